@@ -261,7 +261,7 @@ def _plain_policy(s, logp):
         lr = torch.where(mask, s["ref"].double() - logp, 0.0)
         kl = lr.exp() - lr - 1
         d = d + c["beta"] * (1 - lr.exp())
-    n = mask.sum(1, keepdim=True)
+    n = mask.sum(1, keepdim=True).double()
     w = mask / n.sum() if c["normalizer"] == "tokens" else \
         mask / n.clamp(min=1) / (n > 0).sum()
     loss = ((c["beta"] * kl - gain) * w).sum()
