@@ -1,0 +1,77 @@
+// Dropout with a mask that is made where it is needed and never stored (philox.hpp):
+// y = dt(x * scale) where kept, 0 where dropped; the backward is the same call on the
+// gradient.
+#include <algorithm>
+
+#include "philox.hpp"
+
+using namespace grpo;
+
+namespace {
+
+enum Dtype { BF16 = 0, F16 = 1, F32 = 2 };
+
+// One thread: eight consecutive values, one generator block.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) dropout_kernel(const void* x, void* y, int64_t n,
+                                                      Dropout d) {
+  const DropKey key = drop_key(d.rng);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; 8 * i < n;
+       i += (int64_t)gridDim.x * 256) {
+  const int64_t e = 8 * i;
+  const uint4 w = philox((uint64_t)i, key);
+  if (VEC && e + 8 <= n) {
+    if (DT == F32) {
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(x) + e);
+      const float4 a = s[0], b = s[1];
+      auto keep = [&](float v, int j) __attribute__((always_inline)) {
+        return drop_keeps(w, j, d.threshold) ? v * d.scale : 0.f;
+      };
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(y) + e);
+      o[0] = make_float4(keep(a.x, 0), keep(a.y, 1), keep(a.z, 2), keep(a.w, 3));
+      o[1] = make_float4(keep(b.x, 4), keep(b.y, 5), keep(b.z, 6), keep(b.w, 7));
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + e);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(y) + e) =
+          drop8<DT == F16>(v, w, d.threshold, d.scale);
+    }
+    continue;
+  }
+  for (int j = 0; j < 8 && e + j < n; ++j) {
+    const bool on = drop_keeps(w, j, d.threshold);
+    if (DT == F32) {
+      const float v = static_cast<const float*>(x)[e + j];
+      static_cast<float*>(y)[e + j] = on ? v * d.scale : 0.f;
+    } else {
+      const float v = e2f<DT == F16>(static_cast<const uint16_t*>(x)[e + j]);
+      static_cast<uint16_t*>(y)[e + j] = f2e<DT == F16>(on ? v * d.scale : 0.f);
+    }
+  }
+  }
+}
+
+template <int DT>
+int launch(const void* x, void* y, int64_t n, const Dropout& d, hipStream_t st) {
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(n, 8 * 256), 1 << 20);
+  if (aligned16(x) && aligned16(y))
+    dropout_kernel<DT, true><<<grid, 256, 0, st>>>(x, y, n, d);
+  else
+    dropout_kernel<DT, false><<<grid, 256, 0, st>>>(x, y, n, d);
+  return launch_check("dropout");
+}
+
+}  // namespace
+
+extern "C" int grpo_dropout(const void* x, void* y, int64_t numel, int dtype, double p,
+                            const int64_t* rng, grpo_stream_t stream) {
+  if (numel < 0) return einval("negative numel");
+  if (dtype < 0 || dtype > 2) return einval("dtype must be 0 (bf16), 1 (float16) or 2 (float32)");
+  Dropout d;
+  if (int rc = drop_args(rng, p, &d)) return rc;
+  if (numel == 0) return GRPO_OK;
+  if (!x || !y || !rng) return einval("null pointer");
+  hipStream_t st = as_stream(stream);
+  if (dtype == BF16) return launch<BF16>(x, y, numel, d, st);
+  if (dtype == F16) return launch<F16>(x, y, numel, d, st);
+  return launch<F32>(x, y, numel, d, st);
+}

@@ -67,6 +67,23 @@ class TileLinear(ctypes.Structure):
 
 _TILE = ctypes.POINTER(TileLinear)
 
+
+class Policy(ctypes.Structure):
+    """``grpo_policy_t``: clip range, cap, KL weight and normalization of the policy loss."""
+
+    _fields_ = [
+        ("eps_low", _c.c_double),
+        ("eps_high", _c.c_double),
+        ("delta", _c.c_double),
+        ("beta", _c.c_double),
+        ("denom", _c.c_double),
+        ("normalizer", _I32),
+    ]
+
+
+_POLICY = ctypes.POINTER(Policy)
+_ROWS = [_VP, _I32, _I64, _I64, _I32, _I32, _I32, _VP, _VP, _F32]  # logits .. temperature
+
 # name -> (restype, argtypes); mirrors include/grpo_hip.h one to one.
 SIGNATURES = {
     "grpo_version": (_I32, []),
@@ -77,6 +94,16 @@ SIGNATURES = {
     "grpo_nf4_absmax_expand": (_I32, [_VP, _VP, _VP, _I32, _F32, _I64, _VP, _VP]),
     "grpo_nf4_grad_x": (_I32, [_VP, _I64, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _VP, _I64, _VP,
                                 _I64, _VP]),
+    "grpo_token_logprobs": (_I32, [*_ROWS, _VP, _VP, _VP, _VP]),
+    "grpo_token_logprobs_backward": (_I32, [*_ROWS, _VP, _VP, _VP, _VP, _VP]),
+    "grpo_policy_loss_workspace_bytes": (_SZ, [_I32, _I32, _I32]),
+    "grpo_policy_loss": (
+        _I32, [_VP, _VP, _VP, _VP, _I32, _VP, _I32, _I32, _POLICY, _VP, _VP, _VP, _SZ, _VP]),
+    "grpo_policy_loss_backward": (
+        _I32, [_VP, _VP, _VP, _VP, _I32, _VP, _I32, _I32, _POLICY, _VP, _VP, _VP, _SZ, _VP]),
+    "grpo_policy_loss_logits": (
+        _I32, [*_ROWS, _VP, _VP, _VP, _I32, _POLICY, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "grpo_dropout": (_I32, [_VP, _VP, _I64, _I32, _c.c_double, _VP, _VP]),
     "grpo_nf4_dequant_t": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _VP]),
     "grpo_gemm16_tile": (_I32, [_I32, _I32, _c.POINTER(_I32), _c.POINTER(_I32)]),
     "grpo_nf4_lora_train_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32, _I32]),

@@ -8,6 +8,9 @@ Exports the reference's hot-path operator surface:
   (``__init__.py:234-262``), else to the model-level decode
   (``__init__.py:264-296``);
 * ``lora_fused_forward(...)`` (``__init__.py:323-354``);
+* the policy update's ``fused_grpo_loss`` (``__init__.py:300``), with its parts
+  ``token_logprobs`` and ``grpo_policy_loss``;
+* ``counter_dropout``, the LoRA layers' dropout without a stored mask;
 * ``HIP_AVAILABLE`` (and ``TRITON_AVAILABLE``, the reference's flag name, as an
   alias so callers such as ``src/grpo/trainer.py:387`` keep working).
 
@@ -33,6 +36,10 @@ _kernel_cache: dict[str, Callable[..., object] | None] = {}
 _EXPLICIT_MODULES = {
     "paged_kv_decode": "grpo_mi355x.kernels.paged_kv",
     "lora_fused_forward": "grpo_mi355x.kernels.lora_forward",
+    "fused_grpo_loss": "grpo_mi355x.kernels.policy_loss",
+    "token_logprobs": "grpo_mi355x.kernels.policy_loss",
+    "grpo_policy_loss": "grpo_mi355x.kernels.policy_loss",
+    "counter_dropout": "grpo_mi355x.kernels.dropout",
     "paged_kv_decode_model": "grpo_mi355x.rollout.decode",
 }
 
@@ -113,4 +120,35 @@ def lora_fused_forward(x: object, base_layer: object | None = None, lora_A: obje
                   dropout=dropout, lora_layer=lora_layer, prefer_base_layer=prefer_base_layer)
 
 
-__all__ = ["HIP_AVAILABLE", "TRITON_AVAILABLE", "paged_kv_decode", "lora_fused_forward"]
+def _call(name: str, *args: object, **kwargs: object) -> object:
+    kernel = _get_hip_kernel(name)
+    if kernel is None:
+        raise _unavailable(name)
+    return kernel(*args, **kwargs)
+
+
+def token_logprobs(logits: object, token_ids: object, mask: object | None = None,
+                   **kwargs: object) -> object:
+    """``policy_loss.token_logprobs``."""
+    return _call("token_logprobs", logits, token_ids, mask, **kwargs)
+
+
+def grpo_policy_loss(logps: object, old_logps: object, advantages: object,
+                     mask: object | None = None, **kwargs: object) -> object:
+    """``policy_loss.grpo_policy_loss``."""
+    return _call("grpo_policy_loss", logps, old_logps, advantages, mask, **kwargs)
+
+
+def fused_grpo_loss(logits: object, token_ids: object, old_logps: object, advantages: object,
+                    mask: object | None = None, **kwargs: object) -> object:
+    """``policy_loss.fused_grpo_loss``."""
+    return _call("fused_grpo_loss", logits, token_ids, old_logps, advantages, mask, **kwargs)
+
+
+def counter_dropout(x: object, p: float, rng: object) -> object:
+    """``dropout.counter_dropout``."""
+    return _call("counter_dropout", x, p, rng)
+
+
+__all__ = ["HIP_AVAILABLE", "TRITON_AVAILABLE", "paged_kv_decode", "lora_fused_forward",
+           "token_logprobs", "grpo_policy_loss", "fused_grpo_loss", "counter_dropout"]

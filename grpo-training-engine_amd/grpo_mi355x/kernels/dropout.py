@@ -1,0 +1,81 @@
+"""``counter_dropout`` -- dropout whose mask is never stored (``csrc/dropout.hip``).
+
+The mask is a function of the element's index and of ``rng``, two int64 on the device
+(seed and offset): the backward, and every kernel that needs it, makes it again.  ``rng`` is
+read on the device, so a captured graph draws new masks when the tensor changes.
+"""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def check_dropout(p: float, rng: torch.Tensor, device: torch.device) -> float:
+    """``p`` as a float, after the checks that every dropout entry point makes."""
+    p = float(p)
+    if not (0.0 <= p and p * 65536.0 + 0.5 < 65536.0):
+        raise ValueError(f"dropout p must be in [0, 1) (in steps of 1/65536), got {p}.")
+    if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
+        raise ValueError("rng must be a contiguous int64 tensor of two values, seed and offset.")
+    if rng.device != device:
+        raise ValueError(f"rng must be on {device}, got {rng.device}.")
+    return p
+
+
+def _dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
+    x = x.detach()
+    if not x.is_contiguous():
+        x = x.contiguous()
+    y = torch.empty_like(x)
+    dev = x.device
+    with (contextlib.nullcontext() if dev.index == torch.cuda.current_device()
+          else torch.cuda.device(dev)):
+        rc = _lib.device_library().grpo_dropout(x.data_ptr(), y.data_ptr(), x.numel(),
+                                                _DTYPES[x.dtype], p, rng.data_ptr(),
+                                                _lib.stream_handle(dev))
+    if rc:
+        _lib.check(rc, "grpo_dropout")
+    return y
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, rng):
+        ctx.p = p
+        ctx.save_for_backward(rng)
+        return _dropout(x, p, rng)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        return _dropout(grad, ctx.p, ctx.saved_tensors[0]), None, None
+
+
+def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
+    """``x`` with each element dropped with probability ``p``, the others scaled.
+
+    Element ``e`` of ``x`` (row-major) is dropped iff ``u(e) < t``, ``t = round(65536 p)``,
+    where ``u(e)`` are 16 bits of the Philox4x32-10 block with counter ``(e // 8, offset)``
+    and key ``seed``, ``rng = [seed, offset]``; the rest is multiplied by
+    ``65536 / (65536 - t)`` and rounded once.  A dropped element gives 0, also where x is
+    not finite.  The same ``rng`` gives the same mask; the caller changes the offset from
+    call to call (``CounterDropout`` does), and leaves ``rng`` unchanged until the backward
+    has run.  bfloat16, float16 or float32, any shape."""
+    if not x.is_cuda:
+        raise ValueError("x must be on the ROCm/HIP device.")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}.")
+    p = check_dropout(p, rng, x.device)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dropout.apply(x, p, rng)
+    return _dropout(x, p, rng)
+
+
+__all__ = ["counter_dropout", "check_dropout"]

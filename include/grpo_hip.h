@@ -87,6 +87,83 @@ int grpo_nf4_grad_x(const void* grad, int64_t ldg, const uint8_t* w, const float
                     const float* code16, int blocksize, int M, int N, int K, const void* addend,
                     int64_t ld_add, void* out, int64_t ldo, grpo_stream_t stream);
 
+/* ------------------------------------------------- the policy update --
+ * dtype of logits and of dropout's tensors: 0 bf16, 1 float16, 2 float32. Positions are
+ * B sequences of S tokens, R = B * S rows; row (b, s) of the logits starts at element
+ * b * stride_b + s * stride_s and its V values are contiguous (strides >= 0; aligned to
+ * the type, not more). ids int64 [R]; mask uint8 [R] (0: not counted) or NULL: all are
+ * counted. What is not counted is not read: its results are 0. An id outside [0, V) at a
+ * counted row gives NaN. At most 2^22 - 1 rows of logits. */
+
+/* Log-probabilities of given tokens, logp[r] = x_id / T - log sum_v exp(x_v / T), the
+ * log-probability half of _fused_grpo_loss_kernel (src/triton_kernels/grpo_loss.py:47-139).
+ *   logp    : float32 [R]
+ *   entropy : float32 [R], -sum_v p_v log p_v, or NULL
+ *   stat    : float32 [R][4] for grpo_token_logprobs_backward, 16-byte aligned, or NULL */
+int grpo_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_s, int B,
+                        int S, int V, const int64_t* ids, const uint8_t* mask, float temperature,
+                        float* logp, float* entropy, float* stat, grpo_stream_t stream);
+/* grad_logits[r][v] = g / T * (1[v = id] - p_v), g = grad_logp[r] * *scale (scale: one
+ * float32 on the device, or NULL: 1); grad_logits [R][V] contiguous, in the logits' type. */
+int grpo_token_logprobs_backward(const void* logits, int dtype, int64_t stride_b,
+                                 int64_t stride_s, int B, int S, int V, const int64_t* ids,
+                                 const uint8_t* mask, float temperature, const float* stat,
+                                 const float* grad_logp, const float* scale, void* grad_logits,
+                                 grpo_stream_t stream);
+
+/* The two-sided clipped policy loss (GRPOTrainer.compute_grpo_loss, src/grpo/algorithm.py:
+ * 115-254): per counted token, r = exp(logp - old), q = ref - logp, A its advantage,
+ *   l = beta (exp(q) - q - 1) - min(min(r, delta) A, clip(r, 1 - eps_low, 1 + eps_high) A)
+ *   loss = sum w l,  w = 1 / counted tokens (normalizer 0), 1 / (counted tokens of the
+ *   sequence * sequences that have some) (1), 1 / denom (2). */
+typedef struct {
+  double eps_low, eps_high;
+  double delta; /* INFINITY: no cap */
+  double beta;
+  double denom; /* normalizer 2 */
+  int normalizer;
+} grpo_policy_t;
+
+/* Workspace bytes of the entry points below (from_logits: grpo_policy_loss_logits). */
+size_t grpo_policy_loss_workspace_bytes(int B, int S, int from_logits);
+/*   logp, old_logp, ref_logp : float32 [R]; old_logp NULL: logp itself; ref_logp NULL: no
+ *                              KL term
+ *   advantages : float32 [B], or [R] (adv_tokens != 0)
+ *   loss       : float32 [1]
+ *   metrics    : float32 [4], means over the counted tokens: r, tokens whose gain no
+ *                longer follows r, the KL term exp(q) - q - 1, old - logp
+ * Nothing counted: loss and metrics are 0. */
+int grpo_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
+                     const float* advantages, int adv_tokens, const uint8_t* mask, int B, int S,
+                     const grpo_policy_t* policy, float* loss, float* metrics, void* workspace,
+                     size_t workspace_bytes, grpo_stream_t stream);
+/* grad_logp[r] = *grad_loss * d loss / d logp[r], float32 [R]; the workspace is the one
+ * that grpo_policy_loss filled for the same mask. */
+int grpo_policy_loss_backward(const float* logp, const float* old_logp, const float* ref_logp,
+                              const float* advantages, int adv_tokens, const uint8_t* mask, int B,
+                              int S, const grpo_policy_t* policy, const float* grad_loss,
+                              float* grad_logp, void* workspace, size_t workspace_bytes,
+                              grpo_stream_t stream);
+/* Both in one (fused_grpo_loss, src/triton_kernels/grpo_loss.py:571-625): logp, loss and
+ * metrics from the logits; stat [R][4] and coef [R] (both or neither) are what
+ * grpo_token_logprobs_backward takes as stat and grad_logp, with the loss's gradient as
+ * its scale. */
+int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b, int64_t stride_s,
+                            int B, int S, int V, const int64_t* ids, const uint8_t* mask,
+                            float temperature, const float* old_logp, const float* ref_logp,
+                            const float* advantages, int adv_tokens, const grpo_policy_t* policy,
+                            float* loss, float* logp, float* metrics, float* stat, float* coef,
+                            void* workspace, size_t workspace_bytes, grpo_stream_t stream);
+
+/* Dropout with a mask that is never stored: y[e] = dt(x[e] * scale), 0 where dropped.
+ * Element e is dropped iff u(e) < t, t = round(65536 p), where u(e) are 16 bits of the
+ * Philox4x32-10 block with counter (e / 8, offset) and key seed: word e % 8 / 2, low half
+ * first; scale = 65536 / (65536 - t). rng: int64 [2] on the device, seed and offset. The
+ * backward is the same call on the gradient. x and y [numel], contiguous; may be the same.
+ * 0 <= p and t < 65536. */
+int grpo_dropout(const void* x, void* y, int64_t numel, int dtype, double p, const int64_t* rng,
+                 grpo_stream_t stream);
+
 /* ------------------------------------------- LoRA side of the training --
  * dtype of every 16-bit operand: bf16 (f16 == 0) or float16 (f16 != 0). */
 

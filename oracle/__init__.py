@@ -19,6 +19,9 @@ This package restates, in numpy, the arithmetic of the reference's hot path
 * ``oracle.sampling``    -- the sampled-token rule of the device sampler for a
                             given uniform draw (temperature, top-p cut, ties),
                             and the SplitMix64 draw of (seed, row, step).
+* ``oracle.policy_loss`` -- token log-probabilities, the two-sided clipped policy
+                            loss (``src/grpo/algorithm.py:115-254``) and their
+                            gradients in float64; the counter-based dropout mask.
 
 Only ``tests/``, ``__graft_entry__.smoke()`` and the ``cpu_baseline`` leg of
 ``bench.py`` may import this package, and only as the checker or as the timed
@@ -57,6 +60,9 @@ Pinning (what each function is checked against, besides the GPU kernels):
                                     ``exp_nonpos`` against float64 ``exp``;
                                     ``splitmix64`` against published vectors
                                     (``tests/test_oracle_sampling.py``).
+* ``policy_loss``                -- torch's CPU autograd in float64, central
+                                    differences; Philox's published known
+                                    answers (``tests/test_oracle_policy_loss.py``).
 """
 
-__all__ = ["bf16", "nf4", "lora_linear", "paged", "decode", "sampling"]
+__all__ = ["bf16", "nf4", "lora_linear", "paged", "decode", "sampling", "policy_loss"]

@@ -1,0 +1,544 @@
+"""The policy update's loss kernels against ``oracle.policy_loss`` in float64.
+
+Bounds, with e = 2^-24 (half a float32 step), per counted row of V logits:
+
+* every term exp2(x k - M) is off by at most 2 e (the exponential's ulp) and, from its
+  argument a, by ln 2 |a| e relative, weighted by 2^a <= 1: 0.54 e; a sum of n terms in
+  order adds at most n e of the whole, and a thread sums at most ceil(V / 512) + 8 terms
+  before ten more levels; so S is off by (V / 512 + 24) e relative, logp by as much.
+* k is off by e relative: logp by e times the distance of the token's logit from the
+  distribution's mean, at most |logp| + H.
+* logp's rounding: e |logp|.
+
+The entropy adds t / S: sums of terms e^a a of one sign up to |a| <= 2 log2 V + 32, bounded
+by (V / 512 + 26) e (H + 1) in the same way. A gradient c / T (1[v = id] - p_v) is off by p's
+relative error (that of S, 2.6 e for its own exponential with |a| up to 150: 104 e) plus three
+roundings, then half a step of its type.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import policy_loss as P
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def within(got, want, tol):
+    """|got - want| <= tol everywhere (a NaN fails), with what is wrong in a few words."""
+    if isinstance(got, torch.Tensor):
+        got = got.detach().cpu().double().numpy()
+    got = np.asarray(got).reshape(np.shape(want))
+    with np.errstate(invalid="ignore"):
+        bad = ~(np.abs(got - want) <= tol)
+    at = tuple(int(i[0]) for i in np.nonzero(bad)) if bad.any() else None
+    assert at is None, (f"{bad.sum()} of {bad.size} off, first {at}: {got[at]} for {want[at]}, "
+                        f"bound {np.broadcast_to(tol, bad.shape)[at]}")
+
+
+def _ops():
+    from grpo_mi355x import kernels
+
+    return kernels
+
+
+def make(rows, vocab, dtype, seed, std=2.0, shift=0.0, counted=0.75):
+    """CPU inputs: logits in the type, ids (-100 where not counted), mask."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, vocab, generator=g) * std + shift
+    ids = torch.randint(0, vocab, (rows,), generator=g)
+    x[torch.arange(rows), ids] += 6 * torch.rand(rows, generator=g)
+    mask = torch.rand(rows, generator=g) < counted
+    return x.to(DT[dtype]), torch.where(mask, ids, -100), mask
+
+
+def bounds(x, ids, mask, t):
+    """(logp, entropy, softmax) in float64 and the bounds on the first two."""
+    logp, ent, p = P.token_logprobs(x.double().numpy(), ids.numpy(), mask.numpy(), t)
+    n = x.shape[1] / 512 + 24
+    return logp, ent, p, E * (n + 2 * np.abs(logp) + ent), E * (n + 2) * (2 * ent + 2)
+
+
+def grad_bound(want, p, coef, t, dtype):
+    c = np.abs(coef / t)[:, None]
+    half = torch.finfo(DT[dtype]).eps / 2
+    tiny = {"f16": 2.0 ** -25, "bf16": 0.0, "f32": 0.0}[dtype] + 2.0 ** -126
+    return E * c * (p * (p.shape[1] / 512 + 130) + 3) * (p > 0) + half * np.abs(want) + tiny
+
+
+VOCABS = [1, 2, 7, 8, 9, 511, 1000, 4097, 32003]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vocab", VOCABS)
+@pytest.mark.parametrize("t", [1.0, 0.7])
+def test_token_logprobs_and_gradient(dev, dtype, vocab, t):
+    rows = 5
+    x, ids, mask = make(rows, vocab, dtype, seed=vocab + int(10 * t))
+    logp, ent, p, tol, tol_ent = bounds(x, ids, mask, t)
+    leaf = x.to(dev).requires_grad_()
+    got, got_ent = _ops().token_logprobs(leaf, ids.to(dev), mask.to(dev), temperature=t,
+                                         return_entropy=True)
+    assert got.dtype == got_ent.dtype == torch.float32
+    assert not got_ent.requires_grad
+    within(got, logp, tol)
+    within(got_ent, ent, tol_ent)
+    coef = torch.randn(rows, generator=torch.Generator().manual_seed(1))
+    grad, = torch.autograd.grad(got, leaf, coef.to(dev))
+    want = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy(), t)
+    assert grad.dtype == x.dtype and grad.shape == x.shape
+    within(grad, want, grad_bound(want, p, coef.double().numpy(), t, dtype))
+    assert not grad[~mask.to(dev)].any()
+    with torch.no_grad():  # the form without a gradient gives the same values
+        again = _ops().token_logprobs(leaf, ids.to(dev), mask.to(dev), temperature=t)
+    assert torch.equal(again, got.detach())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [151936, 152064, 262147])
+def test_whole_vocabularies(dev, dtype, vocab):
+    x, ids, mask = make(3, vocab, dtype, seed=5, counted=1.1)
+    logp, ent, p, tol, tol_ent = bounds(x, ids, mask, 1.0)
+    leaf = x.to(dev).requires_grad_()
+    got, got_ent = _ops().token_logprobs(leaf, ids.to(dev), return_entropy=True)
+    within(got, logp, tol)
+    within(got_ent, ent, tol_ent)
+    coef = torch.tensor([1.0, -2.0, 0.5])
+    grad, = torch.autograd.grad(got, leaf, coef.to(dev))
+    want = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy())
+    within(grad, want, grad_bound(want, p, coef.double().numpy(), 1.0, dtype))
+
+
+def test_an_offset_of_all_logits_changes_nothing(dev):
+    x, ids, mask = make(4, 5000, "f32", seed=2, counted=1.1)
+    x = torch.round(x * 64) / 64  # so that the shifted logits are exact too
+    for shift in (0.0, 1000.0, -4096.0, 65536.0):
+        y = x + shift
+        logp, _, _, tol, _ = bounds(x, ids, mask, 0.7)
+        got = _ops().token_logprobs(y.to(dev), ids.to(dev), temperature=0.7)
+        assert torch.equal(y - shift, x)
+        # x k - M has one rounding at the size of its result: no shift in the bound
+        within(got, logp, tol)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_masked_vocabulary_and_lowest_values(dev, dtype):
+    x, ids, _ = make(6, 777, dtype, seed=9, counted=1.1)
+    low = torch.finfo(x.dtype).min
+    x[0, 100:] = -math.inf
+    ids[0] = 3
+    x[1, 100:] = low
+    ids[1] = 5
+    x[2] = low                      # the whole row at the lowest value: uniform
+    x[3, ids[3]] = -math.inf        # the token itself is ruled out
+    x[4, :] = -math.inf
+    x[4, 9] = 2.0
+    ids[4] = 9                      # only one token is left
+    mask = torch.ones(6, dtype=torch.bool)
+    logp, ent, p, tol, tol_ent = bounds(x, ids, mask, 1.0)
+    leaf = x.to(dev).requires_grad_()
+    got, got_ent = _ops().token_logprobs(leaf, ids.to(dev), return_entropy=True)
+    g = got.detach().cpu().double().numpy()
+    assert g[3] == -math.inf and logp[3] == -math.inf
+    keep = np.array([0, 1, 2, 4, 5])
+    within(g[keep], logp[keep], tol[keep])
+    within(got_ent, ent, tol_ent)
+    assert abs(g[4]) <= 3 * E  # one term: its own error, not a sum's
+    coef = torch.ones(6)
+    grad, = torch.autograd.grad(got, leaf, coef.to(dev))
+    want = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy())
+    within(grad, want, grad_bound(want, p, np.ones(6), 1.0, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_values_that_are_not_finite(dev, dtype):
+    x, ids, mask = make(6, 1030, dtype, seed=4, counted=1.1)
+    x[0] = -math.inf                # nothing left: NaN, as a log-softmax
+    x[1, 7] = math.inf
+    x[2, 900] = math.nan
+    x[3] = math.nan                 # not counted: not read
+    x[4, 0] = math.inf
+    mask[3] = mask[4] = False
+    ids[3], ids[4] = -100, 10 ** 12
+    leaf = x.to(dev).requires_grad_()
+    got, ent = _ops().token_logprobs(leaf, ids.to(dev), mask.to(dev), return_entropy=True)
+    want = torch.log_softmax(x.double(), -1)[torch.arange(6), ids.clamp(0, 1029)]
+    g = got.detach().cpu()
+    assert torch.isnan(g[:3]).all() and torch.isnan(want[:3]).all()
+    assert g[3] == g[4] == 0 and ent[3] == ent[4] == 0
+    assert abs(float(g[5]) - float(want[5])) <= 64 * E * (1 + abs(float(want[5])))
+    grad, = torch.autograd.grad(got.sum(), leaf)
+    assert torch.isnan(grad[:3]).any(1).all()
+    assert not grad[3:5].any()
+    assert torch.isfinite(grad[5]).all()
+
+
+def test_ids_outside_the_vocabulary_give_nan(dev):
+    x, ids, mask = make(4, 100, "f32", seed=1, counted=1.1)
+    ids[0], ids[1], ids[2] = -1, 100, 2 ** 40
+    got = _ops().token_logprobs(x.to(dev), ids.to(dev))
+    assert torch.isnan(got[:3]).all() and torch.isfinite(got[3])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_strided_and_unaligned_logits(dev, dtype):
+    """Rows at every alignment: slices of the vocabulary, of the positions, an expanded
+    batch and a transposed one give what their contiguous copies give."""
+    base, _, _ = make(6 * 5, 135, dtype, seed=8)
+    base = base.view(6, 5, 135).to(dev)
+    views = [base[:, :-1], base[:, 1:, 3:130], base[::2, :, 1:], base.transpose(0, 1),
+             base[:1].expand(3, -1, -1), base[..., ::2], base[:, 2]]
+    for v in views:
+        ids = torch.randint(0, v.shape[-1], v.shape[:-1], device=dev)
+        mask = torch.rand(ids.shape, device=dev) < 0.8
+        out = []
+        for x in (v, v.contiguous()):
+            leaf = x.detach().requires_grad_()
+            assert leaf.stride() == x.stride()
+            got, ent = _ops().token_logprobs(leaf, ids, mask, return_entropy=True)
+            grad, = torch.autograd.grad(got, leaf, torch.ones_like(got))
+            out.append((got.detach(), ent, grad))
+        # another split of the row over the threads: the sums' order differs
+        assert torch.allclose(out[0][0], out[1][0], rtol=4 * E, atol=64 * E)
+        assert torch.allclose(out[0][1], out[1][1], rtol=64 * E, atol=64 * E)
+        assert torch.allclose(out[0][2].float(), out[1][2].float(),
+                              rtol=2 * torch.finfo(v.dtype).eps, atol=64 * E)
+
+
+def test_leading_shapes(dev):
+    x, ids, _ = make(24, 50, "f32", seed=3)
+    ids = ids.clamp(min=0).to(dev)
+    flat = _ops().token_logprobs(x.to(dev), ids)
+    four = _ops().token_logprobs(x.to(dev).view(2, 3, 4, 50), ids.view(2, 3, 4))
+    assert torch.equal(four.reshape(-1), flat)
+    for shape in ((0, 5, 50), (3, 0, 50), (0, 50)):
+        leaf = torch.zeros(shape, device=dev, requires_grad=True)
+        got = _ops().token_logprobs(leaf, torch.zeros(shape[:-1], dtype=torch.int64, device=dev))
+        assert got.shape == shape[:-1]
+        got.sum().backward()
+        assert leaf.grad.shape == shape
+
+
+def test_refusals_on_the_device(dev):
+    x = torch.zeros(2, 3, 8, device=dev)
+    ids = torch.zeros(2, 3, dtype=torch.int64, device=dev)
+    ops = _ops()
+    for bad, message in [((x.double(), ids), "bfloat16"), ((x, ids.int()), "int64"),
+                         ((x, ids[:1]), "token_ids must be"), ((x, ids.cpu()), "must be on"),
+                         ((x[..., :0], ids), "at least one"), ((x[0, 0], ids[0, 0]), "vocab"),
+                         ((x, ids, ids[:, :2]), "mask must be")]:
+        with pytest.raises(ValueError, match=message):
+            ops.token_logprobs(*bad)
+    for t in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_logprobs(x, ids, temperature=t)
+    with pytest.raises(ValueError, match="batch, seq, vocab"):
+        ops.fused_grpo_loss(x[0], ids[0], None, torch.zeros(3, device=dev))
+    leaf = x.clone().requires_grad_()
+    got = ops.token_logprobs(leaf, ids)
+    grad, = torch.autograd.grad(got.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivative
+        grad.sum().backward()
+
+
+# ------------------------------------------------------------- policy loss --
+
+def tokens(b, s, seed, counted=0.75, spread=0.4):
+    """Log-probabilities whose ratios keep 1e-3 from every border used below."""
+    g = np.random.default_rng(seed)
+    logp = (-3 * g.random((b, s))).astype(np.float32)
+    diff = spread * g.standard_normal((b, s))
+    for border in (math.log(0.8), math.log(1.2), math.log(1.28), math.log(1.5)):
+        near = np.abs(diff - border) < 1e-3
+        diff[near] = border + 2e-3
+    old = (logp - diff).astype(np.float32)
+    ref = (logp + 0.3 * g.standard_normal((b, s))).astype(np.float32)
+    mask = g.random((b, s)) < counted
+    if b > 2:
+        mask[1] = False
+    return logp, old, ref, g.standard_normal(b).astype(np.float32), mask
+
+
+def close(got, want, scale, n):
+    """float64 work on float32 inputs: one rounding of the result, sums of n terms of
+    absolute sum ``scale`` in float64."""
+    got = float(got.detach())
+    return abs(got - want) <= 1.01 * E * abs(want) + (n + 64) * 2.0 ** -52 * scale + 1e-45
+
+
+@pytest.mark.parametrize("b, s", [(1, 1), (3, 1), (1, 257), (5, 333), (64, 200), (700, 3),
+                                  (2, 40000)])
+@pytest.mark.parametrize("normalizer", ["tokens", "sequences", 1234.5])
+@pytest.mark.parametrize("beta, delta", [(0.0, None), (0.04, 1.5)])
+def test_policy_loss_and_gradient(dev, b, s, normalizer, beta, delta):
+    logp, old, ref, adv, mask = tokens(b, s, seed=b * 1000 + s)
+    want, want_metrics, want_grad = P.policy_loss(
+        logp, old, adv, mask, ref if beta else None, 0.2, 0.28, delta or math.inf, beta,
+        normalizer)
+    put = lambda a: torch.from_numpy(a).to(dev)  # noqa: E731
+    leaf = put(logp).requires_grad_()
+    loss, metrics = _ops().grpo_policy_loss(
+        leaf, put(old), put(adv), put(mask), ref_logps=put(ref) if beta else None, eps_low=0.2,
+        eps_high=0.28, delta=delta, beta=beta, normalizer=normalizer)
+    n = mask.sum()
+    # exp is off by a step or two of float64; the terms' absolute sum is at most
+    scale = float(np.abs(adv).max() * 4 + 1) * (1.0 if isinstance(normalizer, str)
+                                                else n / normalizer)
+    assert loss.shape == () and loss.dtype == torch.float32
+    assert close(loss, want, scale, n)
+    assert not metrics.requires_grad
+    for j in range(4):
+        assert close(metrics[j], want_metrics[j], 8.0, n), j
+    factor = -0.75
+    grad, = torch.autograd.grad(loss * factor, leaf)
+    # the derivative, its product with the upstream gradient and one rounding
+    within(grad, factor * want_grad, 1.01 * E * np.abs(factor * want_grad) + 2.0 ** -149)
+    assert not grad[~put(mask)].any()
+
+
+def test_policy_loss_by_differences(dev):
+    """The gradient is the difference quotient of the loss itself."""
+    logp, old, ref, adv, mask = tokens(3, 4, seed=11, counted=1.1)
+    mask[:] = True
+    put = lambda a: torch.from_numpy(a).to(dev)  # noqa: E731
+
+    def loss(lp):
+        return _ops().grpo_policy_loss(lp, put(old), put(adv), put(mask), ref_logps=put(ref),
+                                       beta=0.1, eps_high=0.28, normalizer=1.0)
+
+    leaf = put(logp).requires_grad_()
+    grad, = torch.autograd.grad(loss(leaf)[0], leaf)
+    h = 2.0 ** -11
+    for b in range(3):
+        for s in range(4):
+            d = torch.zeros_like(leaf)
+            d[b, s] = h
+            up, down = float(loss(leaf.detach() + d)[0]), float(loss(leaf.detach() - d)[0])
+            # the loss's own rounding (12 terms of a size up to 4: 48 e each way) over 2 h,
+            # and a third derivative of at most 16
+            assert abs((up - down) / (2 * h) - float(grad[b, s])) <= 96 * E / h + 16 * h * h
+
+
+def test_policy_loss_options(dev):
+    logp, old, ref, adv, mask = tokens(6, 50, seed=21)
+    put = lambda a: torch.from_numpy(a).to(dev)  # noqa: E731
+    ops = _ops()
+    leaf = put(logp).requires_grad_()
+    # on-policy: no old log-probabilities, every ratio 1
+    loss, metrics = ops.grpo_policy_loss(leaf, None, put(adv), put(mask))
+    want, _, want_grad = P.policy_loss(logp, None, adv, mask)
+    assert close(loss, want, 8.0, mask.size)
+    assert metrics[0] == 1 and metrics[1] == 0 and metrics[3] == 0
+    grad, = torch.autograd.grad(loss, leaf)
+    within(grad, want_grad, 1.01 * E * np.abs(want_grad))
+    # an advantage for each token, masks of other types, no mask
+    wide = np.ascontiguousarray(np.broadcast_to(adv[:, None], logp.shape))
+    base = ops.grpo_policy_loss(put(logp), put(old), put(adv), put(mask))
+    for m in (put(mask).long(), put(mask).float(), put(mask).to(torch.uint8)):
+        got = ops.grpo_policy_loss(put(logp), put(old), put(wide), m)
+        assert torch.equal(got[0], base[0]) and torch.equal(got[1], base[1])
+    full = ops.grpo_policy_loss(put(logp), put(old), put(adv))
+    ones = ops.grpo_policy_loss(put(logp), put(old), put(adv), torch.ones_like(put(mask)))
+    assert torch.equal(full[0], ones[0]) and torch.equal(full[1], ones[1])
+    # strided and 16-bit inputs are taken at their values
+    t = put(logp).t().contiguous().t()
+    got = ops.grpo_policy_loss(t, put(old).double(), put(adv), put(mask))
+    assert torch.equal(got[0], base[0])
+
+
+@pytest.mark.parametrize("normalizer", ["tokens", "sequences", 7.0])
+def test_nothing_counted(dev, normalizer):
+    b, s, v = 3, 4, 40
+    nan = torch.full((b, s), math.nan, device=dev)
+    mask = torch.zeros(b, s, dtype=torch.bool, device=dev)
+    adv = torch.full((b,), math.nan, device=dev)
+    leaf = nan.clone().requires_grad_()
+    loss, metrics = _ops().grpo_policy_loss(leaf, nan, adv, mask, ref_logps=nan, beta=0.1,
+                                            normalizer=normalizer)
+    loss.backward()
+    assert loss == 0 and not metrics.any() and not leaf.grad.any()
+    logits = torch.full((b, s, v), math.nan, device=dev, requires_grad=True)
+    ids = torch.full((b, s), -100, device=dev)
+    loss, logp, metrics = _ops().fused_grpo_loss(logits, ids, nan, adv, mask, ref_logps=nan,
+                                                 beta=0.1, normalizer=normalizer)
+    loss.backward()
+    assert loss == 0 and not metrics.any() and not logp.any() and not logits.grad.any()
+    for shape in ((0, 4), (3, 0)):
+        e = torch.zeros(shape, device=dev, requires_grad=True)
+        loss, metrics = _ops().grpo_policy_loss(e, None, torch.zeros(shape[0], device=dev),
+                                                normalizer=normalizer)
+        loss.backward()
+        assert loss == 0 and not metrics.any() and e.grad.shape == shape
+
+
+# ------------------------------------------------------ loss from the logits --
+
+def loss_inputs(b, s, vocab, dtype, seed, t=1.0, beta=0.04):
+    x, ids, _ = make(b * s, vocab, dtype, seed, counted=1.1)
+    _, _, _, adv, mask = tokens(b, s, seed)
+    flat = torch.from_numpy(mask.reshape(-1))
+    logp, _, p = P.token_logprobs(x.double().numpy(), ids.numpy(), np.ones(b * s, bool), t)
+    diff = (tokens(b, s, seed + 1)[0] - tokens(b, s, seed + 1)[1]).reshape(-1).astype(np.float64)
+    old = np.float32(logp - diff).reshape(b, s)
+    ref = np.float32(logp + 0.1).reshape(b, s) if beta else None
+    ids = torch.where(flat, ids, -100)
+    return x.view(b, s, vocab), ids.view(b, s), old, ref, adv, mask, logp, p
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("b, s, vocab", [(1, 1, 9), (3, 5, 1000), (4, 33, 4097), (2, 3, 151936),
+                                         (1, 2, 262147), (40, 16, 300)])
+@pytest.mark.parametrize("normalizer, t, beta", [("tokens", 1.0, 0.0), ("sequences", 0.7, 0.04)])
+def test_fused_loss_and_gradient(dev, dtype, b, s, vocab, normalizer, t, beta):
+    x, ids, old, ref, adv, mask, logp, p = loss_inputs(b, s, vocab, dtype, seed=vocab + b, t=t,
+                                                       beta=beta)
+    if not mask.any():
+        mask[0, 0] = True
+        ids[0, 0] = 3
+        logp, _, p = P.token_logprobs(x.view(b * s, vocab).double().numpy(),
+                                      ids.clamp(min=0).reshape(-1).numpy(),
+                                      np.ones(b * s, bool), t)
+    want, want_metrics, d = P.policy_loss(logp.reshape(b, s), old, adv, mask, ref, 0.2, 0.28,
+                                          math.inf, beta, normalizer)
+    put = lambda a: None if a is None else torch.as_tensor(a).to(dev)  # noqa: E731
+    leaf = put(x).requires_grad_()
+    loss, got_logp, metrics = _ops().fused_grpo_loss(
+        leaf, put(ids), put(old), put(adv), put(mask), ref_logps=put(ref), temperature=t,
+        eps_high=0.28, beta=beta, normalizer=normalizer)
+    assert not got_logp.requires_grad and not metrics.requires_grad
+    tol = E * (vocab / 512 + 24 + 2 * np.abs(logp.reshape(b, s)) + math.log(vocab))
+    within(got_logp, np.where(mask, logp.reshape(b, s), 0), tol)
+    top = float(tol.max())  # logp's error moves a ratio below 8 by at most 8 of it
+    scale = float(np.abs(adv).max()) * 8 + 1
+    assert abs(float(loss.detach()) - want) <= top * scale + E * abs(want)
+    for j in range(4):
+        assert abs(float(metrics[j]) - want_metrics[j]) <= 8 * top + E * abs(want_metrics[j]), j
+    factor = 0.5
+    grad, = torch.autograd.grad(loss * factor, leaf)
+    coef = factor * d.reshape(-1)
+    wantg = P.logits_grad(p, ids.clamp(min=0).reshape(-1).numpy(), mask.reshape(-1), coef, t)
+    # the row's factor is off by 2 of logp's error relative (r, and the KL term's exp)
+    slack = (np.abs(coef) * 4 + (0.1 if beta else 0.0)) * top
+    tol = grad_bound(wantg, p, coef, t, dtype) + (slack / t)[:, None] * (
+        p + (np.arange(vocab)[None] == ids.reshape(-1, 1).numpy()))
+    within(grad, wantg, tol * mask.reshape(-1, 1))
+
+
+def test_fused_loss_is_its_parts(dev):
+    """One call equals token_logprobs then grpo_policy_loss, to logp's rounding."""
+    x, ids, old, ref, adv, mask, logp, _ = loss_inputs(4, 20, 3001, "f32", seed=6)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    kw = dict(ref_logps=put(ref), beta=0.04, delta=3.0)
+    one, two = put(x).requires_grad_(), put(x).requires_grad_()
+    loss, lp, metrics = _ops().fused_grpo_loss(one, put(ids), put(old), put(adv), put(mask), **kw)
+    parts = _ops().token_logprobs(two, put(ids), put(mask))
+    assert torch.equal(parts.detach(), lp)
+    loss2, metrics2 = _ops().grpo_policy_loss(parts, put(old), put(adv), put(mask), **kw)
+    tol = 16 * E * float(np.abs(logp).max())
+    assert abs(float(loss) - float(loss2)) <= tol
+    assert torch.allclose(metrics, metrics2, rtol=4 * E, atol=tol)
+    loss.backward()
+    loss2.backward()
+    assert torch.allclose(one.grad, two.grad, rtol=64 * E, atol=tol / mask.sum())
+
+
+def test_backward_twice_and_scaled(dev):
+    """A second backward of a kept graph, and any upstream gradient, give the gradient."""
+    x, ids, old, _, adv, mask, _, _ = loss_inputs(2, 9, 2000, "bf16", seed=3, beta=0.0)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    leaf = put(x).requires_grad_()
+    loss, _, _ = _ops().fused_grpo_loss(leaf, put(ids), put(old), put(adv), put(mask))
+    one, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    kept = one.clone()
+    one.mul_(3.0)  # the caller owns what it was given
+    two, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    assert torch.equal(two, kept)
+    half, = torch.autograd.grad(0.5 * loss, leaf, retain_graph=True)
+    assert torch.equal(half, kept * 0.5)  # a power of two: the same roundings
+    leaf.grad = None
+    loss.backward(retain_graph=True)
+    loss.backward()
+    assert torch.equal(leaf.grad, kept + kept)
+
+
+def test_logits_changed_before_the_backward_are_refused(dev):
+    x, ids, old, _, adv, mask, _, _ = loss_inputs(2, 3, 64, "f32", seed=3, beta=0.0)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    leaf = put(x).requires_grad_()
+    logits = leaf * 1.0
+    loss, _, _ = _ops().fused_grpo_loss(logits, put(ids), put(old), put(adv), put(mask))
+    with torch.no_grad():
+        logits.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_another_stream_and_many_calls(dev):
+    """Calls on a side stream, two in flight, equal those on the default stream."""
+    sets = [loss_inputs(3, 17, 5003, "bf16", seed=s) for s in (1, 2)]
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+
+    def go(x, ids, old, ref, adv, mask, *_):
+        leaf = put(x).requires_grad_()
+        loss, lp, m = _ops().fused_grpo_loss(leaf, put(ids), put(old), put(adv), put(mask),
+                                             ref_logps=put(ref), beta=0.04)
+        return [loss.detach(), lp, m, *torch.autograd.grad(loss, leaf)]
+
+    want = [go(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st, s in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append(go(*s))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+
+
+def test_captured_and_replayed(dev):
+    """Forward and backward in one graph, replayed with other inputs between eager work."""
+    b, s, vocab = 3, 7, 4099
+    sets = [loss_inputs(b, s, vocab, "bf16", seed=k) for k in (1, 2, 3)]
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+
+    def eager(v):
+        leaf = put(v[0]).requires_grad_()
+        loss, lp, m = _ops().fused_grpo_loss(leaf, put(v[1]), put(v[2]), put(v[4]), put(v[5]),
+                                             ref_logps=put(v[3]), beta=0.04)
+        return [loss.detach(), lp, m, *torch.autograd.grad(loss, leaf)]
+
+    want = [eager(v) for v in sets]
+    held = [put(sets[0][i]).clone() for i in range(6)]
+    held[0].requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        loss, lp, m = _ops().fused_grpo_loss(held[0], held[1], held[2], held[4], held[5],
+                                             ref_logps=held[3], beta=0.04)
+        return [loss.detach(), lp, m, *torch.autograd.grad(loss, held[0])]
+
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in (0, 1, 2, 1):
+        with torch.no_grad():
+            for h, v in zip(held, sets[k]):
+                h.copy_(put(v))
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(out, want[k]):
+            assert torch.equal(u, v)
+        eager(sets[k])  # eager work between the replays
+        torch.cuda.synchronize()
