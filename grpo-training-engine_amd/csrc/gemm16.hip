@@ -184,13 +184,18 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
   wait_vm<0>();  // nothing lands after the workgroup's end
 
   const float sc = MODE == GEMM16_LORA ? round_e<F16>(g.scaling) : 1.f;
+  DropKey key{};
+  if (MODE == GEMM16_ADD_DROP) key = drop_key(g.drop.rng);
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
     const int m = m0 + (wm * RM + i) * 16 + ln;
     const uint4 tv = *reinterpret_cast<const uint4*>(g.t + (int64_t)min(m, g.M - 1) * 32 + 8 * lg);
     uint32_t o[2 * RN];
+    uint4 bits{};  // of the eight columns of tiles j and j + 1
 #pragma unroll
     for (int j = 0; j < RN; ++j) {
+      if (MODE == GEMM16_ADD_DROP && j % 2 == 0)
+        bits = philox(((uint64_t)m * g.N + nl + 4 * j) >> 3, key);
       const f32x4_t u = mfma16x16x32_e<F16>(low[j], tv, f32x4_t{0.f, 0.f, 0.f, 0.f});
       float v[4];
 #pragma unroll
@@ -203,6 +208,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
                 v[q] + e2f<F16>((uint16_t)(bias[2 * j + (q >> 1)] >> (16 * (q & 1)))));
           w = round_e<F16>(w * sc);
         }
+        if (MODE == GEMM16_ADD_DROP)
+          w = drop_keeps(bits, 4 * (j & 1) + q, g.drop.threshold) ? round_e<F16>(w * g.drop.scale)
+                                                                  : 0.f;
         v[q] += w;
       }
       o[2 * j] = pack_e2<F16>(v[0], v[1]);
@@ -284,7 +292,10 @@ int gemm16_launch(const Gemm16& g, Gemm16Mode mode, bool f16, hipStream_t st) {
     return einval("GEMM rows must be 16-byte aligned");
   if (g.lda < g.K || g.ldb < g.K || g.ldc < g.N || g.ldl < g.r || g.r < 1 || g.r > 32)
     return einval("row stride too small or rank outside [1, 32]");
+  if (mode == GEMM16_ADD_DROP && !g.drop.rng) return einval("null pointer");
   const Args a{g, 0, 0, g.r % 8 == 0 && g.ldl % 8 == 0 && aligned16(g.low)};
+  if (mode == GEMM16_ADD_DROP)
+    return f16 ? pick<true, GEMM16_ADD_DROP>(a, st) : pick<false, GEMM16_ADD_DROP>(a, st);
   if (mode == GEMM16_ADD)
     return f16 ? pick<true, GEMM16_ADD>(a, st) : pick<false, GEMM16_ADD>(a, st);
   return f16 ? pick<true, GEMM16_LORA>(a, st) : pick<false, GEMM16_LORA>(a, st);

@@ -1,14 +1,15 @@
 // 16-bit MFMA GEMM with the LoRA term in its epilogue (gemm16.hip).
 #pragma once
 
-#include "common.hpp"
+#include "philox.hpp"
 
 namespace grpo {
 
 // C[m, n] = dt(sum_k A[m, k] B[n, k]), both operands contiguous along k, then
 //   GEMM16_ADD   C = dt(C + dt(t low^T))
 //   GEMM16_LORA  C = dt(dt(C [+ bias]) + dt(dt(t low^T) * dt(scaling)))
-enum Gemm16Mode { GEMM16_ADD, GEMM16_LORA };
+//   GEMM16_ADD_DROP  C = dt(C + drop(dt(t low^T))), the mask of a contiguous [M][N]
+enum Gemm16Mode { GEMM16_ADD, GEMM16_LORA, GEMM16_ADD_DROP };
 
 struct Gemm16 {
   const uint16_t* a;  // [M][K], row stride lda
@@ -24,6 +25,7 @@ struct Gemm16 {
   const uint16_t* bias;  // GEMM16_LORA: [N] or null
   int r;                 // 1..32
   float scaling;         // GEMM16_LORA
+  Dropout drop;          // GEMM16_ADD_DROP
 };
 
 // K % 32 == 0 and N % 8 == 0; rows of a, b and c 16-byte aligned; row strides of

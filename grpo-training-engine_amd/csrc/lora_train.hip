@@ -5,6 +5,9 @@
 //   xa = dt(x A^T)                    gi = dt(dt(g * dt(s)) B)
 //   grad_A = dt(gi^T x)               grad_B = dt(dt(g * dt(s))^T xa)
 //   grad_x = dt(dt(g W) + dt(gi A))   y = dt(dt(dt(x W^T) [+ bias]) + dt(dt(t B^T) * dt(s)))
+// With dropout on the adapter's input, drop(x) = dt(x * scale) where kept and 0 elsewhere
+// (philox.hpp), x is drop(x) in xa, t and grad_A, and grad_x adds drop(dt(gi A)); the mask is
+// made again in each of the four kernels that need it.
 //
 // The weight is decoded once per call, not once per row tile: from about 5 million
 // outputs (fewer where the decoding GEMM's ring kernel does not run) the two passes over
@@ -149,6 +152,7 @@ struct PrepArgs {
   const uint16_t* la;  // A [r][K]
   uint16_t* at;        // [K][32] (ranks >= r zero)
   int K;
+  Dropout drop;        // of job 0's rows
 };
 
 template <bool F16>
@@ -167,11 +171,13 @@ __device__ __forceinline__ uint4 keep(bool on, uint4 v) {
 
 // One job's product for rows m0 .. m0 + 15: wave w takes the 64-column steps w,
 // w + 8, ...; lane (row ln, group lg) the columns c0 + 16 lg .. + 15.
-template <int TC, bool F16, bool BT>
+template <int TC, bool F16, bool BT, bool DROP>
 __device__ __forceinline__ void rows_product(const RowsJob& j, const PrepArgs& p, int m0, int wave,
                                              int ln, int lg, f32x4_t (&acc)[TC]) {
   const float sc = BT ? round_e<F16>(p.scaling) : 1.f;
   const uint16_t* const xr = j.src + (int64_t)min(m0 + ln, p.M - 1) * j.ld;
+  DropKey key{};
+  if (DROP) key = drop_key(p.drop.rng);
   int rk[TC];  // ranks >= r repeat rank r - 1; their results are not used
 #pragma unroll
   for (int tc = 0; tc < TC; ++tc) rk[tc] = min(16 * tc + ln, p.r - 1);
@@ -198,13 +204,16 @@ __device__ __forceinline__ void rows_product(const RowsJob& j, const PrepArgs& p
         b[tc] = keep(on, b[tc]);
       }
       if (BT) a = scale8<F16>(a, sc);
+      if (DROP)  // the row's eight values are one block: C % 8 == 0
+        a = drop8<F16>(a, philox(((uint64_t)(m0 + ln) * j.C + cc) >> 3, key), p.drop.threshold,
+                       p.drop.scale);
 #pragma unroll
       for (int tc = 0; tc < TC; ++tc) acc[tc] = mfma16x16x32_e<F16>(a, b[tc], acc[tc]);
     }
   }
 }
 
-template <int TC, bool F16>
+template <int TC, bool F16, bool DROP>
 __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) {
   constexpr int LD = 16 * TC + 1;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -217,9 +226,9 @@ __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) 
 #pragma unroll
   for (int tc = 0; tc < TC; ++tc) acc[tc] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (bt)
-    rows_product<TC, F16, true>(j, p, m0, wave, ln, lg, acc);
+    rows_product<TC, F16, true, false>(j, p, m0, wave, ln, lg, acc);
   else
-    rows_product<TC, F16, false>(j, p, m0, wave, ln, lg, acc);
+    rows_product<TC, F16, false, DROP>(j, p, m0, wave, ln, lg, acc);
 #pragma unroll
   for (int tc = 0; tc < TC; ++tc)
 #pragma unroll
@@ -239,13 +248,13 @@ __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) 
   if (j.cols && rank < 16 * TC) j.cols[(int64_t)rank * p.Mp + m] = v;
 }
 
-template <int TC, bool F16, bool TR>
+template <int TC, bool F16, bool TR, bool DROP>
 __global__ void __launch_bounds__(512) train_prep_kernel(PrepArgs p) {
   __shared__ __align__(16) char lds[TR ? DT * DT_LD * 2 : 8 * 16 * (16 * TC + 1) * 4];
   static_assert(8 * 16 * (16 * TC + 1) * 4 <= DT * DT_LD * 2, "both uses fit");
   int b = blockIdx.x;
   if (b < 2 * p.rows) {
-    rows_tile<TC, F16>(p, b, reinterpret_cast<float*>(lds));
+    rows_tile<TC, F16, DROP>(p, b, reinterpret_cast<float*>(lds));
     return;
   }
   b -= 2 * p.rows;
@@ -285,9 +294,10 @@ struct WgradArgs {
   float* pa;   // [S][r][K]
   uint16_t* gb;
   uint16_t* ga;
+  Dropout drop;  // of x
 };
 
-template <int TC, bool F16>
+template <int TC, bool F16, bool DROP>
 __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
   constexpr int LD = 16 * TC + 1;
   __shared__ float red[2][WG_C * LD];
@@ -300,6 +310,8 @@ __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
   const uint16_t* const src = isg ? p.g : p.x;
   const uint16_t* const low = isg ? p.xat : p.git;
   const float sc = round_e<F16>(p.scaling);
+  DropKey key{};
+  if (DROP) key = drop_key(p.drop.rng);
   const int c = c0 + 8 * ln;
   const bool con = c < C;  // C % 8 == 0
   const uint16_t* const sc0 = src + (con ? c : 0);
@@ -325,6 +337,9 @@ __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
     for (int i = 0; i < 8; ++i) {
       v[i] = keep(con && m + i < p.M, v[i]);  // no 0 * inf from rows past the end
       if (isg) v[i] = scale8<F16>(v[i], sc);
+      else if (DROP)
+        v[i] = drop8<F16>(v[i], philox(((uint64_t)(m + i) * p.K + c) >> 3, key), p.drop.threshold,
+                          p.drop.scale);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -445,8 +460,13 @@ TrainWs train_ws(int M, int N, int K, int r) {
 template <bool F16, bool TR>
 int launch_prep(const PrepArgs& a, hipStream_t st) {
   const unsigned grid = 2u * a.rows + a.dequant.blocks + (a.at ? (unsigned)cdiv(a.K, 128) : 0u);
-  if (a.r > 16) train_prep_kernel<2, F16, TR><<<grid, 512, 0, st>>>(a);
-  else train_prep_kernel<1, F16, TR><<<grid, 512, 0, st>>>(a);
+  if (a.drop.threshold) {
+    if (a.r > 16) train_prep_kernel<2, F16, TR, true><<<grid, 512, 0, st>>>(a);
+    else train_prep_kernel<1, F16, TR, true><<<grid, 512, 0, st>>>(a);
+  } else {
+    if (a.r > 16) train_prep_kernel<2, F16, TR, false><<<grid, 512, 0, st>>>(a);
+    else train_prep_kernel<1, F16, TR, false><<<grid, 512, 0, st>>>(a);
+  }
   return launch_check("train_prep");
 }
 
@@ -470,6 +490,7 @@ struct TrainCall {
   int M, N, K;
   char* ws;
   hipStream_t st;
+  Dropout drop;  // of x on its way to A
 };
 
 template <bool F16>
@@ -481,6 +502,7 @@ int run_forward(const TrainCall& c, const uint16_t* bias, uint16_t* y, int64_t l
   a.M = c.M;
   a.Mp = (int)pad32(c.M);
   a.r = c.r;
+  a.drop = c.drop;
   a.job[0] = RowsJob{c.x, c.ldx, c.la, c.K, rows, nullptr};
   a.rows = a.Mp / 16;
   a.dequant = DequantJob{c.w, c.absmax, c.code16, wd, c.N, c.K, c.bs_shift,
@@ -522,6 +544,7 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
   a.scaling = c.scaling;
   a.rows = Mp / 16;
   a.K = c.K;
+  a.drop = c.drop;
   if (grad_b) a.job[0] = RowsJob{c.x, c.ldx, c.la, c.K, nullptr, xat};
   if (grad_x || grad_a)
     a.job[1] = RowsJob{grad, ldg, c.lb, c.N, grad_x ? rows : nullptr, grad_a ? git : nullptr};
@@ -547,7 +570,9 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
     g.low = at;
     g.ldl = 32;
     g.r = c.r;
-    if (int rc = gemm16_launch(g, GEMM16_ADD, F16, c.st)) return rc;
+    g.drop = c.drop;
+    const Gemm16Mode mode = c.drop.threshold ? GEMM16_ADD_DROP : GEMM16_ADD;
+    if (int rc = gemm16_launch(g, mode, F16, c.st)) return rc;
   }
   if (!grad_a && !grad_b) return GRPO_OK;
   WgradArgs w{};
@@ -572,8 +597,14 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
     w.pa = reinterpret_cast<float*>(c.ws + o.pa);
   }
   const dim3 grid((unsigned)(w.tn + (grad_a ? cdiv(c.K, WG_C) : 0)), (unsigned)S);
-  if (c.r > 16) lora_wgrad_kernel<2, F16><<<grid, 256, 0, c.st>>>(w);
-  else lora_wgrad_kernel<1, F16><<<grid, 256, 0, c.st>>>(w);
+  w.drop = c.drop;
+  if (grad_a && c.drop.threshold) {
+    if (c.r > 16) lora_wgrad_kernel<2, F16, true><<<grid, 256, 0, c.st>>>(w);
+    else lora_wgrad_kernel<1, F16, true><<<grid, 256, 0, c.st>>>(w);
+  } else {
+    if (c.r > 16) lora_wgrad_kernel<2, F16, false><<<grid, 256, 0, c.st>>>(w);
+    else lora_wgrad_kernel<1, F16, false><<<grid, 256, 0, c.st>>>(w);
+  }
   if (int rc = launch_check("lora_wgrad")) return rc;
   if (S == 1) return GRPO_OK;
   const SumArgs sa{w.pb, w.pa, grad_b, grad_a, grad_b ? (int64_t)c.N * c.r : 0,
@@ -607,11 +638,53 @@ int train_check(const void* x, int64_t ldx, const uint8_t* w, const float* absma
 TrainCall train_call(const void* x, int64_t ldx, const uint8_t* w, const float* absmax,
                      const float* code16, int blocksize, const void* lora_a, const void* lora_b,
                      int r, float scaling, int M, int N, int K, void* workspace,
-                     grpo_stream_t stream) {
+                     grpo_stream_t stream, const Dropout& drop) {
   return TrainCall{static_cast<const uint16_t*>(x), ldx, w, absmax, code16,
                    __builtin_ctz((unsigned)blocksize), static_cast<const uint16_t*>(lora_a),
                    static_cast<const uint16_t*>(lora_b), r, scaling, M, N, K,
-                   static_cast<char*>(workspace), as_stream(stream)};
+                   static_cast<char*>(workspace), as_stream(stream), drop};
+}
+
+// The whole of both directions' entry points; drop.threshold 0: no dropout.
+int train_forward(const void* x, int64_t ldx, const uint8_t* w, const float* absmax,
+                  const float* code16, int blocksize, const void* bias, const void* lora_a,
+                  const void* lora_b, int r, float scaling, void* y, int64_t ldy, int M, int N,
+                  int K, int f16, const Dropout& drop, void* workspace, size_t workspace_bytes,
+                  grpo_stream_t stream) {
+  if (int rc = train_check(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, M, N, K,
+                           workspace, workspace_bytes))
+    return rc;
+  if (!y) return einval("null pointer");
+  if (ldy < N || ldy % 8 || !aligned16(y)) return einval("y rows must be 16-byte aligned");
+  const TrainCall c = train_call(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, scaling,
+                                 M, N, K, workspace, stream, drop);
+  const uint16_t* const b = static_cast<const uint16_t*>(bias);
+  uint16_t* const o = static_cast<uint16_t*>(y);
+  return f16 ? run_forward<true>(c, b, o, ldy) : run_forward<false>(c, b, o, ldy);
+}
+
+int train_backward(const void* x, int64_t ldx, const void* grad, int64_t ldg, const uint8_t* w,
+                   const float* absmax, const float* code16, int blocksize, const void* lora_a,
+                   const void* lora_b, int r, float scaling, int M, int N, int K, int f16,
+                   const Dropout& drop, void* grad_x, int64_t ldgx, void* grad_a, void* grad_b,
+                   void* workspace, size_t workspace_bytes, grpo_stream_t stream) {
+  if (int rc = train_check(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, M, N, K,
+                           workspace, workspace_bytes))
+    return rc;
+  if (!grad_x && !grad_a && !grad_b) return GRPO_OK;
+  if (!grad) return einval("null pointer");
+  if (ldg < N || ldg % 8 || ldg >= (1 << 22) || !aligned16(grad))
+    return einval("grad rows must be 16-byte aligned");
+  if (grad_x && (ldgx < K || ldgx % 8 || !aligned16(grad_x)))
+    return einval("grad_x rows must be 16-byte aligned");
+  if (!aligned16(grad_a) || !aligned16(grad_b))
+    return einval("the adapters' gradients must be 16-byte aligned");
+  const TrainCall c = train_call(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, scaling,
+                                 M, N, K, workspace, stream, drop);
+  const uint16_t* const g = static_cast<const uint16_t*>(grad);
+  auto u = [](void* q) { return static_cast<uint16_t*>(q); };
+  return f16 ? run_backward<true>(c, g, ldg, u(grad_x), ldgx, u(grad_a), u(grad_b))
+             : run_backward<false>(c, g, ldg, u(grad_x), ldgx, u(grad_a), u(grad_b));
 }
 
 }  // namespace
@@ -646,16 +719,19 @@ extern "C" int grpo_nf4_lora_train_forward(const void* x, int64_t ldx, const uin
                                            int64_t ldy, int M, int N, int K, int f16,
                                            void* workspace, size_t workspace_bytes,
                                            grpo_stream_t stream) {
-  if (int rc = train_check(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, M, N, K,
-                           workspace, workspace_bytes))
-    return rc;
-  if (!y) return einval("null pointer");
-  if (ldy < N || ldy % 8 || !aligned16(y)) return einval("y rows must be 16-byte aligned");
-  const TrainCall c = train_call(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, scaling,
-                                 M, N, K, workspace, stream);
-  const uint16_t* const b = static_cast<const uint16_t*>(bias);
-  uint16_t* const o = static_cast<uint16_t*>(y);
-  return f16 ? run_forward<true>(c, b, o, ldy) : run_forward<false>(c, b, o, ldy);
+  return train_forward(x, ldx, w, absmax, code16, blocksize, bias, lora_a, lora_b, r, scaling, y,
+                       ldy, M, N, K, f16, Dropout{}, workspace, workspace_bytes, stream);
+}
+
+extern "C" int grpo_nf4_lora_train_forward_dropout(
+    const void* x, int64_t ldx, const uint8_t* w, const float* absmax, const float* code16,
+    int blocksize, const void* bias, const void* lora_a, const void* lora_b, int r, float scaling,
+    void* y, int64_t ldy, int M, int N, int K, int f16, double p, const int64_t* rng,
+    void* workspace, size_t workspace_bytes, grpo_stream_t stream) {
+  Dropout drop;
+  if (int rc = drop_args(rng, p, &drop)) return rc;
+  return train_forward(x, ldx, w, absmax, code16, blocksize, bias, lora_a, lora_b, r, scaling, y,
+                       ldy, M, N, K, f16, drop, workspace, workspace_bytes, stream);
 }
 
 extern "C" int grpo_nf4_lora_train_backward(const void* x, int64_t ldx, const void* grad,
@@ -666,21 +742,20 @@ extern "C" int grpo_nf4_lora_train_backward(const void* x, int64_t ldx, const vo
                                             void* grad_x, int64_t ldgx, void* grad_a,
                                             void* grad_b, void* workspace,
                                             size_t workspace_bytes, grpo_stream_t stream) {
-  if (int rc = train_check(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, M, N, K,
-                           workspace, workspace_bytes))
-    return rc;
-  if (!grad_x && !grad_a && !grad_b) return GRPO_OK;
-  if (!grad) return einval("null pointer");
-  if (ldg < N || ldg % 8 || ldg >= (1 << 22) || !aligned16(grad))
-    return einval("grad rows must be 16-byte aligned");
-  if (grad_x && (ldgx < K || ldgx % 8 || !aligned16(grad_x)))
-    return einval("grad_x rows must be 16-byte aligned");
-  if (!aligned16(grad_a) || !aligned16(grad_b))
-    return einval("the adapters' gradients must be 16-byte aligned");
-  const TrainCall c = train_call(x, ldx, w, absmax, code16, blocksize, lora_a, lora_b, r, scaling,
-                                 M, N, K, workspace, stream);
-  const uint16_t* const g = static_cast<const uint16_t*>(grad);
-  auto u = [](void* q) { return static_cast<uint16_t*>(q); };
-  return f16 ? run_backward<true>(c, g, ldg, u(grad_x), ldgx, u(grad_a), u(grad_b))
-             : run_backward<false>(c, g, ldg, u(grad_x), ldgx, u(grad_a), u(grad_b));
+  return train_backward(x, ldx, grad, ldg, w, absmax, code16, blocksize, lora_a, lora_b, r,
+                        scaling, M, N, K, f16, Dropout{}, grad_x, ldgx, grad_a, grad_b, workspace,
+                        workspace_bytes, stream);
+}
+
+extern "C" int grpo_nf4_lora_train_backward_dropout(
+    const void* x, int64_t ldx, const void* grad, int64_t ldg, const uint8_t* w,
+    const float* absmax, const float* code16, int blocksize, const void* lora_a,
+    const void* lora_b, int r, float scaling, int M, int N, int K, int f16, double p,
+    const int64_t* rng, void* grad_x, int64_t ldgx, void* grad_a, void* grad_b, void* workspace,
+    size_t workspace_bytes, grpo_stream_t stream) {
+  Dropout drop;
+  if (int rc = drop_args(rng, p, &drop)) return rc;
+  return train_backward(x, ldx, grad, ldg, w, absmax, code16, blocksize, lora_a, lora_b, r,
+                        scaling, M, N, K, f16, drop, grad_x, ldgx, grad_a, grad_b, workspace,
+                        workspace_bytes, stream);
 }

@@ -117,6 +117,16 @@ SIGNATURES = {
         [_VP, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _VP, _I32, _F32, _I32, _I32, _I32, _I32,
          _VP, _I64, _VP, _VP, _VP, _SZ, _VP],
     ),
+    "grpo_nf4_lora_train_forward_dropout": (
+        _I32,
+        [_VP, _I64, _VP, _VP, _VP, _I32, _VP, _VP, _VP, _I32, _F32, _VP, _I64, _I32, _I32, _I32,
+         _I32, _c.c_double, _VP, _VP, _SZ, _VP],
+    ),
+    "grpo_nf4_lora_train_backward_dropout": (
+        _I32,
+        [_VP, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _VP, _I32, _F32, _I32, _I32, _I32, _I32,
+         _c.c_double, _VP, _VP, _I64, _VP, _VP, _VP, _SZ, _VP],
+    ),
     "grpo_nf4_linear_plan": (
         _I32,
         [_I32, _I32, _I32, _I32, _I32, _I32, _c.POINTER(_I32), _c.POINTER(_SZ),

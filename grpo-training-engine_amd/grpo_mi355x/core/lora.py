@@ -7,7 +7,9 @@ prefer_base_layer, lora_A, lora_B, lora_dropout``) and ``forward`` dispatch
 ``RuntimeError`` or ``ValueError`` run ``base_layer(x) + B(A(x)) * scaling``
 (``lora.py:125-137``).  ``base_layer`` is a ``Linear4bitNF4`` (or a
 bitsandbytes ``Linear4bit``); its own forward dequantizes on the GPU, so no
-branch here computes on the CPU.
+branch here computes on the CPU.  ``counter_dropout=True`` makes a ``dropout`` > 0 one
+whose mask is counter-based and never stored (``CounterDropout``), which the fused kernel
+runs; the default stays ``nn.Dropout``, which it refuses.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import torch
 import torch.nn as nn
 
 from ..kernels import lora_fused_forward
+from ..kernels.dropout import CounterDropout
 from .nf4 import Linear4bitNF4
 
 
@@ -42,7 +45,8 @@ class ManualLoRALayer(nn.Module):
     """``Y = W_4bit(x) + B(A(x)) * (alpha / rank)`` (``lora.py:50-163``)."""
 
     def __init__(self, base_layer, rank: int = 16, alpha: int = 32, dropout: float = 0.0,
-                 use_triton: bool = True, prefer_base_layer: bool = False):
+                 use_triton: bool = True, prefer_base_layer: bool = False,
+                 counter_dropout: bool = False):
         super().__init__()
         self.base_layer = base_layer
         self.rank = rank
@@ -55,15 +59,20 @@ class ManualLoRALayer(nn.Module):
         out_features = base_layer.out_features
         self.lora_A = nn.Linear(in_features, rank, bias=False)
         self.lora_B = nn.Linear(rank, out_features, bias=False)
-        self.lora_dropout = nn.Dropout(p=dropout) if dropout > 0 else nn.Identity()
+        kind = CounterDropout if counter_dropout else nn.Dropout
+        self.lora_dropout = kind(p=dropout) if dropout > 0 else nn.Identity()
         nn.init.kaiming_uniform_(self.lora_A.weight, a=5 ** 0.5)
         nn.init.zeros_(self.lora_B.weight)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        # one draw for a call, whichever branch below runs
+        drop = self.lora_dropout
+        rng = drop.draw(x.device) if isinstance(drop, CounterDropout) and drop.active() else None
         if self.use_triton:
             try:
                 return cast(torch.Tensor, lora_fused_forward(
-                    x, lora_layer=self, prefer_base_layer=self.prefer_base_layer))
+                    x, lora_layer=self, prefer_base_layer=self.prefer_base_layer,
+                    dropout_rng=rng))
             except (ImportError, RuntimeError, ValueError):
                 pass
         try:
@@ -71,7 +80,8 @@ class ManualLoRALayer(nn.Module):
             if base_output.requires_grad:
                 base_output = base_output.clone()
             x_adapt = x.to(self.lora_A.weight.dtype)
-            lora_output = self.lora_B(self.lora_A(self.lora_dropout(x_adapt)))
+            x_adapt = drop(x_adapt) if rng is None else drop(x_adapt, rng)
+            lora_output = self.lora_B(self.lora_A(x_adapt))
             lora_output = lora_output * self.scaling
             if lora_output.dtype != base_output.dtype:
                 lora_output = lora_output.to(base_output.dtype)
@@ -79,7 +89,7 @@ class ManualLoRALayer(nn.Module):
         except Exception:
             if not self.use_triton:
                 raise
-            return cast(torch.Tensor, lora_fused_forward(x, lora_layer=self))
+            return cast(torch.Tensor, lora_fused_forward(x, lora_layer=self, dropout_rng=rng))
 
     def merge_weights(self) -> torch.Tensor:
         """``W_base + B A * scaling`` with the base dequantized on the GPU (``lora.py:149-163``)."""
@@ -91,7 +101,8 @@ class ManualLoRALayer(nn.Module):
 def inject_lora_layers(model: nn.Module, target_modules: List[str], rank: int = 16,
                        alpha: int = 32, dropout: float = 0.0, use_triton: bool = True,
                        prefer_base_layer: bool = False, verbose: bool = True,
-                       dtype: torch.dtype = torch.bfloat16) -> int:
+                       dtype: torch.dtype = torch.bfloat16,
+                       counter_dropout: bool = False) -> int:
     """Wrap every 4-bit linear whose short name is in ``target_modules`` (``lora.py:166-233``)."""
     injected = 0
     for name, module in list(model.named_modules()):
@@ -100,7 +111,8 @@ def inject_lora_layers(model: nn.Module, target_modules: List[str], rank: int = 
             parent_name = ".".join(name.split(".")[:-1])
             parent = model.get_submodule(parent_name) if parent_name else model
             layer = ManualLoRALayer(module, rank=rank, alpha=alpha, dropout=dropout,
-                                    use_triton=use_triton, prefer_base_layer=prefer_base_layer)
+                                    use_triton=use_triton, prefer_base_layer=prefer_base_layer,
+                                    counter_dropout=counter_dropout)
             layer = layer.to(device=module.weight.device, dtype=dtype)
             setattr(parent, short, layer)
             injected += 1

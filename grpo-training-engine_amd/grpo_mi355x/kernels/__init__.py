@@ -112,12 +112,14 @@ def paged_kv_decode(model: object, input_ids: object, attention_mask: object | N
 def lora_fused_forward(x: object, base_layer: object | None = None, lora_A: object | None = None,
                        lora_B: object | None = None, scaling: float | None = None,
                        dropout: object | None = None, lora_layer: object | None = None,
-                       prefer_base_layer: bool = False) -> object:
+                       prefer_base_layer: bool = False,
+                       dropout_rng: object | None = None) -> object:
     kernel = _get_hip_kernel("lora_fused_forward")
     if kernel is None:
         raise _unavailable("lora_fused_forward")
     return kernel(x, base_layer=base_layer, lora_A=lora_A, lora_B=lora_B, scaling=scaling,
-                  dropout=dropout, lora_layer=lora_layer, prefer_base_layer=prefer_base_layer)
+                  dropout=dropout, lora_layer=lora_layer, prefer_base_layer=prefer_base_layer,
+                  dropout_rng=dropout_rng)
 
 
 def _call(name: str, *args: object, **kwargs: object) -> object:

@@ -78,4 +78,32 @@ def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tenso
     return _dropout(x, p, rng)
 
 
-__all__ = ["counter_dropout", "check_dropout"]
+class CounterDropout(torch.nn.Module):
+    """``nn.Dropout`` on ``counter_dropout``: seed and offset of each call are drawn on the
+    device from torch's generator, so ``torch.manual_seed``, activation checkpointing and
+    graph capture govern the mask as they do any of torch's random numbers."""
+
+    def __init__(self, p: float = 0.5):
+        super().__init__()
+        if not 0.0 <= p < 1.0:
+            raise ValueError(f"dropout p must be in [0, 1), got {p}.")
+        self.p = float(p)
+
+    @staticmethod
+    def draw(device: torch.device) -> torch.Tensor:
+        """Seed and offset of one mask."""
+        return torch.randint(0, 2 ** 63 - 1, (2,), dtype=torch.int64, device=device)
+
+    def active(self) -> bool:
+        return self.training and self.p > 0.0
+
+    def forward(self, x: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        if not self.active():
+            return x
+        return counter_dropout(x, self.p, self.draw(x.device) if rng is None else rng)
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}"
+
+
+__all__ = ["CounterDropout", "counter_dropout", "check_dropout"]

@@ -5,7 +5,9 @@ Same call surface and dispatch as the reference's
 
 * ``lora_layer`` (a ``ManualLoRALayer``-like object) or explicit
   ``base_layer/lora_A/lora_B/scaling/dropout``;
-* dropout p > 0 -> ``ValueError`` (``:958-960``);
+* dropout p > 0 -> ``ValueError`` (``:958-960``), unless its mask is counter-based: a
+  ``CounterDropout`` in training mode, or ``dropout_rng`` with the draw for any dropout
+  module; it then runs inside the training linear (``FusedLoRADropoutFunction``);
 * a base weight with ``quant_state`` and ``prefer_base_layer=False`` -> the
   fused kernel (``FusedLoRAFunction``, ``:966-984``); otherwise the adapter
   branch ``base_layer(x) + B(A(x)) * scaling`` (``:986-1037``);
@@ -34,9 +36,11 @@ from typing import Optional
 import torch
 import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ..core.nf4 import float_absmax
 from . import ops
+from .dropout import CounterDropout, check_dropout, counter_dropout
 
 
 _HALF = (torch.bfloat16, torch.float16)
@@ -203,8 +207,15 @@ def _train_workspace(w: torch.Tensor, blocksize: int, lora_A: torch.Tensor,
     return nbytes if low % 16 == 0 else 0
 
 
-def _run_forward(x, weight_4bit, quant_state, lora_A, lora_B, scaling, bias):
-    """The fused linear: (output, what its backward needs)."""
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """The tensor, contiguous and on a 16-byte boundary."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _run_forward(x, weight_4bit, quant_state, lora_A, lora_B, scaling, bias, drop=None):
+    """The fused linear: (output, what its backward needs). ``drop``: (p, rng) of the
+    dropout on the adapter's input, which the training linear alone has."""
     m, n, k, r = _validate_inputs(x, weight_4bit, quant_state, lora_A, lora_B)
     if r <= 0:
         raise ValueError(f"LoRA rank must be > 0, got {r}.")
@@ -221,13 +232,18 @@ def _run_forward(x, weight_4bit, quant_state, lora_A, lora_B, scaling, bias):
         raise ValueError("packed weight or absmax too short for the quant_state's shape.")
     if bias is not None and (not bias.is_cuda or bias.numel() != n):
         raise ValueError(f"bias must have {n} elements on the ROCm/HIP device.")
+    if drop is not None:
+        x_flat, w, lora_A = _aligned(x_flat), _aligned(w), _aligned(lora_A)
     nbytes = (_train_workspace(w, blocksize, lora_A, lora_B, x_flat)
-              if train_forward_pays(m, n, k, r, blocksize, dt) else 0)
+              if drop is not None or train_forward_pays(m, n, k, r, blocksize, dt) else 0)
+    if drop is not None and m and not nbytes:
+        raise ValueError("dropout in the fused linear needs N and K to be multiples of 32, "
+                         "a rank of at most 32 and a power-of-two blocksize >= 32.")
     if nbytes:
         if bias is not None and (bias.dtype != dt or not bias.is_contiguous()):
             bias = bias.to(dt).contiguous()
         out = ops.train_forward(x_flat, w, absmax, code, blocksize, lora_A.contiguous(),
-                                lora_B.contiguous(), scaling, bias, nbytes)
+                                lora_B.contiguous(), scaling, bias, nbytes, drop)
     else:
         out = _forward_any(x_flat, w, absmax, code, blocksize, n, lora_A, lora_B, scaling, bias)
     return out.view(x.shape[:-1] + (n,)), (x_flat, lora_A, lora_B, w, absmax, code), blocksize
@@ -312,10 +328,65 @@ class FusedLoRAFunction(torch.autograd.Function):
         return grad_x.view(ctx.x_shape), None, None, grad_A, grad_B, None, grad_bias
 
 
+class FusedLoRADropoutFunction(torch.autograd.Function):
+    """``FusedLoRAFunction`` with counter-based dropout on the adapter's input: the
+    training linear both ways, the mask made again from ``rng`` where it is needed."""
+
+    @staticmethod
+    def forward(ctx, x, weight_4bit, quant_state, lora_A, lora_B, scaling, bias, p, rng):
+        out, saved, blocksize = _run_forward(x, weight_4bit, quant_state, lora_A, lora_B, scaling,
+                                             bias, (p, rng))
+        ctx.save_for_backward(*saved, rng)
+        ctx.blocksize, ctx.scaling, ctx.p, ctx.x_shape = blocksize, scaling, p, x.shape
+        ctx.has_bias = bias is not None
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, lora_A, lora_B, w, absmax, code, rng = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = grad_out.reshape(-1, lora_B.shape[0])
+        g = _aligned(g if g.dtype == x.dtype else g.to(x.dtype))
+        grad_bias = g.sum(dim=0) if ctx.has_bias and need[6] else None
+        if x.shape[0] == 0:
+            grads = (torch.empty_like(x), torch.zeros_like(lora_A), torch.zeros_like(lora_B))
+        else:
+            nbytes = _train_workspace(w, ctx.blocksize, lora_A, lora_B, x, g)
+            grads = ops.train_backward(x, g, w, absmax, code, ctx.blocksize, lora_A,
+                                       lora_B.contiguous(), ctx.scaling, need[0], need[3],
+                                       need[4], nbytes, (ctx.p, rng))
+        gx, ga, gb = grads
+        return (None if gx is None else gx.view(ctx.x_shape), None, None, ga, gb, None, grad_bias,
+                None, None)
+
+
+def _dropout_of(dropout, rng, device):
+    """(p, rng) of the counter-based dropout asked for, or None where nothing is dropped;
+    any other dropout is refused."""
+    p = (0.0 if dropout is None or type(dropout) is torch.nn.Identity
+         else getattr(dropout, "p", 0.0))
+    if not p or not p > 0.0:
+        return None
+    counter = isinstance(dropout, CounterDropout)
+    if rng is None and not counter:
+        raise ValueError("Dropout is not supported in lora_fused_forward.")
+    if not getattr(dropout, "training", True):
+        return None
+    rng = CounterDropout.draw(device) if rng is None else rng
+    return check_dropout(p, rng, device), rng
+
+
 def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=None,
                        scaling: Optional[float] = None, dropout=None, lora_layer=None,
-                       prefer_base_layer: bool = False) -> torch.Tensor:
-    """Drop-in for ``src.triton_kernels.lora_forward.lora_fused_forward``."""
+                       prefer_base_layer: bool = False,
+                       dropout_rng: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Drop-in for ``src.triton_kernels.lora_forward.lora_fused_forward``.
+
+    ``dropout_rng``: seed and offset (int64 [2], on x's device) of the mask that ``dropout``
+    (any module with a ``p``) puts on the adapter's input, ``y = W x + B(A(drop(x))) s``;
+    None: none, or a ``CounterDropout``'s own draw.  The mask is ``counter_dropout``'s and
+    is never stored; a module in eval mode drops nothing."""
     if lora_layer is not None:
         base_layer = getattr(lora_layer, "base_layer", None)
         lora_A = getattr(lora_layer, "lora_A", None)
@@ -324,10 +395,7 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
         dropout = getattr(lora_layer, "lora_dropout", None)
     if base_layer is None or lora_A is None or lora_B is None or scaling is None:
         raise ValueError("Provide lora_layer or base_layer/lora_A/lora_B/scaling for fused LoRA.")
-    dropout_p = (0.0 if dropout is None or type(dropout) is torch.nn.Identity
-                 else getattr(dropout, "p", 0.0))
-    if dropout_p and dropout_p > 0.0:
-        raise ValueError("Dropout is not supported in lora_fused_forward.")
+    drop = _dropout_of(dropout, dropout_rng, x.device)
 
     weight_4bit = getattr(base_layer, "weight", None)
     lora_A_weight = getattr(lora_A, "weight", lora_A)
@@ -337,6 +405,10 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
             and getattr(weight_4bit, "quant_state", None) is not None):
         args = (x, weight_4bit, weight_4bit.quant_state, lora_A_weight, lora_B_weight,
                 float(scaling), getattr(base_layer, "bias", None))
+        if drop is not None:
+            if torch.is_grad_enabled():
+                return FusedLoRADropoutFunction.apply(*args, *drop)
+            return _run_forward(*args, drop)[0]
         # With nothing to record (no grad mode, no forward-mode level, no transform)
         # the autograd function's own bookkeeping, 5 us of a decode call's 25, is left out.
         if not torch.is_grad_enabled() and fwAD._current_level < 0 and \
@@ -360,7 +432,8 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
     base_output = base_layer(x.contiguous())
     if getattr(base_output, "requires_grad", False):
         base_output = base_output.clone()
-    x_lora = x.reshape(-1, x.shape[-1]).to(lora_A_weight.dtype)
+    x_lora = x if drop is None else counter_dropout(x, *drop)
+    x_lora = x_lora.reshape(-1, x.shape[-1]).to(lora_A_weight.dtype)
     t = (x_lora.float() @ lora_A_weight.float().t()).to(lora_A_weight.dtype)
     u = (t.float() @ lora_B_weight.float().t()).to(lora_A_weight.dtype)
     u = u * float(scaling)
@@ -369,4 +442,4 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
     return base_output + u.view(base_output.shape)
 
 
-__all__ = ["lora_fused_forward", "FusedLoRAFunction"]
+__all__ = ["lora_fused_forward", "FusedLoRAFunction", "FusedLoRADropoutFunction"]

@@ -166,35 +166,45 @@ def _check_train(x, packed, absmax, code, blocksize, lora_a, lora_b, others) -> 
     return nf4_lora_train_workspace_bytes(m, n, k, r, int(blocksize))
 
 
-def train_forward(x, packed, absmax, code, blocksize, lora_a, lora_b, scaling, bias, nbytes):
-    """``nf4_lora_train_forward`` of checked arguments (``nbytes``: their workspace)."""
+def train_forward(x, packed, absmax, code, blocksize, lora_a, lora_b, scaling, bias, nbytes,
+                  drop=None):
+    """``nf4_lora_train_forward`` of checked arguments (``nbytes``: their workspace;
+    ``drop``: (p, rng) of the dropout on the adapter's input, or None)."""
     (m, k), (n, r), dev = x.shape, lora_b.shape, x.device
     y = torch.empty((m, n), dtype=x.dtype, device=dev)
     ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
-    rc = _lib.device_library().grpo_nf4_lora_train_forward(
-        x.data_ptr(), k, packed.data_ptr(), absmax.data_ptr(), code.data_ptr(), blocksize,
-        None if bias is None else bias.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), r,
-        scaling, y.data_ptr(), n, m, n, k, x.dtype == torch.float16, ws.data_ptr(), nbytes,
-        _lib.stream_handle(dev))
+    args = (x.data_ptr(), k, packed.data_ptr(), absmax.data_ptr(), code.data_ptr(), blocksize,
+            None if bias is None else bias.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(), r,
+            scaling, y.data_ptr(), n, m, n, k, x.dtype == torch.float16)
+    end = (ws.data_ptr(), nbytes, _lib.stream_handle(dev))
+    if drop is None:
+        rc = _lib.device_library().grpo_nf4_lora_train_forward(*args, *end)
+    else:
+        rc = _lib.device_library().grpo_nf4_lora_train_forward_dropout(
+            *args, drop[0], drop[1].data_ptr(), *end)
     if rc:
         _lib.check(rc, "grpo_nf4_lora_train_forward")
     return y
 
 
 def train_backward(x, grad, packed, absmax, code, blocksize, lora_a, lora_b, scaling, want_x,
-                   want_a, want_b, nbytes):
-    """``nf4_lora_train_backward`` of checked arguments (``nbytes``: their workspace)."""
+                   want_a, want_b, nbytes, drop=None):
+    """``nf4_lora_train_backward`` of checked arguments (``nbytes`` and ``drop`` as there)."""
     (m, k), (n, r), dev = x.shape, lora_b.shape, x.device
     gx = torch.empty_like(x) if want_x else None
     ga = torch.empty_like(lora_a) if want_a else None
     gb = torch.empty_like(lora_b) if want_b else None
     ws = torch.empty(nbytes or 16, dtype=torch.uint8, device=dev)
-    rc = _lib.device_library().grpo_nf4_lora_train_backward(
-        x.data_ptr(), k, grad.data_ptr(), n, packed.data_ptr(), absmax.data_ptr(),
-        code.data_ptr(), blocksize, lora_a.data_ptr(), lora_b.data_ptr(), r, scaling, m, n, k,
-        x.dtype == torch.float16, None if gx is None else gx.data_ptr(), k,
-        None if ga is None else ga.data_ptr(), None if gb is None else gb.data_ptr(),
-        ws.data_ptr(), nbytes, _lib.stream_handle(dev))
+    args = (x.data_ptr(), k, grad.data_ptr(), n, packed.data_ptr(), absmax.data_ptr(),
+            code.data_ptr(), blocksize, lora_a.data_ptr(), lora_b.data_ptr(), r, scaling, m, n, k,
+            x.dtype == torch.float16)
+    end = (None if gx is None else gx.data_ptr(), k, None if ga is None else ga.data_ptr(),
+           None if gb is None else gb.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_handle(dev))
+    if drop is None:
+        rc = _lib.device_library().grpo_nf4_lora_train_backward(*args, *end)
+    else:
+        rc = _lib.device_library().grpo_nf4_lora_train_backward_dropout(
+            *args, drop[0], drop[1].data_ptr(), *end)
     if rc:
         _lib.check(rc, "grpo_nf4_lora_train_backward")
     return gx, ga, gb

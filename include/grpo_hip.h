@@ -209,6 +209,27 @@ int grpo_nf4_lora_train_backward(const void* x, int64_t ldx, const void* grad, i
                                  int64_t ldgx, void* grad_a, void* grad_b, void* workspace,
                                  size_t workspace_bytes, grpo_stream_t stream);
 
+/* Both with dropout on the adapter's input: x is drop(x) (grpo_dropout of a contiguous
+ * [M, K] in x's type, with p and rng) in t, in x A^T and in grad_A, and
+ *   grad_x = dt(dt(g W) + drop(dt(gi A))).
+ * p and rng as in grpo_dropout; p that rounds to 0: the calls above. */
+int grpo_nf4_lora_train_forward_dropout(const void* x, int64_t ldx, const uint8_t* w,
+                                        const float* absmax, const float* code16, int blocksize,
+                                        const void* bias, const void* lora_a, const void* lora_b,
+                                        int r, float scaling, void* y, int64_t ldy, int M, int N,
+                                        int K, int f16, double p, const int64_t* rng,
+                                        void* workspace, size_t workspace_bytes,
+                                        grpo_stream_t stream);
+int grpo_nf4_lora_train_backward_dropout(const void* x, int64_t ldx, const void* grad,
+                                         int64_t ldg, const uint8_t* w, const float* absmax,
+                                         const float* code16, int blocksize, const void* lora_a,
+                                         const void* lora_b, int r, float scaling, int M, int N,
+                                         int K, int f16, double p, const int64_t* rng,
+                                         void* grad_x, int64_t ldgx, void* grad_a, void* grad_b,
+                                         void* workspace, size_t workspace_bytes,
+                                         grpo_stream_t stream);
+
+
 /* ------------------------------------------------ split-K NF4 linear --
  * The fast NF4 (+ LoRA) linear runs as a split-K kernel: workgroups own a
  * 16-row tile of W and one slice of K, so every CU gets work even when N/16
