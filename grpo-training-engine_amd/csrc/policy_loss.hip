@@ -13,12 +13,14 @@
 // sequences) or 1 / (a given number). Rows that are not counted are not read: their
 // logp, loss and gradient are 0 whatever stands there.
 //
-// M is an integer, so x k - M is one fused multiply-add with a single rounding at the
-// size of its result, and sums taken against different M are brought together by exact
-// powers of two. k is the float32 nearest log2(e) / T, and logp uses that same k, so its
-// rounding moves logp by less than half a step of float32 and does not grow with an
-// offset common to all logits. Everything per row is float64 from S on: the ratio of a
-// token next to a border of the clip decides whether it has a gradient at all.
+// x k - M is two fused multiply-adds, k = khi + klo: each rounds at the size of its result,
+// whatever offset the logits have in common. (With k rounded to float32 every logp of a
+// batch moves the same way, and a loss whose advantages cancel shows it: 1.4e-5 relative at
+// T = 0.7.) M is an integer, so sums taken against different M are brought together by
+// exact powers of two. Everything per row is float64 from the threads' sums on: the ratio of
+// a token next to a border of the clip decides whether it has a gradient at all.
+#include <type_traits>
+
 #include "common.hpp"
 
 using namespace grpo;
@@ -36,14 +38,21 @@ struct Rows {
   int S, V;
   const int64_t* ids;   // [rows]
   const uint8_t* mask;  // [rows] or null: every row is counted
-  float k;              // log2(e) / T
+  double k;             // log2(e) / T
+  float khi, klo;       // khi < k, khi + klo = k; klo > 0 keeps -inf * klo from being NaN
 };
+// (Rows is never passed by reference to a function that is not inlined: it would have to
+// live in memory, and its pointers would no longer be known to be global.)
 
-// What the gradient needs of a row: e_v = exp2(x_v k - M), or exp2((x_v - m) k) where M
+// What the gradient needs of a row: e_v = exp2(x_v k - M), or exp2((x_v - m) khi) where M
 // is not finite (rows whose logits are all below -1e30, or not finite).
 struct RowStat {
   float M, S, m, pad;
 };
+
+__device__ __forceinline__ float exponent(float x, float khi, float klo, float M) {
+  return fmaf(x, klo, fmaf(x, khi, -M));
+}
 
 using Policy = grpo_policy_t;
 
@@ -92,119 +101,209 @@ __device__ __forceinline__ int head_of(const void* p, int n) {
 
 // ------------------------------------------------------- softmax statistics --
 
-// S, and t = sum e (x k - M) for the entropy, against an M of its own.
+// A difference of two Ms as ldexp takes it; beyond 2^-4096 nothing is left anyway.
+__device__ __forceinline__ int shift(float d) { return (int)fmaxf(d, -4096.f); }
+
+// S, and t = sum e (x k - M) for the entropy, against an M of its own. What is added is at
+// most 2^4: its exponent x k - M is rounded at 4 at most, so the largest terms are exact to
+// little more than the exponential's own last bit; the sums are float64, one addition for
+// each N terms that were added to each other in float32.
 template <bool ENT>
 struct Sums {
-  float M = LOWEST, S = 0.f, t = 0.f;
-  __device__ __forceinline__ void raise(float to) {  // M is an integer, to > M
-    const float f = __builtin_amdgcn_exp2f(M - to);
-    if (ENT) t = f * (t + (M - to) * S);
-    S *= f;
-    M = to;
+  float M = LOWEST;
+  double S = 0.0, t = 0.0;
+  __device__ __forceinline__ void admit(float top, const Rows& q) {
+    if (top * q.khi > M + 4.f) {
+      const float to = rintf(top * q.khi) + 4.f;
+      const int by = shift(M - to);
+      if (ENT) t = ldexp(t + (double)(M - to) * S, by);
+      S = ldexp(S, by);
+      M = to;
+    }
   }
-  // 32 above M is still far from the end of float32's range: M moves rarely.
-  __device__ __forceinline__ void admit(float top, float k) {
-    if (top * k > M + 32.f) raise(rintf(top * k));
-  }
-  __device__ __forceinline__ void add(float x, float k) {
-    const float a = fmaf(x, k, -M), e = __builtin_amdgcn_exp2f(a);
-    S += e;
-    if (ENT) t = fmaf(e, fmaxf(a, -1024.f), t);  // a = -inf: 0, not 0 * inf
-  }
-  __device__ __forceinline__ void join(float M2, float S2, float t2) {
-    if (M2 > M) raise(M2);
-    const float f = __builtin_amdgcn_exp2f(M2 - M);
-    if (ENT) t = fmaf(f, t2 + (M2 - M) * S2, t);
-    S = fmaf(f, S2, S);
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], const Rows& q) {
+    float e[N], u[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float a = exponent(x[j], q.khi, q.klo, M);
+      e[j] = __builtin_amdgcn_exp2f(a);
+      u[j] = ENT ? e[j] * fmaxf(a, -1024.f) : 0.f;  // a = -inf: 0, not 0 * inf
+    }
+#pragma unroll
+    for (int w = 1; w < N; w *= 2)
+#pragma unroll
+      for (int j = 0; j + w < N; j += 2 * w) {
+        e[j] += e[j + w];
+        if (ENT) u[j] += u[j + w];
+      }
+    S += e[0];
+    if (ENT) t += u[0];
   }
 };
 
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* red) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, red[w]);
   return v;
 }
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = wave_sum_dpp(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < NT / 64; ++w) v += red[w];
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
 
-// The statistics of a row by one workgroup, the same in every thread.
+struct Joined {  // of a workgroup, the same in every thread
+  float M;
+  double S, t;
+};
+template <int NT>
+struct JoinSpace {
+  double S[NT / 64], t[NT / 64];
+  float M[NT / 64];
+};
+
+template <bool ENT, int NT>
+__device__ __forceinline__ Joined join(const Sums<ENT>& s, JoinSpace<NT>& red) {
+  const float M = wave_max(s.M);
+  const int by = shift(s.M - M);
+  const double S = wave_sum64(ldexp(s.S, by));
+  const double t = ENT ? wave_sum64(ldexp(s.t + (double)(s.M - M) * s.S, by)) : 0.0;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red.M[threadIdx.x >> 6] = M;
+    red.S[threadIdx.x >> 6] = S;
+    if (ENT) red.t[threadIdx.x >> 6] = t;
+  }
+  __syncthreads();
+  Joined j{red.M[0], 0.0, 0.0};
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) j.M = fmaxf(j.M, red.M[w]);
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    const int b = shift(red.M[w] - j.M);
+    j.S += ldexp(red.S[w], b);
+    if (ENT) j.t += ldexp(red.t[w] + (double)(red.M[w] - j.M) * red.S[w], b);
+  }
+  return j;
+}
+
+template <int NT>
+__device__ __forceinline__ double block_sum64(double v, JoinSpace<NT>& red) {
+  v = wave_sum64(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red.S[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int w = 0; w < NT / 64; ++w) v += red.S[w];
+  return v;
+}
+
+// A row as one workgroup sees it: vectors from the first 16-byte boundary on, and the
+// fewer than 2 PER values around them, one a thread.
+template <int DT>
+struct Span {
+  const void* row;
+  const uint4* vec;
+  int head, nvec, tail, odd;
+  __device__ __forceinline__ Span(const void* p, int V) : row(p) {
+    head = head_of<DT>(p, V);
+    nvec = (V - head) / PER<DT>;
+    tail = head + nvec * PER<DT>;
+    odd = head + V - tail;
+    vec = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + (int64_t)head * SIZE<DT>);
+  }
+  __device__ __forceinline__ int odd_at(int i) const { return i < head ? i : tail + i - head; }
+};
+
+template <int DT>
+__device__ __forceinline__ float top_of(const float (&f)[PER<DT>]) {
+  float top = f[0];
+#pragma unroll
+  for (int j = 1; j < PER<DT>; ++j) top = fmaxf(top, f[j]);
+  return top;
+}
+
+// The statistics of a row whose sums came out 0 or not finite: nothing above -1e30, or
+// values that are not finite. The maximum, then the sum against it.
+struct PlainStat {
+  double S, t;
+  float m;
+};
 template <int DT, bool ENT, int NT>
-__device__ __forceinline__ RowStat row_stat(const void* row, int V, float k, float* red,
-                                            float* ent) {
-  const int head = head_of<DT>(row, V), nvec = (V - head) / PER<DT>;
-  const uint4* const vec = reinterpret_cast<const uint4*>(static_cast<const char*>(row) +
-                                                          (int64_t)head * SIZE<DT>);
-  const int tail = head + nvec * PER<DT>;
-  Sums<ENT> s;
-  for (int i = threadIdx.x; i < nvec; i += NT) {
-    float f[PER<DT>];
-    unpack<DT>(vec[i], f);
-    float top = f[0];
-#pragma unroll
-    for (int j = 1; j < PER<DT>; ++j) top = fmaxf(top, f[j]);
-    s.admit(top, k);
-#pragma unroll
-    for (int j = 0; j < PER<DT>; ++j) s.add(f[j], k);
-  }
-  if ((int)threadIdx.x < head + V - tail) {
-    const float x = load1<DT>(row, (int)threadIdx.x < head ? threadIdx.x
-                                                           : tail + threadIdx.x - head);
-    s.admit(x, k);
-    s.add(x, k);
-  }
-  RowStat r;
-  r.M = block_max<NT>(s.M, red);
-  Sums<ENT> all;
-  all.M = r.M;
-  all.join(s.M, s.S, s.t);
-  r.S = block_sum<NT>(all.S, red);
-  const float t = ENT ? block_sum<NT>(all.t, red) : 0.f;
-  r.m = 0.f;
-  r.pad = 0.f;
-  if (ENT) *ent = (float)(LN2 * (log2((double)r.S) - (double)t / (double)r.S));
-  if (r.S > 0.f && r.S < INFINITY) return r;
-  // no finite logit above -1e30, or one that is not finite: the maximum, then the sum
-  float m = -INFINITY;
-  for (int v = threadIdx.x; v < V; v += NT) m = fmaxf(m, load1<DT>(row, v));
-  m = block_max<NT>(m, red);
-  float S = 0.f, u = 0.f;
+__device__ __noinline__ PlainStat plain_stat(const void* row, int V, float k, float* red) {
+  __syncthreads();
+  float top = -INFINITY;
+  for (int v = threadIdx.x; v < V; v += NT) top = fmaxf(top, load1<DT>(row, v));
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int w = 0; w < NT / 64; ++w) top = fmaxf(top, red[w]);
+  double S = 0.0, t = 0.0;
   for (int v = threadIdx.x; v < V; v += NT) {
-    const float a = (load1<DT>(row, v) - m) * k, e = __builtin_amdgcn_exp2f(a);
+    const float a = (load1<DT>(row, v) - top) * k, e = __builtin_amdgcn_exp2f(a);
     S += e;
-    if (ENT) u = fmaf(e, fmaxf(a, -1024.f), u);
+    if (ENT) t += e * fmaxf(a, -1024.f);
   }
-  r.M = INFINITY;
-  r.S = block_sum<NT>(S, red);
-  r.m = m;
-  if (ENT) {
-    u = block_sum<NT>(u, red);
-    *ent = (float)(LN2 * (log2((double)r.S) - (double)u / (double)r.S));
+  double* const sum = reinterpret_cast<double*>(red);
+  S = wave_sum64(S);
+  t = wave_sum64(t);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    sum[threadIdx.x >> 6] = S;
+    sum[NT / 64 + (threadIdx.x >> 6)] = t;
   }
-  return r;
+  __syncthreads();
+  S = t = 0.0;
+  for (int w = 0; w < NT / 64; ++w) {
+    S += sum[w];
+    t += sum[NT / 64 + w];
+  }
+  return PlainStat{S, t, top};
+}
+
+// Vectors [i0, i1) of a row, and the values around the vectors if `odd`, added to s.
+template <int DT, bool ENT, int NT>
+__device__ __forceinline__ void add_span(const Span<DT>& sp, int i0, int i1, bool odd,
+                                         const Rows& q, Sums<ENT>& s) {
+  for (int i = i0 + (int)threadIdx.x; i < i1; i += NT) {
+    float f[PER<DT>];
+    unpack<DT>(sp.vec[i], f);
+    s.admit(top_of<DT>(f), q);
+    s.add(f, q);
+  }
+  if (odd && (int)threadIdx.x < sp.odd) {
+    const float x[1] = {load1<DT>(sp.row, sp.odd_at(threadIdx.x))};
+    s.admit(x[0], q);
+    s.add(x, q);
+  }
+}
+
+// The statistics of a row from its threads' sums, and what the row's gradient needs of them.
+template <int DT, bool ENT, int NT>
+__device__ __forceinline__ Joined row_stat(const Sums<ENT>& s, const void* row, const Rows& q,
+                                           JoinSpace<NT>& red, RowStat* st) {
+  Joined j = join<ENT, NT>(s, red);
+  float m = 0.f;
+  if (!(j.S > 0.0 && j.S < (double)INFINITY)) {
+    const PlainStat ps =
+        plain_stat<DT, ENT, NT>(row, q.V, q.khi, reinterpret_cast<float*>(&red));
+    j = Joined{INFINITY, ps.S, ps.t};
+    m = ps.m;
+  }
+  *st = RowStat{j.M, (float)j.S, m, 0.f};
+  return j;
 }
 
 // logp of the row's token; NaN for an id outside the vocabulary.
 template <int DT>
-__device__ __forceinline__ double row_logp(const void* row, int64_t id, int V, float k,
-                                           const RowStat& r) {
-  if (id < 0 || id >= V) return __builtin_nan("");
+__device__ __forceinline__ double row_logp(const void* row, int64_t id, const Rows& q,
+                                           const Joined& j, float m) {
+  if (id < 0 || id >= q.V) return __builtin_nan("");
   const double x = load1<DT>(row, id);
-  const double a = r.M < INFINITY ? fma(x, (double)k, -(double)r.M) : (x - (double)r.m) * (double)k;
-  return LN2 * (a - log2((double)r.S));
+  const double a = j.M < INFINITY ? fma(x, q.k, -(double)j.M)
+                                  : (x - (double)m) * (double)q.khi;
+  return LN2 * (a - log2(j.S));
 }
 
 template <int DT>
@@ -215,77 +314,200 @@ __device__ __forceinline__ const void* row_at(const Rows& q, int64_t r) {
 
 constexpr int NT = 512;
 
+struct LogpOut {
+  double* logp64;  // any but logp may be null
+  float* logp;
+  float* entropy;
+  RowStat* stat;
+};
+
 template <int DT, bool ENT>
-__global__ void __launch_bounds__(NT) logp_kernel(Rows q, double* logp64, float* logp,
-                                                  float* entropy, RowStat* stat) {
-  __shared__ float red[NT / 64];
+__device__ __forceinline__ void write_logp(const LogpOut& o, int64_t r, const void* row,
+                                           const Rows& q, const Joined& j, const RowStat& st) {
+  const double lp = row_logp<DT>(row, q.ids[r], q, j, st.m);
+  if (o.logp64) o.logp64[r] = lp;
+  o.logp[r] = (float)lp;
+  if (ENT) o.entropy[r] = (float)(LN2 * (log2(j.S) - j.t / j.S));
+  if (o.stat) o.stat[r] = st;
+}
+template <bool ENT>
+__device__ __forceinline__ void write_uncounted(const LogpOut& o, int64_t r) {
+  if (o.logp64) o.logp64[r] = 0.0;
+  o.logp[r] = 0.f;
+  if (ENT) o.entropy[r] = 0.f;
+  if (o.stat) o.stat[r] = RowStat{0.f, 1.f, 0.f, 0.f};
+}
+
+// One workgroup a row.
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(NT) logp_kernel(Rows q, LogpOut o) {
+  __shared__ JoinSpace<NT> red;
   const int64_t r = blockIdx.x;
-  float ent = 0.f;
-  double lp = 0.0;
-  RowStat st{0.f, 1.f, 0.f, 0.f};
-  if (!q.mask || q.mask[r]) {
-    const void* row = row_at<DT>(q, r);
-    st = row_stat<DT, ENT, NT>(row, q.V, q.k, red, &ent);
-    if (threadIdx.x == 0) lp = row_logp<DT>(row, q.ids[r], q.V, q.k, st);
+  if (q.mask && !q.mask[r]) {
+    if (threadIdx.x == 0) write_uncounted<ENT>(o, r);
+    return;
   }
-  if (threadIdx.x == 0) {
-    if (logp64) logp64[r] = lp;
-    logp[r] = (float)lp;
-    if (ENT) entropy[r] = ent;
-    if (stat) stat[r] = st;
+  const void* row = row_at<DT>(q, r);
+  const Span<DT> sp(row, q.V);
+  Sums<ENT> s;
+  add_span<DT, ENT, NT>(sp, 0, sp.nvec, true, q, s);
+  RowStat st;
+  const Joined j = row_stat<DT, ENT, NT>(s, row, q, red, &st);
+  if (threadIdx.x == 0) write_logp<DT, ENT>(o, r, row, q, j, st);
+}
+
+// Few rows: each cut over gridDim.y workgroups, whose sums are then joined.
+struct Part {
+  double S, t;
+  float M, pad;
+};
+
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(NT) logp_part_kernel(Rows q, Part* parts) {
+  __shared__ JoinSpace<NT> red;
+  const int64_t r = blockIdx.x;
+  if (q.mask && !q.mask[r]) return;
+  const Span<DT> sp(row_at<DT>(q, r), q.V);
+  const int n = (int)gridDim.y, y = (int)blockIdx.y, per = (sp.nvec + n - 1) / n;
+  Sums<ENT> s;
+  add_span<DT, ENT, NT>(sp, min(sp.nvec, y * per), min(sp.nvec, (y + 1) * per), y == 0, q, s);
+  const Joined j = join<ENT, NT>(s, red);
+  if (threadIdx.x == 0) parts[r * n + y] = Part{j.S, j.t, j.M, 0.f};
+}
+
+template <int DT, bool ENT>
+__global__ void __launch_bounds__(NT) logp_join_kernel(Rows q, const Part* parts, int n,
+                                                       LogpOut o) {
+  __shared__ JoinSpace<NT> red;
+  const int64_t r = blockIdx.x;
+  if (q.mask && !q.mask[r]) {
+    if (threadIdx.x == 0) write_uncounted<ENT>(o, r);
+    return;
+  }
+  Sums<ENT> s;
+  if ((int)threadIdx.x < n) {
+    const Part p = parts[r * n + threadIdx.x];
+    s.M = p.M;
+    s.S = p.S;
+    s.t = p.t;
+  }
+  const void* row = row_at<DT>(q, r);
+  RowStat st;
+  const Joined j = row_stat<DT, ENT, NT>(s, row, q, red, &st);
+  if (threadIdx.x == 0) write_logp<DT, ENT>(o, r, row, q, j, st);
+}
+
+// One row's gradient: value(x) = -c / T e(x) / S, and c / T more at id.
+struct RowGrad {
+  float khi, klo, M, m, neg, c;
+  int id;  // -1: outside the vocabulary
+};
+
+__device__ __forceinline__ RowGrad row_grad(const Rows& q, const RowStat& st, float c,
+                                            int64_t id) {
+  return RowGrad{q.khi, q.klo, st.M, st.m, -c / st.S, c, id >= 0 && id < q.V ? (int)id : -1};
+}
+__device__ __forceinline__ float grad_value(const RowGrad& g, float x) {
+  return __builtin_amdgcn_exp2f(exponent(x, g.khi, g.klo, g.M)) * g.neg;
+}
+// ... of rows whose M is not finite
+__device__ __forceinline__ float grad_plain(const RowGrad& g, float x) {
+  return __builtin_amdgcn_exp2f((x - g.m) * g.khi) * g.neg;
+}
+
+// A vector of a row's gradient. For 16-bit results |neg| goes into the exponent, so a value
+// takes one multiply-add, the exponential and half a conversion: 2^(x khi + base), base =
+// log2 |neg| - M + klo (M / khi). base rounds at 2^-24 of its size, klo is applied at the row's
+// top instead of at x: together below 2^-13 of a value while |M| < 1024, a sixteenth of
+// float16's half step; rows beyond that go value by value.
+struct VecGrad {
+  float khi, klo, M, neg, base;
+  uint32_t sign;
+};
+__device__ __forceinline__ VecGrad vec_grad(const RowGrad& g) {
+  return VecGrad{g.khi, g.klo, g.M, g.neg,
+                 __builtin_amdgcn_logf(fabsf(g.neg)) - fmaf(-g.klo, g.M / g.khi, g.M),
+                 __float_as_uint(g.neg) >> 31 ? 0x80008000u : 0u};
+}
+template <int DT>
+__device__ __forceinline__ uint4 grad_vector(const VecGrad& g, const uint4& v) {
+  float f[PER<DT>];
+  unpack<DT>(v, f);
+#pragma unroll
+  for (int j = 0; j < PER<DT>; ++j)
+    f[j] = DT == F32 ? __builtin_amdgcn_exp2f(exponent(f[j], g.khi, g.klo, g.M)) * g.neg
+                     : __builtin_amdgcn_exp2f(fmaf(f[j], g.khi, g.base));
+  uint4 o = pack<DT>(f);
+  if (DT != F32) o = make_uint4(o.x ^ g.sign, o.y ^ g.sign, o.z ^ g.sign, o.w ^ g.sign);
+  return o;
+}
+// Whether grad_vector holds for a row.
+template <int DT>
+__device__ __forceinline__ bool by_vectors(const RowGrad& g) {
+  return DT == F32 ? g.M < INFINITY : fabsf(g.M) < 1024.f;
+}
+
+__device__ __forceinline__ void store_stream(void* p, uint4 v) {
+  __builtin_nontemporal_store(u32x4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<u32x4_t*>(p));
+}
+
+template <int DT, int NT>
+__device__ __forceinline__ void zero_row(void* out, int V) {
+  const Span<DT> sp(out, V);
+  char* const o = static_cast<char*>(out) + (int64_t)sp.head * SIZE<DT>;
+  for (int i = threadIdx.x; i < sp.nvec; i += NT)
+    store_stream(o + (int64_t)i * 16, make_uint4(0, 0, 0, 0));
+  if ((int)threadIdx.x < sp.odd) store1<DT>(out, sp.odd_at(threadIdx.x), 0.f);
+}
+
+// Rows that cannot be stored 16 bytes at a time where they are loaded so, and rows whose M
+// is not finite: value by value.
+template <int DT, int NT>
+__device__ __noinline__ void grad_by_value(RowGrad g, const void* row, void* out, int V) {
+  for (int v = threadIdx.x; v < V; v += NT) {
+    const float x = load1<DT>(row, v);
+    const float y = g.M < INFINITY ? grad_value(g, x) : grad_plain(g, x);
+    store1<DT>(out, v, v == g.id ? y + g.c : y);
   }
 }
 
 // grad[r][v] = coef[r] scale / T (1[v = id] - e_v / S); scale: a device scalar or null.
+// skip_one: the gradient for scale 1 is there already.
 template <int DT>
-__global__ void __launch_bounds__(NT) logits_grad_kernel(Rows q, const RowStat* stat,
+__global__ void __launch_bounds__(NT) logits_grad_kernel(Rows q, int R, const RowStat* stat,
                                                          const float* coef, const float* scale,
-                                                         float inv_t, void* grad) {
-  const int64_t r = blockIdx.x;
-  const void* row = row_at<DT>(q, r);
-  char* const out = static_cast<char*>(grad) + r * q.V * SIZE<DT>;
-  const int V = q.V;
-  const bool on = !q.mask || q.mask[r];
-  RowStat st{0.f, 1.f, 0.f, 0.f};
-  float c = 0.f;
-  int64_t id = -1;
-  if (on) {
-    st = stat[r];
-    c = coef[r] * (scale ? *scale : 1.f) * inv_t;
-    id = q.ids[r];
-  }
-  const float neg = -c / st.S, k = q.k;
-  auto value = [&](float x) __attribute__((always_inline)) {
-    const float a = st.M < INFINITY ? fmaf(x, k, -st.M) : (x - st.m) * k;
-    return __builtin_amdgcn_exp2f(a) * neg;
-  };
-  const int head = head_of<DT>(out, V), nvec = (V - head) / PER<DT>, tail = head + nvec * PER<DT>;
-  const char* const src = static_cast<const char*>(row) + (int64_t)head * SIZE<DT>;
-  uint4* const dst = reinterpret_cast<uint4*>(out + (int64_t)head * SIZE<DT>);
-  const bool same = aligned16(src);
-  for (int i = threadIdx.x; i < nvec; i += NT) {
-    float f[PER<DT>];
-    if (on) {
-      if (same) {
-        unpack<DT>(reinterpret_cast<const uint4*>(src)[i], f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < PER<DT>; ++j) f[j] = load1<DT>(src, (int64_t)i * PER<DT> + j);
-      }
-#pragma unroll
-      for (int j = 0; j < PER<DT>; ++j) {
-        const int64_t v = head + (int64_t)i * PER<DT> + j;
-        f[j] = value(f[j]) + (v == id ? c : 0.f);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < PER<DT>; ++j) f[j] = 0.f;
+                                                         float inv_t, void* grad, bool skip_one) {
+  const float by = scale ? *scale : 1.f;
+  if (skip_one && by == 1.f) return;
+  const int y = (int)blockIdx.y, ny = (int)gridDim.y;
+  for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
+    char* const out = static_cast<char*>(grad) + r * q.V * SIZE<DT>;
+    if (q.mask && !q.mask[r]) {
+      if (!skip_one && y == 0) zero_row<DT, NT>(out, q.V);
+      continue;
     }
-    dst[i] = pack<DT>(f);
-  }
-  if ((int)threadIdx.x < head + V - tail) {
-    const int v = (int)threadIdx.x < head ? threadIdx.x : tail + threadIdx.x - head;
-    store1<DT>(out, v, on ? value(load1<DT>(row, v)) + (v == id ? c : 0.f) : 0.f);
+    const void* row = row_at<DT>(q, r);
+    const RowGrad g = row_grad(q, stat[r], coef[r] * by * inv_t, q.ids[r]);
+    const Span<DT> sp(row, q.V);
+    char* const o = out + (int64_t)sp.head * SIZE<DT>;
+    if (!aligned16(o) || !by_vectors<DT>(g)) {
+      if (y == 0) grad_by_value<DT, NT>(g, row, out, q.V);
+      continue;
+    }
+    const int idv = (g.id - sp.head) / PER<DT>;  // id's vector, if it is in one
+    const bool in_vec = g.id >= sp.head && g.id < sp.tail;
+    const VecGrad vg = vec_grad(g);
+    for (int i = y * NT + (int)threadIdx.x; i < sp.nvec; i += ny * NT) {
+      store_stream(o + (int64_t)i * 16, grad_vector<DT>(vg, sp.vec[i]));
+      // the same thread's store to the same place comes after
+      if (in_vec && i == idv)
+        store1<DT>(out, g.id, grad_value(g, load1<DT>(row, g.id)) + g.c);
+    }
+    if (y == 0 && (int)threadIdx.x < sp.odd) {
+      const int v = sp.odd_at(threadIdx.x);
+      const float d = grad_value(g, load1<DT>(row, v));
+      store1<DT>(out, v, v == g.id ? d + g.c : d);
+    }
   }
 }
 
@@ -293,14 +515,36 @@ __global__ void __launch_bounds__(NT) logits_grad_kernel(Rows q, const RowStat* 
 
 // Counted tokens of each sequence.
 __global__ void __launch_bounds__(256) count_kernel(const uint8_t* mask, int S, int* counts) {
-  __shared__ float red[4];
+  __shared__ JoinSpace<256> red;
   const uint8_t* m = mask + (int64_t)blockIdx.x * S;
   int n = 0;
   for (int s = threadIdx.x; s < S; s += 256) n += m[s] != 0;
-  // at most 2^31 tokens of a sequence, summed as two exact float32 halves
-  const float lo = block_sum<256>((float)(n & 4095), red);
-  const float hi = block_sum<256>((float)(n >> 12), red);
-  if (threadIdx.x == 0) counts[blockIdx.x] = (int)hi * 4096 + (int)lo;
+  const double all = block_sum64<256>((double)n, red);
+  if (threadIdx.x == 0) counts[blockIdx.x] = (int)all;
+}
+
+// Batches small enough for every workgroup to count for itself, in its LDS.
+constexpr int SMALL_TOKENS = 8192, SMALL_BATCH = 1024;
+
+// counts[b] for a small batch: 64 positions a wave, one addition for them where they are of
+// one sequence.
+template <int NT_>
+__device__ __forceinline__ void count_small(const uint8_t* mask, int B, int S, int* counts) {
+  for (int b = threadIdx.x; b < B; b += NT_) counts[b] = 0;
+  __syncthreads();
+  const int R = B * S, lane = threadIdx.x & 63;
+  for (int r0 = (int)(threadIdx.x & ~63u); r0 < R; r0 += NT_) {
+    const int r = r0 + lane;
+    const bool on = r < R && mask[r];
+    const int b0 = r0 / S;
+    const uint64_t set = __ballot(on);
+    if (min(r0 + 63, R - 1) / S == b0) {
+      if (lane == 0) atomicAdd(&counts[b0], __popcll(set));
+    } else if (on) {
+      atomicAdd(&counts[r / S], 1);
+    }
+  }
+  __syncthreads();
 }
 
 struct Tokens {
@@ -310,7 +554,7 @@ struct Tokens {
   const float* ref;      // [R] or null
   const float* adv;      // [B], or [R] (adv_tokens)
   const uint8_t* mask;   // [R] or null
-  const int* counts;     // [B] or null: S each
+  const int* counts;     // [B], or null: S each (no mask), or to be counted (a small batch)
   int B, S;
   bool adv_tokens;
 };
@@ -320,25 +564,24 @@ struct TokenSums {
   double v[5];
 };
 
-// Counted tokens and sequences of the batch, the same in every thread.
+// Counted tokens and sequences of the batch, the same in every thread; counts: [B] or
+// null (S each).
 template <int NT_>
-__device__ __forceinline__ void totals(const Tokens& t, double* red, double* tokens,
-                                       double* seqs) {
-  double n = 0.0, q = 0.0;
-  if (!t.counts) {
-    *tokens = (double)t.B * t.S;
-    *seqs = t.B;
+__device__ __forceinline__ void totals(const int* counts, int B, int S, double* red,
+                                       double* tokens, double* seqs) {
+  if (!counts) {
+    *tokens = (double)B * S;
+    *seqs = B;
     return;
   }
-  for (int b = threadIdx.x; b < t.B; b += NT_) {
-    const int c = t.counts[b];
+  double n = 0.0, q = 0.0;
+  for (int b = threadIdx.x; b < B; b += NT_) {
+    const int c = counts[b];
     n += c;
     q += c > 0;
   }
-  for (int o = 32; o; o >>= 1) {
-    n += __shfl_xor(n, o);
-    q += __shfl_xor(q, o);
-  }
+  n = wave_sum64(n);
+  q = wave_sum64(q);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
     red[threadIdx.x >> 6] = n;
@@ -388,74 +631,222 @@ __device__ __forceinline__ double token_loss(const Policy& p, double lp, double 
   return d * w;
 }
 
-__device__ __forceinline__ double token_at(const Policy& p, const Tokens& t, int64_t r,
-                                           double tokens, double seqs, TokenSums& s) {
-  if (t.mask && !t.mask[r]) return 0.0;
-  const int b = (int)(r / t.S);
-  const double lp = t.logp64 ? t.logp64[r] : (double)t.logp[r];
-  const double w = token_weight(p, t.counts ? t.counts[b] : t.S, tokens, seqs);
+// Token r of sequence b, of which `in_row` tokens are counted.
+__device__ __forceinline__ double token_at(const Policy& p, const Tokens& t, int64_t r, int b,
+                                           double lp, int in_row, double tokens, double seqs,
+                                           TokenSums& s) {
   return token_loss(p, lp, t.old ? (double)t.old[r] : lp, t.ref != nullptr,
-                    t.ref ? (double)t.ref[r] : 0.0, t.adv[t.adv_tokens ? r : b], w, s);
+                    t.ref ? (double)t.ref[r] : 0.0, t.adv[t.adv_tokens ? r : b],
+                    token_weight(p, in_row, tokens, seqs), s);
 }
 
 // The workgroup's sums, in wave order (thread 0 writes them).
 template <int NT_>
 __device__ __forceinline__ void write_sums(TokenSums s, double* red, double* out) {
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    double v = s.v[i];
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      v = red[0];
-      for (int w = 1; w < NT_ / 64; ++w) v += red[w];
-      out[i] = v;
-    }
+  for (int i = 0; i < 5; ++i) s.v[i] = wave_sum64(s.v[i]);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) red[5 * (threadIdx.x >> 6) + i] = s.v[i];
+  __syncthreads();
+  if (threadIdx.x < 5) {
+    double v = red[threadIdx.x];
+    for (int w = 1; w < NT_ / 64; ++w) v += red[5 * w + threadIdx.x];
+    out[threadIdx.x] = v;
   }
+  __syncthreads();
 }
 
-// coef (null: none): d loss / d logp of every token, 0 where not counted.
-__global__ void __launch_bounds__(256) policy_kernel(Policy p, Tokens t, float* coef,
-                                                     const float* scale, double* sums) {
-  __shared__ double red[8];
-  double tokens, seqs;
-  totals<256>(t, red, &tokens, &seqs);
+// What the forward leaves for the backward: d loss / d logp of every token, 0 where not
+// counted, in float64 (the log-probabilities' gradient) or float32 (the logits').
+struct Coef {
+  double* f64;
+  float* f32;
+};
+
+struct LossOut {
+  float* loss;
+  float* metrics;
+};
+
+__device__ __forceinline__ void write_loss(const LossOut& o, const double* sums, double tokens) {
+  *o.loss = (float)sums[0];
+  for (int j = 0; j < 4; ++j) o.metrics[j] = tokens > 0.0 ? (float)(sums[1 + j] / tokens) : 0.f;
+}
+
+// ONE: a small batch by one workgroup, from its counts to the loss.
+template <bool ONE, int NT_>
+__global__ void __launch_bounds__(NT_) policy_kernel(Policy p, Tokens t, Coef coef, double* sums,
+                                                     LossOut o) {
+  __shared__ double red[5 * (NT_ / 64)], all[5];
+  __shared__ int own[ONE ? SMALL_BATCH : 1];
   const int64_t R = (int64_t)t.B * t.S;
-  const double g = scale ? *scale : 1.0;
+  const bool count = ONE && t.mask;
+  if (count) count_small<NT_>(t.mask, t.B, t.S, own);
+  double tokens, seqs;
+  if (count) totals<NT_>(own, t.B, t.S, red, &tokens, &seqs);
+  else totals<NT_>(t.counts, t.B, t.S, red, &tokens, &seqs);
   TokenSums s{};
-  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < R; r += (int64_t)gridDim.x * 256) {
-    const double d = token_at(p, t, r, tokens, seqs, s);
-    if (coef) coef[r] = (float)(d * g);
+  for (int64_t r = (int64_t)blockIdx.x * NT_ + threadIdx.x; r < R; r += (int64_t)gridDim.x * NT_) {
+    double d = 0.0;
+    if (!t.mask || t.mask[r]) {
+      const int b = ONE ? (int)r / t.S : (int)(r / t.S);
+      const int in_row = count ? own[b] : t.counts ? t.counts[b] : t.S;
+      d = token_at(p, t, r, b, t.logp64 ? t.logp64[r] : (double)t.logp[r], in_row, tokens, seqs,
+                   s);
+    }
+    if (coef.f64) coef.f64[r] = d;
+    if (coef.f32) coef.f32[r] = (float)d;
   }
-  if (sums) write_sums<256>(s, red, sums + 5 * (int64_t)blockIdx.x);
+  write_sums<NT_>(s, red, ONE ? all : sums + 5 * (int64_t)blockIdx.x);
+  if (ONE && threadIdx.x == 0) write_loss(o, all, tokens);
 }
 
 // loss and metrics from the workgroups' sums, in their order.
 __global__ void __launch_bounds__(256) finish_kernel(Tokens t, const double* sums, int blocks,
-                                                     float* loss, float* metrics) {
-  __shared__ double red[8], out[5];
+                                                     LossOut o) {
+  __shared__ double red[20], all[5];
   double tokens, seqs;
-  totals<256>(t, red, &tokens, &seqs);
+  totals<256>(t.counts, t.B, t.S, red, &tokens, &seqs);
   TokenSums s{};
   for (int i = threadIdx.x; i < blocks; i += 256)
     for (int j = 0; j < 5; ++j) s.v[j] += sums[5 * i + j];
-  write_sums<256>(s, red, out);
-  if (threadIdx.x) return;
-  *loss = (float)out[0];
-  for (int j = 0; j < 4; ++j) metrics[j] = tokens > 0.0 ? (float)(out[1 + j] / tokens) : 0.f;
+  write_sums<256>(s, red, all);
+  if (threadIdx.x == 0) write_loss(o, all, tokens);
+}
+
+// grad[r] = coef[r] * *by
+__global__ void __launch_bounds__(256) scale_kernel(const double* coef, const float* by, int64_t n,
+                                                    float* grad) {
+  const double f = *by;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    grad[i] = (float)(coef[i] * f);
+}
+
+// ------------------------------------------- loss and gradient in one pass --
+
+// A row of logits stays in registers from its sums to its gradient, so it is read once:
+// NV vectors a thread, one row a workgroup.
+template <int DT, int NT_, int NV>
+__global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tokens t,
+                                                           float inv_t, double* logp64,
+                                                           float* logp, RowStat* stat,
+                                                           float* coef, void* grad) {
+  __shared__ JoinSpace<NT_> red;
+  __shared__ double total[2 * (NT_ / 64)];
+  __shared__ float shared_coef;
+  __shared__ int own[SMALL_BATCH];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  char* const out = static_cast<char*>(grad) + r * q.V * SIZE<DT>;
+  if (q.mask && !q.mask[r]) {
+    zero_row<DT, NT_>(out, q.V);
+    if (tid == 0) {
+      logp64[r] = 0.0;
+      logp[r] = 0.f;
+      stat[r] = RowStat{0.f, 1.f, 0.f, 0.f};
+      coef[r] = 0.f;
+    }
+    return;
+  }
+  const void* row = row_at<DT>(q, r);
+  const Span<DT> sp(row, q.V);
+  uint4 v[NV];
+  // whole strides of the workgroup, then the last one's threads; -inf adds nothing
+  constexpr uint32_t LOW = DT == F32 ? 0xFF800000u : DT == F16 ? 0xFC00FC00u : 0xFF80FF80u;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if ((i + 1) * NT_ <= sp.nvec) {
+      v[i] = load_stream(sp.vec + i * NT_ + tid);
+    } else {
+      v[i] = make_uint4(LOW, LOW, LOW, LOW);
+      if (i * NT_ + tid < sp.nvec) v[i] = load_stream(sp.vec + i * NT_ + tid);
+    }
+  }
+  const float odd = tid < sp.odd ? load1<DT>(row, sp.odd_at(tid)) : -INFINITY;
+  // counted while the row is on its way
+  const bool count = t.mask && !t.counts;
+  if (count) count_small<NT_>(t.mask, t.B, t.S, own);
+  double tokens, seqs;
+  if (count) totals<NT_>(own, t.B, t.S, total, &tokens, &seqs);
+  else totals<NT_>(t.counts, t.B, t.S, total, &tokens, &seqs);
+  Sums<false> s;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * NT_ < sp.nvec) {
+      float f[PER<DT>];
+      unpack<DT>(v[i], f);
+      s.admit(top_of<DT>(f), q);
+      s.add(f, q);
+    }
+  }
+  if (sp.odd) {
+    const float x[1] = {odd};
+    s.admit(odd, q);
+    s.add(x, q);
+  }
+  RowStat st;
+  const Joined j = row_stat<DT, false, NT_>(s, row, q, red, &st);
+  const int64_t id = q.ids[r];
+  if (tid == 0) {
+    const int b = (int)(r / t.S);
+    const double lp = row_logp<DT>(row, id, q, j, st.m);
+    const int in_row = count ? own[b] : t.counts ? t.counts[b] : t.S;
+    TokenSums unused{};
+    const float c = (float)token_at(p, t, r, b, lp, in_row, tokens, seqs, unused);
+    logp64[r] = lp;
+    logp[r] = (float)lp;
+    stat[r] = st;
+    coef[r] = c;
+    shared_coef = c;
+  }
+  __syncthreads();
+  const RowGrad g = row_grad(q, st, shared_coef * inv_t, id);
+  char* const o = out + (int64_t)sp.head * SIZE<DT>;
+  if (!aligned16(o) || !by_vectors<DT>(g)) {
+    grad_by_value<DT, NT_>(g, row, out, q.V);
+    return;
+  }
+  const VecGrad vg = vec_grad(g);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * NT_ + tid < sp.nvec)
+      store_stream(o + (int64_t)(i * NT_ + tid) * 16, grad_vector<DT>(vg, v[i]));
+  }
+  if (tid < sp.odd) {
+    const int at = sp.odd_at(tid);
+    const float y = grad_value(g, odd);
+    store1<DT>(out, at, at == g.id ? y + g.c : y);
+  }
+  // the token's own value, by the thread that stored its vector (its later store to the
+  // same place comes after)
+  if (g.id >= sp.head && g.id < sp.tail && (g.id - sp.head) / PER<DT> % NT_ == tid)
+    store1<DT>(out, g.id, grad_value(g, load1<DT>(row, g.id)) + g.c);
 }
 
 // ----------------------------------------------------------------- host --
 
-// Workspace of the loss entry points: counted tokens per sequence, the workgroups'
-// sums, and (from logits) the float64 log-probabilities.
+// Workgroups a row of the log-probabilities is cut over: enough for 512 in all (two a CU:
+// 8 rows of 151936 bf16 logits 17.3 us with one workgroup each), each with 2048 vectors or more.
+int logp_cuts(int64_t R, int dtype, int V) {
+  const int64_t vecs = (int64_t)V * (dtype == F32 ? 4 : 2) / 16;
+  const int64_t n = R ? (512 + R - 1) / R : 1;
+  const int64_t most = vecs / 2048 < 64 ? vecs / 2048 : 64;
+  return (int)(n < most ? n : most > 1 ? most : 1);
+}
+size_t logp_ws(int64_t R, int dtype, int V) {
+  const int n = logp_cuts(R, dtype, V);
+  return n > 1 ? (size_t)R * n * sizeof(Part) : 0;
+}
+
+// Workspace of the loss entry points: counted tokens per sequence, the workgroups' sums, and
+// (from logits) the float64 log-probabilities and the parts of few rows.
 constexpr int SUM_BLOCKS = 256;
 struct PolicyWs {
-  size_t counts, sums, logp64, total;
+  size_t counts, sums, logp64, parts, total;
 };
-PolicyWs policy_ws(int B, int S, bool logits) {
+PolicyWs policy_ws(int B, int S, int dtype, int V) {  // V 0: from log-probabilities
   PolicyWs w{};
   size_t o = 0;
   auto take = [&](size_t n) {
@@ -463,9 +854,11 @@ PolicyWs policy_ws(int B, int S, bool logits) {
     o += (n + 255) / 256 * 256;
     return at;
   };
+  const int64_t R = (int64_t)B * S;
   w.counts = take((size_t)B * 4);
   w.sums = take(SUM_BLOCKS * 5 * 8);
-  w.logp64 = take(logits ? (size_t)B * S * 8 : 0);
+  w.logp64 = take(V ? (size_t)R * 8 : 0);
+  w.parts = take(V ? logp_ws(R, dtype, V) : 0);
   w.total = o;
   return w;
 }
@@ -477,14 +870,14 @@ int batch_check(int B, int S) {
 }
 
 int rows_check(const void* x, int dtype, int64_t sb, int64_t ss, int B, int S, int V,
-               const int64_t* ids, float temperature) {
+               const int64_t* ids, double temperature) {
   if (int rc = batch_check(B, S)) return rc;
   if ((int64_t)B * S >= (1 << 22)) return einval("2^22 rows of logits or more");
   if (V < 1) return einval("an empty vocabulary");
   if (dtype < 0 || dtype > 2) return einval("dtype must be 0 (bf16), 1 (float16) or 2 (float32)");
-  if (!(temperature > 0.f) || !(temperature < INFINITY))
+  if (!(temperature > 0.0) || !(temperature < (double)INFINITY))
     return einval("temperature must be positive and finite");
-  const float k = (float)(1.0 / LN2 / (double)temperature);
+  const float k = (float)(1.0 / LN2 / temperature);
   if (!(k >= 1e-30f) || !(k <= 1e30f)) return einval("temperature out of range");
   if ((int64_t)B * S == 0) return GRPO_OK;
   if (!x || !ids) return einval("null pointer");
@@ -495,40 +888,81 @@ int rows_check(const void* x, int dtype, int64_t sb, int64_t ss, int B, int S, i
 }
 
 Rows rows_of(const void* x, int64_t sb, int64_t ss, int S, int V, const int64_t* ids,
-             const uint8_t* mask, float temperature) {
-  return Rows{x, sb, ss, S, V, ids, mask, (float)(1.0 / LN2 / (double)temperature)};
+             const uint8_t* mask, double temperature) {
+  const double k = 1.0 / LN2 / temperature;
+  float hi = (float)k;
+  if ((double)hi >= k) hi = nextafterf(hi, 0.f);
+  return Rows{x, sb, ss, S, V, ids, mask, k, hi, (float)(k - (double)hi)};
 }
 
-template <int DT>
-int launch_logp(const Rows& q, int64_t R, double* logp64, float* logp, float* entropy,
-                RowStat* stat, hipStream_t st) {
-  if (entropy) logp_kernel<DT, true><<<(unsigned)R, NT, 0, st>>>(q, logp64, logp, entropy, stat);
-  else logp_kernel<DT, false><<<(unsigned)R, NT, 0, st>>>(q, logp64, logp, entropy, stat);
-  return launch_check("token_logprobs");
+template <int DT, bool ENT>
+int launch_logp(const Rows& q, int64_t R, const LogpOut& o, Part* parts, hipStream_t st) {
+  const int n = logp_cuts(R, DT, q.V);
+  if (n == 1) {
+    logp_kernel<DT, ENT><<<(unsigned)R, NT, 0, st>>>(q, o);
+    return launch_check("token_logprobs");
+  }
+  logp_part_kernel<DT, ENT><<<dim3((unsigned)R, (unsigned)n), NT, 0, st>>>(q, parts);
+  if (int rc = launch_check("token_logprobs_part")) return rc;
+  logp_join_kernel<DT, ENT><<<(unsigned)R, NT, 0, st>>>(q, parts, n, o);
+  return launch_check("token_logprobs_join");
 }
 
-int run_logp(int dtype, const Rows& q, int64_t R, double* logp64, float* logp, float* entropy,
-             RowStat* stat, hipStream_t st) {
-  if (dtype == BF16) return launch_logp<BF16>(q, R, logp64, logp, entropy, stat, st);
-  if (dtype == F16) return launch_logp<F16>(q, R, logp64, logp, entropy, stat, st);
-  return launch_logp<F32>(q, R, logp64, logp, entropy, stat, st);
+int run_logp(int dtype, const Rows& q, int64_t R, const LogpOut& o, void* parts, hipStream_t st) {
+  Part* const p = static_cast<Part*>(parts);
+  auto go = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    return o.entropy ? launch_logp<DT, true>(q, R, o, p, st) : launch_logp<DT, false>(q, R, o, p, st);
+  };
+  if (dtype == BF16) return go(std::integral_constant<int, BF16>{});
+  if (dtype == F16) return go(std::integral_constant<int, F16>{});
+  return go(std::integral_constant<int, F32>{});
 }
 
 int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const float* coef,
-             const float* scale, float temperature, void* grad, hipStream_t st) {
-  const float inv_t = 1.f / temperature;
-  const unsigned n = (unsigned)R;
+             const float* scale, double temperature, void* grad, bool skip_one, hipStream_t st) {
+  const float inv_t = (float)(1.0 / temperature);
+  const int n = (int)R;
+  // with a gradient that is most likely there already, few workgroups to find that out; few
+  // rows are cut over several
+  const dim3 grid(skip_one && n > 1024 ? 1024u : (unsigned)n,
+                  n < 256 ? (unsigned)logp_cuts(R, dtype, q.V) : 1u);
   if (dtype == BF16)
-    logits_grad_kernel<BF16><<<n, NT, 0, st>>>(q, stat, coef, scale, inv_t, grad);
+    logits_grad_kernel<BF16><<<grid, NT, 0, st>>>(q, n, stat, coef, scale, inv_t, grad, skip_one);
   else if (dtype == F16)
-    logits_grad_kernel<F16><<<n, NT, 0, st>>>(q, stat, coef, scale, inv_t, grad);
+    logits_grad_kernel<F16><<<grid, NT, 0, st>>>(q, n, stat, coef, scale, inv_t, grad, skip_one);
   else
-    logits_grad_kernel<F32><<<n, NT, 0, st>>>(q, stat, coef, scale, inv_t, grad);
+    logits_grad_kernel<F32><<<grid, NT, 0, st>>>(q, n, stat, coef, scale, inv_t, grad, skip_one);
   return launch_check("token_logprobs_backward");
 }
 
+// Rows of at most this many bytes stay in registers: 19 vectors a thread of a workgroup
+// that fills a CU's registers.
+constexpr int HELD = 19;
+bool rows_held(int dtype, int V) {
+  return (int64_t)V * (dtype == F32 ? 4 : 2) <= (int64_t)HELD * 1024 * 16;
+}
+
+template <int DT>
+int launch_loss_rows(const Rows& q, int64_t R, const Policy& p, const Tokens& t, float inv_t,
+                     double* logp64, float* logp, RowStat* stat, float* coef, void* grad,
+                     hipStream_t st) {
+  const int64_t bytes = (int64_t)q.V * SIZE<DT>;
+  const unsigned n = (unsigned)R;
+  if (bytes <= HELD * 256 * 16)
+    loss_rows_kernel<DT, 256, HELD><<<n, 256, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
+                                                       grad);
+  else if (bytes <= HELD * 512 * 16)
+    loss_rows_kernel<DT, 512, HELD><<<n, 512, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
+                                                       grad);
+  else
+    loss_rows_kernel<DT, 1024, HELD><<<n, 1024, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
+                                                         grad);
+  return launch_check("policy_loss_rows");
+}
+
 int policy_check(const grpo_policy_t* p, int B, int S, const float* adv, const void* ws,
-                 size_t ws_bytes, bool logits) {
+                 size_t ws_bytes, const PolicyWs& need) {
   if (int rc = batch_check(B, S)) return rc;
   if (!p) return einval("null policy parameters");
   if (!(p->eps_low >= 0.0) || !(p->eps_high >= 0.0)) return einval("clip range must be >= 0");
@@ -539,52 +973,76 @@ int policy_check(const grpo_policy_t* p, int B, int S, const float* adv, const v
   if ((int64_t)B * S && !adv) return einval("null pointer");
   if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u))
     return einval("the workspace must be 16-byte aligned");
-  if (ws_bytes < policy_ws(B, S, logits).total) {
+  if (ws_bytes < need.total) {
     set_error("workspace too small");
     return GRPO_EWORKSPACE;
   }
   return GRPO_OK;
 }
 
-// Counts, then the tokens' losses and derivatives, then the sums' end.
-int run_policy(const Policy& p, Tokens t, char* ws, const PolicyWs& o, float* coef, float* loss,
-               float* metrics, hipStream_t st) {
+bool small_batch(const Tokens& t) {
+  return (int64_t)t.B * t.S <= SMALL_TOKENS && t.B <= SMALL_BATCH;
+}
+
+// Counts ahead of the kernels that need them (a small batch is counted in those).
+int run_counts(Tokens* t, char* ws, const PolicyWs& o, hipStream_t st) {
+  if (!t->mask || small_batch(*t)) return GRPO_OK;
+  int* counts = reinterpret_cast<int*>(ws + o.counts);
+  count_kernel<<<(unsigned)t->B, 256, 0, st>>>(t->mask, t->S, counts);
+  t->counts = counts;
+  return launch_check("policy_count");
+}
+
+// The tokens' losses and derivatives, and the sums' end. One workgroup takes a small batch
+// (4096 tokens: one launch of 8 us for three of 3.6, 5.3 and 4.0).
+int run_policy(const Policy& p, const Tokens& t, char* ws, const PolicyWs& o, Coef coef,
+               const LossOut& out, hipStream_t st) {
   const int64_t R = (int64_t)t.B * t.S;
-  if (t.mask && R) {
-    int* counts = reinterpret_cast<int*>(ws + o.counts);
-    count_kernel<<<(unsigned)t.B, 256, 0, st>>>(t.mask, t.S, counts);
-    if (int rc = launch_check("policy_count")) return rc;
-    t.counts = counts;
-  }
   double* sums = reinterpret_cast<double*>(ws + o.sums);
-  const int blocks = (int)(R ? cdiv(R, 256) < SUM_BLOCKS ? cdiv(R, 256) : SUM_BLOCKS : 0);
-  if (blocks) {
-    policy_kernel<<<blocks, 256, 0, st>>>(p, t, coef, nullptr, sums);
-    if (int rc = launch_check("policy_loss")) return rc;
+  if (small_batch(t)) {
+    policy_kernel<true, 1024><<<1, 1024, 0, st>>>(p, t, coef, sums, out);
+    return launch_check("policy_loss");
   }
-  finish_kernel<<<1, 256, 0, st>>>(t, sums, blocks, loss, metrics);
+  const int64_t most = R ? cdiv(R, 256) : 1;
+  const int blocks = (int)(most < SUM_BLOCKS ? most : SUM_BLOCKS);
+  policy_kernel<false, 256><<<blocks, 256, 0, st>>>(p, t, coef, sums, out);
+  if (int rc = launch_check("policy_loss")) return rc;
+  finish_kernel<<<1, 256, 0, st>>>(t, sums, blocks, out);
   return launch_check("policy_finish");
 }
 
 }  // namespace
 
+extern "C" size_t grpo_token_logprobs_workspace_bytes(int dtype, int B, int S, int V) {
+  return dtype < 0 || dtype > 2 || B < 0 || S < 0 || V < 1 ? 0 : logp_ws((int64_t)B * S, dtype, V);
+}
+
 extern "C" int grpo_token_logprobs(const void* logits, int dtype, int64_t stride_b,
                                    int64_t stride_s, int B, int S, int V, const int64_t* ids,
-                                   const uint8_t* mask, float temperature, float* logp,
-                                   float* entropy, float* stat, grpo_stream_t stream) {
+                                   const uint8_t* mask, double temperature, float* logp,
+                                   float* entropy, float* stat, void* workspace,
+                                   size_t workspace_bytes, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
   const int64_t R = (int64_t)B * S;
   if (!R) return GRPO_OK;
   if (!logp) return einval("null pointer");
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
-  return run_logp(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R,
-                  nullptr, logp, entropy, reinterpret_cast<RowStat*>(stat), as_stream(stream));
+  if (const size_t need = logp_ws(R, dtype, V)) {
+    if (!workspace || !aligned16(workspace)) return einval("the workspace must be 16-byte aligned");
+    if (workspace_bytes < need) {
+      set_error("workspace too small");
+      return GRPO_EWORKSPACE;
+    }
+  }
+  const LogpOut o{nullptr, logp, entropy, reinterpret_cast<RowStat*>(stat)};
+  return run_logp(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R, o,
+                  workspace, as_stream(stream));
 }
 
 extern "C" int grpo_token_logprobs_backward(const void* logits, int dtype, int64_t stride_b,
                                             int64_t stride_s, int B, int S, int V,
                                             const int64_t* ids, const uint8_t* mask,
-                                            float temperature, const float* stat,
+                                            double temperature, const float* stat,
                                             const float* grad_logp, const float* scale,
                                             void* grad_logits, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
@@ -596,69 +1054,104 @@ extern "C" int grpo_token_logprobs_backward(const void* logits, int dtype, int64
     return einval("grad_logits is not aligned to its type");
   return run_grad(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R,
                   reinterpret_cast<const RowStat*>(stat), grad_logp, scale, temperature,
-                  grad_logits, as_stream(stream));
+                  grad_logits, false, as_stream(stream));
 }
 
-extern "C" size_t grpo_policy_loss_workspace_bytes(int B, int S, int from_logits) {
-  return B < 0 || S < 0 ? 0 : policy_ws(B, S, from_logits != 0).total;
+extern "C" size_t grpo_policy_loss_workspace_bytes(int B, int S) {
+  return B < 0 || S < 0 ? 0 : policy_ws(B, S, 0, 0).total;
 }
 
 extern "C" int grpo_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
                                 const float* advantages, int adv_tokens, const uint8_t* mask,
                                 int B, int S, const grpo_policy_t* policy, float* loss,
-                                float* metrics, void* workspace, size_t workspace_bytes,
-                                grpo_stream_t stream) {
-  if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, false)) return rc;
+                                float* metrics, double* coef, void* workspace,
+                                size_t workspace_bytes, grpo_stream_t stream) {
+  if (int rc = batch_check(B, S)) return rc;
+  const PolicyWs o = policy_ws(B, S, 0, 0);
+  if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, o)) return rc;
   if (((int64_t)B * S && !logp) || !loss || !metrics) return einval("null pointer");
   Tokens t{nullptr, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
-  return run_policy(*policy, t, static_cast<char*>(workspace), policy_ws(B, S, false),
-                    nullptr, loss, metrics, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  char* const ws = static_cast<char*>(workspace);
+  if (int rc = run_counts(&t, ws, o, st)) return rc;
+  return run_policy(*policy, t, ws, o, Coef{coef, nullptr}, LossOut{loss, metrics}, st);
 }
 
-extern "C" int grpo_policy_loss_backward(const float* logp, const float* old_logp,
-                                         const float* ref_logp, const float* advantages,
-                                         int adv_tokens, const uint8_t* mask, int B, int S,
-                                         const grpo_policy_t* policy, const float* grad_loss,
-                                         float* grad_logp, void* workspace,
-                                         size_t workspace_bytes, grpo_stream_t stream) {
-  if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, false)) return rc;
-  const int64_t R = (int64_t)B * S;
-  if (!R) return GRPO_OK;
-  if (!logp || !grad_loss || !grad_logp) return einval("null pointer");
-  hipStream_t st = as_stream(stream);
-  Tokens t{nullptr, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
-  if (mask) {  // the forward's counts, in the same workspace
-    t.counts = reinterpret_cast<const int*>(static_cast<char*>(workspace) +
-                                            policy_ws(B, S, false).counts);
-  }
-  const int blocks = (int)(cdiv(R, 256) < 2048 ? cdiv(R, 256) : 2048);
-  policy_kernel<<<blocks, 256, 0, st>>>(*policy, t, grad_logp, grad_loss, nullptr);
+extern "C" int grpo_policy_loss_backward(const double* coef, const float* grad_loss,
+                                         int64_t tokens, float* grad_logp, grpo_stream_t stream) {
+  if (tokens < 0) return einval("negative dimension");
+  if (!tokens) return GRPO_OK;
+  if (!coef || !grad_loss || !grad_logp) return einval("null pointer");
+  const int blocks = (int)(cdiv(tokens, 256) < 2048 ? cdiv(tokens, 256) : 2048);
+  scale_kernel<<<blocks, 256, 0, as_stream(stream)>>>(coef, grad_loss, tokens, grad_logp);
   return launch_check("policy_loss_backward");
+}
+
+extern "C" size_t grpo_policy_loss_logits_workspace_bytes(int dtype, int B, int S, int V) {
+  return dtype < 0 || dtype > 2 || B < 0 || S < 0 || V < 1 ? 0 : policy_ws(B, S, dtype, V).total;
 }
 
 extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b,
                                        int64_t stride_s, int B, int S, int V, const int64_t* ids,
-                                       const uint8_t* mask, float temperature,
+                                       const uint8_t* mask, double temperature,
                                        const float* old_logp, const float* ref_logp,
                                        const float* advantages, int adv_tokens,
                                        const grpo_policy_t* policy, float* loss, float* logp,
-                                       float* metrics, float* stat, float* coef, void* workspace,
+                                       float* metrics, float* stat, float* coef,
+                                       void* grad_logits, void* workspace,
                                        size_t workspace_bytes, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
-  if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, true)) return rc;
+  const PolicyWs o = policy_ws(B, S, dtype, V);
+  if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, o)) return rc;
   const int64_t R = (int64_t)B * S;
   if ((R && !logp) || !loss || !metrics) return einval("null pointer");
   if ((stat == nullptr) != (coef == nullptr)) return einval("stat and coef go together");
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
+  if (grad_logits && R && (!stat || !rows_held(dtype, V)))
+    return einval("grad_logits needs stat and coef and a row of at most 311296 bytes");
+  if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == F32 ? 4 : 2))
+    return einval("grad_logits is not aligned to its type");
   hipStream_t st = as_stream(stream);
   char* const ws = static_cast<char*>(workspace);
-  const PolicyWs o = policy_ws(B, S, true);
   double* const lp = reinterpret_cast<double*>(ws + o.logp64);
+  RowStat* const rs = reinterpret_cast<RowStat*>(stat);
+  Tokens t{lp, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
+  if (int rc = run_counts(&t, ws, o, st)) return rc;
   if (R) {
     const Rows q = rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature);
-    if (int rc = run_logp(dtype, q, R, lp, logp, nullptr, reinterpret_cast<RowStat*>(stat), st))
-      return rc;
+    const float inv_t = (float)(1.0 / temperature);
+    int rc;
+    if (!grad_logits) {
+      rc = run_logp(dtype, q, R, LogpOut{lp, logp, nullptr, rs}, ws + o.parts, st);
+    } else {
+      auto go = dtype == BF16 ? launch_loss_rows<BF16>
+                : dtype == F16 ? launch_loss_rows<F16> : launch_loss_rows<F32>;
+      rc = go(q, R, *policy, t, inv_t, lp, logp, rs, coef, grad_logits, st);
+      coef = nullptr;  // written
+    }
+    if (rc) return rc;
   }
-  Tokens t{lp, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
-  return run_policy(*policy, t, ws, o, coef, loss, metrics, st);
+  return run_policy(*policy, t, ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
+}
+
+extern "C" int grpo_policy_loss_logits_held(int dtype, int V) {
+  return dtype >= 0 && dtype <= 2 && V >= 1 && rows_held(dtype, V);
+}
+
+extern "C" int grpo_policy_loss_logits_rescale(const void* logits, int dtype, int64_t stride_b,
+                                               int64_t stride_s, int B, int S, int V,
+                                               const int64_t* ids, const uint8_t* mask,
+                                               double temperature, const float* stat,
+                                               const float* coef, const float* grad_loss,
+                                               void* grad_logits, grpo_stream_t stream) {
+  if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
+  const int64_t R = (int64_t)B * S;
+  if (!R) return GRPO_OK;
+  if (!stat || !coef || !grad_loss || !grad_logits) return einval("null pointer");
+  if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == F32 ? 4 : 2))
+    return einval("grad_logits is not aligned to its type");
+  return run_grad(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R,
+                  reinterpret_cast<const RowStat*>(stat), coef, grad_loss, temperature,
+                  grad_logits, true, as_stream(stream));
 }

@@ -6,20 +6,21 @@
 * ``grpo_policy_loss``: the two-sided clipped policy loss with a cap on the ratio and a
   KL term (``src/grpo/algorithm.py:115-254``) from per-token log-probabilities;
 * ``fused_grpo_loss``: the loss straight from the logits (``src/triton_kernels/
-  grpo_loss.py:571-625``), the vocabulary read once forward.
+  grpo_loss.py:571-625``), the vocabulary read once for the loss and its gradient.
 
 Positions are ``[batch, seq]``; ``logits[b, s]`` scores ``token_ids[b, s]`` (shifting
 logits against tokens is the caller's slice: ``logits[:, :-1]`` is taken as it is, without
 a copy).  ``mask`` says which positions count; the others are not read, whatever stands
 there, and get logp 0 and gradient 0.  Softmax statistics, losses and gradients are
 float32 or float64; the logits' gradient is rounded once, to the logits' type.
-Arguments that do not fit raise ``ValueError``, a missing device ``ImportError``.
+Arguments that do not fit raise ``ValueError``, a missing device ``ImportError``.  Nothing is
+kept between calls: every buffer is the call's own.
 """
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -30,132 +31,157 @@ from .. import _lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NORMALIZERS = {"tokens": 0, "sequences": 1}
+_MAX_ROWS = 1 << 22
 
 
-def _on(device: torch.device):
-    """The device's context where it is not the current one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _run(device: torch.device, name: str, *args) -> None:
+    """The C entry point on the device's current stream."""
+    fn = getattr(_lib.device_library(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _same_device(device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must be on {device}, got {t.device}.")
+def _once(backward):
+    """``once_differentiable``, its bookkeeping left out where no graph is being made."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
 
 
-def _float_rows(t: Optional[torch.Tensor], name: str, shape) -> Optional[torch.Tensor]:
-    """A float32 contiguous tensor of ``shape`` (any float type is taken)."""
+# ------------------------------------------------------- argument checks --
+
+def _float_rows(t: Optional[torch.Tensor], name: str, shape,
+                device: torch.device) -> Optional[torch.Tensor]:
+    """``t`` as a contiguous float32 tensor of ``shape`` without a graph."""
     if t is None:
         return None
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}.")
     if not t.dtype.is_floating_point:
         raise ValueError(f"{name} must be a floating-point tensor, got {t.dtype}.")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}.")
-    t = t.detach()
+    if t.requires_grad:
+        t = t.detach()
     if t.dtype != torch.float32:
         t = t.float()
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _mask_rows(mask: Optional[torch.Tensor], shape) -> Optional[torch.Tensor]:
+def _mask_rows(mask: Optional[torch.Tensor], shape,
+               device: torch.device) -> Optional[torch.Tensor]:
     """The mask as contiguous bool (any type: nonzero counts)."""
     if mask is None:
         return None
-    if tuple(mask.shape) != tuple(shape):
+    if mask.device != device:
+        raise ValueError(f"mask must be on {device}, got {mask.device}.")
+    if mask.shape != shape:
         raise ValueError(f"mask must be {list(shape)}, got {list(mask.shape)}.")
     if mask.dtype != torch.bool:
         mask = mask != 0
     return mask if mask.is_contiguous() else mask.contiguous()
 
 
-class _Rows:
-    """Checked logits with their ids and mask, and the C arguments that describe them."""
-
-    def __init__(self, logits, token_ids, mask, temperature):
-        if logits.ndim < 2:
-            raise ValueError(f"logits must be [..., vocab], got {list(logits.shape)}.")
-        if not logits.is_cuda:
-            raise ValueError("logits must be on the ROCm/HIP device.")
-        if logits.dtype not in _DTYPES:
-            raise ValueError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}.")
-        lead = logits.shape[:-1]
-        if tuple(token_ids.shape) != tuple(lead):
-            raise ValueError(f"token_ids must be {list(lead)}, got {list(token_ids.shape)}.")
-        if token_ids.dtype != torch.int64:
-            raise ValueError(f"token_ids must be int64, got {token_ids.dtype}.")
-        if logits.shape[-1] < 1:
-            raise ValueError("logits must have a vocabulary of at least one token.")
-        t = float(temperature)
-        if not (0.0 < t < math.inf):
-            raise ValueError(f"temperature must be positive and finite, got {temperature}.")
-        _same_device(logits.device, token_ids=token_ids, mask=mask)
-        x = logits.detach()
-        if x.stride(-1) != 1 and x.shape[-1] > 1 or any(v < 0 for v in x.stride()):
-            x = x.contiguous()
-        if x.ndim > 3:
-            x = x.reshape(-1, x.shape[-2], x.shape[-1])
-        self.shape, self.t = tuple(lead), t
-        self.x, self.ids = x, token_ids.contiguous()
-        self.mask = _mask_rows(mask, lead)
-        self.vocab = x.shape[-1]
-        if x.ndim == 3:
-            self.b, self.s, self.sb, self.ss = x.shape[0], x.shape[1], x.stride(0), x.stride(1)
-        else:
-            self.b, self.s, self.sb, self.ss = x.shape[0], 1, x.stride(0), 0
-        if self.b * self.s >= 1 << 22:
-            raise ValueError("at most 2**22 - 1 rows of logits in a call.")
-
-    def args(self):
-        return (self.x.data_ptr(), _DTYPES[self.x.dtype], self.sb, self.ss, self.b, self.s,
-                self.vocab, self.ids.data_ptr(), _lib.ptr(self.mask), self.t)
+def _check_logits(logits, token_ids, mask, temperature):
+    """(contiguous ids, mask, temperature) that fit the logits."""
+    if logits.ndim < 2:
+        raise ValueError(f"logits must be [..., vocab], got {list(logits.shape)}.")
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the ROCm/HIP device.")
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits must be bfloat16, float16 or float32, got {logits.dtype}.")
+    *lead, vocab = logits.shape
+    lead = torch.Size(lead)
+    if token_ids.shape != lead:
+        raise ValueError(f"token_ids must be {list(lead)}, got {list(token_ids.shape)}.")
+    if token_ids.dtype != torch.int64:
+        raise ValueError(f"token_ids must be int64, got {token_ids.dtype}.")
+    if token_ids.device != logits.device:
+        raise ValueError(f"token_ids must be on {logits.device}, got {token_ids.device}.")
+    if not vocab:
+        raise ValueError("logits must have a vocabulary of at least one token.")
+    if lead.numel() >= _MAX_ROWS:
+        raise ValueError(f"at most {_MAX_ROWS - 1} rows of logits in a call.")
+    t = float(temperature)
+    if not 0.0 < t < math.inf:
+        raise ValueError(f"temperature must be positive and finite, got {temperature}.")
+    if not token_ids.is_contiguous():
+        token_ids = token_ids.contiguous()
+    return token_ids, _mask_rows(mask, lead, logits.device), t
 
 
-def _grad_of(rows: _Rows, stat, coef, scale) -> torch.Tensor:
-    """The logits' gradient, of the logits' shape."""
-    out = torch.empty((*rows.shape, rows.vocab), dtype=rows.x.dtype, device=rows.x.device)
-    with _on(out.device):
-        rc = _lib.device_library().grpo_token_logprobs_backward(
-            *rows.args(), stat.data_ptr(), coef.data_ptr(), _lib.ptr(scale), out.data_ptr(),
-            _lib.stream_handle(out.device))
-    if rc:
-        _lib.check(rc, "grpo_token_logprobs_backward")
+def _rows(logits, ids, mask, t):
+    """(the tensor read, the C arguments that describe its rows)."""
+    x = logits.detach()
+    if x.ndim == 2:
+        x = x.unsqueeze(1)
+    elif x.ndim > 3:
+        x = x.reshape(-1, x.shape[-2], x.shape[-1])
+    b, s, v = x.shape
+    sb, ss, sv = x.stride()
+    if sv != 1 and v > 1:
+        x = x.contiguous()
+        sb, ss, sv = x.stride()
+    return x, (x.data_ptr(), _DTYPES[x.dtype], sb, ss, b, s, v, ids.data_ptr(), _lib.ptr(mask), t)
+
+
+# ---------------------------------------------------- log-probabilities --
+
+@functools.lru_cache(maxsize=256)
+def _logp_bytes(dtype: int, b: int, s: int, v: int) -> int:
+    return _lib.library().grpo_token_logprobs_workspace_bytes(dtype, b, s, v)
+
+
+def _grad_of(logits, ids, mask, t, stat: int, coef: int, scale) -> torch.Tensor:
+    """The logits' gradient, of the logits' shape (stat, coef: addresses)."""
+    x, rows = _rows(logits, ids, mask, t)
+    out = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
+    _run(x.device, "grpo_token_logprobs_backward", *rows, stat, coef, _lib.ptr(scale),
+         out.data_ptr())
     return out
 
 
-def _logprobs(rows: _Rows, entropy: bool, train: bool):
-    dev, n = rows.x.device, rows.b * rows.s
-    logp = torch.empty(rows.shape, dtype=torch.float32, device=dev)
-    ent = torch.empty(rows.shape, dtype=torch.float32, device=dev) if entropy else None
-    stat = torch.empty((n, 4), dtype=torch.float32, device=dev) if train else None
-    with _on(dev):
-        rc = _lib.device_library().grpo_token_logprobs(
-            *rows.args(), logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stat),
-            _lib.stream_handle(dev))
-    if rc:
-        _lib.check(rc, "grpo_token_logprobs")
+def _logprobs(logits, ids, mask, t, entropy: bool, train: bool):
+    x, rows = _rows(logits, ids, mask, t)
+    dev, (b, s, v) = x.device, x.shape
+    logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(logp) if entropy else None
+    stat = torch.empty((b * s, 4), dtype=torch.float32, device=dev) if train else None
+    nbytes = _logp_bytes(rows[1], b, s, v)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _run(dev, "grpo_token_logprobs", *rows, logp.data_ptr(), _lib.ptr(ent), _lib.ptr(stat),
+         _lib.ptr(ws), nbytes)
     return logp, ent, stat
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, token_ids, mask, temperature, entropy):
-        rows = _Rows(logits, token_ids, mask, temperature)
-        logp, ent, stat = _logprobs(rows, entropy, True)
-        ctx.save_for_backward(logits, rows.ids, rows.mask, stat)
-        ctx.temperature = rows.t
+    def forward(ctx, logits, ids, mask, t, entropy):
+        logp, ent, stat = _logprobs(logits, ids, mask, t, entropy, True)
+        ctx.save_for_backward(logits, ids, mask, stat)
+        ctx.t = t
+        ctx.set_materialize_grads(False)
         if ent is not None:
             ctx.mark_non_differentiable(ent)
         return logp, ent
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_logp, _):
+    @_once
+    def backward(ctx, grad, _):
+        if grad is None:
+            return None, None, None, None, None
         logits, ids, mask, stat = ctx.saved_tensors
-        rows = _Rows(logits, ids, mask, ctx.temperature)
-        grad = _float_rows(grad_logp, "grad", rows.shape)
-        return _grad_of(rows, stat, grad, None), None, None, None, None
+        grad = _float_rows(grad, "grad", ids.shape, ids.device)
+        return (_grad_of(logits, ids, mask, ctx.t, stat.data_ptr(), grad.data_ptr(), None), None,
+                None, None, None)
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
@@ -168,102 +194,98 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     Differentiable by ``logits``.  With ``return_entropy`` also the entropy of each
     position's distribution, which carries no gradient.  An id outside the vocabulary at a
     counted position gives NaN there."""
+    ids, mask, t = _check_logits(logits, token_ids, mask, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
-        logp, ent = _TokenLogprobs.apply(logits, token_ids, mask, temperature, return_entropy)
+        logp, ent = _TokenLogprobs.apply(logits, ids, mask, t, return_entropy)
     else:
-        logp, ent, _ = _logprobs(_Rows(logits, token_ids, mask, temperature), return_entropy,
-                                 False)
+        logp, ent, _ = _logprobs(logits, ids, mask, t, return_entropy, False)
     return (logp, ent) if return_entropy else logp
 
 
 # ------------------------------------------------------------ policy loss --
 
-def _policy(eps_low, eps_high, delta, beta, normalizer) -> _lib.Policy:
-    eps_low, eps_high, beta = float(eps_low), float(eps_high), float(beta)
-    cap = math.inf if delta is None else float(delta)
+@functools.lru_cache(maxsize=64)
+def _policy_of(eps_low: float, eps_high: float, cap: float, beta: float, normalizer):
     if not (0.0 <= eps_low < math.inf and 0.0 <= eps_high < math.inf):
         raise ValueError("eps_low and eps_high must be >= 0 and finite.")
     if not cap > 0.0:
-        raise ValueError(f"delta must be positive, got {delta}.")
+        raise ValueError(f"delta must be positive, got {cap}.")
     if not 0.0 <= beta < math.inf:
         raise ValueError(f"beta must be >= 0 and finite, got {beta}.")
     if isinstance(normalizer, str):
         if normalizer not in _NORMALIZERS:
             raise ValueError(f"normalizer must be 'tokens', 'sequences' or a number, got "
                              f"{normalizer!r}.")
-        return _lib.Policy(eps_low, eps_high, cap, beta, 1.0, _NORMALIZERS[normalizer])
-    denom = float(normalizer)
-    if not 0.0 < denom < math.inf:
+        return ctypes.byref(_lib.Policy(eps_low, eps_high, cap, beta, 1.0,
+                                        _NORMALIZERS[normalizer]))
+    if not 0.0 < normalizer < math.inf:
         raise ValueError(f"the normalizer must be positive and finite, got {normalizer}.")
-    return _lib.Policy(eps_low, eps_high, cap, beta, denom, 2)
+    return ctypes.byref(_lib.Policy(eps_low, eps_high, cap, beta, normalizer, 2))
 
 
-class _Tokens:
-    """Checked per-token inputs of the policy loss, and the C arguments they make."""
-
-    def __init__(self, device, shape, old_logps, ref_logps, advantages, mask):
-        if len(shape) != 2:
-            raise ValueError(f"positions must be [batch, seq], got {list(shape)}.")
-        _same_device(device, old_logps=old_logps, ref_logps=ref_logps, advantages=advantages,
-                     mask=mask)
-        self.old = _float_rows(old_logps, "old_logps", shape)
-        self.ref = _float_rows(ref_logps, "ref_logps", shape)
-        self.per_token = advantages.ndim == 2
-        self.adv = _float_rows(advantages, "advantages",
-                               shape if self.per_token else shape[:1])
-        self.mask = _mask_rows(mask, shape)
-        self.shape = tuple(shape)
-
-    def args(self):
-        return (_lib.ptr(self.old), _lib.ptr(self.ref), self.adv.data_ptr(), self.per_token)
-
-
-def _need_ref(beta: float, ref_logps) -> None:
+def _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps):
+    beta = float(beta)
+    policy = _policy_of(float(eps_low), float(eps_high),
+                        math.inf if delta is None else float(delta), beta,
+                        normalizer if isinstance(normalizer, str) else float(normalizer))
     if beta and ref_logps is None:
         raise ValueError("beta > 0 needs ref_logps.")
+    return policy
+
+
+def _check_tokens(shape, device, old_logps, ref_logps, advantages):
+    """(old, ref, advantages as float32, whether these are per token) that fit ``shape``."""
+    if len(shape) != 2:
+        raise ValueError(f"positions must be [batch, seq], got {list(shape)}.")
+    per_token = advantages.ndim == 2
+    return (_float_rows(old_logps, "old_logps", shape, device),
+            _float_rows(ref_logps, "ref_logps", shape, device),
+            _float_rows(advantages, "advantages", shape if per_token else shape[:1], device),
+            per_token)
+
+
+@functools.lru_cache(maxsize=256)
+def _policy_bytes(b: int, s: int) -> int:
+    return _lib.library().grpo_policy_loss_workspace_bytes(b, s)
+
+
+def _policy_loss(lp, tokens, mask, policy, train: bool):
+    old, ref, adv, per_token = tokens
+    dev, (b, s) = lp.device, lp.shape
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    metrics = torch.empty(4, dtype=torch.float32, device=dev)
+    # the float64 derivatives, where the backward wants them, then the workspace
+    keep = -(-8 * b * s // 256) * 256 if train else 0
+    nbytes = _policy_bytes(b, s)
+    buf = torch.empty(keep + nbytes, dtype=torch.uint8, device=dev)
+    at = buf.data_ptr()
+    _run(dev, "grpo_policy_loss", lp.data_ptr(), _lib.ptr(old), _lib.ptr(ref), adv.data_ptr(),
+         per_token, _lib.ptr(mask), b, s, policy, loss.data_ptr(), metrics.data_ptr(),
+         at if train else None, at + keep, nbytes)
+    return loss, metrics, buf
 
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logps, tokens, policy):
-        lp = _float_rows(logps, "logps", tokens.shape)
-        loss, metrics, ws = _policy_loss(lp, tokens, policy)
-        ctx.save_for_backward(logps, tokens.old, tokens.ref, tokens.adv, tokens.mask, ws)
-        ctx.per_token, ctx.policy = tokens.per_token, policy
+    def forward(ctx, logps, lp, tokens, mask, policy):
+        loss, metrics, ctx.coef = _policy_loss(lp, tokens, mask, policy, True)
+        ctx.shape, ctx.dtype = logps.shape, logps.dtype
+        ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(metrics)
         return loss, metrics
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_loss, _):
-        logps, old, ref, adv, mask, ws = ctx.saved_tensors
-        lp = _float_rows(logps, "logps", logps.shape)
-        g = grad_loss.to(torch.float32).contiguous()
-        out = torch.empty_like(lp)
-        b, s = lp.shape
-        with _on(lp.device):
-            rc = _lib.device_library().grpo_policy_loss_backward(
-                lp.data_ptr(), _lib.ptr(old), _lib.ptr(ref), adv.data_ptr(), ctx.per_token,
-                _lib.ptr(mask), b, s, ctypes.byref(ctx.policy), g.data_ptr(), out.data_ptr(),
-                ws.data_ptr(), ws.numel(), _lib.stream_handle(lp.device))
-        if rc:
-            _lib.check(rc, "grpo_policy_loss_backward")
-        return (out if out.dtype == logps.dtype else out.to(logps.dtype)), None, None
-
-
-def _policy_loss(lp, tokens, policy):
-    lib, dev, (b, s) = _lib.device_library(), lp.device, tokens.shape
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    metrics = torch.empty(4, dtype=torch.float32, device=dev)
-    nbytes = lib.grpo_policy_loss_workspace_bytes(b, s, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = lib.grpo_policy_loss(
-            lp.data_ptr(), *tokens.args(), _lib.ptr(tokens.mask), b, s, ctypes.byref(policy),
-            loss.data_ptr(), metrics.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_handle(dev))
-    if rc:
-        _lib.check(rc, "grpo_policy_loss")
-    return loss, metrics, ws
+        if grad_loss is None:
+            return None, None, None, None, None
+        if grad_loss.dtype != torch.float32:
+            grad_loss = grad_loss.float()
+        dev = grad_loss.device
+        out = torch.empty(ctx.shape, dtype=torch.float32, device=dev)
+        _run(dev, "grpo_policy_loss_backward", ctx.coef.data_ptr(), grad_loss.data_ptr(),
+             out.numel(), out.data_ptr())
+        return out if ctx.dtype == torch.float32 else out.to(ctx.dtype), None, None, None, None
 
 
 def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
@@ -287,52 +309,78 @@ def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
     gradient) are means over the counted tokens: r, the share whose gain no longer moves
     with r (clipped or capped), ``exp(q) - q - 1`` and ``old_logps - logps``.  With nothing
     counted, loss and metrics are 0."""
-    policy = _policy(eps_low, eps_high, delta, beta, normalizer)
-    _need_ref(policy.beta, ref_logps)
+    policy = _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps)
     if not logps.is_cuda:
         raise ValueError("logps must be on the ROCm/HIP device.")
-    tokens = _Tokens(logps.device, logps.shape, old_logps, ref_logps, advantages, mask)
+    shape, dev = logps.shape, logps.device
+    tokens = _check_tokens(shape, dev, old_logps, ref_logps, advantages)
+    mask = _mask_rows(mask, shape, dev)
+    lp = _float_rows(logps, "logps", shape, dev)
     if torch.is_grad_enabled() and logps.requires_grad:
-        return _PolicyLoss.apply(logps, tokens, policy)
-    loss, metrics, _ = _policy_loss(_float_rows(logps, "logps", logps.shape), tokens, policy)
-    return loss, metrics
+        return _PolicyLoss.apply(logps, lp, tokens, mask, policy)
+    return _policy_loss(lp, tokens, mask, policy, False)[:2]
+
+
+# ------------------------------------------------- the loss from logits --
+
+@functools.lru_cache(maxsize=256)
+def _logits_plan(dtype: int, b: int, s: int, v: int):
+    """(workspace bytes, whether a row stays in a workgroup's registers)."""
+    lib = _lib.library()
+    return (lib.grpo_policy_loss_logits_workspace_bytes(dtype, b, s, v),
+            bool(lib.grpo_policy_loss_logits_held(dtype, v)))
+
+
+def _logits_loss(logits, ids, mask, t, tokens, policy, train: bool):
+    old, ref, adv, per_token = tokens
+    x, rows = _rows(logits, ids, mask, t)
+    dev, (b, s, v) = x.device, x.shape
+    nbytes, held = _logits_plan(rows[1], b, s, v)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    metrics = torch.empty(4, dtype=torch.float32, device=dev)
+    logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
+    grad = torch.empty(logits.shape, dtype=x.dtype, device=dev) if train and held else None
+    # what the backward needs of each row (16 bytes of statistics, 4 of its derivative), then
+    # the workspace
+    keep = -(-20 * b * s // 256) * 256 if train else 0
+    buf = torch.empty(keep + nbytes, dtype=torch.uint8, device=dev)
+    at = buf.data_ptr()
+    _run(dev, "grpo_policy_loss_logits", *rows, _lib.ptr(old), _lib.ptr(ref), adv.data_ptr(),
+         per_token, policy, loss.data_ptr(), logp.data_ptr(), metrics.data_ptr(),
+         at if train else None, at + 16 * b * s if train else None, _lib.ptr(grad), at + keep,
+         nbytes)
+    return loss, logp, metrics, buf, grad
 
 
 class _LogitsLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, rows, tokens, policy):
-        loss, logp, metrics, stat, coef = _logits_loss(rows, tokens, policy, True)
-        ctx.save_for_backward(logits, rows.ids, rows.mask, stat, coef)
-        ctx.temperature = rows.t
+    def forward(ctx, logits, ids, mask, t, tokens, policy):
+        loss, logp, metrics, ctx.buf, ctx.grad = _logits_loss(logits, ids, mask, t, tokens,
+                                                              policy, True)
+        ctx.save_for_backward(logits, ids, mask)
+        ctx.t = t
         ctx.mark_non_differentiable(logp, metrics)
+        ctx.set_materialize_grads(False)
         return loss, logp, metrics
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_loss, *_):
-        logits, ids, mask, stat, coef = ctx.saved_tensors
-        rows = _Rows(logits, ids, mask, ctx.temperature)
-        g = grad_loss.to(torch.float32).contiguous()
-        return _grad_of(rows, stat, coef, g), None, None, None
-
-
-def _logits_loss(rows: _Rows, tokens: _Tokens, policy, train: bool):
-    lib, dev, n = _lib.device_library(), rows.x.device, rows.b * rows.s
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    metrics = torch.empty(4, dtype=torch.float32, device=dev)
-    logp = torch.empty(rows.shape, dtype=torch.float32, device=dev)
-    stat = torch.empty((n, 4), dtype=torch.float32, device=dev) if train else None
-    coef = torch.empty(n, dtype=torch.float32, device=dev) if train else None
-    nbytes = lib.grpo_policy_loss_workspace_bytes(rows.b, rows.s, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = lib.grpo_policy_loss_logits(
-            *rows.args(), *tokens.args(), ctypes.byref(policy), loss.data_ptr(), logp.data_ptr(),
-            metrics.data_ptr(), _lib.ptr(stat), _lib.ptr(coef), ws.data_ptr(), nbytes,
-            _lib.stream_handle(dev))
-    if rc:
-        _lib.check(rc, "grpo_policy_loss_logits")
-    return loss, logp, metrics, stat, coef
+        if grad_loss is None:
+            return None, None, None, None, None, None
+        logits, ids, mask = ctx.saved_tensors
+        if grad_loss.dtype != torch.float32:
+            grad_loss = grad_loss.float()
+        stat = ctx.buf.data_ptr()
+        coef = stat + 16 * ids.numel()
+        grad, ctx.grad = ctx.grad, None  # handed out once: it is the caller's from here on
+        if grad is None:
+            grad = _grad_of(logits, ids, mask, ctx.t, stat, coef, grad_loss)
+        else:
+            x, rows = _rows(logits, ids, mask, ctx.t)
+            _run(x.device, "grpo_policy_loss_logits_rescale", *rows, stat, coef,
+                 grad_loss.data_ptr(), grad.data_ptr())
+        return grad, None, None, None, None, None
 
 
 def fused_grpo_loss(logits: torch.Tensor, token_ids: torch.Tensor,
@@ -346,17 +394,17 @@ def fused_grpo_loss(logits: torch.Tensor, token_ids: torch.Tensor,
 
     ``logits [batch, seq, V]``; the other arguments are those of the two operators.
     Differentiable by ``logits`` alone; ``logps`` (float32, 0 where not counted) and
-    ``metrics`` carry no gradient."""
-    policy = _policy(eps_low, eps_high, delta, beta, normalizer)
-    _need_ref(policy.beta, ref_logps)
+    ``metrics`` carry no gradient.  Rows of up to 311296 bytes are read once: their gradient
+    is made with the loss, for an upstream gradient of 1, and the backward hands it out (or
+    computes it again where the upstream gradient is another, and for a second backward)."""
+    policy = _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps)
     if logits.ndim != 3:
         raise ValueError(f"logits must be [batch, seq, vocab], got {list(logits.shape)}.")
-    rows = _Rows(logits, token_ids, mask, temperature)
-    tokens = _Tokens(logits.device, rows.shape, old_logps, ref_logps, advantages, rows.mask)
+    ids, mask, t = _check_logits(logits, token_ids, mask, temperature)
+    tokens = _check_tokens(ids.shape, logits.device, old_logps, ref_logps, advantages)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _LogitsLoss.apply(logits, rows, tokens, policy)
-    loss, logp, metrics, _, _ = _logits_loss(rows, tokens, policy, False)
-    return loss, logp, metrics
+        return _LogitsLoss.apply(logits, ids, mask, t, tokens, policy)
+    return _logits_loss(logits, ids, mask, t, tokens, policy, False)[:3]
 
 
 __all__ = ["token_logprobs", "grpo_policy_loss", "fused_grpo_loss"]

@@ -99,15 +99,18 @@ int grpo_nf4_grad_x(const void* grad, int64_t ldg, const uint8_t* w, const float
  * log-probability half of _fused_grpo_loss_kernel (src/triton_kernels/grpo_loss.py:47-139).
  *   logp    : float32 [R]
  *   entropy : float32 [R], -sum_v p_v log p_v, or NULL
- *   stat    : float32 [R][4] for grpo_token_logprobs_backward, 16-byte aligned, or NULL */
+ *   stat    : float32 [R][4] for grpo_token_logprobs_backward, 16-byte aligned, or NULL
+ *   workspace : few long rows are cut over several workgroups; 0 bytes otherwise */
+size_t grpo_token_logprobs_workspace_bytes(int dtype, int B, int S, int V);
 int grpo_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t stride_s, int B,
-                        int S, int V, const int64_t* ids, const uint8_t* mask, float temperature,
-                        float* logp, float* entropy, float* stat, grpo_stream_t stream);
+                        int S, int V, const int64_t* ids, const uint8_t* mask, double temperature,
+                        float* logp, float* entropy, float* stat, void* workspace,
+                        size_t workspace_bytes, grpo_stream_t stream);
 /* grad_logits[r][v] = g / T * (1[v = id] - p_v), g = grad_logp[r] * *scale (scale: one
  * float32 on the device, or NULL: 1); grad_logits [R][V] contiguous, in the logits' type. */
 int grpo_token_logprobs_backward(const void* logits, int dtype, int64_t stride_b,
                                  int64_t stride_s, int B, int S, int V, const int64_t* ids,
-                                 const uint8_t* mask, float temperature, const float* stat,
+                                 const uint8_t* mask, double temperature, const float* stat,
                                  const float* grad_logp, const float* scale, void* grad_logits,
                                  grpo_stream_t stream);
 
@@ -124,36 +127,46 @@ typedef struct {
   int normalizer;
 } grpo_policy_t;
 
-/* Workspace bytes of the entry points below (from_logits: grpo_policy_loss_logits). */
-size_t grpo_policy_loss_workspace_bytes(int B, int S, int from_logits);
+size_t grpo_policy_loss_workspace_bytes(int B, int S);
 /*   logp, old_logp, ref_logp : float32 [R]; old_logp NULL: logp itself; ref_logp NULL: no
  *                              KL term
  *   advantages : float32 [B], or [R] (adv_tokens != 0)
  *   loss       : float32 [1]
  *   metrics    : float32 [4], means over the counted tokens: r, tokens whose gain no
  *                longer follows r, the KL term exp(q) - q - 1, old - logp
+ *   coef       : float64 [R], d loss / d logp, or NULL
  * Nothing counted: loss and metrics are 0. */
 int grpo_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
                      const float* advantages, int adv_tokens, const uint8_t* mask, int B, int S,
-                     const grpo_policy_t* policy, float* loss, float* metrics, void* workspace,
-                     size_t workspace_bytes, grpo_stream_t stream);
-/* grad_logp[r] = *grad_loss * d loss / d logp[r], float32 [R]; the workspace is the one
- * that grpo_policy_loss filled for the same mask. */
-int grpo_policy_loss_backward(const float* logp, const float* old_logp, const float* ref_logp,
-                              const float* advantages, int adv_tokens, const uint8_t* mask, int B,
-                              int S, const grpo_policy_t* policy, const float* grad_loss,
-                              float* grad_logp, void* workspace, size_t workspace_bytes,
-                              grpo_stream_t stream);
+                     const grpo_policy_t* policy, float* loss, float* metrics, double* coef,
+                     void* workspace, size_t workspace_bytes, grpo_stream_t stream);
+/* grad_logp[r] = coef[r] * *grad_loss, float32 [tokens]. */
+int grpo_policy_loss_backward(const double* coef, const float* grad_loss, int64_t tokens,
+                              float* grad_logp, grpo_stream_t stream);
 /* Both in one (fused_grpo_loss, src/triton_kernels/grpo_loss.py:571-625): logp, loss and
  * metrics from the logits; stat [R][4] and coef [R] (both or neither) are what
  * grpo_token_logprobs_backward takes as stat and grad_logp, with the loss's gradient as
- * its scale. */
+ * its scale.
+ *   grad_logits : [R][V] contiguous, in the logits' type, or NULL: the gradient of the loss
+ *                 itself (its upstream gradient 1), made in the same pass over the logits;
+ *                 needs stat and coef and a vocabulary that grpo_policy_loss_logits_held
+ *                 takes (a row stays in one workgroup's registers) */
+size_t grpo_policy_loss_logits_workspace_bytes(int dtype, int B, int S, int V);
 int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b, int64_t stride_s,
                             int B, int S, int V, const int64_t* ids, const uint8_t* mask,
-                            float temperature, const float* old_logp, const float* ref_logp,
+                            double temperature, const float* old_logp, const float* ref_logp,
                             const float* advantages, int adv_tokens, const grpo_policy_t* policy,
                             float* loss, float* logp, float* metrics, float* stat, float* coef,
-                            void* workspace, size_t workspace_bytes, grpo_stream_t stream);
+                            void* grad_logits, void* workspace, size_t workspace_bytes,
+                            grpo_stream_t stream);
+int grpo_policy_loss_logits_held(int dtype, int V);
+/* grad_logits of the call above for an upstream gradient *grad_loss: left as it is where
+ * that is 1, computed again from the logits otherwise (decided on the device). */
+int grpo_policy_loss_logits_rescale(const void* logits, int dtype, int64_t stride_b,
+                                    int64_t stride_s, int B, int S, int V, const int64_t* ids,
+                                    const uint8_t* mask, double temperature, const float* stat,
+                                    const float* coef, const float* grad_loss, void* grad_logits,
+                                    grpo_stream_t stream);
 
 /* Dropout with a mask that is never stored: y[e] = dt(x[e] * scale), 0 where dropped.
  * Element e is dropped iff u(e) < t, t = round(65536 p), where u(e) are 16 bits of the

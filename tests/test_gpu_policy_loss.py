@@ -127,8 +127,9 @@ def test_an_offset_of_all_logits_changes_nothing(dev):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_masked_vocabulary_and_lowest_values(dev, dtype):
-    x, ids, _ = make(6, 777, dtype, seed=9, counted=1.1)
+@pytest.mark.parametrize("vocab", [777, 50257])
+def test_masked_vocabulary_and_lowest_values(dev, dtype, vocab):
+    x, ids, _ = make(6, vocab, dtype, seed=9, counted=1.1)
     low = torch.finfo(x.dtype).min
     x[0, 100:] = -math.inf
     ids[0] = 3
@@ -156,8 +157,9 @@ def test_masked_vocabulary_and_lowest_values(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_values_that_are_not_finite(dev, dtype):
-    x, ids, mask = make(6, 1030, dtype, seed=4, counted=1.1)
+@pytest.mark.parametrize("vocab", [1030, 70001])  # one workgroup a row, and several
+def test_values_that_are_not_finite(dev, dtype, vocab):
+    x, ids, mask = make(6, vocab, dtype, seed=4, counted=1.1)
     x[0] = -math.inf                # nothing left: NaN, as a log-softmax
     x[1, 7] = math.inf
     x[2, 900] = math.nan
@@ -167,7 +169,7 @@ def test_values_that_are_not_finite(dev, dtype):
     ids[3], ids[4] = -100, 10 ** 12
     leaf = x.to(dev).requires_grad_()
     got, ent = _ops().token_logprobs(leaf, ids.to(dev), mask.to(dev), return_entropy=True)
-    want = torch.log_softmax(x.double(), -1)[torch.arange(6), ids.clamp(0, 1029)]
+    want = torch.log_softmax(x.double(), -1)[torch.arange(6), ids.clamp(0, vocab - 1)]
     g = got.detach().cpu()
     assert torch.isnan(g[:3]).all() and torch.isnan(want[:3]).all()
     assert g[3] == g[4] == 0 and ent[3] == ent[4] == 0
@@ -176,6 +178,24 @@ def test_values_that_are_not_finite(dev, dtype):
     assert torch.isnan(grad[:3]).any(1).all()
     assert not grad[3:5].any()
     assert torch.isfinite(grad[5]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [100.0, 900.0, 20000.0])
+def test_gradients_of_large_logits(dev, dtype, size):
+    """Whatever their size: below and beyond where 16-bit gradients go by vectors."""
+    x, ids, mask = make(5, 4096, "f32", seed=7, counted=1.1)
+    x = (x + size).to(DT[dtype])
+    logp, ent, p, tol, _ = bounds(x, ids, mask, 0.7)
+    coef = torch.tensor([1.0, -2.0, 0.5, 3.0, -0.25])
+    leaf = x.to(dev).requires_grad_()
+    got = _ops().token_logprobs(leaf, ids.to(dev), temperature=0.7)
+    within(got, logp, tol)
+    grad, = torch.autograd.grad(got, leaf, coef.to(dev))
+    want = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy(), 0.7)
+    # by vectors the exponent is off by 2^-13 of the value at most
+    extra = 0.0 if dtype == "f32" else 2.0 ** -13 * np.abs(coef.numpy() / 0.7)[:, None] * p
+    within(grad, want, grad_bound(want, p, coef.double().numpy(), 0.7, dtype) + extra)
 
 
 def test_ids_outside_the_vocabulary_give_nan(dev):
@@ -272,7 +292,7 @@ def close(got, want, scale, n):
 
 
 @pytest.mark.parametrize("b, s", [(1, 1), (3, 1), (1, 257), (5, 333), (64, 200), (700, 3),
-                                  (2, 40000)])
+                                  (1500, 2), (2, 40000)])
 @pytest.mark.parametrize("normalizer", ["tokens", "sequences", 1234.5])
 @pytest.mark.parametrize("beta, delta", [(0.0, None), (0.04, 1.5)])
 def test_policy_loss_and_gradient(dev, b, s, normalizer, beta, delta):
@@ -391,7 +411,7 @@ def loss_inputs(b, s, vocab, dtype, seed, t=1.0, beta=0.04):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("b, s, vocab", [(1, 1, 9), (3, 5, 1000), (4, 33, 4097), (2, 3, 151936),
+@pytest.mark.parametrize("b, s, vocab", [(1, 1, 9), (300, 30, 65), (1100, 1, 17), (3, 5, 1000), (4, 33, 4097), (2, 3, 151936),
                                          (1, 2, 262147), (40, 16, 300)])
 @pytest.mark.parametrize("normalizer, t, beta", [("tokens", 1.0, 0.0), ("sequences", 0.7, 0.04)])
 def test_fused_loss_and_gradient(dev, dtype, b, s, vocab, normalizer, t, beta):
@@ -440,7 +460,7 @@ def test_fused_loss_is_its_parts(dev):
     assert torch.equal(parts.detach(), lp)
     loss2, metrics2 = _ops().grpo_policy_loss(parts, put(old), put(adv), put(mask), **kw)
     tol = 16 * E * float(np.abs(logp).max())
-    assert abs(float(loss) - float(loss2)) <= tol
+    assert abs(float(loss.detach()) - float(loss2.detach())) <= tol
     assert torch.allclose(metrics, metrics2, rtol=4 * E, atol=tol)
     loss.backward()
     loss2.backward()

@@ -37,23 +37,37 @@ def test_policy_parameters_are_refused(kw, message):
 
 
 def test_shapes_of_the_tokens_are_refused():
-    dev, shape = torch.device("cpu"), (2, 3)
-    make = policy_loss._Tokens
-    good = torch.zeros(2)
+    dev, shape = torch.device("cpu"), torch.Size((2, 3))
+
+    def make(old=None, ref=None, adv=torch.zeros(2), shape=shape):
+        return policy_loss._check_tokens(shape, dev, old, ref, adv)
+
     with pytest.raises(ValueError, match="positions"):
-        make(dev, (2, 3, 4), None, None, good, None)
+        make(shape=torch.Size((2, 3, 4)))
     with pytest.raises(ValueError, match="old_logps must be"):
-        make(dev, shape, torch.zeros(2, 4), None, good, None)
+        make(old=torch.zeros(2, 4))
     with pytest.raises(ValueError, match="ref_logps must be a floating"):
-        make(dev, shape, None, torch.zeros(2, 3, dtype=torch.int64), good, None)
-    with pytest.raises(ValueError, match="advantages must be"):
-        make(dev, shape, None, None, torch.zeros(3), None)
-    with pytest.raises(ValueError, match="advantages must be"):
-        make(dev, shape, None, None, torch.zeros(3, 2), None)
+        make(ref=torch.zeros(2, 3, dtype=torch.int64))
+    for adv in (torch.zeros(3), torch.zeros(3, 2), torch.zeros(2, 3, 1), torch.zeros(())):
+        with pytest.raises(ValueError, match="advantages must be"):
+            make(adv=adv)
     with pytest.raises(ValueError, match="mask must be"):
-        make(dev, shape, None, None, good, torch.ones(3, 2, dtype=torch.bool))
-    with pytest.raises(ValueError, match="must be on cpu"):
-        make(dev, shape, None, None, torch.zeros(2, device="meta"), None)
+        policy_loss._mask_rows(torch.ones(3, 2, dtype=torch.bool), shape, dev)
+    for name in ("old", "ref", "adv"):
+        with pytest.raises(ValueError, match="must be on cpu"):
+            make(**{name: torch.zeros(2 if name == "adv" else shape, device="meta")})
+
+
+def test_policy_parameters_are_read_at_every_call():
+    """The parameters kept for equal arguments are those of the values, not of a tensor."""
+    n = torch.tensor(4.0)
+    args = (0.2, 0.2, None, 0.0)
+    four = policy_loss._policy(*args, n, None)._obj
+    n.fill_(8.0)
+    eight = policy_loss._policy(*args, n, None)._obj
+    assert (four.denom, eight.denom) == (4.0, 8.0)
+    assert policy_loss._policy(*args, 8, None)._obj.normalizer == 2
+    assert policy_loss._policy(*args, "sequences", None)._obj.normalizer == 1
 
 
 @pytest.mark.parametrize("p", [-0.1, 1.0, math.nan, 1 - 2 ** -18])
@@ -82,7 +96,8 @@ def lib():
 
 
 def _rows(lib, dtype=0, sb=8, ss=8, b=2, s=3, v=8, ids=FAKE, t=1.0, x=FAKE, logp=FAKE, stat=FAKE):
-    return lib.grpo_token_logprobs(x, dtype, sb, ss, b, s, v, ids, None, t, logp, None, stat, None)
+    return lib.grpo_token_logprobs(x, dtype, sb, ss, b, s, v, ids, None, t, logp, None, stat, None,
+                                   0, None)
 
 
 @pytest.mark.parametrize("kw", [
@@ -92,6 +107,36 @@ def _rows(lib, dtype=0, sb=8, ss=8, b=2, s=3, v=8, ids=FAKE, t=1.0, x=FAKE, logp
 ])
 def test_c_entry_refuses_logits(lib, kw):
     assert _rows(lib, **kw) == -1, lib.grpo_last_error()
+
+
+def test_c_entry_wants_a_workspace_where_rows_are_cut(lib):
+    need = lib.grpo_token_logprobs_workspace_bytes(0, 8, 1, 151936)
+    assert need > 0
+    for rows, vocab in ((4096, 151936), (8, 2000)):  # enough rows; short ones
+        assert lib.grpo_token_logprobs_workspace_bytes(0, rows, 1, vocab) == 0
+    args = (FAKE, 0, 151936, 0, 8, 1, 151936, FAKE, None, 1.0, FAKE, None, None)
+    assert lib.grpo_token_logprobs(*args, None, need, None) == -1
+    assert lib.grpo_token_logprobs(*args, FAKE + 8, need, None) == -1
+    assert lib.grpo_token_logprobs(*args, FAKE, need - 1, None) == -3
+
+
+def test_rows_that_stay_in_registers(lib):
+    held = lib.grpo_policy_loss_logits_held
+    assert [held(0, v) for v in (1, 151936, 152064, 155648, 155649, 0)] == [1, 1, 1, 1, 0, 0]
+    assert [held(2, v) for v in (50257, 77824, 77825)] == [1, 1, 0] and held(3, 8) == 0
+
+
+def test_c_entry_refuses_a_gradient_it_cannot_make(lib):
+    need = 1 << 30
+
+    def go(v, stat, coef, grad):
+        return lib.grpo_policy_loss_logits(
+            FAKE, 0, v, v, 2, 3, v, FAKE, None, 1.0, None, None, FAKE, 0, ctypes.byref(_policy()),
+            FAKE, FAKE, FAKE, stat, coef, grad, FAKE, need, None)
+
+    assert go(8, FAKE, None, None) == -1 and go(8, FAKE + 4, FAKE, None) == -1
+    assert go(8, None, None, FAKE) == -1  # no place for the statistics
+    assert go(160000, FAKE, FAKE, FAKE) == -1 and go(8, FAKE, FAKE, FAKE + 1) == -1
 
 
 def test_c_entry_with_no_rows_does_nothing(lib):
@@ -109,8 +154,8 @@ def _policy(**kw):
 
 def _loss(lib, policy, logp=FAKE, adv=FAKE, b=2, s=3, ws=FAKE, nbytes=1 << 20):
     return lib.grpo_policy_loss(logp, None, None, adv, 0, None, b, s,
-                                None if policy is None else ctypes.byref(policy), FAKE, FAKE, ws,
-                                nbytes, None)
+                                None if policy is None else ctypes.byref(policy), FAKE, FAKE, None,
+                                ws, nbytes, None)
 
 
 @pytest.mark.parametrize("kw", [
@@ -127,8 +172,8 @@ def test_c_entry_refuses_buffers(lib):
     assert _loss(lib, _policy(), adv=None) == -1
     assert _loss(lib, _policy(), ws=None) == -1
     assert _loss(lib, _policy(), ws=FAKE + 8) == -1
-    need = lib.grpo_policy_loss_workspace_bytes(2, 3, 0)
-    assert 0 < need <= lib.grpo_policy_loss_workspace_bytes(2, 3, 1)
+    need = lib.grpo_policy_loss_workspace_bytes(2, 3)
+    assert 0 < need <= lib.grpo_policy_loss_logits_workspace_bytes(0, 2, 3, 8)
     assert _loss(lib, _policy(), nbytes=need - 1) == -3
     assert _loss(lib, _policy(), b=1 << 16, s=1 << 16) == -1
 
