@@ -57,9 +57,19 @@ __device__ __forceinline__ float exponent(float x, float khi, float klo, float M
 using Policy = grpo_policy_t;
 
 template <int DT>
+using Raw = std::conditional_t<DT == F32, float, uint16_t>;
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const void* x, int64_t i) {
+  return static_cast<const Raw<DT>*>(x)[i];
+}
+template <int DT>
+__device__ __forceinline__ float to_float(Raw<DT> v) {
+  if constexpr (DT == F32) return v;
+  else return e2f<DT == F16>(v);
+}
+template <int DT>
 __device__ __forceinline__ float load1(const void* x, int64_t i) {
-  if (DT == F32) return static_cast<const float*>(x)[i];
-  return e2f<DT == F16>(static_cast<const uint16_t*>(x)[i]);
+  return to_float<DT>(load_raw<DT>(x, i));
 }
 template <int DT>
 __device__ __forceinline__ void store1(void* x, int64_t i, float v) {
@@ -142,15 +152,36 @@ struct Sums {
   }
 };
 
+// Over the 64 lanes of a wave, every lane gets the result (as wave_sum_dpp).
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
+  v = fmaxf(v, dpp_move<0xB1>(v));
+  v = fmaxf(v, dpp_move<0x4E>(v));
+  v = fmaxf(v, dpp_move<0x141>(v));
+  v = fmaxf(v, dpp_move<0x140>(v));
+  return pair32_max(pair16_max(v));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_move64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+  v += dpp_move64<0xB1>(v);
+  v += dpp_move64<0x4E>(v);
+  v += dpp_move64<0x141>(v);
+  v += dpp_move64<0x140>(v);
+  uint64_t u = __builtin_bit_cast(uint64_t, v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  v = __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+      __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+  u = __builtin_bit_cast(uint64_t, v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+         __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
 }
 
 struct Joined {  // of a workgroup, the same in every thread
@@ -163,29 +194,40 @@ struct JoinSpace {
   float M[NT / 64];
 };
 
+// A wave's sums against the largest M among its lanes.
+template <bool ENT>
+__device__ __forceinline__ Joined join_wave(float M, double S, double t) {
+  const float top = wave_max(M);
+  const int by = shift(M - top);
+  return Joined{top, wave_sum64(ldexp(S, by)),
+                ENT ? wave_sum64(ldexp(t + (double)(M - top) * S, by)) : 0.0};
+}
+// The waves' sums into LDS ...
+template <bool ENT, int NT>
+__device__ __forceinline__ void leave(const Sums<ENT>& s, JoinSpace<NT>& red) {
+  const Joined w = join_wave<ENT>(s.M, s.S, s.t);
+  if ((threadIdx.x & 63) == 0) {
+    red.M[threadIdx.x >> 6] = w.M;
+    red.S[threadIdx.x >> 6] = w.S;
+    if (ENT) red.t[threadIdx.x >> 6] = w.t;
+  }
+}
+// ... and joined by any wave, a lane each, after a barrier.
+template <bool ENT, int NT>
+__device__ __forceinline__ Joined gather(const JoinSpace<NT>& red) {
+  const int l = threadIdx.x & 63;
+  const bool in = l < NT / 64;
+  return join_wave<ENT>(in ? red.M[l] : LOWEST, in ? red.S[l] : 0.0, in && ENT ? red.t[l] : 0.0);
+}
 template <bool ENT, int NT>
 __device__ __forceinline__ Joined join(const Sums<ENT>& s, JoinSpace<NT>& red) {
-  const float M = wave_max(s.M);
-  const int by = shift(s.M - M);
-  const double S = wave_sum64(ldexp(s.S, by));
-  const double t = ENT ? wave_sum64(ldexp(s.t + (double)(s.M - M) * s.S, by)) : 0.0;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red.M[threadIdx.x >> 6] = M;
-    red.S[threadIdx.x >> 6] = S;
-    if (ENT) red.t[threadIdx.x >> 6] = t;
-  }
+  leave<ENT, NT>(s, red);
   __syncthreads();
-  Joined j{red.M[0], 0.0, 0.0};
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) j.M = fmaxf(j.M, red.M[w]);
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) {
-    const int b = shift(red.M[w] - j.M);
-    j.S += ldexp(red.S[w], b);
-    if (ENT) j.t += ldexp(red.t[w] + (double)(red.M[w] - j.M) * red.S[w], b);
-  }
-  return j;
+  return gather<ENT, NT>(red);
+}
+__device__ __forceinline__ bool usable(const Joined& j) {
+  return j.S > 0.0 && j.S < (double)INFINITY;
 }
 
 template <int NT>
@@ -285,7 +327,7 @@ __device__ __forceinline__ Joined row_stat(const Sums<ENT>& s, const void* row, 
                                            JoinSpace<NT>& red, RowStat* st) {
   Joined j = join<ENT, NT>(s, red);
   float m = 0.f;
-  if (!(j.S > 0.0 && j.S < (double)INFINITY)) {
+  if (!usable(j)) {
     const PlainStat ps =
         plain_stat<DT, ENT, NT>(row, q.V, q.khi, reinterpret_cast<float*>(&red));
     j = Joined{INFINITY, ps.S, ps.t};
@@ -295,20 +337,20 @@ __device__ __forceinline__ Joined row_stat(const Sums<ENT>& s, const void* row, 
   return j;
 }
 
-// logp of the row's token; NaN for an id outside the vocabulary.
+// The row's value at its token; NaN for an id outside the vocabulary.
 template <int DT>
-__device__ __forceinline__ double row_logp(const void* row, int64_t id, const Rows& q,
-                                           const Joined& j, float m) {
-  if (id < 0 || id >= q.V) return __builtin_nan("");
-  const double x = load1<DT>(row, id);
-  const double a = j.M < INFINITY ? fma(x, q.k, -(double)j.M)
-                                  : (x - (double)m) * (double)q.khi;
-  return LN2 * (a - log2(j.S));
+__device__ __forceinline__ float row_at_id(const void* row, int64_t id, int V) {
+  return id < 0 || id >= V ? __builtin_nanf("") : load1<DT>(row, id);
+}
+// Its exponent: logp is ln 2 (this - log2 S).
+__device__ __forceinline__ double id_exponent(float x, const Rows& q, const Joined& j, float m) {
+  return j.M < INFINITY ? fma((double)x, q.k, -(double)j.M)
+                        : ((double)x - (double)m) * (double)q.khi;
 }
 
 template <int DT>
 __device__ __forceinline__ const void* row_at(const Rows& q, int64_t r) {
-  const int64_t b = r / q.S, s = r - b * q.S;
+  const uint32_t b = (uint32_t)r / (uint32_t)q.S, s = (uint32_t)r - b * q.S;  // < 2^22 rows
   return static_cast<const char*>(q.x) + (b * q.sb + s * q.ss) * SIZE<DT>;
 }
 
@@ -324,7 +366,8 @@ struct LogpOut {
 template <int DT, bool ENT>
 __device__ __forceinline__ void write_logp(const LogpOut& o, int64_t r, const void* row,
                                            const Rows& q, const Joined& j, const RowStat& st) {
-  const double lp = row_logp<DT>(row, q.ids[r], q, j, st.m);
+  const double lp =
+      LN2 * (id_exponent(row_at_id<DT>(row, q.ids[r], q.V), q, j, st.m) - log2(j.S));
   if (o.logp64) o.logp64[r] = lp;
   o.logp[r] = (float)lp;
   if (ENT) o.entropy[r] = (float)(LN2 * (log2(j.S) - j.t / j.S));
@@ -513,6 +556,15 @@ __global__ void __launch_bounds__(NT) logits_grad_kernel(Rows q, int R, const Ro
 
 // ------------------------------------------------------------- policy loss --
 
+// What a token counts, by sequence: with n_b counted tokens in sequence b, n in all and B'
+// sequences with some, 1 / n, 1 / (n_b B') or 1 / denom.
+__device__ __forceinline__ double token_weight(const Policy& p, int in_row, double tokens,
+                                               double seqs) {
+  if (p.normalizer == 0) return 1.0 / tokens;
+  if (p.normalizer == 1) return 1.0 / (in_row * seqs);
+  return 1.0 / p.denom;
+}
+
 // Counted tokens of each sequence.
 __global__ void __launch_bounds__(256) count_kernel(const uint8_t* mask, int S, int* counts) {
   __shared__ JoinSpace<256> red;
@@ -523,8 +575,9 @@ __global__ void __launch_bounds__(256) count_kernel(const uint8_t* mask, int S, 
   if (threadIdx.x == 0) counts[blockIdx.x] = (int)all;
 }
 
-// Batches small enough for every workgroup to count for itself, in its LDS.
-constexpr int SMALL_TOKENS = 8192, SMALL_BATCH = 1024;
+// A batch of at most SMALL_TOKENS tokens in SMALL_BATCH sequences is counted by one workgroup,
+// in its LDS: one launch instead of two.
+constexpr int SMALL_BATCH = 1024, SMALL_TOKENS = 4096;
 
 // counts[b] for a small batch: 64 positions a wave, one addition for them where they are of
 // one sequence.
@@ -547,14 +600,57 @@ __device__ __forceinline__ void count_small(const uint8_t* mask, int B, int S, i
   __syncthreads();
 }
 
+// Counted tokens and sequences of the batch, the same in every thread.
+template <int NT_>
+__device__ __forceinline__ void totals(const int* counts, int B, double* red, double* tokens,
+                                       double* seqs) {
+  double n = 0.0, q = 0.0;
+  for (int b = threadIdx.x; b < B; b += NT_) {
+    const int c = counts[b];
+    n += c;
+    q += c > 0;
+  }
+  n = wave_sum64(n);
+  q = wave_sum64(q);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = n;
+    red[NT_ / 64 + (threadIdx.x >> 6)] = q;
+  }
+  __syncthreads();
+  n = q = 0.0;
+  for (int w = 0; w < NT_ / 64; ++w) {
+    n += red[w];
+    q += red[NT_ / 64 + w];
+  }
+  *tokens = n;
+  *seqs = q;
+}
+
+// weights[b] of each sequence, and weights[B] = n, for the launches that follow.
+template <bool SMALL>
+__global__ void __launch_bounds__(1024) weight_kernel(Policy p, const uint8_t* mask, int B, int S,
+                                                      const int* counts, double* weights) {
+  __shared__ double red[2 * 16];
+  __shared__ int own[SMALL ? SMALL_BATCH : 1];
+  if (SMALL) count_small<1024>(mask, B, S, own);
+  const int* const n = SMALL ? own : counts;
+  double tokens, seqs;
+  totals<1024>(n, B, red, &tokens, &seqs);
+  for (int b = threadIdx.x; b < B; b += 1024) weights[b] = token_weight(p, n[b], tokens, seqs);
+  if (threadIdx.x == 0) weights[B] = tokens;
+}
+
 struct Tokens {
-  const double* logp64;  // [R], or null: logp
-  const float* logp;     // [R]
+  const double* logp64;  // [R], or null
+  const double2* parts;  // [R] (the token's exponent, S), or null: logp is made of them
+  float* logp;           // [R]: read where both are null, written where parts are given
   const float* old;      // [R] or null: logp itself
   const float* ref;      // [R] or null
   const float* adv;      // [B], or [R] (adv_tokens)
   const uint8_t* mask;   // [R] or null
-  const int* counts;     // [B], or null: S each (no mask), or to be counted (a small batch)
+  const double* weights; // [B + 1], or null: no mask, all of `weight`
+  double weight;
   int B, S;
   bool adv_tokens;
 };
@@ -598,46 +694,44 @@ __device__ __forceinline__ void totals(const int* counts, int B, int S, double* 
   *seqs = q;
 }
 
-__device__ __forceinline__ double token_weight(const Policy& p, int in_row, double tokens,
-                                               double seqs) {
-  if (p.normalizer == 0) return 1.0 / tokens;
-  if (p.normalizer == 1) return 1.0 / (in_row * seqs);
-  return 1.0 / p.denom;
+// One token of ratio r and eq = exp(ref - logp): d l / d logp.
+struct Slope {
+  double d, gain;
+  bool follows;  // the smaller gain moves with r
+};
+__device__ __forceinline__ Slope token_slope(const Policy& p, double r, double a, bool has_ref,
+                                             double eq) {
+  const double lo = 1.0 - p.eps_low, hi = 1.0 + p.eps_high;
+  const double clipped = fmin(fmax(r, lo), hi);
+  const double free_gain = fmin(r, p.delta) * a, clip_gain = clipped * a;
+  Slope s;
+  s.follows = (free_gain <= clip_gain && r <= p.delta) ||
+              (clip_gain <= free_gain && clipped == r);
+  s.gain = fmin(free_gain, clip_gain);
+  s.d = s.follows ? -r * a : 0.0;
+  if (r != r || a != a) s.d = s.gain = r * a;  // fmin would hide a NaN
+  if (has_ref) s.d += p.beta * (1.0 - eq);
+  return s;
 }
 
-// One counted token: d loss / d logp, its terms added to s.
-__device__ __forceinline__ double token_loss(const Policy& p, double lp, double old, bool has_ref,
-                                             double ref, double a, double w, TokenSums& s) {
-  const double r = exp(lp - old);
-  const double lo = 1.0 - p.eps_low, hi = 1.0 + p.eps_high, cap = p.delta;
-  const double clipped = fmin(fmax(r, lo), hi);
-  const double free_gain = fmin(r, cap) * a, clip_gain = clipped * a;
-  // whether the smaller gain moves with r
-  const bool follows = (free_gain <= clip_gain && r <= cap) ||
-                       (clip_gain <= free_gain && clipped == r);
-  double l = -fmin(free_gain, clip_gain), d = follows ? -r * a : 0.0, kl = 0.0;
-  if (r != r || a != a) l = d = r * a;  // fmin would hide a NaN
-  if (has_ref) {
-    const double q = ref - lp, e = exp(q);
-    kl = e - q - 1.0;
-    l += p.beta * kl;
-    d += p.beta * (1.0 - e);
+// Token r of sequence b and weight w: d loss / d logp, its terms added to s.
+__device__ __forceinline__ double token_at(const Policy& p, const Tokens& t, int64_t r, int b,
+                                           double lp, double w, TokenSums& s) {
+  const double old = t.old ? (double)t.old[r] : lp, a = t.adv[t.adv_tokens ? r : b];
+  const double ratio = exp(lp - old);
+  double q = 0.0, eq = 1.0;
+  if (t.ref) {
+    q = (double)t.ref[r] - lp;
+    eq = exp(q);
   }
-  s.v[0] += w * l;
-  s.v[1] += r;
-  s.v[2] += follows ? 0.0 : 1.0;
+  const Slope g = token_slope(p, ratio, a, t.ref != nullptr, eq);
+  const double kl = t.ref ? eq - q - 1.0 : 0.0;
+  s.v[0] += w * (p.beta * kl - g.gain);
+  s.v[1] += ratio;
+  s.v[2] += g.follows ? 0.0 : 1.0;
   s.v[3] += kl;
   s.v[4] += old - lp;
-  return d * w;
-}
-
-// Token r of sequence b, of which `in_row` tokens are counted.
-__device__ __forceinline__ double token_at(const Policy& p, const Tokens& t, int64_t r, int b,
-                                           double lp, int in_row, double tokens, double seqs,
-                                           TokenSums& s) {
-  return token_loss(p, lp, t.old ? (double)t.old[r] : lp, t.ref != nullptr,
-                    t.ref ? (double)t.ref[r] : 0.0, t.adv[t.adv_tokens ? r : b],
-                    token_weight(p, in_row, tokens, seqs), s);
+  return g.d * w;
 }
 
 // The workgroup's sums, in wave order (thread 0 writes them).
@@ -675,26 +769,39 @@ __device__ __forceinline__ void write_loss(const LossOut& o, const double* sums,
   for (int j = 0; j < 4; ++j) o.metrics[j] = tokens > 0.0 ? (float)(sums[1 + j] / tokens) : 0.f;
 }
 
-// ONE: a small batch by one workgroup, from its counts to the loss.
+// ONE: a small batch by one workgroup, to the loss (and from the counts, without weights).
 template <bool ONE, int NT_>
 __global__ void __launch_bounds__(NT_) policy_kernel(Policy p, Tokens t, Coef coef, double* sums,
                                                      LossOut o) {
   __shared__ double red[5 * (NT_ / 64)], all[5];
   __shared__ int own[ONE ? SMALL_BATCH : 1];
   const int64_t R = (int64_t)t.B * t.S;
-  const bool count = ONE && t.mask;
-  if (count) count_small<NT_>(t.mask, t.B, t.S, own);
-  double tokens, seqs;
-  if (count) totals<NT_>(own, t.B, t.S, red, &tokens, &seqs);
-  else totals<NT_>(t.counts, t.B, t.S, red, &tokens, &seqs);
+  const bool count = ONE && t.mask && !t.weights;
+  double tokens = R, seqs = t.B;
+  if (count) {
+    count_small<NT_>(t.mask, t.B, t.S, own);
+    totals<NT_>(own, t.B, red, &tokens, &seqs);
+  } else if (t.weights) {
+    tokens = t.weights[t.B];
+  }
   TokenSums s{};
   for (int64_t r = (int64_t)blockIdx.x * NT_ + threadIdx.x; r < R; r += (int64_t)gridDim.x * NT_) {
     double d = 0.0;
     if (!t.mask || t.mask[r]) {
-      const int b = ONE ? (int)r / t.S : (int)(r / t.S);
-      const int in_row = count ? own[b] : t.counts ? t.counts[b] : t.S;
-      d = token_at(p, t, r, b, t.logp64 ? t.logp64[r] : (double)t.logp[r], in_row, tokens, seqs,
-                   s);
+      const int b = (int)((uint32_t)r / (uint32_t)t.S);  // < 2^31 tokens
+      const double w = count ? token_weight(p, own[b], tokens, seqs)
+                       : t.weights ? t.weights[b] : t.weight;
+      double lp;
+      if (t.parts) {
+        const double2 e = t.parts[r];
+        lp = LN2 * (e.x - log2(e.y));
+        t.logp[r] = (float)lp;
+      } else {
+        lp = t.logp64 ? t.logp64[r] : (double)t.logp[r];
+      }
+      d = token_at(p, t, r, b, lp, w, s);
+    } else if (t.parts) {
+      t.logp[r] = 0.f;
     }
     if (coef.f64) coef.f64[r] = d;
     if (coef.f32) coef.f32[r] = (float)d;
@@ -707,13 +814,11 @@ __global__ void __launch_bounds__(NT_) policy_kernel(Policy p, Tokens t, Coef co
 __global__ void __launch_bounds__(256) finish_kernel(Tokens t, const double* sums, int blocks,
                                                      LossOut o) {
   __shared__ double red[20], all[5];
-  double tokens, seqs;
-  totals<256>(t.counts, t.B, t.S, red, &tokens, &seqs);
   TokenSums s{};
   for (int i = threadIdx.x; i < blocks; i += 256)
     for (int j = 0; j < 5; ++j) s.v[j] += sums[5 * i + j];
   write_sums<256>(s, red, all);
-  if (threadIdx.x == 0) write_loss(o, all, tokens);
+  if (threadIdx.x == 0) write_loss(o, all, t.weights ? t.weights[t.B] : (double)t.B * t.S);
 }
 
 // grad[r] = coef[r] * *by
@@ -727,24 +832,23 @@ __global__ void __launch_bounds__(256) scale_kernel(const double* coef, const fl
 // ------------------------------------------- loss and gradient in one pass --
 
 // A row of logits stays in registers from its sums to its gradient, so it is read once:
-// NV vectors a thread, one row a workgroup.
+// NV vectors a thread, one row a workgroup. Between the sums and the gradient every wave but
+// one waits, so that stretch is kept short: the token's inputs are loaded with the row, the
+// ratio and exp(ref - logp) are made of the token's exponent and S without a logarithm, and
+// logp itself is left to policy_kernel.
 template <int DT, int NT_, int NV>
 __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tokens t,
-                                                           float inv_t, double* logp64,
-                                                           float* logp, RowStat* stat,
-                                                           float* coef, void* grad) {
+                                                           float inv_t, double2* parts,
+                                                           RowStat* stat, float* coef,
+                                                           void* grad) {
   __shared__ JoinSpace<NT_> red;
-  __shared__ double total[2 * (NT_ / 64)];
-  __shared__ float shared_coef;
-  __shared__ int own[SMALL_BATCH];
-  const int64_t r = blockIdx.x;
+  __shared__ RowGrad shared_grad;
+  const uint32_t r = blockIdx.x;
   const int tid = threadIdx.x;
-  char* const out = static_cast<char*>(grad) + r * q.V * SIZE<DT>;
+  char* const out = static_cast<char*>(grad) + (int64_t)r * q.V * SIZE<DT>;
   if (q.mask && !q.mask[r]) {
     zero_row<DT, NT_>(out, q.V);
     if (tid == 0) {
-      logp64[r] = 0.0;
-      logp[r] = 0.f;
       stat[r] = RowStat{0.f, 1.f, 0.f, 0.f};
       coef[r] = 0.f;
     }
@@ -752,57 +856,79 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
   }
   const void* row = row_at<DT>(q, r);
   const Span<DT> sp(row, q.V);
+  // Stride i of the workgroup holds vectors start(i) + tid; the last one is moved back to end
+  // with the row, and of it only what no stride before it holds counts (in_stride). So every
+  // thread loads NV vectors in any case, at scalar addresses: were some loads skipped, the
+  // compiler could not tell how many are behind the one it needs, and would wait for all.
+  const int last = max(sp.nvec - NT_, 0), tail0 = min(tid, max(sp.nvec - 1, 0));
+  auto start = [&](int i) __attribute__((always_inline)) { return min(i * NT_, last); };
+  auto in_stride = [&](int i) __attribute__((always_inline)) {
+    return i ? tid >= i * NT_ - start(i) : tid < sp.nvec;
+  };
+  const uint4* const vec = sp.nvec ? sp.vec : reinterpret_cast<const uint4*>(parts);
   uint4 v[NV];
-  // whole strides of the workgroup, then the last one's threads; -inf adds nothing
-  constexpr uint32_t LOW = DT == F32 ? 0xFF800000u : DT == F16 ? 0xFC00FC00u : 0xFF80FF80u;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if ((i + 1) * NT_ <= sp.nvec) {
-      v[i] = load_stream(sp.vec + i * NT_ + tid);
-    } else {
-      v[i] = make_uint4(LOW, LOW, LOW, LOW);
-      if (i * NT_ + tid < sp.nvec) v[i] = load_stream(sp.vec + i * NT_ + tid);
-    }
-  }
-  const float odd = tid < sp.odd ? load1<DT>(row, sp.odd_at(tid)) : -INFINITY;
-  // counted while the row is on its way
-  const bool count = t.mask && !t.counts;
-  if (count) count_small<NT_>(t.mask, t.B, t.S, own);
-  double tokens, seqs;
-  if (count) totals<NT_>(own, t.B, t.S, total, &tokens, &seqs);
-  else totals<NT_>(t.counts, t.B, t.S, total, &tokens, &seqs);
+  for (int i = 0; i < NV; ++i) v[i] = load_stream(vec + start(i) + tail0);
+  // Loads come back in order: what is used before the row's last vector is loaded by scalar
+  // loads, and what is a vector load is left as it stands (unconverted, and at an address
+  // that looks as if it differed between lanes) until after the row's sums.
+  int lane0 = 0;
+  asm("" : "+v"(lane0));
+  const int64_t id = load_uniform(q.ids + r);
+  const bool known = id >= 0 && id < q.V;
+  const Raw<DT> raw = load_raw<DT>(row, (known ? id : 0) + lane0);
+  const Raw<DT> raw_odd = load_raw<DT>(row, tid < sp.odd ? sp.odd_at(tid) : 0);
+  const uint32_t b = r / (uint32_t)t.S;
+  const double adv = load_uniform(t.adv + (t.adv_tokens ? r : b));
+  const double old = t.old ? (double)load_uniform(t.old + r) : 0.0;
+  const double ref = t.ref ? (double)load_uniform(t.ref + r) : 0.0;
+  const double w = t.weights ? load_uniform(t.weights + b) : t.weight;
   Sums<false> s;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i * NT_ < sp.nvec) {
+    if (in_stride(i)) {
       float f[PER<DT>];
       unpack<DT>(v[i], f);
       s.admit(top_of<DT>(f), q);
       s.add(f, q);
     }
   }
-  if (sp.odd) {
+  const float odd = to_float<DT>(raw_odd);
+  if (tid < sp.odd) {
     const float x[1] = {odd};
     s.admit(odd, q);
     s.add(x, q);
   }
-  RowStat st;
-  const Joined j = row_stat<DT, false, NT_>(s, row, q, red, &st);
-  const int64_t id = q.ids[r];
-  if (tid == 0) {
-    const int b = (int)(r / t.S);
-    const double lp = row_logp<DT>(row, id, q, j, st.m);
-    const int in_row = count ? own[b] : t.counts ? t.counts[b] : t.S;
-    TokenSums unused{};
-    const float c = (float)token_at(p, t, r, b, lp, in_row, tokens, seqs, unused);
-    logp64[r] = lp;
-    logp[r] = (float)lp;
-    stat[r] = st;
-    coef[r] = c;
-    shared_coef = c;
+  // by the first wave: d loss / d logp, and what the row's values need of it
+  auto token = [&](const Joined& j, float m) __attribute__((always_inline)) {
+    const float xid = known ? to_float<DT>(raw) : __builtin_nanf("");
+    const double a = id_exponent(xid, q, j, m);
+    const double ratio = t.old ? exp(fma(LN2, a, -old)) / j.S : 1.0 + 0.0 * a;
+    const double eq = t.ref ? exp(fma(-LN2, a, ref)) * j.S : 1.0;
+    const float c = (float)(token_slope(p, ratio, adv, t.ref != nullptr, eq).d * w);
+    const RowStat st{j.M, (float)j.S, m, 0.f};
+    if (tid == 0) {
+      shared_grad = row_grad(q, st, c * inv_t, id);
+      parts[r] = make_double2(a, j.S);
+      stat[r] = st;
+      coef[r] = c;
+    }
+  };
+  leave<false, NT_>(s, red);
+  __syncthreads();
+  if (tid < 64) {
+    const Joined j = gather<false, NT_>(red);
+    if (usable(j)) token(j, 0.f);
+    else if (tid == 0) shared_grad.neg = INFINITY, shared_grad.M = LOWEST;
   }
   __syncthreads();
-  const RowGrad g = row_grad(q, st, shared_coef * inv_t, id);
+  if (shared_grad.M == LOWEST) {  // no such row gets here through token()
+    const PlainStat ps =
+        plain_stat<DT, false, NT_>(row, q.V, q.khi, reinterpret_cast<float*>(&red));
+    if (tid < 64) token(Joined{INFINITY, ps.S, 0.0}, ps.m);
+    __syncthreads();
+  }
+  const RowGrad g = shared_grad;
   char* const o = out + (int64_t)sp.head * SIZE<DT>;
   if (!aligned16(o) || !by_vectors<DT>(g)) {
     grad_by_value<DT, NT_>(g, row, out, q.V);
@@ -811,8 +937,8 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
   const VecGrad vg = vec_grad(g);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i * NT_ + tid < sp.nvec)
-      store_stream(o + (int64_t)(i * NT_ + tid) * 16, grad_vector<DT>(vg, v[i]));
+    if (in_stride(i))
+      store_stream(o + (int64_t)start(i) * 16 + tid * 16, grad_vector<DT>(vg, v[i]));
   }
   if (tid < sp.odd) {
     const int at = sp.odd_at(tid);
@@ -821,8 +947,9 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
   }
   // the token's own value, by the thread that stored its vector (its later store to the
   // same place comes after)
-  if (g.id >= sp.head && g.id < sp.tail && (g.id - sp.head) / PER<DT> % NT_ == tid)
-    store1<DT>(out, g.id, grad_value(g, load1<DT>(row, g.id)) + g.c);
+  const int at_id = (g.id - sp.head) / PER<DT>;
+  if (g.id >= sp.head && g.id < sp.tail && at_id - start(at_id / NT_) == tid)
+    store1<DT>(out, g.id, grad_value(g, to_float<DT>(raw)) + g.c);
 }
 
 // ----------------------------------------------------------------- host --
@@ -840,11 +967,11 @@ size_t logp_ws(int64_t R, int dtype, int V) {
   return n > 1 ? (size_t)R * n * sizeof(Part) : 0;
 }
 
-// Workspace of the loss entry points: counted tokens per sequence, the workgroups' sums, and
+// Workspace of the loss entry points: counts and weights per sequence, the workgroups' sums, and
 // (from logits) the float64 log-probabilities and the parts of few rows.
 constexpr int SUM_BLOCKS = 256;
 struct PolicyWs {
-  size_t counts, sums, logp64, parts, total;
+  size_t counts, weights, sums, logp64, parts, total;
 };
 PolicyWs policy_ws(int B, int S, int dtype, int V) {  // V 0: from log-probabilities
   PolicyWs w{};
@@ -856,8 +983,9 @@ PolicyWs policy_ws(int B, int S, int dtype, int V) {  // V 0: from log-probabili
   };
   const int64_t R = (int64_t)B * S;
   w.counts = take((size_t)B * 4);
+  w.weights = take((size_t)(B + 1) * 8);
   w.sums = take(SUM_BLOCKS * 5 * 8);
-  w.logp64 = take(V ? (size_t)R * 8 : 0);
+  w.logp64 = take(V ? (size_t)R * 16 : 0);  // or the parts that logp is made of
   w.parts = take(V ? logp_ws(R, dtype, V) : 0);
   w.total = o;
   return w;
@@ -936,28 +1064,35 @@ int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const flo
   return launch_check("token_logprobs_backward");
 }
 
-// Rows of at most this many bytes stay in registers: 19 vectors a thread of a workgroup
-// that fills a CU's registers.
-constexpr int HELD = 19;
-bool rows_held(int dtype, int V) {
-  return (int64_t)V * (dtype == F32 ? 4 : 2) <= (int64_t)HELD * 1024 * 16;
-}
+// Rows of at most this many vectors stay in registers: 19 a thread of a workgroup that fills
+// a CU's registers.
+constexpr int64_t HELD = 19 * 1024;
+int64_t row_vectors(int dtype, int V) { return ((int64_t)V * (dtype == F32 ? 4 : 2) + 15) / 16; }
+bool rows_held(int dtype, int V) { return row_vectors(dtype, V) <= HELD; }
 
 template <int DT>
 int launch_loss_rows(const Rows& q, int64_t R, const Policy& p, const Tokens& t, float inv_t,
-                     double* logp64, float* logp, RowStat* stat, float* coef, void* grad,
-                     hipStream_t st) {
-  const int64_t bytes = (int64_t)q.V * SIZE<DT>;
-  const unsigned n = (unsigned)R;
-  if (bytes <= HELD * 256 * 16)
-    loss_rows_kernel<DT, 256, HELD><<<n, 256, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
-                                                       grad);
-  else if (bytes <= HELD * 512 * 16)
-    loss_rows_kernel<DT, 512, HELD><<<n, 512, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
-                                                       grad);
-  else
-    loss_rows_kernel<DT, 1024, HELD><<<n, 1024, 0, st>>>(q, p, t, inv_t, logp64, logp, stat, coef,
-                                                         grad);
+                     double2* parts, RowStat* stat, float* coef, void* grad, hipStream_t st) {
+  // the smallest of these that holds the row: loads past it are loads all the same
+  const int64_t vecs = row_vectors(DT, q.V);
+  auto go = [&](auto threads, auto each) {
+    constexpr int NT_ = decltype(threads)::value, NV = decltype(each)::value;
+    if (vecs > NT_ * NV) return false;
+    loss_rows_kernel<DT, NT_, NV><<<(unsigned)R, NT_, 0, st>>>(q, p, t, inv_t, parts, stat, coef,
+                                                               grad);
+    return true;
+  };
+  const std::integral_constant<int, 256> n256;
+  const std::integral_constant<int, 512> n512;
+  const std::integral_constant<int, 1024> n1024;
+  const std::integral_constant<int, 10> v10;
+  const std::integral_constant<int, 14> v14;
+  const std::integral_constant<int, 19> v19;
+  if (!(go(n256, v10) || go(n256, v19) || go(n512, v14) || go(n512, v19) || go(n1024, v14) ||
+        go(n1024, v19))) {
+    set_error("row too long");
+    return GRPO_EUNSUPPORTED;
+  }
   return launch_check("policy_loss_rows");
 }
 
@@ -984,22 +1119,30 @@ bool small_batch(const Tokens& t) {
   return (int64_t)t.B * t.S <= SMALL_TOKENS && t.B <= SMALL_BATCH;
 }
 
-// Counts ahead of the kernels that need them (a small batch is counted in those).
-int run_counts(Tokens* t, char* ws, const PolicyWs& o, hipStream_t st) {
-  if (!t->mask || small_batch(*t)) return GRPO_OK;
-  int* counts = reinterpret_cast<int*>(ws + o.counts);
+// The weights for the launches that follow.
+int run_weights(const Policy& p, Tokens* t, char* ws, const PolicyWs& o, hipStream_t st) {
+  const double R = (double)t->B * t->S;
+  t->weight = p.normalizer == 0 ? 1.0 / R : p.normalizer == 1 ? 1.0 / R : 1.0 / p.denom;
+  if (!t->mask || R == 0.0) return GRPO_OK;
+  int* const counts = reinterpret_cast<int*>(ws + o.counts);
+  double* const weights = reinterpret_cast<double*>(ws + o.weights);
+  t->weights = weights;
+  if (small_batch(*t)) {
+    weight_kernel<true><<<1, 1024, 0, st>>>(p, t->mask, t->B, t->S, nullptr, weights);
+    return launch_check("policy_weights");
+  }
   count_kernel<<<(unsigned)t->B, 256, 0, st>>>(t->mask, t->S, counts);
-  t->counts = counts;
-  return launch_check("policy_count");
+  if (int rc = launch_check("policy_count")) return rc;
+  weight_kernel<false><<<1, 1024, 0, st>>>(p, t->mask, t->B, t->S, counts, weights);
+  return launch_check("policy_weights");
 }
 
-// The tokens' losses and derivatives, and the sums' end. One workgroup takes a small batch
-// (4096 tokens: one launch of 8 us for three of 3.6, 5.3 and 4.0).
-int run_policy(const Policy& p, const Tokens& t, char* ws, const PolicyWs& o, Coef coef,
+// The tokens' losses and derivatives, and the sums' end; `one`: by one workgroup.
+int run_policy(const Policy& p, const Tokens& t, bool one, char* ws, const PolicyWs& o, Coef coef,
                const LossOut& out, hipStream_t st) {
   const int64_t R = (int64_t)t.B * t.S;
   double* sums = reinterpret_cast<double*>(ws + o.sums);
-  if (small_batch(t)) {
+  if (one) {
     policy_kernel<true, 1024><<<1, 1024, 0, st>>>(p, t, coef, sums, out);
     return launch_check("policy_loss");
   }
@@ -1070,11 +1213,17 @@ extern "C" int grpo_policy_loss(const float* logp, const float* old_logp, const 
   const PolicyWs o = policy_ws(B, S, 0, 0);
   if (int rc = policy_check(policy, B, S, advantages, workspace, workspace_bytes, o)) return rc;
   if (((int64_t)B * S && !logp) || !loss || !metrics) return einval("null pointer");
-  Tokens t{nullptr, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
+  Tokens t{nullptr, nullptr, const_cast<float*>(logp), old_logp, ref_logp, advantages, mask,
+           nullptr, 0.0, B, S, adv_tokens != 0};
   hipStream_t st = as_stream(stream);
   char* const ws = static_cast<char*>(workspace);
-  if (int rc = run_counts(&t, ws, o, st)) return rc;
-  return run_policy(*policy, t, ws, o, Coef{coef, nullptr}, LossOut{loss, metrics}, st);
+  // one launch where it does (4096 tokens: 15 us of the GPU's time for 13 and a finish, and
+  // 5 us less of the host's, which is what such a call waits for)
+  const bool one = small_batch(t);
+  if (!one || !mask) {
+    if (int rc = run_weights(*policy, &t, ws, o, st)) return rc;
+  }
+  return run_policy(*policy, t, one, ws, o, Coef{coef, nullptr}, LossOut{loss, metrics}, st);
 }
 
 extern "C" int grpo_policy_loss_backward(const double* coef, const float* grad_loss,
@@ -1115,8 +1264,9 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   char* const ws = static_cast<char*>(workspace);
   double* const lp = reinterpret_cast<double*>(ws + o.logp64);
   RowStat* const rs = reinterpret_cast<RowStat*>(stat);
-  Tokens t{lp, logp, old_logp, ref_logp, advantages, mask, nullptr, B, S, adv_tokens != 0};
-  if (int rc = run_counts(&t, ws, o, st)) return rc;
+  Tokens t{lp, nullptr, logp, old_logp, ref_logp, advantages, mask, nullptr, 0.0, B, S,
+           adv_tokens != 0};
+  if (int rc = run_weights(*policy, &t, ws, o, st)) return rc;
   if (R) {
     const Rows q = rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature);
     const float inv_t = (float)(1.0 / temperature);
@@ -1126,12 +1276,17 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
     } else {
       auto go = dtype == BF16 ? launch_loss_rows<BF16>
                 : dtype == F16 ? launch_loss_rows<F16> : launch_loss_rows<F32>;
-      rc = go(q, R, *policy, t, inv_t, lp, logp, rs, coef, grad_logits, st);
+      double2* const parts = reinterpret_cast<double2*>(lp);
+      rc = go(q, R, *policy, t, inv_t, parts, rs, coef, grad_logits, st);
+      t.logp64 = nullptr;
+      t.parts = parts;
       coef = nullptr;  // written
     }
     if (rc) return rc;
   }
-  return run_policy(*policy, t, ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
+  // one workgroup ends up to 1024 tokens (7.8 us), more are faster in two launches (10.6 at
+  // 4096, one 16)
+  return run_policy(*policy, t, R <= 1024, ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
 }
 
 extern "C" int grpo_policy_loss_logits_held(int dtype, int V) {

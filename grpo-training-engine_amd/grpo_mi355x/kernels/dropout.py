@@ -7,10 +7,7 @@ read on the device, so a captured graph draws new masks when the tensor changes.
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -30,16 +27,16 @@ def check_dropout(p: float, rng: torch.Tensor, device: torch.device) -> float:
 
 
 def _dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
-    x = x.detach()
     if not x.is_contiguous():
         x = x.contiguous()
-    y = torch.empty_like(x)
-    dev = x.device
-    with (contextlib.nullcontext() if dev.index == torch.cuda.current_device()
-          else torch.cuda.device(dev)):
-        rc = _lib.device_library().grpo_dropout(x.data_ptr(), y.data_ptr(), x.numel(),
-                                                _DTYPES[x.dtype], p, rng.data_ptr(),
-                                                _lib.stream_handle(dev))
+    y, dev = torch.empty_like(x), x.device
+    args = (x.data_ptr(), y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, rng.data_ptr())
+    fn = _lib.device_library().grpo_dropout
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream_handle(dev))
     if rc:
         _lib.check(rc, "grpo_dropout")
     return y
@@ -53,9 +50,9 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, p, rng)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        return _dropout(grad, ctx.p, ctx.saved_tensors[0]), None, None
+        # the mask again: its own gradient is the same call, so it differentiates twice
+        return counter_dropout(grad, ctx.p, ctx.saved_tensors[0]), None, None
 
 
 def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
@@ -73,7 +70,7 @@ def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tenso
     if x.dtype not in _DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}.")
     p = check_dropout(p, rng, x.device)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         return _Dropout.apply(x, p, rng)
     return _dropout(x, p, rng)
 

@@ -114,3 +114,13 @@ def test_captured_graph_draws_from_the_tensor(dev):
         assert torch.equal(y.cpu(), want(x, 0.4, 11, k))
         drop(held, 0.1, rng)
         torch.cuda.synchronize()
+
+
+def test_differentiates_twice(dev):
+    """Linear in x for a given mask: the second derivative's mask is the same one."""
+    x = torch.randn(5, 9, dtype=torch.float32, device=dev, requires_grad=True)
+    y = drop(x, 0.5, state(dev, 8, 1)) ** 2
+    first, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    second, = torch.autograd.grad(first.sum(), x)
+    f = torch.from_numpy(dropout_factors(45, 0.5, 8, 1)).view(5, 9).float().to(dev)
+    assert torch.equal(second, 2 * f * f)  # powers of two: exact
