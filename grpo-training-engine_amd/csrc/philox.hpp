@@ -29,16 +29,21 @@ __device__ __forceinline__ DropKey drop_key(const int64_t* rng) {
   return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
 }
 
-// The four words of block i.
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // one instruction of gfx950
+}
+
+// The four words of block i: twenty 32 x 32 -> 64 products (a quarter of the full rate) and
+// twenty three-way xors.
 __device__ __forceinline__ uint4 philox(uint64_t i, const DropKey& key) {
   uint32_t c0 = (uint32_t)i, c1 = (uint32_t)(i >> 32), c2 = key.o0, c3 = key.o1;
   uint32_t k0 = key.k0, k1 = key.k1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p = (uint64_t)c0 * 0xD2511F53u, q = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
+    c0 = xor3((uint32_t)(q >> 32), c1, k0);
     c1 = (uint32_t)q;
-    c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+    c2 = xor3((uint32_t)(p >> 32), c3, k1);
     c3 = (uint32_t)p;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
