@@ -20,6 +20,7 @@
 // exact powers of two. Everything per row is float64 from the threads' sums on: the ratio of
 // a token next to a border of the clip decides whether it has a gradient at all.
 #include <type_traits>
+#include <algorithm>
 
 #include "common.hpp"
 
@@ -1070,14 +1071,19 @@ int run_logp(int dtype, const Rows& q, int64_t R, const LogpOut& o, void* parts,
   return go(std::integral_constant<int, F32>{});
 }
 
+// Rows of at most this many vectors stay in registers: 19 a thread of a workgroup that fills
+// a CU's registers.
+constexpr int64_t HELD = 19 * 1024;
+int64_t row_vectors(int dtype, int V) { return ((int64_t)V * (dtype == F32 ? 4 : 2) + 15) / 16; }
 int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const float* coef,
              const float* scale, double temperature, void* grad, bool skip_one, hipStream_t st) {
   const float inv_t = (float)(1.0 / temperature);
   const int n = (int)R;
-  // with a gradient that is most likely there already, few workgroups to find that out; few
-  // rows are cut over several
+  // with a gradient that is most likely there already, few workgroups to find that out; fewer
+  // than 4096 rows are cut over several, of 1024 vectors or more each (993 x 50257 float32: 59
+  // us with one each, 53)
   const dim3 grid(skip_one && n > 1024 ? 1024u : (unsigned)n,
-                  n < 256 ? (unsigned)logp_cuts(R, dtype, q.V) : 1u);
+                  n < 4096 ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(4096 / n, row_vectors(dtype, q.V) / 1024)) : 1u);
   if (dtype == BF16)
     logits_grad_kernel<BF16><<<grid, NT, 0, st>>>(q, n, stat, coef, scale, inv_t, grad, skip_one);
   else if (dtype == F16)
@@ -1087,10 +1093,6 @@ int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const flo
   return launch_check("token_logprobs_backward");
 }
 
-// Rows of at most this many vectors stay in registers: 19 a thread of a workgroup that fills
-// a CU's registers.
-constexpr int64_t HELD = 19 * 1024;
-int64_t row_vectors(int dtype, int V) { return ((int64_t)V * (dtype == F32 ? 4 : 2) + 15) / 16; }
 bool rows_held(int dtype, int V) { return row_vectors(dtype, V) <= HELD; }
 
 template <int DT>

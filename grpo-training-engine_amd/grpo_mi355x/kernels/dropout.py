@@ -51,8 +51,10 @@ class _Dropout(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        # the mask again: its own gradient is the same call, so it differentiates twice
-        return counter_dropout(grad, ctx.p, ctx.saved_tensors[0]), None, None
+        # the mask again; its own gradient is the same call, so it differentiates twice
+        rng, = ctx.saved_tensors
+        run = _Dropout.apply if torch.is_grad_enabled() and grad.requires_grad else _dropout
+        return run(grad, ctx.p, rng), None, None
 
 
 def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
