@@ -7,7 +7,11 @@
 //   grad_x = dt(dt(g W) + dt(gi A))   y = dt(dt(dt(x W^T) [+ bias]) + dt(dt(t B^T) * dt(s)))
 // With dropout on the adapter's input, drop(x) = dt(x * scale) where kept and 0 elsewhere
 // (philox.hpp), x is drop(x) in xa, t and grad_A, and grad_x adds drop(dt(gi A)); the mask is
-// made again in each of the four kernels that need it.
+// made again in each of the four kernels that need it: 4184 rows of 3584 x 3584, r = 16, 9
+// us more than without dropout (GEMM epilogue 4, weight gradients 4, preparation 1) in 265,
+// where a mask of a byte each would be written once and read three times (60 MB, 12 us) and
+// kept from forward to backward. The rounding points are those without dropout, drop(x)
+// rounded to the type as the layer that drops ahead of A rounds it.
 //
 // The weight is decoded once per call, not once per row tile: from about 5 million
 // outputs (fewer where the decoding GEMM's ring kernel does not run) the two passes over

@@ -180,6 +180,7 @@ def test_c_entry_refuses_buffers(lib):
 
 @pytest.mark.parametrize("kw", [dict(p=1.0), dict(p=-0.5), dict(p=math.nan), dict(dtype=3),
                                 dict(n=-1), dict(x=None), dict(rng=None), dict(rng=FAKE + 4),
+                                dict(x=FAKE + 1), dict(y=FAKE + 2, dtype=2),
                                 dict(p=1 - 2 ** -18)])
 def test_c_entry_refuses_dropout(lib, kw):
     a = dict(x=FAKE, y=FAKE, n=8, dtype=0, p=0.1, rng=FAKE)
