@@ -352,7 +352,8 @@ class FusedLoRADropoutFunction(torch.autograd.Function):
         if x.shape[0] == 0:
             grads = (torch.empty_like(x), torch.zeros_like(lora_A), torch.zeros_like(lora_B))
         else:
-            nbytes = _train_workspace(w, ctx.blocksize, lora_A, lora_B, x, g)
+            nbytes = ops.nf4_lora_train_workspace_bytes(*g.shape, x.shape[1], lora_A.shape[0],
+                                                        ctx.blocksize)  # all aligned by now
             grads = ops.train_backward(x, g, w, absmax, code, ctx.blocksize, lora_A,
                                        lora_B.contiguous(), ctx.scaling, need[0], need[3],
                                        need[4], nbytes, (ctx.p, rng))

@@ -267,3 +267,29 @@ def test_captured_and_replayed(dev):
         for u, v in zip(out, step(fresh(), _state(dev, SEED, k))):
             assert torch.equal(u, v)
         torch.cuda.synchronize()
+
+
+def test_checkpointed_layer(dev):
+    """Activation checkpointing draws the mask again and gets the same one."""
+    from torch.utils.checkpoint import checkpoint
+
+    from grpo_mi355x.core.lora import ManualLoRALayer
+    from grpo_mi355x.core.nf4 import Linear4bitNF4
+
+    g = torch.Generator().manual_seed(4)
+    base = Linear4bitNF4.from_weight(torch.randn(64, 64, generator=g) * 0.05, None)
+    layer = ManualLoRALayer(base, rank=8, alpha=16, dropout=0.3,
+                            counter_dropout=True).to(dev).to(torch.bfloat16)
+    with torch.no_grad():
+        layer.lora_B.weight.normal_(std=0.05)
+    x = torch.randn(2, 9, 64, generator=g).bfloat16().to(dev)
+    got = []
+    for run in (lambda t: layer(layer(t)),
+                lambda t: checkpoint(lambda u: layer(layer(u)), t, use_reentrant=False)):
+        layer.zero_grad()
+        torch.manual_seed(5)
+        leaf = x.clone().requires_grad_()
+        (run(leaf).float() ** 2).sum().backward()
+        got.append((leaf.grad, layer.lora_A.weight.grad.clone(), layer.lora_B.weight.grad.clone()))
+    for u, v in zip(*got):
+        assert torch.equal(u, v)

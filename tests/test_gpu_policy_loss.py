@@ -100,7 +100,7 @@ def test_token_logprobs_and_gradient(dev, dtype, vocab, t):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("vocab", [151936, 152064, 262147])
+@pytest.mark.parametrize("vocab", [151936, 152064, 262147, 2000003])
 def test_whole_vocabularies(dev, dtype, vocab):
     x, ids, mask = make(3, vocab, dtype, seed=5, counted=1.1)
     logp, ent, p, tol, tol_ent = bounds(x, ids, mask, 1.0)
@@ -562,3 +562,67 @@ def test_captured_and_replayed(dev):
             assert torch.equal(u, v)
         eager(sets[k])  # eager work between the replays
         torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(dev):
+    """16384 rows of 151936 values: 5 GB, rows past 2^31 values. The last rows' results are
+    those of a call of their own (the weights do not depend on the batch: a number)."""
+    rows, vocab = 16384, 151936
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(1, rows, vocab, generator=g, device=dev, dtype=torch.bfloat16)
+    ids = torch.randint(0, vocab, (1, rows), generator=g, device=dev)
+    old = torch.full((1, rows), -12.0, device=dev)
+    adv = torch.randn(1, rows, generator=g, device=dev)
+    x.requires_grad_()
+
+    def go(x, ids, old, adv):
+        loss, lp, _ = _ops().fused_grpo_loss(x, ids, old, adv, normalizer=100.0)
+        grad, = torch.autograd.grad(loss, x)
+        lp2 = _ops().token_logprobs(x, ids)
+        grad2, = torch.autograd.grad(lp2, x, adv)
+        return lp, grad, lp2.detach(), grad2
+
+    lp, grad, lp2, grad2 = go(x, ids, old, adv)
+    end = slice(rows - 5, rows)
+    # 4096 rows and more are not cut over workgroups; these five are, and their sums' order
+    # differs: to the roundings of logp, and a gradient's half step either way
+    want = go(x.detach()[:, end].clone().requires_grad_(), ids[:, end], old[:, end], adv[:, end])
+    for a, b in ((lp, want[0]), (lp2, want[2])):
+        assert torch.allclose(a[:, end], b, rtol=4 * E, atol=16 * E)
+    for a, b in ((grad, want[1]), (grad2, want[3])):
+        assert torch.allclose(a[:, end].float(), b.float(), rtol=2.0 ** -7, atol=1e-30)
+
+
+def test_shifted_view_of_a_models_logits(dev):
+    """logits[:, :-1] as a trainer slices them: the gradient reaches the whole tensor."""
+    x, ids, old, ref, adv, mask, _, _ = loss_inputs(3, 8, 2001, "bf16", seed=5)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    whole = torch.cat([put(x), torch.full((3, 1, 2001), math.nan, device=dev).bfloat16()], 1)
+    leaf, part = whole.clone().requires_grad_(), put(x).requires_grad_()
+    kw = dict(ref_logps=put(ref), beta=0.04)
+    args = (put(ids), put(old), put(adv), put(mask))
+    a, lp, _ = _ops().fused_grpo_loss(leaf[:, :-1], *args, **kw)
+    b, lp2, _ = _ops().fused_grpo_loss(part, *args, **kw)
+    a.backward()
+    b.backward()
+    # rows start at other addresses, so their sums' order differs
+    assert torch.allclose(lp, lp2, rtol=4 * E, atol=16 * E)
+    assert torch.allclose(leaf.grad[:, :-1].float(), part.grad.float(), rtol=2.0 ** -7, atol=1e-30)
+    assert not leaf.grad[:, -1].any()
+
+
+def test_saved_tensors_that_moved(dev):
+    """Hooks that keep the saved logits elsewhere: the backward reads what it is given."""
+    x, ids, old, _, adv, mask, _, _ = loss_inputs(2, 9, 2000, "bf16", seed=3, beta=0.0)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    grads = []
+    for hooks in (False, True):
+        leaf = put(x).requires_grad_()
+        with torch.autograd.graph.save_on_cpu() if hooks else torch.enable_grad():
+            loss, _, _ = _ops().fused_grpo_loss(leaf * 1.0, put(ids), put(old), put(adv),
+                                                put(mask))
+            lp = _ops().token_logprobs(leaf * 1.0, put(ids), put(mask))
+        torch.full_like(leaf, math.nan)  # takes the place of what was given back
+        grads.append(torch.autograd.grad(0.5 * loss, leaf) + torch.autograd.grad(lp.sum(), leaf))
+    for u, v in zip(*grads):
+        assert torch.equal(u, v)
