@@ -380,6 +380,17 @@ __device__ __forceinline__ const void* row_at(const Rows& q, int64_t r) {
   return static_cast<const char*>(q.x) + (b * q.sb + s * q.ss) * SIZE<DT>;
 }
 
+// The logits' gradient, rows placed as the logits' are with strides of its own.
+struct Grad {
+  void* x;
+  int64_t sb, ss;
+};
+template <int DT>
+__device__ __forceinline__ char* grad_at(const Grad& g, int S, int64_t r) {
+  const uint32_t b = (uint32_t)r / (uint32_t)S, s = (uint32_t)r - b * S;
+  return static_cast<char*>(g.x) + (b * g.sb + s * g.ss) * SIZE<DT>;
+}
+
 constexpr int NT = 512;
 
 struct LogpOut {
@@ -532,7 +543,7 @@ __device__ __forceinline__ void zero_row(void* out, int V) {
 }
 
 // Rows that cannot be stored 16 bytes at a time where they are loaded so, and rows whose M
-// is not finite: value by value.
+// is not finite: value by value (50257 bf16 values a row: 2.0 times the time).
 template <int DT, int NT>
 __device__ __noinline__ void grad_by_value(RowGrad g, const void* row, void* out, int V) {
   for (int v = threadIdx.x; v < V; v += NT) {
@@ -547,12 +558,12 @@ __device__ __noinline__ void grad_by_value(RowGrad g, const void* row, void* out
 template <int DT>
 __global__ void __launch_bounds__(NT) logits_grad_kernel(Rows q, int R, const RowStat* stat,
                                                          const float* coef, const float* scale,
-                                                         float inv_t, void* grad, bool skip_one) {
+                                                         float inv_t, Grad grad, bool skip_one) {
   const float by = scale ? *scale : 1.f;
   if (skip_one && by == 1.f) return;
   const int y = (int)blockIdx.y, ny = (int)gridDim.y;
   for (int64_t r = blockIdx.x; r < R; r += gridDim.x) {
-    char* const out = static_cast<char*>(grad) + r * q.V * SIZE<DT>;
+    char* const out = grad_at<DT>(grad, q.S, r);
     if (q.mask && !q.mask[r]) {
       if (!skip_one && y == 0) zero_row<DT, NT>(out, q.V);
       continue;
@@ -868,12 +879,12 @@ template <int DT, int NT_, int NV>
 __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tokens t,
                                                            float inv_t, double2* parts,
                                                            RowStat* stat, float* coef,
-                                                           void* grad) {
+                                                           Grad grad) {
   __shared__ JoinSpace<NT_> red;
   __shared__ RowGrad shared_grad;
   const uint32_t r = blockIdx.x;
   const int tid = threadIdx.x;
-  char* const out = static_cast<char*>(grad) + (int64_t)r * q.V * SIZE<DT>;
+  char* const out = grad_at<DT>(grad, q.S, r);
   if (q.mask && !q.mask[r]) {
     zero_row<DT, NT_>(out, q.V);
     if (tid == 0) {
@@ -982,12 +993,13 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
 
 // ----------------------------------------------------------------- host --
 
-// Workgroups a row of the log-probabilities is cut over: enough for 512 in all (two a CU:
-// 8 rows of 151936 bf16 logits 17.3 us with one workgroup each), each with 2048 vectors or more.
+// Workgroups a row of the log-probabilities is cut over: enough for 512 in all (two a CU; 8
+// rows of 151936 bf16 logits 7.8 us, 17.3 with one workgroup each; with 1024 in all 200 rows
+// gain 4 % and 32 lose 15), each with 1024 vectors or more (32 rows 8.5 us, 9.5 with 2048).
 int logp_cuts(int64_t R, int dtype, int V) {
   const int64_t vecs = (int64_t)V * (dtype == F32 ? 4 : 2) / 16;
   const int64_t n = R ? (512 + R - 1) / R : 1;
-  const int64_t most = vecs / 2048 < 64 ? vecs / 2048 : 64;
+  const int64_t most = vecs / 1024 < 64 ? vecs / 1024 : 64;
   return (int)(n < most ? n : most > 1 ? most : 1);
 }
 size_t logp_ws(int64_t R, int dtype, int V) {
@@ -1043,6 +1055,14 @@ int rows_check(const void* x, int dtype, int64_t sb, int64_t ss, int B, int S, i
   return GRPO_OK;
 }
 
+int grad_check(const void* grad, int dtype, int64_t sb, int64_t ss) {
+  if (!grad) return einval("null pointer");
+  if (sb < 0 || ss < 0) return einval("negative row stride");
+  if (reinterpret_cast<uintptr_t>(grad) % (dtype == F32 ? 4 : 2))
+    return einval("grad_logits is not aligned to its type");
+  return GRPO_OK;
+}
+
 Rows rows_of(const void* x, int64_t sb, int64_t ss, int S, int V, const int64_t* ids,
              const uint8_t* mask, double temperature) {
   const double k = 1.0 / LN2 / temperature;
@@ -1088,7 +1108,7 @@ int run_logp(int dtype, const Rows& q, int64_t R, const LogpOut& o, void* parts,
 constexpr int64_t HELD = 19 * 1024;
 int64_t row_vectors(int dtype, int V) { return ((int64_t)V * (dtype == F32 ? 4 : 2) + 15) / 16; }
 int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const float* coef,
-             const float* scale, double temperature, void* grad, bool skip_one, hipStream_t st) {
+             const float* scale, double temperature, const Grad& grad, bool skip_one, hipStream_t st) {
   const float inv_t = (float)(1.0 / temperature);
   const int n = (int)R;
   // with a gradient that is most likely there already, few workgroups to find that out; fewer
@@ -1109,7 +1129,7 @@ bool rows_held(int dtype, int V) { return row_vectors(dtype, V) <= HELD; }
 
 template <int DT>
 int launch_loss_rows(const Rows& q, int64_t R, const Policy& p, const Tokens& t, float inv_t,
-                     double2* parts, RowStat* stat, float* coef, void* grad, hipStream_t st) {
+                     double2* parts, RowStat* stat, float* coef, const Grad& grad, hipStream_t st) {
   // the smallest of these that holds the row: loads past it are loads all the same
   const int64_t vecs = row_vectors(DT, q.V);
   auto go = [&](auto threads, auto each) {
@@ -1224,17 +1244,17 @@ extern "C" int grpo_token_logprobs_backward(const void* logits, int dtype, int64
                                             const int64_t* ids, const uint8_t* mask,
                                             double temperature, const float* stat,
                                             const float* grad_logp, const float* scale,
-                                            void* grad_logits, grpo_stream_t stream) {
+                                            void* grad_logits, int64_t grad_stride_b,
+                                            int64_t grad_stride_s, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
   const int64_t R = (int64_t)B * S;
   if (!R) return GRPO_OK;
-  if (!stat || !grad_logp || !grad_logits) return einval("null pointer");
+  if (!stat || !grad_logp) return einval("null pointer");
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == F32 ? 4 : 2))
-    return einval("grad_logits is not aligned to its type");
+  if (int rc = grad_check(grad_logits, dtype, grad_stride_b, grad_stride_s)) return rc;
   return run_grad(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R,
                   reinterpret_cast<const RowStat*>(stat), grad_logp, scale, temperature,
-                  grad_logits, false, as_stream(stream));
+                  Grad{grad_logits, grad_stride_b, grad_stride_s}, false, as_stream(stream));
 }
 
 extern "C" size_t grpo_policy_loss_workspace_bytes(int B, int S) {
@@ -1284,7 +1304,8 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
                                        const float* advantages, int adv_tokens,
                                        const grpo_policy_t* policy, float* loss, float* logp,
                                        float* metrics, float* stat, float* coef,
-                                       void* grad_logits, void* workspace,
+                                       void* grad_logits, int64_t grad_stride_b,
+                                       int64_t grad_stride_s, void* workspace,
                                        size_t workspace_bytes, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
   const PolicyWs o = policy_ws(B, S, dtype, V);
@@ -1295,8 +1316,9 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
   if (grad_logits && R && (!stat || !rows_held(dtype, V)))
     return einval("grad_logits needs stat and coef and a row of at most 311296 bytes");
-  if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == F32 ? 4 : 2))
-    return einval("grad_logits is not aligned to its type");
+  if (grad_logits) {
+    if (int rc = grad_check(grad_logits, dtype, grad_stride_b, grad_stride_s)) return rc;
+  }
   hipStream_t st = as_stream(stream);
   char* const ws = static_cast<char*>(workspace);
   double* const lp = reinterpret_cast<double*>(ws + o.logp64);
@@ -1314,7 +1336,8 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
       auto go = dtype == BF16 ? launch_loss_rows<BF16>
                 : dtype == F16 ? launch_loss_rows<F16> : launch_loss_rows<F32>;
       double2* const parts = reinterpret_cast<double2*>(lp);
-      rc = go(q, R, *policy, t, inv_t, parts, rs, coef, grad_logits, st);
+      rc = go(q, R, *policy, t, inv_t, parts, rs, coef,
+              Grad{grad_logits, grad_stride_b, grad_stride_s}, st);
       t.logp64 = nullptr;
       t.parts = parts;
       coef = nullptr;  // written
@@ -1335,15 +1358,15 @@ extern "C" int grpo_policy_loss_logits_rescale(const void* logits, int dtype, in
                                                const int64_t* ids, const uint8_t* mask,
                                                double temperature, const float* stat,
                                                const float* coef, const float* grad_loss,
-                                               void* grad_logits, grpo_stream_t stream) {
+                                               void* grad_logits, int64_t grad_stride_b,
+                                               int64_t grad_stride_s, grpo_stream_t stream) {
   if (int rc = rows_check(logits, dtype, stride_b, stride_s, B, S, V, ids, temperature)) return rc;
   const int64_t R = (int64_t)B * S;
   if (!R) return GRPO_OK;
-  if (!stat || !coef || !grad_loss || !grad_logits) return einval("null pointer");
+  if (!stat || !coef || !grad_loss) return einval("null pointer");
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
-  if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == F32 ? 4 : 2))
-    return einval("grad_logits is not aligned to its type");
+  if (int rc = grad_check(grad_logits, dtype, grad_stride_b, grad_stride_s)) return rc;
   return run_grad(dtype, rows_of(logits, stride_b, stride_s, S, V, ids, mask, temperature), R,
                   reinterpret_cast<const RowStat*>(stat), coef, grad_loss, temperature,
-                  grad_logits, true, as_stream(stream));
+                  Grad{grad_logits, grad_stride_b, grad_stride_s}, true, as_stream(stream));
 }

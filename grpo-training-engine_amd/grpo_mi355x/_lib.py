@@ -96,16 +96,18 @@ SIGNATURES = {
                                 _I64, _VP]),
     "grpo_token_logprobs_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
     "grpo_token_logprobs": (_I32, [*_ROWS, _VP, _VP, _VP, _VP, _SZ, _VP]),
-    "grpo_token_logprobs_backward": (_I32, [*_ROWS, _VP, _VP, _VP, _VP, _VP]),
+    "grpo_token_logprobs_backward": (_I32, [*_ROWS, _VP, _VP, _VP, _VP, _I64, _I64, _VP]),
     "grpo_policy_loss_workspace_bytes": (_SZ, [_I32, _I32]),
     "grpo_policy_loss": (
         _I32, [_VP, _VP, _VP, _VP, _I32, _VP, _I32, _I32, _POLICY, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "grpo_policy_loss_backward": (_I32, [_VP, _VP, _I64, _VP, _VP]),
     "grpo_policy_loss_logits_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I32]),
     "grpo_policy_loss_logits": (
-        _I32, [*_ROWS, _VP, _VP, _VP, _I32, _POLICY, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+        _I32, [*_ROWS, _VP, _VP, _VP, _I32, _POLICY, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64,
+               _VP, _SZ, _VP]),
     "grpo_policy_loss_logits_held": (_I32, [_I32, _I32]),
-    "grpo_policy_loss_logits_rescale": (_I32, [*_ROWS, _VP, _VP, _VP, _VP, _VP]),
+    "grpo_policy_loss_logits_rescale": (
+        _I32, [*_ROWS, _VP, _VP, _VP, _VP, _I64, _I64, _VP]),
     "grpo_dropout": (_I32, [_VP, _VP, _I64, _I32, _c.c_double, _VP, _VP]),
     "grpo_nf4_dequant_t": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _VP]),
     "grpo_gemm16_tile": (_I32, [_I32, _I32, _c.POINTER(_I32), _c.POINTER(_I32)]),

@@ -133,6 +133,25 @@ def _rows(logits, ids, mask, t):
     return x, (x.data_ptr(), _DTYPES[x.dtype], sb, ss, b, s, v, ids.data_ptr(), _lib.ptr(mask), t)
 
 
+def _empty_grad(logits, x):
+    """(a tensor for the logits' gradient, its row strides): rows as far from a 16-byte
+    boundary as the logits' own, by their strides where those leave little unused."""
+    b, s, v = x.shape
+    shape, dev = logits.shape, x.device
+    off = x.data_ptr() % 16 // x.element_size()
+    if (off or not x.is_contiguous()) and x.data_ptr() == logits.data_ptr() and logits.ndim <= 3:
+        sb, ss, _ = x.stride()
+        rows = sorted((n, d) for n, d in ((ss, s), (sb, b)) if d > 1)
+        extent, apart = v, True
+        for stride, n in rows:  # the inner rows end before the next outer one begins
+            apart = apart and stride >= extent
+            extent += stride * (n - 1)
+        if apart and extent <= 1.25 * b * s * v:
+            buf = torch.empty(off + extent, dtype=x.dtype, device=dev)
+            return buf.as_strided(shape, logits.stride(), off), sb, ss
+    return torch.empty(shape, dtype=x.dtype, device=dev), s * v, v
+
+
 # ---------------------------------------------------- log-probabilities --
 
 @functools.lru_cache(maxsize=256)
@@ -143,9 +162,9 @@ def _logp_bytes(dtype: int, b: int, s: int, v: int) -> int:
 def _grad_of(logits, ids, mask, t, stat: int, coef: int, scale) -> torch.Tensor:
     """The logits' gradient, of the logits' shape (stat, coef: addresses)."""
     x, rows = _rows(logits, ids, mask, t)
-    out = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
+    out, sb, ss = _empty_grad(logits, x)
     _run(x.device, "grpo_token_logprobs_backward", *rows, stat, coef, _lib.ptr(scale),
-         out.data_ptr())
+         out.data_ptr(), sb, ss)
     return out
 
 
@@ -339,7 +358,7 @@ def _logits_loss(logits, ids, mask, t, tokens, policy, train: bool):
     loss = torch.empty((), dtype=torch.float32, device=dev)
     metrics = torch.empty(4, dtype=torch.float32, device=dev)
     logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
-    grad = torch.empty(logits.shape, dtype=x.dtype, device=dev) if train and held else None
+    grad, sb, ss = _empty_grad(logits, x) if train and held else (None, 0, 0)
     # what the backward needs of each row (16 bytes of statistics, 4 of its derivative), then
     # the workspace
     keep = -(-20 * b * s // 256) * 256 if train else 0
@@ -347,9 +366,9 @@ def _logits_loss(logits, ids, mask, t, tokens, policy, train: bool):
     at = buf.data_ptr()
     _run(dev, "grpo_policy_loss_logits", *rows, _lib.ptr(old), _lib.ptr(ref), adv.data_ptr(),
          per_token, policy, loss.data_ptr(), logp.data_ptr(), metrics.data_ptr(),
-         at if train else None, at + 16 * b * s if train else None, _lib.ptr(grad), at + keep,
-         nbytes)
-    return loss, logp, metrics, buf, grad
+         at if train else None, at + 16 * b * s if train else None, _lib.ptr(grad), sb, ss,
+         at + keep, nbytes)
+    return loss, logp, metrics, buf, (grad, sb, ss)
 
 
 class _LogitsLoss(torch.autograd.Function):
@@ -373,13 +392,14 @@ class _LogitsLoss(torch.autograd.Function):
             grad_loss = grad_loss.float()
         stat = ctx.buf.data_ptr()
         coef = stat + 16 * ids.numel()
-        grad, ctx.grad = ctx.grad, None  # handed out once: it is the caller's from here on
+        # handed out once: it is the caller's from here on
+        (grad, sb, ss), ctx.grad = ctx.grad, (None, 0, 0)
         if grad is None:
             grad = _grad_of(logits, ids, mask, ctx.t, stat, coef, grad_loss)
         else:
             x, rows = _rows(logits, ids, mask, ctx.t)
             _run(x.device, "grpo_policy_loss_logits_rescale", *rows, stat, coef,
-                 grad_loss.data_ptr(), grad.data_ptr())
+                 grad_loss.data_ptr(), grad.data_ptr(), sb, ss)
         return grad, None, None, None, None, None
 
 

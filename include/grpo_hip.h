@@ -107,11 +107,14 @@ int grpo_token_logprobs(const void* logits, int dtype, int64_t stride_b, int64_t
                         float* logp, float* entropy, float* stat, void* workspace,
                         size_t workspace_bytes, grpo_stream_t stream);
 /* grad_logits[r][v] = g / T * (1[v = id] - p_v), g = grad_logp[r] * *scale (scale: one
- * float32 on the device, or NULL: 1); grad_logits [R][V] contiguous, in the logits' type. */
+ * float32 on the device, or NULL: 1); grad_logits in the logits' type, its rows placed like
+ * theirs with strides of its own (rows that do not overlap; 16 bytes are stored at a time
+ * where a row's offset from a 16-byte boundary is that of the logits' row). */
 int grpo_token_logprobs_backward(const void* logits, int dtype, int64_t stride_b,
                                  int64_t stride_s, int B, int S, int V, const int64_t* ids,
                                  const uint8_t* mask, double temperature, const float* stat,
                                  const float* grad_logp, const float* scale, void* grad_logits,
+                                 int64_t grad_stride_b, int64_t grad_stride_s,
                                  grpo_stream_t stream);
 
 /* The two-sided clipped policy loss (GRPOTrainer.compute_grpo_loss, src/grpo/algorithm.py:
@@ -147,7 +150,7 @@ int grpo_policy_loss_backward(const double* coef, const float* grad_loss, int64_
  * metrics from the logits; stat [R][4] and coef [R] (both or neither) are what
  * grpo_token_logprobs_backward takes as stat and grad_logp, with the loss's gradient as
  * its scale.
- *   grad_logits : [R][V] contiguous, in the logits' type, or NULL: the gradient of the loss
+ *   grad_logits : placed as in grpo_token_logprobs_backward, or NULL: the gradient of the loss
  *                 itself (its upstream gradient 1), made in the same pass over the logits;
  *                 needs stat and coef and a vocabulary that grpo_policy_loss_logits_held
  *                 takes (a row stays in one workgroup's registers) */
@@ -157,8 +160,8 @@ int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b, int
                             double temperature, const float* old_logp, const float* ref_logp,
                             const float* advantages, int adv_tokens, const grpo_policy_t* policy,
                             float* loss, float* logp, float* metrics, float* stat, float* coef,
-                            void* grad_logits, void* workspace, size_t workspace_bytes,
-                            grpo_stream_t stream);
+                            void* grad_logits, int64_t grad_stride_b, int64_t grad_stride_s,
+                            void* workspace, size_t workspace_bytes, grpo_stream_t stream);
 int grpo_policy_loss_logits_held(int dtype, int V);
 /* grad_logits of the call above for an upstream gradient *grad_loss: left as it is where
  * that is 1, computed again from the logits otherwise (decided on the device). */
@@ -166,6 +169,7 @@ int grpo_policy_loss_logits_rescale(const void* logits, int dtype, int64_t strid
                                     int64_t stride_s, int B, int S, int V, const int64_t* ids,
                                     const uint8_t* mask, double temperature, const float* stat,
                                     const float* coef, const float* grad_loss, void* grad_logits,
+                                    int64_t grad_stride_b, int64_t grad_stride_s,
                                     grpo_stream_t stream);
 
 /* Dropout with a mask that is never stored: y[e] = dt(x[e] * scale), 0 where dropped.

@@ -129,20 +129,21 @@ def test_rows_that_stay_in_registers(lib):
 def test_c_entry_refuses_a_gradient_it_cannot_make(lib):
     need = 1 << 30
 
-    def go(v, stat, coef, grad):
+    def go(v, stat, coef, grad, sb=24):
         return lib.grpo_policy_loss_logits(
             FAKE, 0, v, v, 2, 3, v, FAKE, None, 1.0, None, None, FAKE, 0, ctypes.byref(_policy()),
-            FAKE, FAKE, FAKE, stat, coef, grad, FAKE, need, None)
+            FAKE, FAKE, FAKE, stat, coef, grad, sb, 8, FAKE, need, None)
 
     assert go(8, FAKE, None, None) == -1 and go(8, FAKE + 4, FAKE, None) == -1
     assert go(8, None, None, FAKE) == -1  # no place for the statistics
     assert go(160000, FAKE, FAKE, FAKE) == -1 and go(8, FAKE, FAKE, FAKE + 1) == -1
+    assert go(8, FAKE, FAKE, FAKE, sb=-1) == -1
 
 
 def test_c_entry_with_no_rows_does_nothing(lib):
     assert _rows(lib, b=0, x=None, ids=None, logp=None) == 0
     assert lib.grpo_token_logprobs_backward(None, 0, 0, 0, 0, 5, 8, None, None, 1.0, None, None,
-                                            None, None, None) == 0
+                                            None, None, 0, 0, None) == 0
     assert lib.grpo_dropout(None, None, 0, 0, 0.1, FAKE, None) == 0
 
 
@@ -186,3 +187,38 @@ def test_c_entry_refuses_dropout(lib, kw):
     a = dict(x=FAKE, y=FAKE, n=8, dtype=0, p=0.1, rng=FAKE)
     a.update(kw)
     assert lib.grpo_dropout(a["x"], a["y"], a["n"], a["dtype"], a["p"], a["rng"], None) == -1
+
+
+@pytest.mark.parametrize("make, kept", [
+    (lambda x: x, False),                       # contiguous and aligned: as it is
+    (lambda x: x[:, :-1], True), (lambda x: x[:, 1:], True),
+    (lambda x: x[..., 3:], False),              # a fifth of each row unused would be too much
+    (lambda x: x[..., 1:], True),
+    (lambda x: x[::2], False), (lambda x: x[:1].expand(4, -1, -1), False),
+    (lambda x: x.transpose(0, 1), True), (lambda x: x[..., ::2], False),
+    (lambda x: x[:, 1], False), (lambda x: x[1:2], True), (lambda x: x.view(-1, 9)[1:], True),
+])
+def test_the_gradients_rows_stand_as_the_logits_do(make, kept):
+    """Rows of the gradient never overlap, and keep the logits' offsets where they can."""
+    base = torch.zeros(5, 6, 9, dtype=torch.bfloat16)
+    v = make(base)
+    ids = torch.zeros(v.shape[:-1], dtype=torch.int64)
+    x, _ = policy_loss._rows(v, ids, None, 1.0)
+    g, sb, ss = policy_loss._empty_grad(v, x)
+    assert g.shape == v.shape and g.dtype == v.dtype
+    size = g.untyped_storage().nbytes() // 2
+    at = [(g.data_ptr() - g.untyped_storage().data_ptr()) // 2 + b * sb + s * ss
+          for b in range(x.shape[0]) for s in range(x.shape[1])]
+    cells = torch.zeros(size, dtype=torch.int32)
+    for a in at:
+        assert a + 9 - (9 - v.shape[-1]) <= size
+        cells[a:a + v.shape[-1]] += 1
+    assert int(cells.max()) == 1 and int(cells.sum()) == v.numel()
+    if kept:
+        assert g.stride() == v.stride()
+        rows = [x.data_ptr() + 2 * (b * x.stride(0) + s * x.stride(1))
+                for b in range(x.shape[0]) for s in range(x.shape[1])]
+        for a, r in zip(at, rows):
+            assert (g.untyped_storage().data_ptr() + 2 * a - r) % 16 == 0
+    else:
+        assert g.is_contiguous()
