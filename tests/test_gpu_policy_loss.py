@@ -626,3 +626,95 @@ def test_saved_tensors_that_moved(dev):
         grads.append(torch.autograd.grad(0.5 * loss, leaf) + torch.autograd.grad(lp.sum(), leaf))
     for u, v in zip(*grads):
         assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("vocab", [600, 160001])  # a row in registers, and beyond
+def test_fused_loss_options(dev, vocab):
+    """On-policy, a cap below the clip's border, an advantage for each token, a number as
+    normalizer, a strided mask and a mask of another type."""
+    b, s = 3, 6
+    x, ids, old, _, _, mask, logp, p = loss_inputs(b, s, vocab, "f32", seed=8, beta=0.0)
+    adv = np.random.default_rng(3).standard_normal((b, s)).astype(np.float32)
+    put = lambda a: None if a is None else torch.as_tensor(a).to(dev)  # noqa: E731
+    wide = torch.zeros(b, s + 2, dtype=torch.int64, device=dev)
+    wide[:, 1:-1] = put(mask)
+    top = E * (vocab / 512 + 24 + 2 * np.abs(logp).max() + math.log(vocab))
+    for o in (None, old):
+        leaf = put(x).requires_grad_()
+        loss, lp, metrics = _ops().fused_grpo_loss(leaf, put(ids), put(o), put(adv),
+                                                   wide[:, 1:-1], delta=1.05, normalizer=77.0)
+        want, want_metrics, d = P.policy_loss(logp.reshape(b, s), o, adv, mask, delta=1.05,
+                                              normalizer=77.0)
+        scale = (8 * np.abs(adv).max() + 1) * mask.sum() / 77
+        assert abs(float(loss.detach()) - want) <= top * scale + E * abs(want)
+        within(metrics, want_metrics, 8 * top + E * np.abs(want_metrics))
+        grad, = torch.autograd.grad(loss, leaf)
+        coef = d.reshape(-1)
+        wantg = P.logits_grad(p, ids.clamp(min=0).reshape(-1).numpy(), mask.reshape(-1), coef)
+        tol = grad_bound(wantg, p, coef, 1.0, "f32") + (np.abs(coef) * 4 * top)[:, None] * (
+            p + (np.arange(vocab)[None] == ids.reshape(-1, 1).numpy()))
+        within(grad.reshape(b * s, vocab), wantg, tol * mask.reshape(-1, 1))
+    # without a gradient: the same loss
+    with torch.no_grad():
+        again = _ops().fused_grpo_loss(put(x), put(ids), put(old), put(adv), put(mask),
+                                       delta=1.05, normalizer=77.0)
+    assert abs(float(again[0]) - float(loss.detach())) <= 2 * top * scale
+    assert torch.allclose(again[1], lp, rtol=4 * E, atol=16 * E)
+
+
+def test_policy_loss_of_16_bit_log_probabilities(dev):
+    logp, old, _, adv, mask = tokens(3, 9, seed=2)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    leaf = put(logp).bfloat16().requires_grad_()
+    loss, _ = _ops().grpo_policy_loss(leaf, put(old), put(adv), put(mask))
+    loss.backward()
+    want, _, grad = P.policy_loss(leaf.detach().cpu().double().numpy(), old, adv, mask)
+    assert close(loss, want, 8.0 * float(np.abs(adv).max()), mask.size)
+    assert leaf.grad.dtype == torch.bfloat16
+    within(leaf.grad, grad, (2.0 ** -8 + E) * np.abs(grad))
+
+
+@pytest.mark.parametrize("rows", [4, 700])  # cut over workgroups, and not
+def test_the_parts_captured_and_replayed(dev, rows):
+    """token_logprobs, grpo_policy_loss and their gradients in one graph, replayed with
+    other inputs between eager work."""
+    vocab = 20001
+    g = torch.Generator(device=dev).manual_seed(4)
+
+    def inputs():
+        x = torch.randn(2, rows // 2, vocab, generator=g, device=dev).bfloat16()
+        ids = torch.randint(0, vocab, (2, rows // 2), generator=g, device=dev)
+        old = -10 + torch.randn(2, rows // 2, generator=g, device=dev)
+        mask = torch.rand(2, rows // 2, generator=g, device=dev) < 0.7
+        return [x, ids, old, torch.randn(2, generator=g, device=dev), mask]
+
+    def step(v):
+        lp, ent = _ops().token_logprobs(v[0], v[1], v[4], return_entropy=True)
+        loss, m = _ops().grpo_policy_loss(lp, v[2], v[3], v[4], normalizer="sequences")
+        return [lp.detach(), ent, loss.detach(), m, *torch.autograd.grad(loss, v[0])]
+
+    sets = [inputs() for _ in range(3)]
+    want = []
+    for v in sets:
+        want.append(step([v[0].clone().requires_grad_(), *v[1:]]))
+    held = [t.clone() for t in sets[0]]
+    held[0].requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(held)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(held)
+    for k in (0, 1, 2, 1):
+        with torch.no_grad():
+            for h, v in zip(held, sets[k]):
+                h.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(out, want[k]):
+            assert torch.equal(u, v)
+        step([sets[k][0].clone().requires_grad_(), *sets[k][1:]])
+        torch.cuda.synchronize()

@@ -222,3 +222,32 @@ def test_the_gradients_rows_stand_as_the_logits_do(make, kept):
             assert (g.untyped_storage().data_ptr() + 2 * a - r) % 16 == 0
     else:
         assert g.is_contiguous()
+
+
+def test_layers_with_counter_dropout():
+    """Injected layers carry the dropout asked for; eval mode and p = 0 drop nothing."""
+    from grpo_mi355x.core.lora import inject_lora_layers
+    from grpo_mi355x.core.nf4 import Linear4bitNF4
+
+    def model():
+        m = torch.nn.Module()
+        m.q_proj = Linear4bitNF4.from_weight(torch.randn(32, 64) * 0.02, None)
+        return m
+
+    for kw, kind in ((dict(), torch.nn.Identity), (dict(dropout=0.1), torch.nn.Dropout),
+                     (dict(dropout=0.1, counter_dropout=True), dropout.CounterDropout),
+                     (dict(counter_dropout=True), torch.nn.Identity)):
+        m = model()
+        assert inject_lora_layers(m, ["q_proj"], rank=4, verbose=False, **kw) == 1
+        assert type(m.q_proj.lora_dropout) is kind
+    d = dropout.CounterDropout(0.1)
+    x = torch.ones(3)
+    assert d.active() and not d.eval().active() and d(x) is x
+    assert dropout.CounterDropout(0.0)(x) is x and "p=0.1" in repr(d)
+    with pytest.raises(ValueError, match="dropout p"):
+        dropout.CounterDropout(1.0)
+    torch.manual_seed(3)
+    a = dropout.CounterDropout.draw(torch.device("cpu"))
+    torch.manual_seed(3)
+    assert torch.equal(a, dropout.CounterDropout.draw(torch.device("cpu")))
+    assert a.dtype == torch.int64 and a.shape == (2,)
