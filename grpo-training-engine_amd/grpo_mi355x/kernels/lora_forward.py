@@ -365,8 +365,7 @@ class FusedLoRADropoutFunction(torch.autograd.Function):
 def _dropout_of(dropout, rng, device):
     """(p, rng) of the counter-based dropout asked for, or None where nothing is dropped;
     any other dropout is refused."""
-    p = (0.0 if dropout is None or type(dropout) is torch.nn.Identity
-         else getattr(dropout, "p", 0.0))
+    p = getattr(dropout, "p", 0.0)
     if not p or not p > 0.0:
         return None
     counter = isinstance(dropout, CounterDropout)
@@ -396,7 +395,8 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
         dropout = getattr(lora_layer, "lora_dropout", None)
     if base_layer is None or lora_A is None or lora_B is None or scaling is None:
         raise ValueError("Provide lora_layer or base_layer/lora_A/lora_B/scaling for fused LoRA.")
-    drop = _dropout_of(dropout, dropout_rng, x.device)
+    drop = (None if dropout is None or type(dropout) is torch.nn.Identity
+            else _dropout_of(dropout, dropout_rng, x.device))
 
     weight_4bit = getattr(base_layer, "weight", None)
     lora_A_weight = getattr(lora_A, "weight", lora_A)
