@@ -29,7 +29,7 @@
 //    (loss_rows_kernel), so the logits are read once and their gradient written once. 4096
 //    rows of 151936 bf16, three quarters of them counted, in 406 us: 2.18 GB at 5.4 TB/s (a
 //    copy of 1 GiB runs at 4.8 to 5.15), where a pass for the sums and one for the gradient
-//    took 168 + 409. Rows beyond 311296 bytes take these two.
+//    took 168 + 409. A few long rows still take these two.
 //  * the loss from log-probabilities: 17 bytes a token; its time is that of its launches.
 #include <type_traits>
 #include <algorithm>
@@ -317,9 +317,9 @@ __device__ __noinline__ PlainStat plain_stat(const void* row, int V, float k, fl
   return PlainStat{S, t, top};
 }
 
-constexpr int AHEAD = 8;  // vectors a thread has on their way
-// Vectors [i0, i1) of a row, and the values around the vectors if `odd`, added to s.
-template <int DT, bool ENT, bool ONCE, int NT>
+// Vectors [i0, i1) of a row, and the values around the vectors if `odd`, added to s; AHEAD
+// vectors of a thread are on their way.
+template <int DT, bool ENT, bool ONCE, int NT, int AHEAD = 8>
 __device__ __forceinline__ void add_span(const Span<DT>& sp, int i0, int i1, bool odd,
                                          const Rows& q, Sums<ENT>& s) {
   auto load = [&](int i) __attribute__((always_inline)) {
@@ -875,7 +875,12 @@ __global__ void __launch_bounds__(256) scale_kernel(const double* coef, const fl
 // one waits, so that stretch is kept short: the token's inputs are loaded with the row, the
 // ratio and exp(ref - logp) are made of the token's exponent and S without a logarithm, and
 // logp itself is left to policy_kernel.
-template <int DT, int NT_, int NV>
+//
+// REST: a row that does not fit into registers (19 vectors a thread, 311296 bytes). What is
+// left is read again for the gradient and found in the last-level cache, since 256 rows are
+// under way, a CU each, and 256 MB hold 1 MB of each: 2048 x 151936 float32 477 us, 5.2 TB/s of
+// logits and gradient, where a pass for the sums and one for the gradient took 680.
+template <int DT, int NT_, int NV, bool REST>
 __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tokens t,
                                                            float inv_t, double2* parts,
                                                            RowStat* stat, float* coef,
@@ -900,11 +905,13 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
   // thread loads NV vectors in any case, at scalar addresses: were some loads skipped, the
   // compiler could not tell how many are behind the one it needs, and would wait for all.
   const int last = max(sp.nvec - NT_, 0), tail0 = min(tid, max(sp.nvec - 1, 0));
-  auto start = [&](int i) __attribute__((always_inline)) { return min(i * NT_, last); };
-  auto in_stride = [&](int i) __attribute__((always_inline)) {
-    return i ? tid >= i * NT_ - start(i) : tid < sp.nvec;
+  auto start = [&](int i) __attribute__((always_inline)) {
+    return REST ? i * NT_ : min(i * NT_, last);
   };
-  const uint4* const vec = sp.nvec ? sp.vec : reinterpret_cast<const uint4*>(parts);
+  auto in_stride = [&](int i) __attribute__((always_inline)) {
+    return REST || (i ? tid >= i * NT_ - start(i) : tid < sp.nvec);
+  };
+  const uint4* const vec = REST || sp.nvec ? sp.vec : reinterpret_cast<const uint4*>(parts);
   uint4 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) v[i] = load_stream(vec + start(i) + tail0);
@@ -932,6 +939,7 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
       s.add(f, q);
     }
   }
+  if (REST) add_span<DT, false, false, NT_, 4>(sp, NV * NT_, sp.nvec, false, q, s);
   const float odd = to_float<DT>(raw_odd);
   if (tid < sp.odd) {
     const float x[1] = {odd};
@@ -979,6 +987,20 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
     if (in_stride(i))
       store_stream(o + (int64_t)start(i) * 16 + tid * 16, grad_vector<DT>(vg, v[i]));
   }
+  if (REST) {
+    constexpr int AHEAD = 4;
+    int i = NV * NT_ + tid;
+    for (; i + (AHEAD - 1) * NT_ < sp.nvec; i += AHEAD * NT_) {
+      uint4 u[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) u[k] = load_stream(sp.vec + i + k * NT_);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        store_stream(o + (int64_t)(i + k * NT_) * 16, grad_vector<DT>(vg, u[k]));
+    }
+    for (; i < sp.nvec; i += NT_)
+      store_stream(o + (int64_t)i * 16, grad_vector<DT>(vg, load_stream(sp.vec + i)));
+  }
   if (tid < sp.odd) {
     const int at = sp.odd_at(tid);
     const float y = grad_value(g, odd);
@@ -987,7 +1009,8 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
   // the token's own value, by the thread that stored its vector (its later store to the
   // same place comes after)
   const int at_id = (g.id - sp.head) / PER<DT>;
-  if (g.id >= sp.head && g.id < sp.tail && at_id - start(at_id / NT_) == tid)
+  const int owner = REST ? at_id % NT_ : at_id - start(at_id / NT_);
+  if (g.id >= sp.head && g.id < sp.tail && owner == tid)
     store1<DT>(out, g.id, grad_value(g, to_float<DT>(raw)) + g.c);
 }
 
@@ -1103,9 +1126,6 @@ int run_logp(int dtype, const Rows& q, int64_t R, const LogpOut& o, void* parts,
   return go(std::integral_constant<int, F32>{});
 }
 
-// Rows of at most this many vectors stay in registers: 19 a thread of a workgroup that fills
-// a CU's registers.
-constexpr int64_t HELD = 19 * 1024;
 int64_t row_vectors(int dtype, int V) { return ((int64_t)V * (dtype == F32 ? 4 : 2) + 15) / 16; }
 int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const float* coef,
              const float* scale, double temperature, const Grad& grad, bool skip_one, hipStream_t st) {
@@ -1114,8 +1134,8 @@ int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const flo
   // with a gradient that is most likely there already, few workgroups to find that out; fewer
   // than 4096 rows are cut over several, of 1024 vectors or more each (993 x 50257 float32: 59
   // us with one each, 53)
-  const dim3 grid(skip_one && n > 1024 ? 1024u : (unsigned)n,
-                  n < 4096 ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(4096 / n, row_vectors(dtype, q.V) / 1024)) : 1u);
+  const int64_t cuts = std::min<int64_t>(4096 / n, row_vectors(dtype, q.V) / 1024);
+  const dim3 grid(skip_one && n > 1024 ? 1024u : (unsigned)n, cuts > 1 ? (unsigned)cuts : 1u);
   if (dtype == BF16)
     logits_grad_kernel<BF16><<<grid, NT, 0, st>>>(q, n, stat, coef, scale, inv_t, grad, skip_one);
   else if (dtype == F16)
@@ -1125,18 +1145,26 @@ int run_grad(int dtype, const Rows& q, int64_t R, const RowStat* stat, const flo
   return launch_check("token_logprobs_backward");
 }
 
-bool rows_held(int dtype, int V) { return row_vectors(dtype, V) <= HELD; }
+// Whether loss and gradient are made by a workgroup a row. Few long rows are cut over the chip
+// instead, for the sums and then for the gradient; us with a workgroup a row / with rows cut:
+//   50257 float32     4 rows 15 / 17, 64 rows 15 / 16, 192 rows 22 / 26
+//   151936 bfloat16   4 rows 23 / 16, 64 rows 24 / 19, 128 rows 25 / 27, 192 rows 30 / 38
+//   151936 float32    64 rows 28 / 24, 128 rows 40 / 43, 512 rows 125 / 173, 2048 rows 477 / 680
+//   262144 bfloat16   128 rows 45 / 41, 256 rows 66 / 72, 2048 rows 453 / 586
+bool by_rows(int dtype, int64_t R, int V) {
+  return row_vectors(dtype, V) <= 14 * 1024 || R >= 128;
+}
 
 template <int DT>
 int launch_loss_rows(const Rows& q, int64_t R, const Policy& p, const Tokens& t, float inv_t,
                      double2* parts, RowStat* stat, float* coef, const Grad& grad, hipStream_t st) {
-  // the smallest of these that holds the row: loads past it are loads all the same
   const int64_t vecs = row_vectors(DT, q.V);
-  auto go = [&](auto threads, auto each) {
+  auto go = [&](auto threads, auto each, auto rest) {
     constexpr int NT_ = decltype(threads)::value, NV = decltype(each)::value;
-    if (vecs > NT_ * NV) return false;
-    loss_rows_kernel<DT, NT_, NV><<<(unsigned)R, NT_, 0, st>>>(q, p, t, inv_t, parts, stat, coef,
-                                                               grad);
+    constexpr bool REST = decltype(rest)::value;
+    if (!REST && vecs > NT_ * NV) return false;
+    loss_rows_kernel<DT, NT_, NV, REST>
+        <<<(unsigned)R, NT_, 0, st>>>(q, p, t, inv_t, parts, stat, coef, grad);
     return true;
   };
   const std::integral_constant<int, 256> n256;
@@ -1145,11 +1173,12 @@ int launch_loss_rows(const Rows& q, int64_t R, const Policy& p, const Tokens& t,
   const std::integral_constant<int, 10> v10;
   const std::integral_constant<int, 14> v14;
   const std::integral_constant<int, 19> v19;
-  if (!(go(n256, v10) || go(n256, v19) || go(n512, v14) || go(n512, v19) || go(n1024, v14) ||
-        go(n1024, v19))) {
-    set_error("row too long");
-    return GRPO_EUNSUPPORTED;
-  }
+  const std::integral_constant<int, DT == F32 ? 16 : 10> some;
+  const std::false_type whole;
+  // the smallest of these that holds the row (loads past it are loads all the same), or the
+  // one that reads what it cannot hold twice, with registers left to do so
+  go(n256, v10, whole) || go(n256, v19, whole) || go(n512, v14, whole) || go(n512, v19, whole) ||
+      go(n1024, v14, whole) || go(n1024, v19, whole) || go(n1024, some, std::true_type{});
   return launch_check("policy_loss_rows");
 }
 
@@ -1314,8 +1343,8 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   if ((R && !logp) || !loss || !metrics) return einval("null pointer");
   if ((stat == nullptr) != (coef == nullptr)) return einval("stat and coef go together");
   if (!aligned16(stat)) return einval("stat must be 16-byte aligned");
-  if (grad_logits && R && (!stat || !rows_held(dtype, V)))
-    return einval("grad_logits needs stat and coef and a row of at most 311296 bytes");
+  if (grad_logits && R && (!stat || !by_rows(dtype, R, V)))
+    return einval("grad_logits needs stat and coef, and rows that are made in one pass");
   if (grad_logits) {
     if (int rc = grad_check(grad_logits, dtype, grad_stride_b, grad_stride_s)) return rc;
   }
@@ -1349,8 +1378,9 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   return run_policy(*policy, t, R <= 1024, ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
 }
 
-extern "C" int grpo_policy_loss_logits_held(int dtype, int V) {
-  return dtype >= 0 && dtype <= 2 && V >= 1 && rows_held(dtype, V);
+extern "C" int grpo_policy_loss_logits_one_pass(int dtype, int B, int S, int V) {
+  return dtype >= 0 && dtype <= 2 && B >= 0 && S >= 0 && V >= 1 &&
+         by_rows(dtype, (int64_t)B * S, V);
 }
 
 extern "C" int grpo_policy_loss_logits_rescale(const void* logits, int dtype, int64_t stride_b,

@@ -105,7 +105,7 @@ SIGNATURES = {
     "grpo_policy_loss_logits": (
         _I32, [*_ROWS, _VP, _VP, _VP, _I32, _POLICY, _VP, _VP, _VP, _VP, _VP, _VP, _I64, _I64,
                _VP, _SZ, _VP]),
-    "grpo_policy_loss_logits_held": (_I32, [_I32, _I32]),
+    "grpo_policy_loss_logits_one_pass": (_I32, [_I32, _I32, _I32, _I32]),
     "grpo_policy_loss_logits_rescale": (
         _I32, [*_ROWS, _VP, _VP, _VP, _VP, _I64, _I64, _VP]),
     "grpo_dropout": (_I32, [_VP, _VP, _I64, _I32, _c.c_double, _VP, _VP]),

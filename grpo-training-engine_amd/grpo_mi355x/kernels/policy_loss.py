@@ -344,21 +344,21 @@ def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
 
 @functools.lru_cache(maxsize=256)
 def _logits_plan(dtype: int, b: int, s: int, v: int):
-    """(workspace bytes, whether a row stays in a workgroup's registers)."""
+    """(workspace bytes, whether the gradient is made with the loss)."""
     lib = _lib.library()
     return (lib.grpo_policy_loss_logits_workspace_bytes(dtype, b, s, v),
-            bool(lib.grpo_policy_loss_logits_held(dtype, v)))
+            bool(lib.grpo_policy_loss_logits_one_pass(dtype, b, s, v)))
 
 
 def _logits_loss(logits, ids, mask, t, tokens, policy, train: bool):
     old, ref, adv, per_token = tokens
     x, rows = _rows(logits, ids, mask, t)
     dev, (b, s, v) = x.device, x.shape
-    nbytes, held = _logits_plan(rows[1], b, s, v)
+    nbytes, one_pass = _logits_plan(rows[1], b, s, v)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     metrics = torch.empty(4, dtype=torch.float32, device=dev)
     logp = torch.empty(ids.shape, dtype=torch.float32, device=dev)
-    grad, sb, ss = _empty_grad(logits, x) if train and held else (None, 0, 0)
+    grad, sb, ss = _empty_grad(logits, x) if train and one_pass else (None, 0, 0)
     # what the backward needs of each row (16 bytes of statistics, 4 of its derivative), then
     # the workspace
     keep = -(-20 * b * s // 256) * 256 if train else 0
@@ -414,9 +414,10 @@ def fused_grpo_loss(logits: torch.Tensor, token_ids: torch.Tensor,
 
     ``logits [batch, seq, V]``; the other arguments are those of the two operators.
     Differentiable by ``logits`` alone; ``logps`` (float32, 0 where not counted) and
-    ``metrics`` carry no gradient.  Rows of up to 311296 bytes are read once: their gradient
-    is made with the loss, for an upstream gradient of 1, and the backward hands it out (or
-    computes it again where the upstream gradient is another, and for a second backward)."""
+    ``metrics`` carry no gradient.  The logits' gradient is made with the loss, for an
+    upstream gradient of 1, and the backward hands it out (or computes it again where the
+    upstream gradient is another, and for a second backward); fewer than 128 rows of more than
+    229376 bytes get theirs in the backward."""
     policy = _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps)
     if logits.ndim != 3:
         raise ValueError(f"logits must be [batch, seq, vocab], got {list(logits.shape)}.")

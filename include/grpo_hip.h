@@ -152,8 +152,8 @@ int grpo_policy_loss_backward(const double* coef, const float* grad_loss, int64_
  * its scale.
  *   grad_logits : placed as in grpo_token_logprobs_backward, or NULL: the gradient of the loss
  *                 itself (its upstream gradient 1), made in the same pass over the logits;
- *                 needs stat and coef and a vocabulary that grpo_policy_loss_logits_held
- *                 takes (a row stays in one workgroup's registers) */
+ *                 needs stat and coef and grpo_policy_loss_logits_one_pass to hold (rows
+ *                 of more than 229376 bytes need to be 128 or more) */
 size_t grpo_policy_loss_logits_workspace_bytes(int dtype, int B, int S, int V);
 int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b, int64_t stride_s,
                             int B, int S, int V, const int64_t* ids, const uint8_t* mask,
@@ -162,7 +162,7 @@ int grpo_policy_loss_logits(const void* logits, int dtype, int64_t stride_b, int
                             float* loss, float* logp, float* metrics, float* stat, float* coef,
                             void* grad_logits, int64_t grad_stride_b, int64_t grad_stride_s,
                             void* workspace, size_t workspace_bytes, grpo_stream_t stream);
-int grpo_policy_loss_logits_held(int dtype, int V);
+int grpo_policy_loss_logits_one_pass(int dtype, int B, int S, int V);
 /* grad_logits of the call above for an upstream gradient *grad_loss: left as it is where
  * that is 1, computed again from the logits otherwise (decided on the device). */
 int grpo_policy_loss_logits_rescale(const void* logits, int dtype, int64_t stride_b,

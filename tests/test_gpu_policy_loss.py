@@ -412,7 +412,7 @@ def loss_inputs(b, s, vocab, dtype, seed, t=1.0, beta=0.04):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("b, s, vocab", [(1, 1, 9), (300, 30, 65), (1100, 1, 17), (3, 5, 1000), (4, 33, 4097), (2, 3, 151936),
-                                         (1, 2, 262147), (40, 16, 300)])
+                                         (1, 2, 262147), (40, 16, 300), (8, 16, 151936), (8, 16, 160003)])
 @pytest.mark.parametrize("normalizer, t, beta", [("tokens", 1.0, 0.0), ("sequences", 0.7, 0.04)])
 def test_fused_loss_and_gradient(dev, dtype, b, s, vocab, normalizer, t, beta):
     x, ids, old, ref, adv, mask, logp, p = loss_inputs(b, s, vocab, dtype, seed=vocab + b, t=t,

@@ -120,10 +120,11 @@ def test_c_entry_wants_a_workspace_where_rows_are_cut(lib):
     assert lib.grpo_token_logprobs(*args, FAKE, need - 1, None) == -3
 
 
-def test_rows_that_stay_in_registers(lib):
-    held = lib.grpo_policy_loss_logits_held
-    assert [held(0, v) for v in (1, 151936, 152064, 155648, 155649, 0)] == [1, 1, 1, 1, 0, 0]
-    assert [held(2, v) for v in (50257, 77824, 77825)] == [1, 1, 0] and held(3, 8) == 0
+def test_rows_that_are_made_in_one_pass(lib):
+    one = lib.grpo_policy_loss_logits_one_pass
+    assert [one(0, 2, 3, v) for v in (1, 114688, 114689, 0)] == [1, 1, 0, 0]
+    assert [one(2, 2, 3, v) for v in (50257, 57344, 57345)] == [1, 1, 0] and one(3, 2, 3, 8) == 0
+    assert [one(2, 8, s, 151936) for s in (15, 16)] == [0, 1]
 
 
 def test_c_entry_refuses_a_gradient_it_cannot_make(lib):
