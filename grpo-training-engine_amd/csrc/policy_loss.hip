@@ -239,9 +239,10 @@ __device__ __forceinline__ Joined join(const Sums<ENT>& s, JoinSpace<NT>& red) {
   __syncthreads();
   return gather<ENT, NT>(red);
 }
-__device__ __forceinline__ bool usable(const Joined& j) {
-  return j.S > 0.0 && j.S < (double)INFINITY;
-}
+// Whether S can be the sum of up to 2^30 terms of which the largest is near 1. Beyond: nothing
+// above -1e30, values that are not finite, or |x k| so large (2^27) that M, a float32, is no
+// longer near it.
+__device__ __forceinline__ bool usable(const Joined& j) { return j.S > 0x1p-8 && j.S < 0x1p40; }
 
 template <int NT>
 __device__ __forceinline__ double block_sum64(double v, JoinSpace<NT>& red) {
@@ -279,8 +280,7 @@ __device__ __forceinline__ float top_of(const float (&f)[PER<DT>]) {
   return top;
 }
 
-// The statistics of a row whose sums came out 0 or not finite: nothing above -1e30, or
-// values that are not finite. The maximum, then the sum against it.
+// The statistics of a row whose sums are not usable: the maximum, then the sum against it.
 struct PlainStat {
   double S, t;
   float m;
@@ -699,40 +699,6 @@ struct TokenSums {
   double v[5];
 };
 
-// Counted tokens and sequences of the batch, the same in every thread; counts: [B] or
-// null (S each).
-template <int NT_>
-__device__ __forceinline__ void totals(const int* counts, int B, int S, double* red,
-                                       double* tokens, double* seqs) {
-  if (!counts) {
-    *tokens = (double)B * S;
-    *seqs = B;
-    return;
-  }
-  double n = 0.0, q = 0.0;
-  for (int b = threadIdx.x; b < B; b += NT_) {
-    const int c = counts[b];
-    n += c;
-    q += c > 0;
-  }
-  n = wave_sum64(n);
-  q = wave_sum64(q);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    red[threadIdx.x >> 6] = n;
-    red[NT_ / 64 + (threadIdx.x >> 6)] = q;
-  }
-  __syncthreads();
-  n = q = 0.0;
-  for (int w = 0; w < NT_ / 64; ++w) {
-    n += red[w];
-    q += red[NT_ / 64 + w];
-  }
-  __syncthreads();
-  *tokens = n;
-  *seqs = q;
-}
-
 // One token of ratio r and eq = exp(ref - logp): d l / d logp.
 struct Slope {
   double d, gain;
@@ -1065,11 +1031,14 @@ int rows_check(const void* x, int dtype, int64_t sb, int64_t ss, int B, int S, i
   if (int rc = batch_check(B, S)) return rc;
   if ((int64_t)B * S >= (1 << 22)) return einval("2^22 rows of logits or more");
   if (V < 1) return einval("an empty vocabulary");
+  // a thread's index and a stride beyond it stay ints
+  if (V > 1 << 30) return einval("a vocabulary of more than 2^30 tokens");
   if (dtype < 0 || dtype > 2) return einval("dtype must be 0 (bf16), 1 (float16) or 2 (float32)");
   if (!(temperature > 0.0) || !(temperature < (double)INFINITY))
     return einval("temperature must be positive and finite");
   const float k = (float)(1.0 / LN2 / temperature);
-  if (!(k >= 1e-30f) || !(k <= 1e30f)) return einval("temperature out of range");
+  // (from 1e-20 on, what khi leaves of k is a normal float32 above 0)
+  if (!(k >= 1e-20f) || !(k <= 1e30f)) return einval("temperature out of range");
   if ((int64_t)B * S == 0) return GRPO_OK;
   if (!x || !ids) return einval("null pointer");
   if (sb < 0 || ss < 0) return einval("negative row stride");

@@ -14,11 +14,16 @@ from .. import _lib
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-def check_dropout(p: float, rng: torch.Tensor, device: torch.device) -> float:
-    """``p`` as a float, after the checks that every dropout entry point makes."""
+def _check_p(p: float) -> float:
     p = float(p)
     if not (0.0 <= p and p * 65536.0 + 0.5 < 65536.0):
         raise ValueError(f"dropout p must be in [0, 1) (in steps of 1/65536), got {p}.")
+    return p
+
+
+def check_dropout(p: float, rng: torch.Tensor, device: torch.device) -> float:
+    """``p`` as a float, after the checks that every dropout entry point makes."""
+    p = _check_p(p)
     if rng.dtype != torch.int64 or rng.numel() != 2 or not rng.is_contiguous():
         raise ValueError("rng must be a contiguous int64 tensor of two values, seed and offset.")
     if rng.device != device:
@@ -84,9 +89,7 @@ class CounterDropout(torch.nn.Module):
 
     def __init__(self, p: float = 0.5):
         super().__init__()
-        if not 0.0 <= p < 1.0:
-            raise ValueError(f"dropout p must be in [0, 1), got {p}.")
-        self.p = float(p)
+        self.p = _check_p(p)
 
     @staticmethod
     def draw(device: torch.device) -> torch.Tensor:

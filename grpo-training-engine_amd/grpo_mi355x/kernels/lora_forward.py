@@ -31,6 +31,7 @@ backward that is itself differentiated run the same products as torch ops.
 
 from __future__ import annotations
 
+import contextlib
 from typing import Optional
 
 import torch
@@ -238,7 +239,8 @@ def _run_forward(x, weight_4bit, quant_state, lora_A, lora_B, scaling, bias, dro
               if drop is not None or train_forward_pays(m, n, k, r, blocksize, dt) else 0)
     if drop is not None and m and not nbytes:
         raise ValueError("dropout in the fused linear needs N and K to be multiples of 32, "
-                         "a rank of at most 32 and a power-of-two blocksize >= 32.")
+                         "adapters of x's type, of rank 32 at most, and a power-of-two "
+                         "blocksize >= 32.")
     if nbytes:
         if bias is not None and (bias.dtype != dt or not bias.is_contiguous()):
             bias = bias.to(dt).contiguous()
@@ -407,9 +409,11 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
         args = (x, weight_4bit, weight_4bit.quant_state, lora_A_weight, lora_B_weight,
                 float(scaling), getattr(base_layer, "bias", None))
         if drop is not None:
-            if torch.is_grad_enabled():
-                return FusedLoRADropoutFunction.apply(*args, *drop)
-            return _run_forward(*args, drop)[0]
+            away = x.is_cuda and x.device.index != torch.cuda.current_device()
+            with torch.cuda.device(x.device) if away else contextlib.nullcontext():
+                if torch.is_grad_enabled():
+                    return FusedLoRADropoutFunction.apply(*args, *drop)
+                return _run_forward(*args, drop)[0]
         # With nothing to record (no grad mode, no forward-mode level, no transform)
         # the autograd function's own bookkeeping, 5 us of a decode call's 25, is left out.
         if not torch.is_grad_enabled() and fwAD._current_level < 0 and \

@@ -32,6 +32,7 @@ from .. import _lib
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NORMALIZERS = {"tokens": 0, "sequences": 1}
 _MAX_ROWS = 1 << 22
+_MAX_VOCAB = 1 << 30
 
 
 def _run(device: torch.device, name: str, *args) -> None:
@@ -108,6 +109,8 @@ def _check_logits(logits, token_ids, mask, temperature):
         raise ValueError(f"token_ids must be on {logits.device}, got {token_ids.device}.")
     if not vocab:
         raise ValueError("logits must have a vocabulary of at least one token.")
+    if vocab > _MAX_VOCAB:
+        raise ValueError(f"a vocabulary of at most {_MAX_VOCAB} tokens, got {vocab}.")
     if lead.numel() >= _MAX_ROWS:
         raise ValueError(f"at most {_MAX_ROWS - 1} rows of logits in a call.")
     t = float(temperature)
@@ -256,6 +259,8 @@ def _check_tokens(shape, device, old_logps, ref_logps, advantages):
     """(old, ref, advantages as float32, whether these are per token) that fit ``shape``."""
     if len(shape) != 2:
         raise ValueError(f"positions must be [batch, seq], got {list(shape)}.")
+    if shape[0] >= 1 << 23 or shape.numel() >= 1 << 31:
+        raise ValueError(f"fewer than 2^23 sequences and 2^31 tokens, got {list(shape)}.")
     per_token = advantages.ndim == 2
     return (_float_rows(old_logps, "old_logps", shape, device),
             _float_rows(ref_logps, "ref_logps", shape, device),

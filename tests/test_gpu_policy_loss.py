@@ -259,11 +259,37 @@ def test_refusals_on_the_device(dev):
             ops.token_logprobs(x, ids, temperature=t)
     with pytest.raises(ValueError, match="batch, seq, vocab"):
         ops.fused_grpo_loss(x[0], ids[0], None, torch.zeros(3, device=dev))
+    wide = x[:1, :1, :1].expand(1, 1, 2 ** 30 + 1)  # no memory of its own
+    with pytest.raises(ValueError, match="vocabulary of at most"):
+        ops.token_logprobs(wide, ids[:1, :1])
+    for shape in ((1, 2 ** 31), (2 ** 23, 1)):
+        with pytest.raises(ValueError, match="2.23 sequences"):
+            ops.grpo_policy_loss(x[0, :1, :1].expand(shape), None, x[0, 0, :1].expand(shape[0]))
     leaf = x.clone().requires_grad_()
     got = ops.token_logprobs(leaf, ids)
     grad, = torch.autograd.grad(got.sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):  # no second derivative
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("t", [1e-20, 1e-10, 3e-9, 1e-8, 1e-7, 1e20])
+def test_temperatures_at_the_ends(dev, t):
+    """Ties share a row whatever the temperature; -inf and (below) anything less has none.
+    Exponents reach 8 in size, with two roundings of 2^-24 each: 2^-20 of ln 2 and up."""
+    x = torch.full((1, 4, 1001), -math.inf, device=dev)
+    x[0, 0, :10], x[0, 1, 5:9], x[0, 2, 1000], x[0, 3, ::7] = 2.3, -3.1, 0.0, 29.7
+    if t < 1.0:
+        x[0, :, 501] = -4.0
+    ids = torch.tensor([[3, 8, 1000, 7]], device=dev)
+    n = torch.tensor([[10.0, 4.0, 1.0, 143.0]], dtype=torch.float64, device=dev)
+    leaf = x.requires_grad_()
+    got = _ops().token_logprobs(leaf, ids, temperature=t)
+    assert torch.allclose(got.double(), -n.log(), rtol=2.0 ** -20, atol=0.0)
+    # the gradient times T: 1 - 1 / n at the token, -1 / n at the ties, 0 elsewhere
+    grad, = torch.autograd.grad(got.sum() * t, leaf)
+    want = -(x.detach() == x.detach().amax(-1, keepdim=True)).double() / n[..., None]
+    want.scatter_add_(2, ids[..., None], torch.ones_like(want[..., :1]))
+    assert torch.allclose(grad.double(), want, rtol=2.0 ** -18, atol=1e-30)
 
 
 # ------------------------------------------------------------- policy loss --

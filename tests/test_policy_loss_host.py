@@ -103,7 +103,8 @@ def _rows(lib, dtype=0, sb=8, ss=8, b=2, s=3, v=8, ids=FAKE, t=1.0, x=FAKE, logp
 @pytest.mark.parametrize("kw", [
     dict(dtype=3), dict(sb=-1), dict(b=-1), dict(v=0), dict(ids=None), dict(t=0.0),
     dict(t=math.inf), dict(t=math.nan), dict(t=1e-36), dict(x=None), dict(x=FAKE + 1),
-    dict(logp=None), dict(stat=FAKE + 4), dict(b=1 << 20, s=4),
+    dict(logp=None), dict(stat=FAKE + 4), dict(b=1 << 20, s=4), dict(v=(1 << 30) + 1),
+    dict(t=1e21),
 ])
 def test_c_entry_refuses_logits(lib, kw):
     assert _rows(lib, **kw) == -1, lib.grpo_last_error()
@@ -247,6 +248,8 @@ def test_layers_with_counter_dropout():
     assert dropout.CounterDropout(0.0)(x) is x and "p=0.1" in repr(d)
     with pytest.raises(ValueError, match="dropout p"):
         dropout.CounterDropout(1.0)
+    with pytest.raises(ValueError, match="dropout p"):
+        dropout.CounterDropout(1 - 2 ** -18)  # rounds to 1 in steps of 1/65536
     torch.manual_seed(3)
     a = dropout.CounterDropout.draw(torch.device("cpu"))
     torch.manual_seed(3)
