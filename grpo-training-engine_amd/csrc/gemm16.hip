@@ -200,6 +200,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
       float v[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        if (MODE == GEMM16_ADD_DROP) {  // one rounding, below
+          v[q] = acc[i][j][q] +
+                 (drop_keeps(bits, 4 * (j & 1) + q, g.drop.threshold) ? u[q] : 0.f);
+          continue;
+        }
         v[q] = round_e<F16>(acc[i][j][q]);
         float w = round_e<F16>(u[q]);
         if (MODE == GEMM16_LORA) {
@@ -208,9 +213,6 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
                 v[q] + e2f<F16>((uint16_t)(bias[2 * j + (q >> 1)] >> (16 * (q & 1)))));
           w = round_e<F16>(w * sc);
         }
-        if (MODE == GEMM16_ADD_DROP)
-          w = drop_keeps(bits, 4 * (j & 1) + q, g.drop.threshold) ? round_e<F16>(w * g.drop.scale)
-                                                                  : 0.f;
         v[q] += w;
       }
       o[2 * j] = pack_e2<F16>(v[0], v[1]);

@@ -8,7 +8,8 @@ namespace grpo {
 // C[m, n] = dt(sum_k A[m, k] B[n, k]), both operands contiguous along k, then
 //   GEMM16_ADD   C = dt(C + dt(t low^T))
 //   GEMM16_LORA  C = dt(dt(C [+ bias]) + dt(dt(t low^T) * dt(scaling)))
-//   GEMM16_ADD_DROP  C = dt(C + drop(dt(t low^T))), the mask of a contiguous [M][N]
+//   GEMM16_ADD_DROP  C = dt(A B^T + keep(t low^T)), keep: 0 where the mask of a contiguous
+//                    [M][N] drops, unscaled
 enum Gemm16Mode { GEMM16_ADD, GEMM16_LORA, GEMM16_ADD_DROP };
 
 struct Gemm16 {

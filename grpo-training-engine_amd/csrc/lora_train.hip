@@ -5,13 +5,18 @@
 //   xa = dt(x A^T)                    gi = dt(dt(g * dt(s)) B)
 //   grad_A = dt(gi^T x)               grad_B = dt(dt(g * dt(s))^T xa)
 //   grad_x = dt(dt(g W) + dt(gi A))   y = dt(dt(dt(x W^T) [+ bias]) + dt(dt(t B^T) * dt(s)))
-// With dropout on the adapter's input, drop(x) = dt(x * scale) where kept and 0 elsewhere
-// (philox.hpp), x is drop(x) in xa, t and grad_A, and grad_x adds drop(dt(gi A)); the mask is
-// made again in each of the four kernels that need it: 4184 rows of 3584 x 3584, r = 16, 9
-// us more than without dropout (GEMM epilogue 4, weight gradients 4, preparation 1) in 265,
-// where a mask of a byte each would be written once and read three times (60 MB, 12 us) and
-// kept from forward to backward. The rounding points are those without dropout, drop(x)
-// rounded to the type as the layer that drops ahead of A rounds it.
+// With dropout on the adapter's input, keep(x) being x where its mask keeps it and 0 elsewhere
+// (philox.hpp), the mask's scale and s are one float32 factor f on the sums of rank r, which
+// leaves x and g as they are and a rounding of each product:
+//   xa = t = dt(f keep(x) A^T)        gi = dt(f g B)
+//   grad_A = dt(gi^T keep(x))         grad_B = dt(g^T xa)
+//   grad_x = dt(g W + keep(gi A))     y = dt(dt(dt(x W^T) [+ bias]) + dt(t B^T))
+// (With the rounding points above, drop(x) and g s rounded too, the adapters' gradients were
+// 1.7 times an exact result's rounding away from 64 bits, 1.4 so.) The mask is made again in
+// each of the four kernels that need it: 4184 rows of 3584 x 3584, r = 16, 6 to 7 us more than
+// without dropout (GEMM epilogue 2, weight gradients 3, preparations 0.6 and 0.7) in 261, where
+// a mask of a byte each would be written once and read three times (60 MB, 12 us) and kept from
+// forward to backward.
 //
 // The weight is decoded once per call, not once per row tile: from about 5 million
 // outputs (fewer where the decoding GEMM's ring kernel does not run) the two passes over
@@ -152,6 +157,7 @@ struct PrepArgs {
   RowsJob job[2];  // job 0: x A^T, job 1: dt(g s) B
   int M, Mp, r, rows;
   float scaling;
+  float factor;  // with dropout: of both products' sums, and g is not scaled
   DequantJob dequant;
   const uint16_t* la;  // A [r][K]
   uint16_t* at;        // [K][32] (ranks >= r zero)
@@ -181,7 +187,7 @@ __device__ __forceinline__ void rows_product(const RowsJob& j, const PrepArgs& p
   const float sc = BT ? round_e<F16>(p.scaling) : 1.f;
   const uint16_t* const xr = j.src + (int64_t)min(m0 + ln, p.M - 1) * j.ld;
   DropKey key{};
-  if (DROP) key = drop_key(p.drop.rng);
+  if (!BT && DROP) key = drop_key(p.drop.rng);
   int rk[TC];  // ranks >= r repeat rank r - 1; their results are not used
 #pragma unroll
   for (int tc = 0; tc < TC; ++tc) rk[tc] = min(16 * tc + ln, p.r - 1);
@@ -207,10 +213,9 @@ __device__ __forceinline__ void rows_product(const RowsJob& j, const PrepArgs& p
         }
         b[tc] = keep(on, b[tc]);
       }
-      if (BT) a = scale8<F16>(a, sc);
-      if (DROP)  // the row's eight values are one block: C % 8 == 0
-        a = drop8<F16>(a, philox(((uint64_t)(m0 + ln) * j.C + cc) >> 3, key), p.drop.threshold,
-                       p.drop.scale);
+      if (BT && !DROP) a = scale8<F16>(a, sc);
+      if (!BT && DROP)  // the row's eight values are one block: C % 8 == 0
+        a = mask8(a, philox(((uint64_t)(m0 + ln) * j.C + cc) >> 3, key), p.drop.threshold);
 #pragma unroll
       for (int tc = 0; tc < TC; ++tc) acc[tc] = mfma16x16x32_e<F16>(a, b[tc], acc[tc]);
     }
@@ -230,7 +235,7 @@ __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) 
 #pragma unroll
   for (int tc = 0; tc < TC; ++tc) acc[tc] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   if (bt)
-    rows_product<TC, F16, true, false>(j, p, m0, wave, ln, lg, acc);
+    rows_product<TC, F16, true, DROP>(j, p, m0, wave, ln, lg, acc);
   else
     rows_product<TC, F16, false, DROP>(j, p, m0, wave, ln, lg, acc);
 #pragma unroll
@@ -246,7 +251,7 @@ __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) 
     float s = red[row * LD + rank];
 #pragma unroll
     for (int w = 1; w < 8; ++w) s += red[(16 * w + row) * LD + rank];
-    v = f2e<F16>(s);
+    v = f2e<F16>(DROP ? s * p.factor : s);
   }
   if (j.rows) j.rows[(int64_t)m * 32 + rank] = v;  // m < Mp: Mp % 16 == 0
   if (j.cols && rank < 16 * TC) j.cols[(int64_t)rank * p.Mp + m] = v;
@@ -285,7 +290,8 @@ __global__ void __launch_bounds__(512) train_prep_kernel(PrepArgs p) {
 constexpr int WG_C = 128;  // columns per workgroup
 
 struct WgradArgs {
-  const uint16_t* g;  // [M][N]: grad_B[n][r] = sum_m dt(g s)[m][n] xa[m][r]
+  const uint16_t* g;  // [M][N]: grad_B[n][r] = sum_m dt(g s)[m][n] xa[m][r], g as it is with
+                      // dropout
   int64_t ldg;
   const uint16_t* x;  // [M][K]: grad_A[r][k] = sum_m gi[m][r] x[m][k]
   int64_t ldx;
@@ -340,10 +346,11 @@ __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = keep(con && m + i < p.M, v[i]);  // no 0 * inf from rows past the end
-      if (isg) v[i] = scale8<F16>(v[i], sc);
-      else if (DROP)
-        v[i] = drop8<F16>(v[i], philox(((uint64_t)(m + i) * p.K + c) >> 3, key), p.drop.threshold,
-                          p.drop.scale);
+      if (isg) {
+        if (!DROP) v[i] = scale8<F16>(v[i], sc);
+      } else if (DROP) {
+        v[i] = mask8(v[i], philox(((uint64_t)(m + i) * p.K + c) >> 3, key), p.drop.threshold);
+      }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -507,6 +514,7 @@ int run_forward(const TrainCall& c, const uint16_t* bias, uint16_t* y, int64_t l
   a.Mp = (int)pad32(c.M);
   a.r = c.r;
   a.drop = c.drop;
+  a.factor = c.scaling * c.drop.scale;
   a.job[0] = RowsJob{c.x, c.ldx, c.la, c.K, rows, nullptr};
   a.rows = a.Mp / 16;
   a.dequant = DequantJob{c.w, c.absmax, c.code16, wd, c.N, c.K, c.bs_shift,
@@ -527,7 +535,7 @@ int run_forward(const TrainCall& c, const uint16_t* bias, uint16_t* y, int64_t l
   g.ldl = c.r;
   g.bias = bias;
   g.r = c.r;
-  g.scaling = c.scaling;
+  g.scaling = c.drop.threshold ? 1.f : c.scaling;  // in t already
   return gemm16_launch(g, GEMM16_LORA, F16, c.st);
 }
 
@@ -549,6 +557,7 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
   a.rows = Mp / 16;
   a.K = c.K;
   a.drop = c.drop;
+  a.factor = c.scaling * c.drop.scale;
   if (grad_b) a.job[0] = RowsJob{c.x, c.ldx, c.la, c.K, nullptr, xat};
   if (grad_x || grad_a)
     a.job[1] = RowsJob{grad, ldg, c.lb, c.N, grad_x ? rows : nullptr, grad_a ? git : nullptr};
@@ -602,7 +611,7 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
   }
   const dim3 grid((unsigned)(w.tn + (grad_a ? cdiv(c.K, WG_C) : 0)), (unsigned)S);
   w.drop = c.drop;
-  if (grad_a && c.drop.threshold) {
+  if (c.drop.threshold) {
     if (c.r > 16) lora_wgrad_kernel<2, F16, true><<<grid, 256, 0, c.st>>>(w);
     else lora_wgrad_kernel<1, F16, true><<<grid, 256, 0, c.st>>>(w);
   } else {

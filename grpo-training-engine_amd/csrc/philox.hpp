@@ -73,6 +73,19 @@ __device__ __forceinline__ uint4 drop8(uint4 x, const uint4& w, uint32_t thresho
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// Eight 16-bit values, 0 (whatever the value) where dropped and unscaled where kept, for a
+// threshold above 0. Two halves at once: w >= t is w - (t - 1) >= 1 in saturating 16 bits.
+__device__ __forceinline__ uint4 mask8(uint4 x, const uint4& w, uint32_t threshold) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 below = (u16x2)(uint16_t)(threshold - 1), one = (u16x2)(uint16_t)1;
+  auto kept = [&](uint32_t v, uint32_t u) __attribute__((always_inline)) {
+    const u16x2 on = __builtin_elementwise_min(
+        __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, u), below), one);
+    return v & __builtin_bit_cast(uint32_t, (u16x2)(-on));
+  };
+  return make_uint4(kept(x.x, w.x), kept(x.y, w.y), kept(x.z, w.z), kept(x.w, w.w));
+}
+
 // Checks of a C entry point; *out is valid when it returns GRPO_OK.
 inline int drop_args(const int64_t* rng, double p, Dropout* out) {
   if (!(p >= 0.0 && p < 1.0)) return einval("dropout p must lie in [0, 1)");

@@ -1,8 +1,8 @@
 """The NF4 + LoRA linear with counter-based dropout on the adapter's input.
 
-The kernels against float64 torch on the same rounding points (those of
-``test_gpu_lora_train``, drop(x) rounded to the type), the mask that of
-``oracle.policy_loss.dropout_factors``. Tolerance as there: the result's rounding u, and an
+The kernels against float64 torch on the same rounding points (x A^T and g B, scaled, in the
+type; the base product and the LoRA term of y), the mask that of
+``oracle.policy_loss.dropout_factors``. Tolerance: the result's rounding u, and an
 intermediate of its size that falls to the other neighbour, 2 u: 3 u of max|result|."""
 
 import math
@@ -52,13 +52,11 @@ def _reference(base, x, g, a, b, s, factor, dt):
                         dtype=dt).view(n, k).double()
     rt = lambda t: t.to(dt).double()  # noqa: E731
     x, g = x.reshape(-1, k), g.reshape(-1, n)
-    drop = lambda t: rt(torch.where(factor > 0, t.float() * factor, 0.0))  # noqa: E731
-    sd, xd = float(torch.tensor(s, dtype=dt)), drop(x)
-    sg = rt(g.double() * sd)
-    gi, xa = rt(sg @ b.double()), rt(xd @ a.double().t())
-    y = rt(rt(x.double() @ w.t()) + base.bias.double()) + rt(rt(xa @ b.double().t()) * sd)
-    gx = rt(g.double() @ w) + drop(rt(gi @ a.double()))
-    return y, gx, gi.t() @ xd, sg.t() @ xa
+    keep = lambda t: torch.where(factor > 0, t.double(), 0.0)  # noqa: E731
+    x, g, a, b, f = x.double(), g.double(), a.double(), b.double(), s * float(factor.max())
+    gi, xa = rt(f * (g @ b)), rt(f * (keep(x) @ a.t()))
+    y = rt(rt(x @ w.t()) + base.bias.double()) + rt(xa @ b.t())
+    return y, g @ w + keep(gi @ a), gi.t() @ keep(x), g.t() @ xa
 
 
 # one row to past each GEMM tile and row slice, remainders of every column tile, ranks
