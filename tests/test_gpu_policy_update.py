@@ -2,9 +2,11 @@
 counter-based dropout, a head, the old and the reference policy's log-probabilities, the
 loss and its gradients, against the same update in float64.
 
-Tolerance: a gradient passes at most 14 tensors rounded to bf16 (drop(x), t, u, y of two
-layers, the logits, their gradient, and gi, gW, gi A and the sum of a layer), each off by at
+Tolerance: a gradient passes at most 14 tensors rounded to bf16 (t, x W, u and y of two
+layers, the logits, their gradient, and gi, grad_x and the adapters' of each), each off by at
 most 2^-8 of its size: 14 * 2^-8 of the gradient's norm."""
+
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -88,3 +90,42 @@ def test_one_update(dev):
             off = (p.weight.grad.double() - d.grad).norm() / d.grad.norm()
             print(f"grad off by {float(off):.2e}", flush=True)
             assert off <= bound
+
+
+def test_where_another_device_is_current(dev, monkeypatch):
+    """Every operator makes its tensors' device the current one for its launches."""
+    from grpo_mi355x import kernels
+    from grpo_mi355x.core.nf4 import quantize_nf4
+
+    g = torch.Generator().manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16().to(dev)  # noqa: E731
+    packed, state = quantize_nf4(rnd(64, 96).float(), 32)
+    packed.quant_state = state
+    base = SimpleNamespace(weight=packed, bias=None)
+    x, a, b, logits = rnd(2, 5, 96), rnd(8, 96), rnd(64, 8), rnd(2, 5, 64)
+    ids, adv = torch.arange(10, device=dev).view(2, 5), torch.tensor([1.0, -1.0], device=dev)
+    rng = torch.tensor([3, 4], device=dev)
+
+    def go():
+        leaf = logits.clone().requires_grad_()
+        logp = kernels.token_logprobs(leaf, ids)
+        return [logp.detach(), kernels.grpo_policy_loss(logp, None, adv)[0].detach(),
+                kernels.fused_grpo_loss(leaf, ids, None, adv)[0].detach(),
+                kernels.counter_dropout(x, 0.3, rng),
+                kernels.lora_fused_forward(x, base_layer=base, lora_A=a, lora_B=b, scaling=2.0,
+                                           dropout=torch.nn.Dropout(0.3), dropout_rng=rng)]
+
+    want, entered = go(), []
+
+    class Entered(torch.cuda.device):
+        def __init__(self, d):
+            entered.append(d)
+            super().__init__(d)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", Entered)
+    got = go()
+    monkeypatch.undo()
+    assert len(entered) == 5 and all(d.index == 0 for d in entered)
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
