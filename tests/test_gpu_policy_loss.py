@@ -512,6 +512,42 @@ def test_backward_twice_and_scaled(dev):
     assert torch.equal(leaf.grad, kept + kept)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vectors, rows", [(300, 7), (2600, 7), (5000, 7), (7200, 7), (9800, 7),
+                                           (14400, 130), (19500, 130)])
+def test_gradient_of_the_one_pass(dev, dtype, vectors, rows):
+    """The gradient made with the loss is, to the bit, what the logits give again (which the
+    test above holds to 64 bits), at every size of row and for rows of every kind."""
+    from grpo_mi355x import _lib
+
+    dt = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[dtype]
+    vocab = vectors * 16 // dt.itemsize + 3
+    assert _lib.library().grpo_policy_loss_logits_one_pass(
+        ["bf16", "f16", "f32"].index(dtype), 1, rows, vocab)
+    g = torch.Generator().manual_seed(vectors)
+    x = torch.randn(1, rows, vocab, generator=g).mul_(3).to(dt)
+    ids = torch.randint(0, vocab, (1, rows), generator=g)
+    mask = torch.ones(1, rows, dtype=torch.bool)
+    x[0, 0, 50:], ids[0, 0] = -math.inf, 7
+    x[0, 1, 50:], ids[0, 1] = torch.finfo(dt).min, vocab - 1
+    x[0, 2], x[0, 3, 9], x[0, 4, vocab - 1] = torch.finfo(dt).min, math.inf, math.nan
+    x[0, 5] += 900.0
+    x[0, 6], mask[0, 6], ids[0, 6] = math.nan, False, -100
+    old = torch.randn(1, rows, generator=g) - 9.0
+    put = lambda t: t.to(dev)  # noqa: E731
+    leaf = put(x).requires_grad_()
+    loss, _, _ = _ops().fused_grpo_loss(leaf, put(ids), put(old), torch.ones(1, device=dev),
+                                        put(mask), temperature=0.9)
+    one, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    two, = torch.autograd.grad(loss, leaf)
+    assert torch.allclose(one, two, rtol=0.0, atol=0.0, equal_nan=True)
+    one = one[0].cpu()
+    assert torch.isfinite(one[[0, 1, 2, 5]]).all() and not one[6].any()
+    assert one[3].isnan().any() and one[4].isnan().all()
+    # (a ratio above the clip leaves a row without a gradient)
+    assert torch.isfinite(one[7:]).all() and one[:3].any() and (rows == 7 or one[7:].any())
+
+
 def test_logits_changed_before_the_backward_are_refused(dev):
     x, ids, old, _, adv, mask, _, _ = loss_inputs(2, 3, 64, "f32", seed=3, beta=0.0)
     put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
