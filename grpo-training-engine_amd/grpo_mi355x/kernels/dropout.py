@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
+from .ops import derivative_recorded
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -52,6 +53,7 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, p, rng):
         ctx.p = p
         ctx.save_for_backward(rng)
+        ctx.save_for_forward(rng)
         return _dropout(x, p, rng)
 
     @staticmethod
@@ -60,6 +62,11 @@ class _Dropout(torch.autograd.Function):
         rng, = ctx.saved_tensors
         run = _Dropout.apply if torch.is_grad_enabled() and grad.requires_grad else _dropout
         return run(grad, ctx.p, rng), None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        # linear in x: the tangent under the same mask
+        return counter_dropout(tangent, ctx.p, ctx.saved_tensors[0])
 
 
 def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
@@ -71,13 +78,13 @@ def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tenso
     ``65536 / (65536 - t)`` and rounded once.  A dropped element gives 0, also where x is
     not finite.  The same ``rng`` gives the same mask; the caller changes the offset from
     call to call (``CounterDropout`` does), and leaves ``rng`` unchanged until the backward
-    has run.  bfloat16, float16 or float32, any shape."""
+    has run.  Differentiable by ``x``, in forward mode too.  bfloat16, float16 or float32, any shape."""
     if not x.is_cuda:
         raise ValueError("x must be on the ROCm/HIP device.")
     if x.dtype not in _DTYPES:
         raise ValueError(f"x must be bfloat16, float16 or float32, got {x.dtype}.")
     p = check_dropout(p, rng, x.device)
-    if x.requires_grad and torch.is_grad_enabled():
+    if derivative_recorded(x):
         return _Dropout.apply(x, p, rng)
     return _dropout(x, p, rng)
 

@@ -35,7 +35,6 @@ import contextlib
 from typing import Optional
 
 import torch
-import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
@@ -411,13 +410,12 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
         if drop is not None:
             away = x.is_cuda and x.device.index != torch.cuda.current_device()
             with torch.cuda.device(x.device) if away else contextlib.nullcontext():
-                if torch.is_grad_enabled():
+                if torch.is_grad_enabled() or ops.derivative_recorded(x):
                     return FusedLoRADropoutFunction.apply(*args, *drop)
                 return _run_forward(*args, drop)[0]
         # With nothing to record (no grad mode, no forward-mode level, no transform)
         # the autograd function's own bookkeeping, 5 us of a decode call's 25, is left out.
-        if not torch.is_grad_enabled() and fwAD._current_level < 0 and \
-                not torch._C._are_functorch_transforms_active():
+        if not torch.is_grad_enabled() and not ops.derivative_recorded(x):
             return _run_forward(*args)[0]
         return FusedLoRAFunction.apply(*args)
 

@@ -10,8 +10,17 @@ from __future__ import annotations
 import functools
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from .. import _lib
+
+
+def derivative_recorded(x: torch.Tensor) -> bool:
+    """Whether a call on ``x`` has to go through its autograd function: for the graph, or
+    under a forward-mode level or a transform, where a tensor carries a tangent without
+    requiring a gradient and a kernel's result would come back without it."""
+    return ((x.requires_grad and torch.is_grad_enabled()) or fwAD._current_level >= 0
+            or torch._C._are_functorch_transforms_active())
 
 # ----------------------------------------------------------- workspaces --
 

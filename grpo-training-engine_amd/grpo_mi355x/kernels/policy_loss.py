@@ -13,7 +13,8 @@ logits against tokens is the caller's slice: ``logits[:, :-1]`` is taken as it i
 a copy).  ``mask`` says which positions count; the others are not read, whatever stands
 there, and get logp 0 and gradient 0.  Softmax statistics, losses and gradients are
 float32 or float64; the logits' gradient is rounded once, to the logits' type.
-Arguments that do not fit raise ``ValueError``, a missing device ``ImportError``.  Nothing is
+Arguments that do not fit raise ``ValueError``, a missing device ``ImportError``; forward-mode
+derivatives raise (``RuntimeError``), as they do from any function that has none.  Nothing is
 kept between calls: every buffer is the call's own.
 """
 
@@ -28,6 +29,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from .ops import derivative_recorded
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _NORMALIZERS = {"tokens": 0, "sequences": 1}
@@ -217,7 +219,7 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     position's distribution, which carries no gradient.  An id outside the vocabulary at a
     counted position gives NaN there."""
     ids, mask, t = _check_logits(logits, token_ids, mask, temperature)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if derivative_recorded(logits):
         logp, ent = _TokenLogprobs.apply(logits, ids, mask, t, return_entropy)
     else:
         logp, ent, _ = _logprobs(logits, ids, mask, t, return_entropy, False)
@@ -340,7 +342,7 @@ def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
     tokens = _check_tokens(shape, dev, old_logps, ref_logps, advantages)
     mask = _mask_rows(mask, shape, dev)
     lp = _float_rows(logps, "logps", shape, dev)
-    if torch.is_grad_enabled() and logps.requires_grad:
+    if derivative_recorded(logps):
         return _PolicyLoss.apply(logps, lp, tokens, mask, policy)
     return _policy_loss(lp, tokens, mask, policy, False)[:2]
 
@@ -428,7 +430,7 @@ def fused_grpo_loss(logits: torch.Tensor, token_ids: torch.Tensor,
         raise ValueError(f"logits must be [batch, seq, vocab], got {list(logits.shape)}.")
     ids, mask, t = _check_logits(logits, token_ids, mask, temperature)
     tokens = _check_tokens(ids.shape, logits.device, old_logps, ref_logps, advantages)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if derivative_recorded(logits):
         return _LogitsLoss.apply(logits, ids, mask, t, tokens, policy)
     return _logits_loss(logits, ids, mask, t, tokens, policy, False)[:3]
 
