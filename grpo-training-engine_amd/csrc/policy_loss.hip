@@ -1170,8 +1170,10 @@ int policy_check(const grpo_policy_t* p, int B, int S, const float* adv, const v
   return GRPO_OK;
 }
 
-bool small_batch(const Tokens& t) {
-  return (int64_t)t.B * t.S <= SMALL_TOKENS && t.B <= SMALL_BATCH;
+// Whether one workgroup ends a batch of up to `most` tokens; its counts have room for
+// SMALL_BATCH sequences, of which there may be more than tokens (S = 0).
+bool small_batch(const Tokens& t, int64_t most = SMALL_TOKENS) {
+  return (int64_t)t.B * t.S <= most && t.B <= SMALL_BATCH;
 }
 
 // The weights for the launches that follow.
@@ -1344,7 +1346,7 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   }
   // one workgroup ends up to 1024 tokens (7.8 us), more are faster in two launches (10.6 at
   // 4096, one 16)
-  return run_policy(*policy, t, R <= 1024, ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
+  return run_policy(*policy, t, small_batch(t, 1024), ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
 }
 
 extern "C" int grpo_policy_loss_logits_one_pass(int dtype, int B, int S, int V) {

@@ -780,3 +780,29 @@ def test_the_parts_captured_and_replayed(dev, rows):
             assert torch.equal(u, v)
         step([sets[k][0].clone().requires_grad_(), *sets[k][1:]])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("b", [0, 7, 1024, 1025, 5000])
+def test_c_entries_with_a_mask_and_no_tokens(dev, b):
+    """Sequences of length 0 and a mask pointer all the same: nothing counted, whatever the
+    number of sequences."""
+    import ctypes
+
+    from grpo_mi355x import _lib
+
+    lib = _lib.device_library()
+    policy = ctypes.byref(_lib.Policy(0.2, 0.2, math.inf, 0.0, 1.0, 1))
+    buf, out = torch.ones(64, dtype=torch.uint8, device=dev), torch.full((5,), 7.0, device=dev)
+    need = max(lib.grpo_policy_loss_workspace_bytes(b, 0),
+               lib.grpo_policy_loss_logits_workspace_bytes(0, b, 0, 8))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    at, loss, metrics = buf.data_ptr(), out.data_ptr(), out[1:].data_ptr()
+    rest = (ws.data_ptr(), need, _lib.stream_handle(dev))
+    assert lib.grpo_policy_loss(at, None, None, at, 0, at, b, 0, policy, loss, metrics, None,
+                                *rest) == 0
+    assert not out.any()
+    out.fill_(7.0)
+    assert lib.grpo_policy_loss_logits(at, 0, 8, 8, b, 0, 8, at, at, 1.0, None, None, at, 0,
+                                       policy, loss, at, metrics, None, None, None, 0, 0,
+                                       *rest) == 0
+    assert not out.any()
