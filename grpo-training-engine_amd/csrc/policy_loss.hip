@@ -699,7 +699,8 @@ struct TokenSums {
   double v[5];
 };
 
-// One token of ratio r and eq = exp(ref - logp): d l / d logp.
+// One token of ratio r and eq = exp(ref - logp): d l / d logp. A KL term of weight 0 is left
+// out, not multiplied by it: eq may be infinite, and the reference be there for the metric alone.
 struct Slope {
   double d, gain;
   bool follows;  // the smaller gain moves with r
@@ -715,7 +716,7 @@ __device__ __forceinline__ Slope token_slope(const Policy& p, double r, double a
   s.gain = fmin(free_gain, clip_gain);
   s.d = s.follows ? -r * a : 0.0;
   if (r != r || a != a) s.d = s.gain = r * a;  // fmin would hide a NaN
-  if (has_ref) s.d += p.beta * (1.0 - eq);
+  if (has_ref && p.beta > 0.0) s.d += p.beta * (1.0 - eq);
   return s;
 }
 
@@ -731,7 +732,7 @@ __device__ __forceinline__ double token_at(const Policy& p, const Tokens& t, int
   }
   const Slope g = token_slope(p, ratio, a, t.ref != nullptr, eq);
   const double kl = t.ref ? eq - q - 1.0 : 0.0;
-  s.v[0] += w * (p.beta * kl - g.gain);
+  s.v[0] += w * ((p.beta > 0.0 ? p.beta * kl : 0.0) - g.gain);
   s.v[1] += ratio;
   s.v[2] += g.follows ? 0.0 : 1.0;
   s.v[3] += kl;

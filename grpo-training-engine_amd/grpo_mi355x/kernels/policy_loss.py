@@ -333,8 +333,8 @@ def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
     ``ref_logps`` are ``[batch, seq]``, ``advantages`` ``[batch]`` or ``[batch, seq]``;
     computed in float64, differentiable by ``logps`` alone.  ``metrics`` (float32 [4], no
     gradient) are means over the counted tokens: r, the share whose gain no longer moves
-    with r (clipped or capped), ``exp(q) - q - 1`` and ``old_logps - logps``.  With nothing
-    counted, loss and metrics are 0."""
+    with r (clipped or capped), ``exp(q) - q - 1`` and ``old_logps - logps``.  ``ref_logps`` with
+    ``beta`` 0 changes the third metric alone.  With nothing counted, loss and metrics are 0."""
     policy = _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps)
     if not logps.is_cuda:
         raise ValueError("logps must be on the ROCm/HIP device.")

@@ -138,7 +138,7 @@ size_t grpo_policy_loss_workspace_bytes(int B, int S);
  *   metrics    : float32 [4], means over the counted tokens: r, tokens whose gain no
  *                longer follows r, the KL term exp(q) - q - 1, old - logp
  *   coef       : float64 [R], d loss / d logp, or NULL
- * Nothing counted: loss and metrics are 0. */
+ * ref_logp with beta 0 changes that metric alone. Nothing counted: loss and metrics are 0. */
 int grpo_policy_loss(const float* logp, const float* old_logp, const float* ref_logp,
                      const float* advantages, int adv_tokens, const uint8_t* mask, int B, int S,
                      const grpo_policy_t* policy, float* loss, float* metrics, double* coef,

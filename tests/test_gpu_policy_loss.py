@@ -806,3 +806,41 @@ def test_c_entries_with_a_mask_and_no_tokens(dev, b):
                                        policy, loss, at, metrics, None, None, None, 0, 0,
                                        *rest) == 0
     assert not out.any()
+
+
+@pytest.mark.parametrize("dtype, vocab", [("bf16", 1000), ("f32", 160001)])  # one pass, and not
+def test_a_reference_without_a_weight_is_a_metric_alone(dev, dtype, vocab):
+    """beta = 0 with ref_logps: loss and gradients are those without it to the bit, also where
+    exp(ref - logp) is not finite."""
+    x, ids, old, _, adv, mask, logp, _ = loss_inputs(3, 6, vocab, dtype, seed=8, beta=0.0)
+    mask[:] = True
+    ids = ids.clamp(min=0)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    kw = dict(eps_high=0.28, normalizer="sequences")
+
+    def run(x, ref):
+        leaf = put(x).requires_grad_()
+        loss, lp, m = _ops().fused_grpo_loss(leaf, put(ids), put(old), put(adv), put(mask),
+                                             ref_logps=ref, **kw)
+        lp2 = lp.clone().requires_grad_()
+        loss2, m2 = _ops().grpo_policy_loss(lp2, put(old), put(adv), put(mask), ref_logps=ref,
+                                            **kw)
+        grads = [*torch.autograd.grad(loss, leaf), *torch.autograd.grad(loss2, lp2)]
+        return [loss.detach(), loss2.detach(), lp, *grads], [m, m2]
+
+    ref = put(np.float32(logp + 0.1).reshape(3, 6))
+    plain, with_ref = run(x, None), run(x, ref)
+    assert all(torch.equal(u, v) for u, v in zip(plain[0], with_ref[0]))
+    at = P.token_logprobs(x.view(18, vocab).double().numpy(), ids.reshape(-1).numpy(),
+                          np.ones(18, bool))[0]
+    q = ref.cpu().double().numpy() - at.reshape(3, 6)
+    want = float((np.exp(q) - q - 1).mean())
+    for m, m0 in zip(with_ref[1], plain[1]):
+        # logp is off by less than 2^-15 here, and each term's slope is e^q - 1
+        assert abs(float(m[2]) - want) <= 2.0 ** -15 * np.abs(np.expm1(q)).mean() + E * want
+        assert m0[2] == 0 and torch.equal(m[[0, 1, 3]], m0[[0, 1, 3]])
+    x[0, 1, ids[0, 1]] = -math.inf  # a token that the mask of the vocabulary forbids
+    x[1, 2, ids[1, 2]] = -3000.0    # ref - logp past the exponential's range
+    plain, with_ref = run(x, None), run(x, ref)
+    assert all(torch.isfinite(u).all() for u in (*plain[0][:2], *plain[0][3:]))
+    assert all(torch.equal(u, v) for u, v in zip(plain[0], with_ref[0]))
