@@ -44,8 +44,6 @@ def _is_linear4bit(module: nn.Module) -> bool:
 class ManualLoRALayer(nn.Module):
     """``Y = W_4bit(x) + B(A(x)) * (alpha / rank)`` (``lora.py:50-163``)."""
 
-    _counter = False  # the dropout is a CounterDropout
-
     def __init__(self, base_layer, rank: int = 16, alpha: int = 32, dropout: float = 0.0,
                  use_triton: bool = True, prefer_base_layer: bool = False,
                  counter_dropout: bool = False):
@@ -63,14 +61,14 @@ class ManualLoRALayer(nn.Module):
         self.lora_B = nn.Linear(rank, out_features, bias=False)
         kind = CounterDropout if counter_dropout else nn.Dropout
         self.lora_dropout = kind(p=dropout) if dropout > 0 else nn.Identity()
-        self._counter = counter_dropout and dropout > 0
         nn.init.kaiming_uniform_(self.lora_A.weight, a=5 ** 0.5)
         nn.init.zeros_(self.lora_B.weight)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        # one draw for a call, whichever branch below runs
+        # one draw for a call, whichever branch below runs, by what the dropout is now
+        drop = self._modules.get("lora_dropout")  # 0.07 us; 0.6 as an attribute
         rng = (CounterDropout.draw(x.device)
-               if self._counter and self.lora_dropout.active() else None)
+               if isinstance(drop, CounterDropout) and drop.active() else None)
         if self.use_triton:
             try:
                 return cast(torch.Tensor, lora_fused_forward(
@@ -83,7 +81,6 @@ class ManualLoRALayer(nn.Module):
             if base_output.requires_grad:
                 base_output = base_output.clone()
             x_adapt = x.to(self.lora_A.weight.dtype)
-            drop = self.lora_dropout
             x_adapt = drop(x_adapt) if rng is None else drop(x_adapt, rng)
             lora_output = self.lora_B(self.lora_A(x_adapt))
             lora_output = lora_output * self.scaling
