@@ -6,8 +6,8 @@ Same call surface and dispatch as the reference's
 * ``lora_layer`` (a ``ManualLoRALayer``-like object) or explicit
   ``base_layer/lora_A/lora_B/scaling/dropout``;
 * dropout p > 0 -> ``ValueError`` (``:958-960``), unless its mask is counter-based: a
-  ``CounterDropout`` in training mode, or ``dropout_rng`` with the draw for any dropout
-  module; it then runs inside the training linear (``FusedLoRADropoutFunction``);
+  ``CounterDropout`` in training mode, or ``dropout_rng`` with the draw for an
+  ``nn.Dropout``; it then runs inside the training linear (``FusedLoRADropoutFunction``);
 * a base weight with ``quant_state`` and ``prefer_base_layer=False`` -> the
   fused kernel (``FusedLoRAFunction``, ``:966-984``); otherwise the adapter
   branch ``base_layer(x) + B(A(x)) * scaling`` (``:986-1037``);
@@ -374,6 +374,9 @@ def _dropout_of(dropout, rng, device):
         raise ValueError("Dropout is not supported in lora_fused_forward.")
     if not getattr(dropout, "training", True):
         return None
+    if not counter and not isinstance(dropout, torch.nn.Dropout):
+        raise ValueError("the dropout of the fused linear must be an nn.Dropout or CounterDropout "
+                         f"(each element by itself), got {type(dropout).__name__}.")
     rng = CounterDropout.draw(device) if rng is None else rng
     return check_dropout(p, rng, device), rng
 
@@ -385,7 +388,7 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
     """Drop-in for ``src.triton_kernels.lora_forward.lora_fused_forward``.
 
     ``dropout_rng``: seed and offset (int64 [2], on x's device) of the mask that ``dropout``
-    (any module with a ``p``) puts on the adapter's input, ``y = W x + B(A(drop(x))) s``;
+    (an ``nn.Dropout`` or ``CounterDropout``) puts on the adapter's input, ``y = W x + B(A(drop(x))) s``;
     None: none, or a ``CounterDropout``'s own draw.  The mask is ``counter_dropout``'s and
     is never stored; a module in eval mode drops nothing."""
     if lora_layer is not None:

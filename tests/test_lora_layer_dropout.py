@@ -5,6 +5,7 @@ import torch
 import torch.nn as nn
 
 from grpo_mi355x.core import lora
+from grpo_mi355x.kernels import lora_forward
 from grpo_mi355x.kernels.dropout import CounterDropout
 
 
@@ -62,3 +63,17 @@ def test_one_draw_for_a_call(monkeypatch, counter):
     layer.eval()
     layer(torch.randn(2, 3, 16))
     assert len(draws) == 1 and fused[1] is None and len(parts) == 1
+
+
+@pytest.mark.parametrize("other", [nn.AlphaDropout, nn.Dropout1d, nn.Dropout2d, nn.Dropout3d,
+                                   nn.FeatureAlphaDropout])
+def test_dropout_of_another_rule_is_refused(other):
+    """A draw makes nn.Dropout's rule, element by element; a module with another rule has to
+    raise rather than run that one. In eval mode none drops anything."""
+    rng, cpu = torch.tensor([1, 2]), torch.device("cpu")
+    with pytest.raises(ValueError, match="nn.Dropout or CounterDropout"):
+        lora_forward._dropout_of(other(0.25), rng, cpu)
+    assert lora_forward._dropout_of(other(0.25).eval(), rng, cpu) is None
+    assert lora_forward._dropout_of(other(0.0), rng, cpu) is None
+    for fine in (nn.Dropout(0.25), CounterDropout(0.25)):
+        assert lora_forward._dropout_of(fine, rng, cpu) == (0.25, rng)
