@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
   }
   const int nl = nw + 4 * RN * lg;  // this lane's first column
   uint32_t bias[2 * RN];
-  if (MODE == GEMM16_LORA && g.bias) {
+  if ((MODE == GEMM16_LORA || MODE == GEMM16_LORA_DROP) && g.bias) {
 #pragma unroll
     for (int i = 0; i < 2 * RN; ++i)
       bias[i] = g.bias[min(nl + 2 * i, g.N - 1)] | (uint32_t)g.bias[min(nl + 2 * i + 1, g.N - 1)]
@@ -183,34 +183,42 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm16_kernel(Args p) {
   if (st < nst) step(st, b0, b1);
   wait_vm<0>();  // nothing lands after the workgroup's end
 
+  constexpr bool ONCE = MODE == GEMM16_ADD_DROP || MODE == GEMM16_LORA_DROP;  // one rounding
   const float sc = MODE == GEMM16_LORA ? round_e<F16>(g.scaling) : 1.f;
   DropKey key{};
   if (MODE == GEMM16_ADD_DROP) key = drop_key(g.drop.rng);
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
     const int m = m0 + (wm * RM + i) * 16 + ln;
-    const uint4 tv = *reinterpret_cast<const uint4*>(g.t + (int64_t)min(m, g.M - 1) * 32 + 8 * lg);
+    const int64_t ti = (int64_t)min(m, g.M - 1) * 32 + 8 * lg;
+    const uint4 tv = *reinterpret_cast<const uint4*>(g.t + ti);
+    uint4 tl{};
+    if (ONCE) tl = *reinterpret_cast<const uint4*>(g.tl + ti);
     uint32_t o[2 * RN];
     uint4 bits{};  // of the eight columns of tiles j and j + 1
 #pragma unroll
     for (int j = 0; j < RN; ++j) {
       if (MODE == GEMM16_ADD_DROP && j % 2 == 0)
         bits = philox(((uint64_t)m * g.N + nl + 4 * j) >> 3, key);
-      const f32x4_t u = mfma16x16x32_e<F16>(low[j], tv, f32x4_t{0.f, 0.f, 0.f, 0.f});
+      f32x4_t u = mfma16x16x32_e<F16>(low[j], tv, f32x4_t{0.f, 0.f, 0.f, 0.f});
+      if (ONCE) u = mfma16x16x32_e<F16>(low[j], tl, u);
       float v[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        if (MODE == GEMM16_ADD_DROP) {  // one rounding, below
-          v[q] = acc[i][j][q] +
-                 (drop_keeps(bits, 4 * (j & 1) + q, g.drop.threshold) ? u[q] : 0.f);
+        auto at_bias = [&]() __attribute__((always_inline)) {
+          return e2f<F16>((uint16_t)(bias[2 * j + (q >> 1)] >> (16 * (q & 1))));
+        };
+        if (ONCE) {
+          v[q] = acc[i][j][q];
+          if (MODE == GEMM16_LORA_DROP && g.bias) v[q] += at_bias();
+          if (MODE == GEMM16_LORA_DROP || drop_keeps(bits, 4 * (j & 1) + q, g.drop.threshold))
+            v[q] += u[q];
           continue;
         }
         v[q] = round_e<F16>(acc[i][j][q]);
         float w = round_e<F16>(u[q]);
         if (MODE == GEMM16_LORA) {
-          if (g.bias)
-            v[q] = round_e<F16>(
-                v[q] + e2f<F16>((uint16_t)(bias[2 * j + (q >> 1)] >> (16 * (q & 1)))));
+          if (g.bias) v[q] = round_e<F16>(v[q] + at_bias());
           w = round_e<F16>(w * sc);
         }
         v[q] += w;
@@ -294,10 +302,14 @@ int gemm16_launch(const Gemm16& g, Gemm16Mode mode, bool f16, hipStream_t st) {
     return einval("GEMM rows must be 16-byte aligned");
   if (g.lda < g.K || g.ldb < g.K || g.ldc < g.N || g.ldl < g.r || g.r < 1 || g.r > 32)
     return einval("row stride too small or rank outside [1, 32]");
-  if (mode == GEMM16_ADD_DROP && !g.drop.rng) return einval("null pointer");
+  const bool once = mode == GEMM16_ADD_DROP || mode == GEMM16_LORA_DROP;
+  if ((mode == GEMM16_ADD_DROP && !g.drop.rng) || (once && (!g.tl || !aligned16(g.tl))))
+    return einval("the GEMM with dropout needs its mask's state and aligned low halves");
   const Args a{g, 0, 0, g.r % 8 == 0 && g.ldl % 8 == 0 && aligned16(g.low)};
   if (mode == GEMM16_ADD_DROP)
     return f16 ? pick<true, GEMM16_ADD_DROP>(a, st) : pick<false, GEMM16_ADD_DROP>(a, st);
+  if (mode == GEMM16_LORA_DROP)
+    return f16 ? pick<true, GEMM16_LORA_DROP>(a, st) : pick<false, GEMM16_LORA_DROP>(a, st);
   if (mode == GEMM16_ADD)
     return f16 ? pick<true, GEMM16_ADD>(a, st) : pick<false, GEMM16_ADD>(a, st);
   return f16 ? pick<true, GEMM16_LORA>(a, st) : pick<false, GEMM16_LORA>(a, st);

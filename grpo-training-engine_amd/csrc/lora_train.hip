@@ -7,12 +7,15 @@
 //   grad_x = dt(dt(g W) + dt(gi A))   y = dt(dt(dt(x W^T) [+ bias]) + dt(dt(t B^T) * dt(s)))
 // With dropout on the adapter's input, keep(x) being x where its mask keeps it and 0 elsewhere
 // (philox.hpp), the mask's scale and s are one float32 factor f on the sums of rank r, which
-// leaves x and g as they are and a rounding of each product:
-//   xa = t = dt(f keep(x) A^T)        gi = dt(f g B)
+// leaves x and g as they are, and every result is rounded once:
+//   xa = t = f keep(x) A^T            gi = f g B
 //   grad_A = dt(gi^T keep(x))         grad_B = dt(g^T xa)
-//   grad_x = dt(g W + keep(gi A))     y = dt(dt(dt(x W^T) [+ bias]) + dt(t B^T))
-// (With the rounding points above, drop(x) and g s rounded too, the adapters' gradients were
-// 1.7 times an exact result's rounding away from 64 bits, 1.4 so.) The mask is made again in
+//   grad_x = dt(g W + keep(gi A))     y = dt(x W^T [+ bias] + t B^T)
+// xa, t and gi are operands of the 16-bit matrix instructions, so they are held as two 16-bit
+// values each, v = dt(v) + dt(v - dt(v)): 2^-16 of v in bf16, and a second instruction a tile,
+// which no timing shows (4184 rows of 3584 x 3584 260 us either way). Results are 1.7e-3 from 64
+// bits, an exact result's rounding to bf16; with one 16-bit value and the rounding points of the
+// formulas above they were 2.4e-3, with drop(x) and g s rounded too 2.9e-3. The mask is made again in
 // each of the four kernels that need it: 4184 rows of 3584 x 3584, r = 16, 6 to 7 us more than
 // without dropout (GEMM epilogue 2, weight gradients 3, preparations 0.6 and 0.7) in 261, where
 // a mask of a byte each would be written once and read three times (60 MB, 12 us) and kept from
@@ -149,6 +152,7 @@ struct RowsJob {
   int C;
   uint16_t* rows;       // [Mp][32] (ranks >= r zero) or null
   uint16_t* cols;       // [16 TC][Mp] (rows m >= M zero) or null
+                        // with dropout: of each two, the values and then what they leave
 };
 
 // One launch: workgroups [0, rows) run job 0, the next `rows` job 1 (a job
@@ -246,15 +250,26 @@ __device__ __forceinline__ void rows_tile(const PrepArgs& p, int b, float* red) 
   // one value per thread, the eight waves' sums in wave order; consecutive
   // threads: consecutive rows of one rank, so the transposed form leaves in runs
   const int row = tid & 15, rank = tid >> 4, m = m0 + row;
-  uint16_t v = 0;
+  uint16_t v = 0, left = 0;
   if (rank < p.r && m < p.M) {
     float s = red[row * LD + rank];
 #pragma unroll
     for (int w = 1; w < 8; ++w) s += red[(16 * w + row) * LD + rank];
-    v = f2e<F16>(DROP ? s * p.factor : s);
+    if (DROP) s *= p.factor;
+    v = f2e<F16>(s);
+    const float d = s - e2f<F16>(v);
+    if (DROP && fabsf(d) < INFINITY) left = f2e<F16>(d);  // an infinite v stays what it is
   }
-  if (j.rows) j.rows[(int64_t)m * 32 + rank] = v;  // m < Mp: Mp % 16 == 0
-  if (j.cols && rank < 16 * TC) j.cols[(int64_t)rank * p.Mp + m] = v;
+  if (j.rows) {  // m < Mp: Mp % 16 == 0
+    uint16_t* const o = j.rows + (int64_t)m * 32 + rank;
+    o[0] = v;
+    if (DROP) o[(int64_t)p.Mp * 32] = left;
+  }
+  if (j.cols && rank < 16 * TC) {
+    uint16_t* const o = j.cols + (int64_t)rank * p.Mp + m;
+    o[0] = v;
+    if (DROP) o[(int64_t)p.Mp * 16 * TC] = left;
+  }
 }
 
 template <int TC, bool F16, bool TR, bool DROP>
@@ -295,8 +310,8 @@ struct WgradArgs {
   int64_t ldg;
   const uint16_t* x;  // [M][K]: grad_A[r][k] = sum_m gi[m][r] x[m][k]
   int64_t ldx;
-  const uint16_t* xat;  // [16 TC][Mp]
-  const uint16_t* git;  // [16 TC][Mp]
+  const uint16_t* xat;  // [16 TC][Mp]; with dropout two of these, to be added
+  const uint16_t* git;  // likewise
   int M, Mp, N, K, r, tn;  // tn: column tiles of g (0: no grad_B)
   float scaling;
   int steps;   // 32-row steps per slice
@@ -339,10 +354,13 @@ __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
       const int mi = min(m + i, p.M - 1);
       v[i] = *reinterpret_cast<const uint4*>(sc0 + (int64_t)mi * ld);
     }
-    uint4 b[TC];
+    uint4 b[TC], bl[TC];
 #pragma unroll
-    for (int tc = 0; tc < TC; ++tc)
-      b[tc] = *reinterpret_cast<const uint4*>(low + (int64_t)(16 * tc + ln) * p.Mp + m);
+    for (int tc = 0; tc < TC; ++tc) {
+      const uint16_t* const q = low + (int64_t)(16 * tc + ln) * p.Mp + m;
+      b[tc] = *reinterpret_cast<const uint4*>(q);
+      if (DROP) bl[tc] = *reinterpret_cast<const uint4*>(q + (int64_t)p.Mp * 16 * TC);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[i] = keep(con && m + i < p.M, v[i]);  // no 0 * inf from rows past the end
@@ -360,7 +378,10 @@ __global__ void __launch_bounds__(256) lora_wgrad_kernel(WgradArgs p) {
                                  perm(word(v[5], j >> 1), word(v[4], j >> 1), sel),
                                  perm(word(v[7], j >> 1), word(v[6], j >> 1), sel));
 #pragma unroll
-      for (int tc = 0; tc < TC; ++tc) acc[j][tc] = mfma16x16x32_e<F16>(a, b[tc], acc[j][tc]);
+      for (int tc = 0; tc < TC; ++tc) {
+        acc[j][tc] = mfma16x16x32_e<F16>(a, b[tc], acc[j][tc]);
+        if (DROP) acc[j][tc] = mfma16x16x32_e<F16>(a, bl[tc], acc[j][tc]);
+      }
     }
   }
   // tile j's row 4 lg + q is column 8 (4 lg + q) + j; waves added as (0 + 2) + (1 + 3)
@@ -442,7 +463,7 @@ int wgrad_slices(int M, int N, int K) {
 }
 
 // Workspace of either direction (byte offsets): the 16-bit weight, t or gi by
-// rows, x A^T and gi by columns, A by columns, the partial sums.
+// rows, x A^T and gi by columns (room for two of each), A by columns, the partial sums.
 struct TrainWs {
   size_t w, rows, xat, git, at, pb, pa, total;
 };
@@ -458,9 +479,9 @@ TrainWs train_ws(int M, int N, int K, int r) {
     return at;
   };
   w.w = take((size_t)N * K * 2);
-  w.rows = take(Mp * 32 * 2);
-  w.xat = take(R * Mp * 2);
-  w.git = take(R * Mp * 2);
+  w.rows = take(2 * Mp * 32 * 2);
+  w.xat = take(2 * R * Mp * 2);
+  w.git = take(2 * R * Mp * 2);
   w.at = take((size_t)K * 32 * 2);
   w.pb = take(S > 1 ? (size_t)S * N * r * 4 : 0);
   w.pa = take(S > 1 ? (size_t)S * K * r * 4 : 0);
@@ -531,12 +552,13 @@ int run_forward(const TrainCall& c, const uint16_t* bias, uint16_t* y, int64_t l
   g.N = c.N;
   g.K = c.K;
   g.t = rows;
+  g.tl = rows + (int64_t)a.Mp * 32;
   g.low = c.lb;
   g.ldl = c.r;
   g.bias = bias;
   g.r = c.r;
-  g.scaling = c.drop.threshold ? 1.f : c.scaling;  // in t already
-  return gemm16_launch(g, GEMM16_LORA, F16, c.st);
+  g.scaling = c.scaling;
+  return gemm16_launch(g, c.drop.threshold ? GEMM16_LORA_DROP : GEMM16_LORA, F16, c.st);
 }
 
 template <bool F16>
@@ -580,6 +602,7 @@ int run_backward(const TrainCall& c, const uint16_t* grad, int64_t ldg, uint16_t
     g.N = c.K;
     g.K = c.N;
     g.t = rows;
+    g.tl = rows + (int64_t)Mp * 32;
     g.low = at;
     g.ldl = 32;
     g.r = c.r;

@@ -227,9 +227,10 @@ int grpo_nf4_lora_train_backward(const void* x, int64_t ldx, const void* grad, i
                                  size_t workspace_bytes, grpo_stream_t stream);
 
 /* Both with dropout on the adapter's input, keep(x) being x with the elements 0 that
- * grpo_dropout of a contiguous [M, K] drops, and f = s times its scale, in float32:
- *   t = xa = dt(f keep(x) A^T)     y = dt(dt(dt(x W^T) [+ bias]) + dt(t B^T))
- *   gi = dt(f g B)                 grad_x = dt(g W + keep(gi A))
+ * grpo_dropout of a contiguous [M, K] drops, and f = s times its scale, in float32; every
+ * result is rounded once (t, xa and gi are held as the sum of two 16-bit values):
+ *   t = xa = f keep(x) A^T         y = dt(x W^T [+ bias] + t B^T)
+ *   gi = f g B                     grad_x = dt(g W + keep(gi A))
  *   grad_A = dt(gi^T keep(x))      grad_B = dt(g^T xa)
  * p and rng as in grpo_dropout; p that rounds to 0: the calls above. */
 int grpo_nf4_lora_train_forward_dropout(const void* x, int64_t ldx, const uint8_t* w,

@@ -291,3 +291,43 @@ def test_checkpointed_layer(dev):
         got.append((leaf.grad, layer.lora_A.weight.grad.clone(), layer.lora_B.weight.grad.clone()))
     for u, v in zip(*got):
         assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("m,n,k,r", [(5, 64, 64, 4), (33, 160, 544, 8), (127, 256, 512, 17),
+                                     (1050, 288, 1024, 16), (1300, 512, 96, 32)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_results_are_rounded_once(dev, m, n, k, r, dt):
+    """The definition in float64, without any rounding on the way. Each element: half a step of
+    its own size, the float32 sums (e = 2^-24 a term of the sums of absolute terms, both
+    stages), and what two 16-bit values leave of x A^T and g B (u^2 of them, and half of
+    float16's least step where that is more) in the products that follow."""
+    from grpo_mi355x.kernels import lora_fused_forward, ops
+
+    base, x, g, a, b = _layer(dev, m, n, k, r, dt, seed=m + n)
+    p, s = 0.25, 1.7
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    y = lora_fused_forward(leaves[0], base_layer=base, lora_A=leaves[1], lora_B=leaves[2],
+                           scaling=s, dropout=torch.nn.Dropout(p), dropout_rng=_state(dev))
+    grads = torch.autograd.grad(y, leaves, g)
+    st = base.weight.quant_state
+    w = ops.nf4_dequant(base.weight.view(-1), st.absmax, st.code, n * k, st.blocksize,
+                        dtype=dt).view(n, k).double().cpu()
+    x, g, a, b, bias = (t.double().cpu() for t in (x[0], g[0], a, b, base.bias))
+    on = torch.from_numpy(dropout_factors(m * k, p, SEED, OFFSET)).view(m, k) > 0
+    f, xk = s / (1 - p), torch.where(on, x, 0.0)
+    t, gi = f * xk @ a.t(), f * g @ b
+    want = [x @ w.t() + bias + t @ b.t(), g @ w + torch.where(on, gi @ a, 0.0), gi.t() @ xk,
+            g.t() @ t]
+    absent = 2.0 ** -25 if dt == torch.float16 else 2.0 ** -134
+    split = lambda v: U[dt] ** 2 * v.abs() + absent  # noqa: E731
+    sums = lambda terms: (terms + 64) * 2.0 ** -24  # noqa: E731
+    xk, x, g, a, b, w = (v.abs() for v in (xk, x, g, a, b, w))
+    ta, ga = f * xk @ a.t(), f * g @ b  # of absolute terms
+    t, gi = split(t) + sums(k) * ta, split(gi) + sums(n) * ga  # what they are off by
+    slack = [sums(k) * (x @ w.t() + bias.abs()) + sums(r) * ta @ b.t() + t @ b.t(),
+             sums(n) * g @ w + sums(r) * ga @ a + gi @ a,
+             sums(m) * ga.t() @ xk + gi.t() @ xk, sums(m) * g.t() @ ta + g.t() @ t]
+    for name, got, v, more in zip(("y", "grad_x", "grad_a", "grad_b"), (y[0], grads[0][0],
+                                                                       *grads[1:]), want, slack):
+        off = (got.detach().double().cpu() - v).abs() - more
+        assert (off <= U[dt] * v.abs() + absent).all(), (name, float((off / v.abs()).max()) / U[dt])
