@@ -331,3 +331,21 @@ def test_results_are_rounded_once(dev, m, n, k, r, dt):
                                                                        *grads[1:]), want, slack):
         off = (got.detach().double().cpu() - v).abs() - more
         assert (off <= U[dt] * v.abs() + absent).all(), (name, float((off / v.abs()).max()) / U[dt])
+
+
+@pytest.mark.parametrize("m", [1, 8, 64, 256])
+@pytest.mark.parametrize("n, k", [(256, 512), (512, 256)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_few_rows_beside_the_linear_without_dropout(dev, m, n, k, dt):
+    """A share of 1/65536 and a draw that drops nothing: the linear without dropout, by its own
+    route and rounding points (three of y and one of x A^T), 5 half steps of the largest."""
+    from grpo_mi355x.kernels import lora_fused_forward
+
+    base, x, _, a, b = _layer(dev, m, n, k, 16, dt, seed=m + n)
+    p = 1 / 65536
+    offset = next(o for o in range(1000) if dropout_factors(m * k, p, SEED, o).all())
+    kw = dict(base_layer=base, lora_A=a, lora_B=b, scaling=2.0)
+    y = lora_fused_forward(x, dropout=torch.nn.Dropout(p), dropout_rng=_state(dev, SEED, offset),
+                           **kw)
+    plain = lora_fused_forward(x, **kw).double()
+    assert float((y.double() - plain).abs().max()) <= 5 * U[dt] * float(plain.abs().max())

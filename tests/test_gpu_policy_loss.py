@@ -844,3 +844,105 @@ def test_a_reference_without_a_weight_is_a_metric_alone(dev, dtype, vocab):
     plain, with_ref = run(x, None), run(x, ref)
     assert all(torch.isfinite(u).all() for u in (*plain[0][:2], *plain[0][3:]))
     assert all(torch.equal(u, v) for u, v in zip(plain[0], with_ref[0]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_gradients_just_inside_the_vector_path(dev, dtype):
+    """|M| just below 1024, where 16-bit gradients by vectors are least exact."""
+    x, ids, mask = make(5, 4096, "f32", seed=7, counted=1.1)
+    x = (x + 478.0).to(DT[dtype])
+    top = x.double().amax(1) / (0.7 * math.log(2.0)) + 4
+    assert 1000 < top.min() and top.max() < 1023
+    logp, ent, p, tol, _ = bounds(x, ids, mask, 0.7)
+    coef = torch.tensor([1.0, -2.0, 0.5, 3.0, -0.25])
+    leaf = x.to(dev).requires_grad_()
+    got = _ops().token_logprobs(leaf, ids.to(dev), temperature=0.7)
+    within(got, logp, tol)
+    grad, = torch.autograd.grad(got, leaf, coef.to(dev))
+    want = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy(), 0.7)
+    extra = 2.0 ** -13 * np.abs(coef.numpy() / 0.7)[:, None] * p
+    within(grad, want, grad_bound(want, p, coef.double().numpy(), 0.7, dtype) + extra)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("fused", [True, False])
+def test_the_scale_is_more_than_one_float(dev, dtype, fused):
+    """log2(e) / 0.7 rounded to float32 is off by 2.0e-8, and every logp with it: a loss whose
+    advantages cancel shows it. Each row has one logit of 0, its token's between -60 and -28
+    and -inf elsewhere, so S is exact to e^(-28 / 0.7) = 4e-18 and logp is x / T to float64's
+    roundings. The tokens of the positive advantages lie 16 below the others in the mean: one
+    float32 would move the loss by 2.0e-8 * 16 / 0.7 / 2 = 2.3e-7."""
+    b, s, vocab = 8, 8, 1000
+    g = torch.Generator().manual_seed(12)
+    tok = -(torch.arange(64) % 16).float() - 28.0
+    tok[:32] -= 16.0
+    x = torch.full((64, vocab), -math.inf)
+    ids = torch.randint(1, vocab, (64,), generator=g)
+    x[:, 0], x[torch.arange(64), ids] = 0.0, tok
+    logp = tok.double().numpy() / 0.7
+    adv = torch.tensor([1.0] * 4 + [-1.0] * 4)
+    old = torch.from_numpy(np.float32(logp)).view(b, s)
+    want, _, _ = P.policy_loss(logp.reshape(b, s), old.numpy(), adv.numpy(), np.ones((b, s), bool))
+    leaf = x.view(b, s, vocab).to(DT[dtype]).to(dev).requires_grad_(fused)
+    loss, got, _ = _ops().fused_grpo_loss(leaf, ids.view(b, s).to(dev), old.to(dev), adv.to(dev),
+                                          temperature=0.7)
+    assert abs(want) < 1e-5  # what old's rounding leaves
+    # float32's rounding of the loss, S, and float64's of logp (86 * 2^-52) and of the sums
+    assert abs(float(loss.detach()) - want) <= E * abs(want) + 1e-13
+    within(got, logp.reshape(b, s), 1.01 * E * np.abs(logp.reshape(b, s)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("vocab, t", [(2403, 1.0), (20803, 0.7), (40003, 1.0), (57003, 0.9)])
+def test_gradient_of_the_one_pass_in_64_bits(dev, dtype, vocab, t):
+    """The gradient that the forward makes, for an upstream gradient of 1, against the oracle."""
+    b, s = 2, 4
+    x, ids, old, ref, adv, mask, logp, p = loss_inputs(b, s, vocab, dtype, seed=vocab, t=t)
+    _, _, d = P.policy_loss(logp.reshape(b, s), old, adv, mask, ref, 0.2, 0.28, math.inf, 0.04,
+                            "tokens")
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    leaf = put(x).requires_grad_()
+    loss, _, _ = _ops().fused_grpo_loss(leaf, put(ids), put(old), put(adv), put(mask),
+                                        ref_logps=put(ref), temperature=t, eps_high=0.28, beta=0.04)
+    grad, = torch.autograd.grad(loss, leaf)
+    coef = d.reshape(-1)
+    at = ids.clamp(min=0).reshape(-1).numpy()
+    want = P.logits_grad(p, at, mask.reshape(-1), coef, t)
+    # the row's factor as in test_fused_loss_and_gradient; 16-bit gradients by vectors 2^-13
+    top = float((E * (vocab / 512 + 24 + 2 * np.abs(logp) + math.log(vocab))).max())
+    slack = (np.abs(coef) * 4 + 0.1) * top
+    tol = grad_bound(want, p, coef, t, dtype) + (slack / t)[:, None] * (
+        p + (np.arange(vocab)[None] == at[:, None]))
+    extra = 0.0 if dtype == "f32" else 2.0 ** -13 * np.abs(coef / t)[:, None] * p
+    within(grad, want, (tol + extra) * mask.reshape(-1, 1))
+
+
+def test_tokens_without_an_advantage(dev):
+    """A = 0: no gain and no gradient at any ratio; the token counts as moving up to delta, on
+    either side of the clip, and as stopped beyond it."""
+    r = torch.tensor([[0.5, 1.0, 1.1, 1.9, 3.0, 7.0]], dtype=torch.float64)
+    logp = torch.full_like(r, -2.0)
+    old = (logp - r.log()).float()
+    adv = torch.zeros(1)
+    for delta, stopped in ((None, 0), (4.0, 1)):
+        want, metrics, grad = P.policy_loss(logp.numpy(), old.numpy(), adv.numpy(),
+                                            np.ones((1, 6), bool), delta=delta or math.inf)
+        leaf = logp.float().to(dev).requires_grad_()
+        loss, m = _ops().grpo_policy_loss(leaf, old.to(dev), adv.to(dev), delta=delta)
+        loss.backward()
+        assert loss == want == 0 and not leaf.grad.any() and not grad.any()
+        assert float(m[1]) == np.float32(stopped / 6) == np.float32(metrics[1])
+
+
+def test_log_probabilities_are_read_as_float32(dev):
+    """float64 log-probabilities are taken to float32 first, and their gradient is float32's."""
+    logp, old, _, adv, mask = tokens(3, 9, seed=4)
+    put = lambda a: torch.as_tensor(a).to(dev)  # noqa: E731
+    wide = (put(logp).double() + 2.0 ** -40).requires_grad_()
+    leaf = put(logp).requires_grad_()
+    one = _ops().grpo_policy_loss(wide, put(old).double(), put(adv).double(), put(mask))[0]
+    two = _ops().grpo_policy_loss(leaf, put(old), put(adv), put(mask))[0]
+    one.backward()
+    two.backward()
+    assert torch.equal(one, two) and wide.grad.dtype == torch.float64
+    assert torch.equal(wide.grad, leaf.grad.double())
