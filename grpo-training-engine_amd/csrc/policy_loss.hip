@@ -24,7 +24,7 @@
 // vector units at about half of that time.
 //  * log-probabilities: a workgroup a row, eight 16-byte loads of a thread on their way;
 //    few rows are cut over several workgroups and joined. 2994 counted rows of 151936 bf16 in
-//    155 us, 5.9 TB/s; 8 rows 8.8 us (17.3 with one workgroup each).
+//    155 us, 5.9 TB/s; 8 rows 8.1 us (17.3 with one workgroup each).
 //  * the loss with the logits' gradient: a row stays in the registers of one workgroup
 //    (loss_rows_kernel), so the logits are read once and their gradient written once. 4096
 //    rows of 151936 bf16, three quarters of them counted, in 406 us: 2.18 GB at 5.4 TB/s (a
@@ -58,7 +58,8 @@ struct Rows {
 // live in memory, and its pointers would no longer be known to be global.)
 
 // What the gradient needs of a row: e_v = exp2(x_v k - M), or exp2((x_v - m) khi) where M
-// is not finite (rows whose logits are all below -1e30, or not finite).
+// is not finite (rows whose logits are all below -1e30, or not finite). S in float32, as is
+// -c / S made of it: a rounding of 2^-24 each, where e_v's exponential alone is off by 2^-23.
 struct RowStat {
   float M, S, m, pad;
 };
@@ -500,8 +501,8 @@ __device__ __forceinline__ float grad_plain(const RowGrad& g, float x) {
 // A vector of a row's gradient. For 16-bit results |neg| goes into the exponent, so a value
 // takes one multiply-add, the exponential and half a conversion: 2^(x khi + base), base =
 // log2 |neg| - M + klo (M / khi). base rounds at 2^-24 of its size, klo is applied at the row's
-// top instead of at x: together below 2^-13 of a value while |M| < 1024, a sixteenth of
-// float16's half step; rows beyond that go value by value.
+// top instead of at x: together below 2^-13 of a value while |M| < 1024, where half a step of
+// float16 is 2^-12 to 2^-11 of it; rows beyond that go value by value.
 struct VecGrad {
   float khi, klo, M, neg, base;
   uint32_t sign;
@@ -984,7 +985,7 @@ __global__ void __launch_bounds__(NT_, 4) loss_rows_kernel(Rows q, Policy p, Tok
 // ----------------------------------------------------------------- host --
 
 // Workgroups a row of the log-probabilities is cut over: enough for 512 in all (two a CU; 8
-// rows of 151936 bf16 logits 7.8 us, 17.3 with one workgroup each; with 1024 in all 200 rows
+// rows of 151936 bf16 logits 8.1 us, 17.3 with one workgroup each; with 1024 in all 200 rows
 // gain 4 % and 32 lose 15), each with 1024 vectors or more (32 rows 8.5 us, 9.5 with 2048).
 int logp_cuts(int64_t R, int dtype, int V) {
   const int64_t vecs = (int64_t)V * (dtype == F32 ? 4 : 2) / 16;

@@ -330,10 +330,12 @@ def grpo_policy_loss(logps: torch.Tensor, old_logps: Optional[torch.Tensor],
     (``normalizer="tokens"``), the mean over sequences of each one's mean
     (``"sequences"``; sequences without a counted token are left out), or the sum divided
     by a number.  ``logps``, ``old_logps`` (None: the policy's own, r = 1) and
-    ``ref_logps`` are ``[batch, seq]``, ``advantages`` ``[batch]`` or ``[batch, seq]``;
-    computed in float64, differentiable by ``logps`` alone.  ``metrics`` (float32 [4], no
+    ``ref_logps`` are ``[batch, seq]``, ``advantages`` ``[batch]`` or ``[batch, seq]``; all of
+    them are read as float32 (other types are converted, float64 included) and computed with
+    in float64; differentiable by ``logps`` alone.  ``metrics`` (float32 [4], no
     gradient) are means over the counted tokens: r, the share whose gain no longer moves
-    with r (clipped or capped), ``exp(q) - q - 1`` and ``old_logps - logps``.  ``ref_logps`` with
+    with r (clipped or capped; with advantage 0 only past both ``delta`` and the clip),
+    ``exp(q) - q - 1`` and ``old_logps - logps``.  ``ref_logps`` with
     ``beta`` 0 changes the third metric alone.  With nothing counted, loss and metrics are 0."""
     policy = _policy(eps_low, eps_high, delta, beta, normalizer, ref_logps)
     if not logps.is_cuda:
