@@ -946,3 +946,42 @@ def test_log_probabilities_are_read_as_float32(dev):
     two.backward()
     assert torch.equal(one, two) and wide.grad.dtype == torch.float64
     assert torch.equal(wide.grad, leaf.grad.double())
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 33), (3, 0, 33), (1500, 0, 33), (0, 0, 1)])
+@pytest.mark.parametrize("masked", [True, False])
+def test_logits_of_no_positions(dev, shape, masked):
+    x = torch.zeros(shape, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    ids = torch.zeros(shape[:2], dtype=torch.int64, device=dev)
+    mask = torch.ones(shape[:2], dtype=torch.bool, device=dev) if masked else None
+    adv = torch.ones(shape[0], device=dev)
+    for normalizer in ("tokens", "sequences", 3.0):
+        loss, logp, metrics = _ops().fused_grpo_loss(x, ids, None, adv, mask, normalizer=normalizer)
+        grad, = torch.autograd.grad(loss, x)
+        assert loss == 0 and not metrics.any() and logp.shape == shape[:2] and grad.shape == shape
+    logp, ent = _ops().token_logprobs(x, ids, mask, return_entropy=True)
+    grad, = torch.autograd.grad(logp.sum(), x)
+    assert logp.shape == ent.shape == shape[:2] and grad.shape == shape
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_an_expanded_leaf_gets_the_sum(dev, dtype):
+    """One row of logits for every position (stride 0): the gradient is the sum over them."""
+    vocab = 777
+    row, ids, _ = make(6, vocab, dtype, seed=3, counted=1.1)
+    row = row[:1]
+    leaf = row.to(dev).requires_grad_()
+    coef = torch.tensor([1.0, 0.5, -0.25, 2.0, -1.0, 0.125])
+    for view in (leaf.expand(6, vocab), leaf[None].expand(2, 3, vocab)):
+        got = _ops().token_logprobs(view, ids.view(view.shape[:-1]).to(dev))
+        grad, = torch.autograd.grad(got, leaf, coef.view(got.shape).to(dev))
+        x = row.expand(6, vocab)
+        mask = torch.ones(6, dtype=torch.bool)
+        logp, _, p, tol, _ = bounds(x, ids, mask, 1.0)
+        within(got.reshape(-1), logp, tol)
+        each = P.logits_grad(p, ids.numpy(), mask.numpy(), coef.double().numpy())
+        # each row rounded to the type, then five additions in it
+        size = np.abs(each).sum(0)
+        half = torch.finfo(DT[dtype]).eps / 2
+        bound = grad_bound(each, p, coef.double().numpy(), 1.0, dtype).sum(0)
+        within(grad[0], each.sum(0), bound + 5 * half * size + 5 * 2.0 ** -25)
