@@ -35,6 +35,7 @@ import contextlib
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
@@ -410,17 +411,16 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
             and getattr(weight_4bit, "quant_state", None) is not None):
         args = (x, weight_4bit, weight_4bit.quant_state, lora_A_weight, lora_B_weight,
                 float(scaling), getattr(base_layer, "bias", None))
+        # With nothing to record (no grad mode, no forward-mode level, no transform)
+        # the autograd function's own bookkeeping, 5 us of a decode call's 25, is left out.
+        bare = (not torch.is_grad_enabled() and fwAD._current_level < 0
+                and not torch._C._are_functorch_transforms_active())
         if drop is not None:
             away = x.is_cuda and x.device.index != torch.cuda.current_device()
             with torch.cuda.device(x.device) if away else contextlib.nullcontext():
-                if torch.is_grad_enabled() or ops.derivative_recorded(x):
-                    return FusedLoRADropoutFunction.apply(*args, *drop)
-                return _run_forward(*args, drop)[0]
-        # With nothing to record (no grad mode, no forward-mode level, no transform)
-        # the autograd function's own bookkeeping, 5 us of a decode call's 25, is left out.
-        if not torch.is_grad_enabled() and not ops.derivative_recorded(x):
-            return _run_forward(*args)[0]
-        return FusedLoRAFunction.apply(*args)
+                return (_run_forward(*args, drop)[0] if bare
+                        else FusedLoRADropoutFunction.apply(*args, *drop))
+        return _run_forward(*args)[0] if bare else FusedLoRAFunction.apply(*args)
 
     # Adapter branch (lora_forward.py:986-1037): base layer + the two adapter
     # products, each rounded to the adapter dtype, scaled, cast, added.

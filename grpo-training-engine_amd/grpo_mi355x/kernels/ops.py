@@ -16,11 +16,12 @@ from .. import _lib
 
 
 def derivative_recorded(x: torch.Tensor) -> bool:
-    """Whether a call on ``x`` has to go through its autograd function: for the graph, or
-    under a forward-mode level or a transform, where a tensor carries a tangent without
-    requiring a gradient and a kernel's result would come back without it."""
-    return ((x.requires_grad and torch.is_grad_enabled()) or fwAD._current_level >= 0
-            or torch._C._are_functorch_transforms_active())
+    """Whether a call on ``x`` has to go through its autograd function: for the graph, or for
+    a tangent, which a dual tensor carries without requiring a gradient and which a kernel's
+    result would come back without.  (A transform's own tensors have no data pointer to be
+    run on, so a call on one raises either way.)"""
+    return ((x.requires_grad and torch.is_grad_enabled())
+            or (fwAD._current_level >= 0 and fwAD.unpack_dual(x).tangent is not None))
 
 # ----------------------------------------------------------- workspaces --
 

@@ -105,4 +105,25 @@ def test_layer_by_parts_has_the_whole_tangent(dev, grad, use_triton):
     assert (want - base_only).abs().max() > 0.1 * want.abs().max()  # the adapter counts
     # two roundings of the base product and of each adapter product, sums apart: 8 half steps
     off = (y.tangent.double() - want).abs().max() / want.abs().max()
-    assert float(off) <= 8 * 2.0 ** -8
+    assert float(off.detach()) <= 8 * 2.0 ** -8
+
+
+def test_transforms(dev):
+    """A batched call's constants give what they give outside; a transform's own tensors raise."""
+    from grpo_mi355x import kernels
+
+    logits, logps, ids, adv = _inputs(dev)
+    rng = torch.tensor([5, 6], device=dev)
+    calls = [(logits, lambda x: kernels.token_logprobs(x, ids)),
+             (logits, lambda x: kernels.fused_grpo_loss(x, ids, None, adv)[0]),
+             (logps, lambda x: kernels.grpo_policy_loss(x, None, adv)[0]),
+             (logits, lambda x: kernels.counter_dropout(x, 0.4, rng))]
+    one = torch.ones(3, device=dev)
+    for x, call in calls:
+        want = call(x).sum()
+        assert torch.equal(torch.vmap(lambda v: v * call(x).sum())(one), one * want)
+        for transform in (lambda f: torch.vmap(f)(torch.stack([x, x])),
+                          lambda f: torch.func.jvp(f, (x,), (x,)),
+                          lambda f: torch.func.grad(lambda v: f(v).sum())(x)):
+            with pytest.raises(RuntimeError):
+                transform(call)
