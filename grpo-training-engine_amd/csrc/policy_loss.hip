@@ -1348,7 +1348,8 @@ extern "C" int grpo_policy_loss_logits(const void* logits, int dtype, int64_t st
   }
   // one workgroup ends up to 1024 tokens (7.8 us), more are faster in two launches (10.6 at
   // 4096, one 16)
-  return run_policy(*policy, t, small_batch(t, 1024), ws, o, Coef{nullptr, coef}, LossOut{loss, metrics}, st);
+  return run_policy(*policy, t, small_batch(t, 1024), ws, o, Coef{nullptr, coef},
+                    LossOut{loss, metrics}, st);
 }
 
 extern "C" int grpo_policy_loss_logits_one_pass(int dtype, int B, int S, int V) {

@@ -78,7 +78,8 @@ def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tenso
     ``65536 / (65536 - t)`` and rounded once.  A dropped element gives 0, also where x is
     not finite.  The same ``rng`` gives the same mask; the caller changes the offset from
     call to call (``CounterDropout`` does), and leaves ``rng`` unchanged until the backward
-    has run.  Differentiable by ``x``, in forward mode too.  bfloat16, float16 or float32, any shape."""
+    has run.  Differentiable by ``x``, in forward mode too.  bfloat16, float16 or float32,
+    any shape."""
     if not x.is_cuda:
         raise ValueError("x must be on the ROCm/HIP device.")
     if x.dtype not in _DTYPES:

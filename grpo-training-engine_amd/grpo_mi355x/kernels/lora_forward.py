@@ -389,9 +389,9 @@ def lora_fused_forward(x: torch.Tensor, base_layer=None, lora_A=None, lora_B=Non
     """Drop-in for ``src.triton_kernels.lora_forward.lora_fused_forward``.
 
     ``dropout_rng``: seed and offset (int64 [2], on x's device) of the mask that ``dropout``
-    (an ``nn.Dropout`` or ``CounterDropout``) puts on the adapter's input, ``y = W x + B(A(drop(x))) s``;
-    None: none, or a ``CounterDropout``'s own draw.  The mask is ``counter_dropout``'s and
-    is never stored; a module in eval mode drops nothing."""
+    (an ``nn.Dropout`` or ``CounterDropout``) puts on the adapter's input,
+    ``y = W x + B(A(drop(x))) s``; None: none, or a ``CounterDropout``'s own draw.  The mask is
+    ``counter_dropout``'s and is never stored; a module in eval mode drops nothing."""
     if lora_layer is not None:
         base_layer = getattr(lora_layer, "base_layer", None)
         lora_A = getattr(lora_layer, "lora_A", None)
