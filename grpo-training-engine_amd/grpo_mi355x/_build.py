@@ -23,7 +23,8 @@ ARCH = "gfx950"
 
 SOURCES = ("capi.hip", "nf4_linear.hip", "nf4_fold.hip", "nf4_tile.hip", "nf4_gemm.hip",
            "paged_attention.hip", "prefill_attention.hip", "decode_ops.hip", "lm_head.hip", "sampling.hip",
-           "nf4_backward.hip", "gemm16.hip", "lora_train.hip", "policy_loss.hip", "dropout.hip")
+           "nf4_backward.hip", "gemm16.hip", "lora_train.hip", "policy_loss.hip", "dropout.hip",
+           "draft_tree.hip", "tree_attention.hip", "sample_tokens.hip")
 
 # Flags of one source only (machine-scheduler strategies measured per source
 # on the decode step): the folded down_proj kernel is scheduled for

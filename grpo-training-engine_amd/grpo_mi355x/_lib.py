@@ -82,6 +82,25 @@ class Policy(ctypes.Structure):
 
 
 _POLICY = ctypes.POINTER(Policy)
+
+
+class Sampler(ctypes.Structure):
+    """``grpo_sampler_t``: temperature and filters of the sampler, one for all rows or, where
+    the ``_rows`` pointer is set, one per row."""
+
+    _fields_ = [
+        ("temperature", _c.c_double),
+        ("top_p", _c.c_double),
+        ("min_p", _c.c_double),
+        ("top_k", _I64),
+        ("temperature_rows", _VP),
+        ("top_k_rows", _VP),
+        ("top_p_rows", _VP),
+        ("min_p_rows", _VP),
+    ]
+
+
+_SAMPLER = ctypes.POINTER(Sampler)
 _ROWS = [_VP, _I32, _I64, _I64, _I32, _I32, _I32, _VP, _VP, _c.c_double]  # logits .. temperature
 
 # name -> (restype, argtypes); mirrors include/grpo_hip.h one to one.
@@ -108,6 +127,18 @@ SIGNATURES = {
     "grpo_policy_loss_logits_one_pass": (_I32, [_I32, _I32, _I32, _I32]),
     "grpo_policy_loss_logits_rescale": (
         _I32, [*_ROWS, _VP, _VP, _VP, _VP, _I64, _I64, _VP]),
+    "grpo_paged_rope_append": (
+        _I32, [*[_VP, _I64, _I64, _I64] * 3, _I32, _VP, _VP, _I32, _I32, _VP, _I64, _VP, _VP, _VP,
+               _VP, _VP, _I64, _VP, _I64, *[_I32] * 7, _VP]),
+    "grpo_paged_tree_attn_workspace_bytes": (_SZ, [_I32] * 5),
+    "grpo_paged_tree_attn": (
+        _I32, [_VP, _I64, _I64, _I64, _I32, _VP, _VP, _I64, _VP, _I64, _I32, _I32, _VP, _VP, _I64,
+               _VP, _F32, _VP, *[_I32] * 5, _VP, _SZ, _VP]),
+    "grpo_draft_tree_accept": (
+        _I32, [_VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _I32, _I64, _VP, _I64,
+               *[_I32] * 6, _I64, _I64, _VP, _VP, _VP, _VP]),
+    "grpo_sample_tokens": (
+        _I32, [_VP, _I32, _I64, _I32, _I32, _VP, _I32, _SAMPLER, _VP, _VP, _VP]),
     "grpo_dropout": (_I32, [_VP, _VP, _I64, _I32, _c.c_double, _VP, _VP]),
     "grpo_nf4_dequant_t": (_I32, [_VP, _VP, _VP, _VP, _I32, _I32, _I32, _I32, _VP]),
     "grpo_gemm16_tile": (_I32, [_I32, _I32, _c.POINTER(_I32), _c.POINTER(_I32)]),

@@ -11,6 +11,8 @@ Exports the reference's hot-path operator surface:
 * the policy update's ``fused_grpo_loss`` (``__init__.py:300``), with its parts
   ``token_logprobs`` and ``grpo_policy_loss``;
 * ``counter_dropout``, the LoRA layers' dropout without a stored mask;
+* checking a tree of drafted tokens in one pass: ``paged_rope_append``,
+  ``paged_tree_attention``, ``sample_tokens`` and ``accept_draft_tree``;
 * ``HIP_AVAILABLE`` (and ``TRITON_AVAILABLE``, the reference's flag name, as an
   alias so callers such as ``src/grpo/trainer.py:387`` keep working).
 
@@ -40,6 +42,10 @@ _EXPLICIT_MODULES = {
     "token_logprobs": "grpo_mi355x.kernels.policy_loss",
     "grpo_policy_loss": "grpo_mi355x.kernels.policy_loss",
     "counter_dropout": "grpo_mi355x.kernels.dropout",
+    "paged_rope_append": "grpo_mi355x.kernels.draft_tree",
+    "paged_tree_attention": "grpo_mi355x.kernels.draft_tree",
+    "accept_draft_tree": "grpo_mi355x.kernels.draft_tree",
+    "sample_tokens": "grpo_mi355x.kernels.sampling",
     "paged_kv_decode_model": "grpo_mi355x.rollout.decode",
 }
 
@@ -152,5 +158,26 @@ def counter_dropout(x: object, p: float, rng: object) -> object:
     return _call("counter_dropout", x, p, rng)
 
 
+def paged_rope_append(*args: object, **kwargs: object) -> object:
+    """``draft_tree.paged_rope_append``."""
+    return _call("paged_rope_append", *args, **kwargs)
+
+
+def paged_tree_attention(*args: object, **kwargs: object) -> object:
+    """``draft_tree.paged_tree_attention``."""
+    return _call("paged_tree_attention", *args, **kwargs)
+
+
+def accept_draft_tree(*args: object, **kwargs: object) -> object:
+    """``draft_tree.accept_draft_tree``."""
+    return _call("accept_draft_tree", *args, **kwargs)
+
+
+def sample_tokens(*args: object, **kwargs: object) -> object:
+    """``sampling.sample_tokens``."""
+    return _call("sample_tokens", *args, **kwargs)
+
+
 __all__ = ["HIP_AVAILABLE", "TRITON_AVAILABLE", "paged_kv_decode", "lora_fused_forward",
-           "token_logprobs", "grpo_policy_loss", "fused_grpo_loss", "counter_dropout"]
+           "token_logprobs", "grpo_policy_loss", "fused_grpo_loss", "counter_dropout",
+           "paged_rope_append", "paged_tree_attention", "sample_tokens", "accept_draft_tree"]

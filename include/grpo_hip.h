@@ -1000,6 +1000,94 @@ int grpo_paged_attn_prefill(const void* q, int64_t q_stride_b, int64_t q_stride_
                             int Hq, int Hkv, int D, int block_size, int max_blocks, float scale,
                             grpo_stream_t stream);
 
+/* ------------------------------------------- trees of drafted tokens --
+ * Checking several drafted tokens per sequence in one pass. Sequence b has context_lens[b]
+ * tokens in the cache and a tree of T <= GRPO_TREE_MAX_NODES nodes after them, counts[b] of
+ * them in use (NULL: all; below 0: none; above T: T); context_lens[b] < 0: none. Node i's keys
+ * and values stand at slot context_lens[b] + i; its parent parents[b][i] is an earlier node of
+ * the tree, or anything else (-1): none. bf16 (f16 == 0) or float16 queries, keys, values and
+ * caches; caches and tables as above, any block size; slots past the table or in blocks
+ * outside [0, num_blocks) are not written, and not attended. */
+#define GRPO_TREE_MAX_NODES 64
+
+/* Rotation of queries and keys to their positions, and the keys and values into the cache:
+ * fused_qkv_rope + the KV update (src/triton_kernels/fused_ops.py:198-219, paged_kv.py:253-319)
+ * for T >= 0 tokens per sequence (any number here).
+ *   q [B, T, Hq, D], k, v [B, T, Hkv, D]: strides of sequence, token and head in values
+ *   cos_table, sin_table : [max_pos, D], float32 (table_f32) or the 16-bit type
+ *   positions : int32 [B, T] (row stride pos_stride; clamped to the table), or NULL:
+ *               context_lens[b] + i
+ *   q_out     : [B, T, Hq, D]; rows past counts[b] become 0
+ * y[d] = x[d] cos[d] - x[d + D/2] sin[d], y[d + D/2] = x[d + D/2] cos[d + D/2] + x[d]
+ * sin[d + D/2] in float32, rounded once. D even. */
+int grpo_paged_rope_append(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
+                           int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb,
+                           int64_t v_st, int64_t v_sh, int f16, const void* cos_table,
+                           const void* sin_table, int table_f32, int max_pos,
+                           const int32_t* positions, int64_t pos_stride,
+                           const int32_t* context_lens, const int32_t* counts, void* q_out,
+                           void* k_cache, void* v_cache, int64_t num_blocks,
+                           const int32_t* block_tables, int64_t bt_stride, int block_size,
+                           int max_blocks, int B, int T, int Hq, int Hkv, int D,
+                           grpo_stream_t stream);
+
+/* Attention of every node over its sequence's context_lens[b] cached tokens, its ancestors and
+ * itself (the decode attention of paged_kv.py:63-251 for a tree): out[b, i, h] = sum_t
+ * softmax_t(scale * q[b, i, h].k_t) v_t, KV head h / (Hq / Hkv). Rows past counts[b], and rows
+ * that attend nothing, are 0. parents: int32 [B, T] (row stride parents_stride), or NULL: a
+ * chain. out: [B, T, Hq, D] in q's type. D <= 512. */
+size_t grpo_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D);
+int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int f16,
+                         const void* k_cache, const void* v_cache, int64_t num_blocks,
+                         const int32_t* block_tables, int64_t bt_stride, int block_size,
+                         int max_blocks, const int32_t* context_lens, const int32_t* parents,
+                         int64_t parents_stride, const int32_t* counts, float scale, void* out,
+                         int B, int T, int Hq, int Hkv, int D, void* workspace,
+                         size_t workspace_bytes, grpo_stream_t stream);
+
+/* The accepted path: node 0 (the pending token) is accepted; after node i comes its first child
+ * whose drafted token is sampled[b][i], the token that the model drew there, unless that is
+ * eos or negative. Path node j's keys and values move to slot context_lens[b] + j in every
+ * layer of k_cache, v_cache [layers, num_blocks, Hkv, block_size, D]; a slot written here is in
+ * no other sequence's table.
+ *   drafted, sampled : int64 [B, T], parents int32 [B, T]; row strides given
+ *   accepted : int32 [B], n: the path's length (0: no node in use)
+ *   path     : int32 [B, T], its nodes, -1 past n
+ *   tokens   : int64 [B, T], sampled[b][path[j]] for j < n, then pad */
+int grpo_draft_tree_accept(const int64_t* drafted, int64_t drafted_stride, const int32_t* parents,
+                           int64_t parents_stride, const int64_t* sampled, int64_t sampled_stride,
+                           const int32_t* context_lens, const int32_t* counts, void* k_cache,
+                           void* v_cache, int layers, int64_t num_blocks,
+                           const int32_t* block_tables, int64_t bt_stride, int block_size,
+                           int max_blocks, int B, int T, int Hkv, int D, int64_t eos, int64_t pad,
+                           int64_t* tokens, int32_t* accepted, int32_t* path,
+                           grpo_stream_t stream);
+
+/* One token per row of logits [M, V] (row stride ld in values; dtype as in the policy update),
+ * with temperature, top-k, top-p and min-p (src/triton_kernels/paged_kv.py:418-450), from given
+ * uniform numbers in [0, 1) (draws: float32, or float64 when draws_f64). w_v = exp((x_v - max)
+ * / T); in descending order of x (ties by index) a token is kept while fewer than top_k stand
+ * before it, the mass before it is below top_p times the mass of those top_k, and w >= min_p;
+ * the first always. The token is the first kept one at which the running mass passes u times
+ * the kept mass. Masses are integers in units of at least 2^-44 (2^-(62 - log2 V)).
+ * Each setting is one number, or one per row where its _rows pointer is not NULL. temperature
+ * <= 0 (or NaN), top_p <= 0 or min_p > 1: the lowest index of the maximum. top_k <= 0, top_p >=
+ * 1, min_p <= 0: no such bound. NaN and -inf are never drawn; where +inf is the maximum only
+ * +inf is. A row with nothing to draw gives token -1, kept 0.
+ *   tokens : int64 [M];  kept : int32 [M], the tokens that the filters leave, or NULL */
+#define GRPO_SAMPLE_MAX_VOCAB (1 << 24)
+typedef struct {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperature_rows;
+  const int32_t* top_k_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+} grpo_sampler_t;
+int grpo_sample_tokens(const void* logits, int dtype, int64_t ld, int M, int V, const void* draws,
+                       int draws_f64, const grpo_sampler_t* sampler, int64_t* tokens,
+                       int32_t* kept, grpo_stream_t stream);
+
 /* Load a batch into an engine's row state (DecodeEngine.start), B rows: tokens,
  * positions (tokens already cached) and limits as int64 [B]; tables int32 [B,
  * width] (row stride ld_tables, 0 for one row shared by all; width <=

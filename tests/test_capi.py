@@ -157,3 +157,50 @@ def test_build_compiles_every_source_with_its_flags():
     assert set(_build.SOURCE_FLAGS) <= set(_build.SOURCES)
     for flags in _build.SOURCE_FLAGS.values():
         assert flags[0] == "-mllvm" and flags[1].startswith("-amdgpu-sched-strategy=")
+
+
+def test_drafted_tree_argument_errors(lib):
+    """Refused before anything is launched (the addresses are never dereferenced)."""
+    import ctypes
+
+    from grpo_mi355x import _lib
+
+    p = 1 << 20
+
+    def append(b=2, t=3, hq=4, hkv=2, d=32, nb=8, bs=16, mb=4, most=64, q=p, tables=p):
+        return lib.grpo_paged_rope_append(q, 0, 0, 0, p, 0, 0, 0, p, 0, 0, 0, 0, p, p, 1, most,
+                                          None, 0, p, None, p, p, p, nb, tables, mb, bs, mb, b, t,
+                                          hq, hkv, d, None)
+
+    def attend(b=2, t=3, hq=4, hkv=2, d=32, nb=8, bs=16, mb=4, q=p, out=p):
+        return lib.grpo_paged_tree_attn(q, 0, 0, 0, 0, p, p, nb, p, mb, bs, mb, p, None, 0, None,
+                                        1.0, out, b, t, hq, hkv, d, None, 0, None)
+
+    def accept(b=2, t=3, hkv=2, d=32, layers=1, nb=8, bs=16, mb=4, drafted=p, path=p):
+        return lib.grpo_draft_tree_accept(drafted, t, p, t, p, t, p, None, p, p, layers, nb, p, mb,
+                                          bs, mb, b, t, hkv, d, -1, 0, p, p, path, None)
+
+    for fn in (append, attend):
+        for kw in (dict(b=-1), dict(hq=3), dict(hkv=0), dict(d=0), dict(nb=0), dict(bs=0),
+                   dict(mb=0), dict(bs=1 << 16, mb=1 << 15), dict(q=None), dict(hq=0)):
+            assert fn(**kw) < 0, (fn.__name__, kw)
+        assert fn(b=0) == 0
+    assert append(t=0) == 0 and append(t=-1) < 0 and append(d=33) < 0 and append(most=0) < 0
+    assert append(tables=None) < 0 and append(b=1 << 16, t=1 << 15) < 0
+    assert attend(t=0) < 0 and attend(t=65) < 0 and attend(d=513) < 0 and attend(out=None) < 0
+    assert b"null" in lib.grpo_last_error()
+    for kw in (dict(b=-1), dict(t=0), dict(t=65), dict(layers=0), dict(hkv=0), dict(d=0),
+               dict(nb=0), dict(b=65536), dict(drafted=None), dict(path=None)):
+        assert accept(**kw) < 0, kw
+    assert accept(b=0) == 0
+
+    def sample(dtype=0, ld=100, m=2, v=100, logits=p, draws=p, tokens=p, sampler=True):
+        s = _lib.Sampler(temperature=1.0, top_p=1.0)
+        return lib.grpo_sample_tokens(logits, dtype, ld, m, v, draws, 0,
+                                      ctypes.byref(s) if sampler else None, tokens, None, None)
+
+    for kw in (dict(m=-1), dict(v=0), dict(v=(1 << 24) + 1), dict(dtype=3), dict(dtype=-1),
+               dict(ld=99), dict(logits=None), dict(draws=None), dict(tokens=None),
+               dict(sampler=False), dict(logits=p + 1), dict(logits=p + 2, dtype=2)):
+        assert sample(**kw) < 0, kw
+    assert sample(m=0) == 0

@@ -1,0 +1,177 @@
+"""``sample_tokens`` against the float64 restatement (oracle/draft_tree.py): the same tokens and
+the same numbers of kept tokens. Both sides' masses are within 2^-36 of each other (units of
+2^-44 over 2^18 tokens at most, relative to a mass of 1 or more), so a draw or a border falls
+between them once in many millions of rows; the seeds here are fixed."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import draft_tree as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def check(dev, logits, u, **kw):
+    """Tokens and kept counts of rows of logits [M, V]; a setting is a number or a list."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    m = logits.shape[0]
+    given = {k: torch.tensor(v, device=dev, dtype=torch.int32 if k == "top_k" else torch.float32)
+             if isinstance(v, list) else v for k, v in kw.items()}
+    tokens, kept = sample_tokens(logits.to(dev), u.to(dev), return_kept=True, **given)
+    assert tokens.dtype == torch.int64 and kept.dtype == torch.int32
+    x = logits.double().numpy()
+    for i in range(m):
+        # a row's float32 setting is the number that the kernel has
+        at = {k: (float(np.float32(v[i])) if k != "top_k" else v[i]) if isinstance(v, list) else v
+              for k, v in kw.items()}
+        want = ref.sample(x[i], float(u[i]), **at)
+        assert (int(tokens[i]), int(kept[i])) == want, (i, at)
+
+
+def rows(seed, m, v, dtype, std=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(m, v, generator=g) * std).to(DTYPES[dtype]), \
+        torch.rand(m, generator=g, dtype=torch.float64)
+
+
+SETTINGS = [dict(), dict(temperature=0.7, top_p=0.9), dict(top_k=50), dict(min_p=0.02),
+            dict(temperature=1.3, top_k=200, top_p=0.8, min_p=0.001), dict(top_k=1),
+            dict(temperature=0.0), dict(top_p=0.0), dict(top_p=1e-30), dict(min_p=1.0),
+            dict(min_p=1.5), dict(temperature=1e-3), dict(temperature=1e6, top_p=0.5),
+            dict(top_k=10 ** 9, top_p=0.999999, min_p=1e-9)]
+
+
+@pytest.mark.parametrize("kw", SETTINGS, ids=str)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("v", [1, 2, 7, 63, 1000, 4097, 32003])
+def test_sizes_and_settings(dev, kw, dtype, v):
+    check(dev, *rows(v, 5, v, dtype), **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("std", [0.0, 1e-38, 1e-6, 0.03, 2.0, 9.0])
+def test_whole_vocabulary(dev, dtype, std):
+    """From one value 151936 times (a tie of all) to a few that stand out."""
+    x, u = rows(3, 4, 151936, dtype, std)
+    for kw in (dict(temperature=0.7, top_p=0.9), dict(top_k=40), dict(min_p=0.1, top_p=0.99),
+               dict()):
+        check(dev, x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_ties_go_to_the_lowest_index(dev, dtype):
+    g = torch.Generator().manual_seed(9)
+    x = torch.randint(-3, 4, (6, 30011), generator=g).to(DTYPES[dtype])  # 0 of both signs
+    x = torch.where((x == 0) & (torch.rand(x.shape, generator=g) < 0.5), -x, x)
+    u = torch.rand(6, generator=g, dtype=torch.float64)
+    for kw in (dict(top_k=100), dict(top_p=0.3), dict(top_k=20000, top_p=0.9), dict(min_p=0.5),
+               dict(temperature=0.5), dict(temperature=0)):
+        check(dev, x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_masked_rows(dev, dtype):
+    """-inf, NaN, the type's lowest value and +inf."""
+    x, u = rows(4, 12, 1003, dtype)
+    lowest = torch.finfo(DTYPES[dtype]).min
+    x[0] = -float("inf")
+    x[1] = float("nan")
+    x[2, 5:] = -float("inf")
+    x[3, ::2] = float("nan")
+    x[4, 1:] = lowest
+    x[5] = lowest
+    x[6, [3, 500, 700]] = float("inf")
+    x[7, :-1] = -float("inf")
+    x[8] = -float("inf")
+    x[8, 77] = lowest
+    x[9] *= 0
+    x[10, :500] = -float("inf")
+    x[11, 200] = torch.finfo(DTYPES[dtype]).max
+    for kw in (dict(), dict(top_k=4), dict(top_p=0.9, temperature=0.6), dict(min_p=0.05),
+               dict(temperature=0), dict(top_k=700, top_p=0.99, temperature=2.0)):
+        check(dev, x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_settings_of_each_row(dev, dtype):
+    x, u = rows(6, 9, 5000, dtype)
+    check(dev, x, u, temperature=[0.0, 0.5, 1.0, 2.0, -1.0, 0.7, 1.0, 1e-4, 1.0],
+          top_k=[0, 5, 5000, -1, 3, 0, 1, 100, 7000],
+          top_p=[0.9, 1.0, 0.5, 0.99, 0.1, 0.95, 1.0, 0.9, 0.2],
+          min_p=[0.0, 0.1, 0.0, 0.01, 0.5, 0.0, 0.2, 0.0, 1.0])
+
+
+def test_ends_of_the_unit_interval(dev):
+    x, _ = rows(7, 6, 1000, "f32")
+    u = torch.tensor([0.0, 1 - 2.0 ** -53, 0.5, 2.0 ** -60, 1 - 2.0 ** -24, 0.25],
+                     dtype=torch.float64)
+    for kw in (dict(), dict(top_k=3), dict(top_p=0.5)):
+        check(dev, x, u, **kw)
+    from grpo_mi355x.kernels import sample_tokens
+
+    flat = torch.zeros(6, 777, device=dev)  # the u-th index; draws outside [0, 1) are its ends
+    at = torch.tensor([-1.0, 0.0, 0.5, 0.999999, 1.0, float("nan")], device=dev)
+    assert sample_tokens(flat, at).tolist() == [0, 0, 388, 776, 776, 0]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_strided_rows(dev, dtype):
+    """Rows at odd addresses, an expanded row, rows inside a larger tensor."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    x, u = rows(8, 6, 2999, dtype)
+    kw = dict(temperature=0.8, top_p=0.9)
+    want = sample_tokens(x.to(dev), u.to(dev), **kw)
+    big = torch.full((6, 4001), 50.0, dtype=x.dtype, device=dev)
+    for at in (0, 1, 3):
+        view = big[:, at:at + 2999]
+        view.copy_(x)
+        assert torch.equal(sample_tokens(view, u.to(dev), **kw), want)
+        big.fill_(50.0)
+    turned = x.t().contiguous().t().to(dev)
+    assert torch.equal(sample_tokens(turned, u.to(dev), **kw), want)
+    one = x[2:3].to(dev).expand(6, 2999)
+    assert torch.equal(sample_tokens(one, u.to(dev), **kw),
+                       sample_tokens(one.contiguous(), u.to(dev), **kw))
+    three = x.to(dev).view(2, 3, 2999)
+    assert torch.equal(sample_tokens(three, u.to(dev).view(2, 3), **kw), want.view(2, 3))
+    assert int(sample_tokens(x[1].to(dev), u[1].to(dev), **kw)) == int(want[1])
+
+
+def test_draws_follow_the_distribution(dev):
+    """20000 draws of one row against its probabilities: chi-squared over 12 tokens (top_k),
+    below its 1 - 1e-6 quantile, 48.0 for 11 degrees of freedom."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    x, _ = rows(12, 1, 300, "bf16")
+    g = torch.Generator().manual_seed(1)
+    n = 20000
+    tokens = sample_tokens(x.to(dev).expand(n, 300), torch.rand(n, generator=g).to(dev), top_k=12)
+    p, at = torch.topk(x[0].double(), 12)
+    p = torch.softmax(p, 0).numpy() * n
+    seen = np.array([(tokens == int(i)).sum().item() for i in at])
+    assert seen.sum() == n
+    assert float(((seen - p) ** 2 / p).sum()) < 48.0
+
+
+def test_refusals(dev):
+    from grpo_mi355x.kernels import sample_tokens
+
+    x, u = rows(1, 4, 100, "bf16")
+    x, u = x.to(dev), u.to(dev)
+    sample_tokens(x, u)
+    for args in ((x.cpu(), u), (x.double(), u), (x.long(), u), (x, u.cpu()), (x, u[:3]),
+                 (x, u.bfloat16()), (x, u[:, None]), (x[:, :0], u)):
+        with pytest.raises(ValueError):
+            sample_tokens(*args)
+    nan, inf = float("nan"), float("inf")
+    for kw in (dict(temperature=nan), dict(temperature=inf), dict(top_p=nan), dict(min_p=inf),
+               dict(top_k=u), dict(top_p=u[:2]), dict(temperature=u.cpu()),
+               dict(min_p=u.to(torch.complex64))):
+        with pytest.raises(ValueError):
+            sample_tokens(x, u, **kw)
+    assert sample_tokens(x[:0], u[:0]).shape == (0,)
