@@ -5,6 +5,9 @@
 //
 // A token that a node does not attend is not read for it: whatever stands there (NaN of a slot
 // never written, another branch) stays out. A node that attends nothing gets 0.
+#include <algorithm>
+
+#include "lds_dma.hpp"
 #include "tree.hpp"
 
 using namespace grpo;
@@ -99,11 +102,439 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
     if (tid + i * GT < D) out[tid + i * GT] = f2e<F16>(l_run == 0.f ? 0.f : acc[i] * inv);
 }
 
+// ------------------------------------------------------------ MFMA kernel --
+// The T (Hq / Hkv) rows (node, head of the group) of one KV head are the columns of 32x32x16
+// MFMAs, so that K and V are read once for all of them:
+//  * A wave owns 32 rows; a workgroup RW waves side by side on rows times TW on tokens, which
+//    take the 32-token parts of each step and meet in LDS at the end. A sequence's tokens are
+//    cut over workgroups where there are few of them (a second kernel joins the parts).
+//  * K and V of a step come to LDS by loads of their own, RING - 1 steps ahead. A token's
+//    16-byte chunks are stored at chunk ^ token, so that the readers (32 tokens, one chunk)
+//    spread over the banks. The cache rows of WIN tokens stand in LDS too.
+//  * S^T = K Q^T leaves lane (row ln, half lh) with 16 of 32 tokens' scores of its row, which
+//    are the operand P^T of O^T = V^T P^T if its contraction index (lh, e) of product j means
+//    token 16 j + 8 (e / 4) + 4 lh + e % 4: P never leaves the lane. V is read as rows, D / 32
+//    neighbouring dims per lane, and its pairs of tokens are turned with v_perm.
+//  * P is rounded to 16 bits (2^-8 of each weight in bf16, 2^-11 in float16), the sum is of the
+//    float32 weights: the roundings are independent, so over many tokens they stay below the
+//    rounding of the result.
+//  * Only steps that reach past the cached tokens, or hold a missing block, look at masks.
+
+constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
+constexpr int MAX_SPLITS = 64;
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+struct FastArgs {
+  TreeArgs t;
+  int splits, RP;  // RP: rows of a (sequence, KV head) in the workspace
+  float* ws_o;     // [B][Hkv][splits][RP][D]
+  float* ws_ml;    // [B][Hkv][splits][RP][2]: max (log2 domain), sum
+};
+
+template <bool F16>
+__device__ __forceinline__ f32x16_t mfma32(uint4 a, uint4 b, f32x16_t c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
+                                                  __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from a 64-bit address of its own to 1 KiB at the wave-uniform LDS address
+// lds (see lds_dma.hpp).
+__device__ __forceinline__ void dma16_at(uint32_t lds, const void* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p)
+               : "memory");
+}
+
+// The tokens of sequence b and how they are cut: split z takes [z chunk, (z + 1) chunk).
+struct Cut {
+  int context, nodes, total, chunk, splits;
+};
+__device__ __forceinline__ Cut cut_of(const TreeArgs& a, int b, int splits, int step) {
+  Cut c;
+  const int len = a.cl[b], cap = a.pages.max_blocks * a.pages.block_size;
+  c.nodes = nodes_of(a.counts, b, a.T, len);
+  c.context = min(max(len, 0), cap);
+  c.total = c.nodes ? (int)min((int64_t)len + c.nodes, (int64_t)cap) : 0;
+  c.chunk = (int)cdiv(cdiv(c.total, splits), step) * step;
+  c.splits = c.total ? (c.total + c.chunk - 1) / c.chunk : 0;
+  return c;
+}
+
+// All ones in the halves of d that are an infinity or NaN (exponent bits all set).
+template <bool F16>
+__device__ __forceinline__ uint32_t inf_halves(uint32_t d) {
+  constexpr uint32_t X = F16 ? 0x7C00u : 0x7F80u;
+  return ((d & X) == X ? 0xFFFFu : 0u) | ((d & (X << 16)) == X << 16 ? 0xFFFF0000u : 0u);
+}
+
+// V^T operand of dims DT row + t from eight tokens' words.
+template <int VW>
+__device__ __forceinline__ uint4 turn(const uint32_t (&v)[8][VW], int t) {
+  const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
+  const int w = t >> 1;
+  return make_uint4(perm(v[1][w], v[0][w], sel), perm(v[3][w], v[2][w], sel),
+                    perm(v[5][w], v[4][w], sel), perm(v[7][w], v[6][w], sel));
+}
+
+template <int D, int TW>
+constexpr int RING_OF = D * TW <= 128 ? 4 : (D * TW <= 256 ? 3 : 2);
+
+template <bool F16, int D, int RW, int TW>
+__global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
+  constexpr int W = RW * TW, STEP = 32 * TW, RING = RING_OF<D, TW>;
+  constexpr int ROWB = 2 * D, NCH = D / 8;          // bytes and 16-byte chunks of a row
+  constexpr int HALF_B = 32 * ROWB, PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
+  constexpr int TPP = 1024 / ROWB, PPK = 32 / TPP;  // tokens of a 1-KiB piece, pieces of K
+  constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
+  static_assert(PIECES % W == 0, "every wave loads as many pieces");
+  constexpr int KS = D / 16, DT = D / 32, VW = DT / 2;  // steps of K, tiles of V, its words
+  constexpr int XCH = 2 + 16 * DT;                      // values per lane in the waves' merge
+  static_assert((TW - 1) * RW * XCH * 256 <= RING * STEP_B, "the merge fits the ring");
+  extern __shared__ __align__(16) char lds[];           // [RING][STEP_B], then WIN rows
+  int* const rows = reinterpret_cast<int*>(lds + RING * STEP_B);
+  const TreeArgs& a = f.t;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = wave / RW, ln = lane & 31, lh = lane >> 5;
+  const int Hkv = a.pages.Hkv, G = a.Hq / Hkv, R = a.T * G;
+  const int pair = blockIdx.x / f.splits, split = blockIdx.x - pair * f.splits;
+  const int b = pair / Hkv, kvh = pair - b * Hkv;
+  if (b >= a.B) return;
+  const Cut c = cut_of(a, b, f.splits, STEP);
+  if (split >= max(c.splits, 1)) return;
+  const int row0 = (blockIdx.y * RW + wave % RW) * 32, row = row0 + ln, rowc = min(row, R - 1);
+  const int node = rowc / G, head = kvh * G + rowc - node * G;
+  const uint64_t all = sees(a, b);
+  const uint64_t mask = (uint64_t)__shfl((long long)all, node);
+
+  uint4 qf[KS];
+  {
+    const uint16_t* const q =
+        a.q + (int64_t)b * a.qsb + (int64_t)node * a.qst + (int64_t)head * a.qsh + 8 * lh;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      qf[i] = *reinterpret_cast<const uint4*>(q + 16 * i);
+      qf[i].x ^= flip, qf[i].y ^= flip, qf[i].z ^= flip, qf[i].w ^= flip;
+    }
+  }
+  const float sl2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // (-inf stays -inf)
+  const int begin = split * c.chunk, end = min(c.total, begin + c.chunk);
+
+  const uint32_t lbase = lds_address(lds);
+  auto fetch = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int pc = wave + W * i, pt = pc / (2 * PPK);
+      const int tok = (pc & (PPK - 1)) * TPP + lane / NCH;
+      const int r = max(rows[s * STEP + 32 * pt + tok], 0);  // a missing one reads row 0
+      const uint16_t* const base = (pc / PPK) & 1 ? a.vc : a.kc;
+      dma16_at(lbase + (s % RING) * STEP_B + pc * 1024,
+               base + (int64_t)r * D + 8 * ((lane ^ tok) & (NCH - 1)));
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;  // of row ln
+  f32x16_t oacc[DT];  // O[ln][DT (8 (i / 4) + 4 lh + i % 4) + t] in oacc[t][i]
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
+  const int kx = 16 * ((lh ^ ln) & (NCH - 1)), ky = ln * ROWB;
+  const int vx = 16 * (((ln * 4 * VW / 16) ^ (4 * lh)) & (NCH - 1));
+  const int vy = 4 * lh * ROWB + ln * 4 * VW % 16;
+  // Wait for q here: at its first use the compiler, which does not count the fetches, would
+  // wait for all of them, in every step.
+#pragma unroll
+  for (int i = 0; i < KS; ++i)
+    asm volatile("" : "+v"(qf[i].x), "+v"(qf[i].y), "+v"(qf[i].z), "+v"(qf[i].w));
+
+  for (int w0 = begin; w0 < end; w0 += WIN) {
+    const int wend = min(end, w0 + WIN), nstep = (wend - w0 + STEP - 1) / STEP;
+    if (w0 != begin) __syncthreads();  // the last window has been read
+    for (int i = tid; i < nstep * STEP; i += 64 * W) {
+      const int64_t at = w0 + i < wend ? a.pages.row(b, w0 + i) : -1;
+      rows[i] = at < 0 ? -1 : (int)at + kvh * a.pages.block_size;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s)
+      if (s < nstep) fetch(s);
+    for (int s = 0; s < nstep; ++s) {
+      if (nstep - 1 - s >= RING - 2)
+        wait_vm<(RING - 2) * LD>();  // step s has landed
+      else
+        wait_vm<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      // The slot filled now was read a step ago: every wave is past that.
+      if (s + RING - 1 < nstep) fetch(s + RING - 1);
+      const int t0 = w0 + s * STEP + 32 * part;
+      if (t0 >= wend || row0 >= R) continue;
+      const char* const kb = lds + (s % RING) * STEP_B + part * PART_B;
+      const char* const vb = kb + HALF_B + vy;
+      f32x16_t sc;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+        sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kb + ky + (kx ^ (32 * i))), qf[i], sc);
+      uint32_t v[2][8][VW];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = 8 * (e >> 2) + (e & 3);
+          const char* const p = vb + (16 * j + k) * ROWB + (vx ^ (16 * (k & (NCH - 1))));
+          if constexpr (VW == 2) {
+            const uint2 w = *reinterpret_cast<const uint2*>(p);
+            v[j][e][0] = w.x, v[j][e][VW - 1] = w.y;
+          } else {
+            v[j][e][0] = *reinterpret_cast<const uint32_t*>(p);
+          }
+        }
+      const uint32_t there = (uint32_t)__ballot(rows[s * STEP + 32 * part + ln] >= 0);
+      if (t0 + 32 > c.context || there != ~0u) {
+        // Bit k: this row attends token t0 + k; of the tokens from `past` on not every row does.
+        const int past = max(c.context - t0, 0);
+        uint32_t on = past >= 32 ? ~0u
+                                 : (past ? (uint32_t)(mask << past) | ((1u << past) - 1)
+                                         : (uint32_t)(mask >> (t0 - c.context)));
+        on = (on & there) >> (4 * lh);
+        const uint32_t gone = ~there >> (4 * lh);
+        const uint32_t some = (past >= 32 ? 0u : ~0u << past) >> (4 * lh);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = 8 * (i >> 2) + (i & 3);  // register i, and token e = i % 8 of product i / 8
+          sc[i] = (on >> k) & 1 ? sc[i] : -INFINITY;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t& d = v[i >> 3][i & 7][w];
+            d = (gone >> k) & 1 ? 0u : d;
+            odd |= (some >> k) & 1 ? inf_halves<F16>(d) : 0u;
+          }
+        }
+        // A value that is not finite, in a token that some row does not attend: 0 times it would
+        // be NaN. It leaves V; the rows that attend its token become NaN there.
+        if (__builtin_expect(__ballot(odd != 0) != 0, 0)) {
+          constexpr uint32_t ONE = F16 ? 0x3C003C00u : 0x3F803F80u;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t one[4], u[8][VW];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int k = 16 * j + 8 * (e >> 2) + (e & 3);
+              const uint32_t bit = (on >> k) & 1 ? ONE & (e & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
+              one[e >> 1] = e & 1 ? one[e >> 1] | bit : bit;
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                const uint32_t x = (some >> k) & 1 ? inf_halves<F16>(v[j][e][w]) : 0u;
+                u[e][w] = x & ONE;
+                v[j][e][w] &= ~x;
+              }
+            }
+            const uint4 ob = make_uint4(one[0], one[1], one[2], one[3]);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+              f32x16_t n;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) n[i] = 0.f;
+              n = mfma32<F16>(turn<VW>(u, t), ob, n);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) oacc[t][i] = n[i] > 0.f ? NAN : oacc[t][i];
+            }
+          }
+        }
+      }
+      float top = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+      const float m_new = fmaxf(m_run, pair32_max(top) * sl2);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no token yet: every P is 0
+      const float corr = __builtin_amdgcn_exp2f(m_run - m_use);
+      float pv[16], ps = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        pv[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], sl2, -m_use));
+        ps += pv[i];
+      }
+      l_run = l_run * corr + pair32_sum(ps);
+      m_run = m_new;
+      if (__ballot(corr != 1.f)) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) oacc[t] *= corr;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint4 p = make_uint4(pack_e2<F16>(pv[8 * j], pv[8 * j + 1]),
+                                   pack_e2<F16>(pv[8 * j + 2], pv[8 * j + 3]),
+                                   pack_e2<F16>(pv[8 * j + 4], pv[8 * j + 5]),
+                                   pack_e2<F16>(pv[8 * j + 6], pv[8 * j + 7]));
+#pragma unroll
+        for (int t = 0; t < DT; ++t) oacc[t] = mfma32<F16>(turn<VW>(v[j], t), p, oacc[t]);
+      }
+    }
+  }
+
+  // The other parts' waves hand (max, sum, O) to the first part's: XCH values per lane.
+  if constexpr (TW > 1) {
+    __syncthreads();  // every wave is past its last read of the ring
+    float* const x = reinterpret_cast<float*>(lds) + (size_t)(wave % RW) * XCH * 64 + lane;
+    constexpr int XP = RW * XCH * 64;  // values of a part
+    if (part > 0) {
+      float* const w = x + (size_t)(part - 1) * XP;
+      w[0] = m_run;
+      w[64] = l_run;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[64 * (2 + 16 * t + i)] = oacc[t][i];
+    }
+    __syncthreads();
+    if (part > 0) return;
+    float m = m_run;
+#pragma unroll
+    for (int p = 1; p < TW; ++p) m = fmaxf(m, x[(p - 1) * XP]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    const float f0 = __builtin_amdgcn_exp2f(m_run - m_use);
+    l_run *= f0;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) oacc[t] *= f0;
+#pragma unroll
+    for (int p = 1; p < TW; ++p) {
+      const float* const w = x + (size_t)(p - 1) * XP;
+      const float fp = __builtin_amdgcn_exp2f(w[0] - m_use);
+      l_run += fp * w[64];
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[t][i] += fp * w[64 * (2 + 16 * t + i)];
+    }
+    m_run = m;
+  }
+  if (row >= R) return;
+  if (c.splits <= 1) {
+    const float inv = node < c.nodes && l_run != 0.f ? 1.f / l_run : 0.f;
+    uint16_t* const o = a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * DT * lh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < DT / 2; ++h) {  // eight neighbouring dims
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 8 * h + 2 * e;  // of the 4 DT dims of this i
+          const float x0 = oacc[d % DT][4 * i + d / DT];
+          const float x1 = oacc[(d + 1) % DT][4 * i + (d + 1) / DT];
+          w[e] = inv == 0.f ? 0u : pack_e2<F16>(x0 * inv, x1 * inv);
+        }
+        *reinterpret_cast<uint4*>(o + 8 * DT * i + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    return;
+  }
+  const int64_t at = ((int64_t)pair * f.splits + split) * f.RP + row;
+  float* const o = f.ws_o + at * D + 4 * DT * lh;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < DT; ++h) {
+      float4 w;
+      w.x = oacc[(4 * h) % DT][4 * i + 4 * h / DT];
+      w.y = oacc[(4 * h + 1) % DT][4 * i + (4 * h + 1) / DT];
+      w.z = oacc[(4 * h + 2) % DT][4 * i + (4 * h + 2) / DT];
+      w.w = oacc[(4 * h + 3) % DT][4 * i + (4 * h + 3) / DT];
+      *reinterpret_cast<float4*>(o + 8 * DT * i + 4 * h) = w;
+    }
+  if (lh == 0) *reinterpret_cast<float2*>(f.ws_ml + 2 * at) = make_float2(m_run, l_run);
+}
+
+// Joins the splits of a row: D / 4 lanes per row, where there are two splits or more.
+constexpr int JT = 256;
+template <bool F16, int D>
+__global__ void __launch_bounds__(JT) tree_attn_join_kernel(FastArgs f, int step) {
+  constexpr int L = D / 4, RPB = JT / L;
+  const TreeArgs& a = f.t;
+  const int Hkv = a.pages.Hkv, G = a.Hq / Hkv, R = a.T * G;
+  const int pair = blockIdx.y, b = pair / Hkv, kvh = pair - b * Hkv;
+  const Cut c = cut_of(a, b, f.splits, step);
+  if (c.splits <= 1) return;
+  const int row = blockIdx.x * RPB + threadIdx.x / L, l = threadIdx.x % L;
+  if (row >= R) return;
+  const int node = row / G, head = kvh * G + row - node * G;
+  const int64_t at = (int64_t)pair * f.splits * f.RP + row;
+  const float2* const ml = reinterpret_cast<const float2*>(f.ws_ml) + at;
+  const float4* const o = reinterpret_cast<const float4*>(f.ws_o) + at * L + l;
+  float m = -INFINITY;
+  for (int z = 0; z < c.splits; ++z) m = fmaxf(m, ml[(int64_t)z * f.RP].x);
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int z = 0; z < c.splits; ++z) {
+    const float2 w = ml[(int64_t)z * f.RP];
+    const float4 v = o[(int64_t)z * f.RP * L];
+    const float x = __builtin_amdgcn_exp2f(w.x - m_use);
+    sum += x * w.y;
+    acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
+  }
+  const float inv = node < c.nodes && sum != 0.f ? 1.f / sum : 0.f;
+  uint2 w = make_uint2(pack_e2<F16>(acc.x * inv, acc.y * inv), pack_e2<F16>(acc.z * inv, acc.w * inv));
+  if (inv == 0.f) w = make_uint2(0u, 0u);
+  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * l) = w;
+}
+
+struct Plan {
+  int rw, tw;      // waves side by side on rows, on tokens
+  int rb, splits;  // blocks of 32 rw rows, parts of a sequence's tokens
+  size_t values;   // rows of the workspace
+};
+Plan plan_of(int B, int T, int Hq, int Hkv) {
+  const int R = T * (Hq / Hkv);
+  Plan p;
+  p.rw = R <= 32 ? 1 : (R <= 64 ? 2 : (R <= 128 ? 4 : 8));
+  p.tw = std::min(8 / p.rw, 4);
+  p.rb = (int)cdiv(R, 32 * p.rw);
+  const int64_t groups = (int64_t)B * Hkv * p.rb;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS, 512 / groups));
+  p.values = p.splits > 1 ? (size_t)B * Hkv * p.splits * p.rb * 32 * p.rw : 0;
+  return p;
+}
+bool fast_dim(int D) { return D == 64 || D == 128; }
+
+template <bool F16, int D, int RW, int TW>
+int go(const FastArgs& a, const Plan& p, hipStream_t st) {
+  constexpr int LDS = RING_OF<D, TW> * TW * 128 * D + WIN * 4;
+  constexpr auto kern = tree_attn_kernel<F16, D, RW, TW>;
+  if (int rc = allow_dynamic_lds<kern, LDS>()) return rc;
+  // Blocks of rows that read the same tokens run on one XCD: their ids are equal modulo 8.
+  int64_t x = (int64_t)a.t.B * a.t.pages.Hkv * p.splits;
+  if (p.rb > 1) x = cdiv(x, 8) * 8;
+  kern<<<dim3((unsigned)x, (unsigned)p.rb), 64 * RW * TW, LDS, st>>>(a);
+  if (p.splits > 1) {
+    const int R = a.t.T * (a.t.Hq / a.t.pages.Hkv);
+    tree_attn_join_kernel<F16, D><<<dim3((unsigned)cdiv(R, JT / (D / 4)),
+                                         (unsigned)(a.t.B * a.t.pages.Hkv)), JT, 0, st>>>(
+        a, 32 * TW);
+  }
+  return launch_check("paged_tree_attn");
+}
+template <bool F16, int D>
+int go_form(const FastArgs& a, const Plan& p, hipStream_t st) {
+  return p.rw == 1   ? go<F16, D, 1, 4>(a, p, st)
+         : p.rw == 2 ? go<F16, D, 2, 4>(a, p, st)
+         : p.rw == 4 ? go<F16, D, 4, 2>(a, p, st)
+                     : go<F16, D, 8, 1>(a, p, st);
+}
+
 }  // namespace
 
 extern "C" size_t grpo_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D) {
-  (void)B, (void)T, (void)Hq, (void)Hkv, (void)D;
-  return 0;
+  if (B < 1 || T < 1 || T > TREE_MAX || Hkv < 1 || Hq < 1 || Hq % Hkv || !fast_dim(D)) return 0;
+  return plan_of(B, T, Hq, Hkv).values * (D + 2) * sizeof(float);
 }
 
 extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
@@ -124,7 +555,6 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
   if (B == 0) return GRPO_OK;
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out)
     return einval("null pointer");
-  (void)workspace, (void)workspace_bytes;
   const TreeArgs a{static_cast<const uint16_t*>(q),
                    q_sb,
                    q_st,
@@ -142,10 +572,25 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
                    Hq,
                    D,
                    scale};
+  hipStream_t st = as_stream(stream);
+  if (fast_dim(D) && ((q_sb | q_st | q_sh) & 7) == 0 && aligned16(q) && aligned16(k_cache) &&
+      aligned16(v_cache) && aligned16(out) && (int64_t)B * Hkv < 65536 &&
+      num_blocks * Hkv * block_size < (1ll << 31)) {
+    const Plan p = plan_of(B, T, Hq, Hkv);
+    const size_t need = p.values * (D + 2) * sizeof(float);
+    if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
+      set_error("tree attention workspace: %zu bytes, 16-byte aligned", need);
+      return GRPO_EWORKSPACE;
+    }
+    float* const ws = static_cast<float*>(workspace);
+    const FastArgs f{a, p.splits, p.rb * 32 * p.rw, ws, ws + p.values * D};
+    if (f16) return D == 64 ? go_form<true, 64>(f, p, st) : go_form<true, 128>(f, p, st);
+    return D == 64 ? go_form<false, 64>(f, p, st) : go_form<false, 128>(f, p, st);
+  }
   const dim3 grid((unsigned)(B * T), (unsigned)Hq);
   if (f16)
-    tree_attn_plain_kernel<true><<<grid, GT, 0, as_stream(stream)>>>(a);
+    tree_attn_plain_kernel<true><<<grid, GT, 0, st>>>(a);
   else
-    tree_attn_plain_kernel<false><<<grid, GT, 0, as_stream(stream)>>>(a);
+    tree_attn_plain_kernel<false><<<grid, GT, 0, st>>>(a);
   return launch_check("paged_tree_attn");
 }
