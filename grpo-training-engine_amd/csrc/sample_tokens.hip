@@ -7,16 +7,18 @@
 // of those k, then w >= min_p; the token is the first kept one at which the running mass
 // passes u times the kept mass.
 //
-//  * Masses are integers: w in units of 2^-S, S = 62 - ceil(log2 V), at most 44. Their sums do
-//    not depend on the order in which threads add them, so the token is a function of the
-//    inputs alone. A weight is a double (degree-11 Taylor polynomial of 2^f on [-1/2, 1/2],
-//    below 1e-14 relative) rounded once to those units; what is more than 45 doublings below
-//    the maximum has no mass.
-//  * "The first place in sorted order where the mass reaches P or the count reaches K" is
-//    found by descending through ranges of order-preserving keys: 4096 bins of the distance
-//    from the maximum, then bins of the keys within one bin until a bin is one value. That
-//    one search gives the top-k, top-p and min-p cuts and the draw itself.
+//  * Masses are integers, in units of 2^-S of the largest weight, S = 62 - ceil(log2 V), at most
+//    44: their sums do not depend on the order in which threads add them, so the token is a
+//    function of the inputs alone. Weights are doubles.
+//  * "The first place in sorted order where the mass reaches P or the count reaches K" gives the
+//    top-k, top-p and min-p cuts and the draw itself. It is found in a histogram of the row: of
+//    its values in bf16, else of 4096 distances from the maximum and then, within the one of
+//    them that holds the place, of the order-preserving keys until a bin is one value.
+//
+// A workgroup of 1024 threads per row.
 #include <math.h>
+
+#include <algorithm>
 
 #include "scan.hpp"
 
@@ -24,13 +26,8 @@ using namespace grpo;
 
 namespace {
 
-constexpr int TT = 1024;           // threads
-constexpr int NB = 4096;           // bins of the distance from the maximum
-constexpr double WINDOW = 48.0;    // doublings that they cover (the last takes the rest)
-constexpr int NK = 2048;           // bins of keys
-constexpr int KEY_BITS = 11;
-constexpr int LIST = 8192;         // values of one bin that LDS holds
-constexpr int SEGS = 2048;         // segments of the row in which a tied token is looked for
+constexpr int TT = 1024;  // threads
+constexpr int SEGS = TT;  // segments of the row in which a tied token is looked for
 
 struct TokArgs {
   const void* logits;
@@ -77,26 +74,22 @@ struct Elem<2> {
   static constexpr int N = 4;
 };
 template <int DT>
-__device__ __forceinline__ float value_of(uint32_t bits) {
-  if constexpr (DT == 0) return bf2f((uint16_t)bits);
-  if constexpr (DT == 1) return h2f((uint16_t)bits);
-  return __uint_as_float(bits);
+__device__ __forceinline__ float value_of(typename Elem<DT>::type x) {
+  if constexpr (DT == 0) return bf2f(x);
+  if constexpr (DT == 1) return h2f(x);
+  if constexpr (DT == 2) return x;
 }
 
-// f(index, value) of every value of the row; 16-byte loads from the first boundary on.
-template <int DT, typename F>
-__device__ __forceinline__ void for_row(const typename Elem<DT>::type* row, int V, F&& f) {
+// one(index, value) of the row's values before the first and after the last 16-byte boundary,
+// many(index of the first, 16 bytes) of what is between, U loads in flight per thread.
+template <int DT, int U, typename One, typename Many>
+__device__ __forceinline__ void for_groups(const typename Elem<DT>::type* row, int V, One&& one,
+                                           Many&& many) {
   typedef typename Elem<DT>::type E;
-  constexpr int N = Elem<DT>::N, U = 4;
+  constexpr int N = Elem<DT>::N;
   const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
   const int head = min(V, mis ? N - mis : 0), G = (V - head) / N, tid = threadIdx.x;
-  auto scalar = [&](int i) {
-    if constexpr (DT == 2)
-      f(i, row[i]);
-    else
-      f(i, value_of<DT>(row[i]));
-  };
-  if (tid < head) scalar(tid);
+  if (tid < head) one(tid, row[tid]);
   const E* const body = row + head;
   for (int g = tid; g < G; g += U * TT) {
     uint4 v[U];
@@ -104,37 +97,33 @@ __device__ __forceinline__ void for_row(const typename Elem<DT>::type* row, int 
     for (int u = 0; u < U; ++u)
       v[u] = *reinterpret_cast<const uint4*>(body + (int64_t)N * min(g + u * TT, G - 1));
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (g + u * TT >= G) break;
-      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      const int at = head + N * (g + u * TT);
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        f(at + e, value_of<DT>(DT == 2 ? w[e & 3] : ((e & 1) ? w[(e >> 1) & 3] >> 16
-                                                             : w[(e >> 1) & 3] & 0xFFFFu)));
-    }
+    for (int u = 0; u < U; ++u)
+      if (g + u * TT < G) many(head + N * (g + u * TT), v[u]);
   }
   const int tail = head + N * G + tid;
-  if (tail < V) scalar(tail);
+  if (tail < V) one(tail, row[tail]);
+}
+// f(index, value as float) of every value.
+template <int DT, typename F>
+__device__ __forceinline__ void for_row(const typename Elem<DT>::type* row, int V, F&& f) {
+  for_groups<DT, 4>(
+      row, V, [&](int i, typename Elem<DT>::type x) { f(i, value_of<DT>(x)); },
+      [&](int i, const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (DT == 2) {
+            f(i + e, __uint_as_float(w[e]));
+          } else {
+            f(i + 2 * e, value_of<DT>((uint16_t)w[e]));
+            f(i + 2 * e + 1, value_of<DT>((uint16_t)(w[e] >> 16)));
+          }
+        }
+      });
 }
 
-// Distance from the maximum in doublings (0 at the maximum itself, infinite ones included;
-// infinite for what has no mass).
-struct Scale {
-  float top;
-  double c;  // log2(e) / T
-  __device__ __forceinline__ double below(float x) const {
-    const double y = ((double)top - (double)x) * c;
-    return x == top ? 0.0 : (y >= 0.0 ? y : (double)INFINITY);
-  }
-};
-__device__ __forceinline__ int bin_of(double y) {
-  return (int)fmin(y * (NB / WINDOW), (double)(NB - 1));
-}
-
-// round(2^(S - y)): the double's last place is 1 after 2^52 is added.
-__device__ __forceinline__ uint64_t mass_of(double y, int shift) {
-  if (!(y < (double)(shift + 1))) return 0;
+// 2^-y as a double, y >= 0, times 2^up: Taylor polynomial of 2^f on [-1/2, 1/2], below 1e-14.
+__device__ __forceinline__ double exp2_neg(double y, int up) {
   const double n = rint(y), f = n - y;
   double p = 4.44553827187081e-10;  // ln(2)^k / k!, k = 11 .. 0
   p = fma(p, f, 7.054911620801121e-09);
@@ -148,274 +137,126 @@ __device__ __forceinline__ uint64_t mass_of(double y, int shift) {
   p = fma(p, f, 0.2402265069591007);
   p = fma(p, f, 0.6931471805599453);
   p = fma(p, f, 1.0);
-  const double r = ldexp(p, shift - (int)n) + 4503599627370496.0;
-  return (uint64_t)__double_as_longlong(r) & ((1ull << 52) - 1);
+  return ldexp(p, up - (int)n);
+}
+// A weight in units of 2^-shift; nothing more than shift + 1 doublings below the maximum.
+__device__ __forceinline__ uint64_t mass_of(double y, int shift) {
+  return y < (double)(shift + 1) ? (uint64_t)rint(exp2_neg(y, shift)) : 0;
 }
 
-struct Lds {
-  unsigned long long mass[NB];
-  unsigned long long kmass[NK];
-  uint32_t cnt[NB];
-  uint32_t kcnt[NK];
-  uint32_t lkey[LIST];
-  uint32_t lidx[LIST];
+// Distance from the maximum in doublings: 0 at the maximum itself (an infinite one included),
+// infinite for what has no mass beside it.
+struct Scale {
+  double top, c;  // the maximum, log2(e) / T
+  __device__ __forceinline__ double below(float x) const {
+    const double y = (top - (double)x) * c;
+    return x == (float)top ? 0.0 : (y >= 0.0 ? y : (double)INFINITY);
+  }
+};
+
+// A row's settings. K: how many tokens top_k leaves; greedy: the maximum is taken.
+struct Row {
+  double T, p, mp;
+  uint32_t K;
+  bool greedy;
+  uint64_t u;  // the draw in units of 2^-64
+};
+__device__ __forceinline__ Row row_of(const TokArgs& a, int m, uint32_t valid) {
+  Row r;
+  r.T = a.temperature ? (double)a.temperature[m] : a.t;
+  r.p = a.top_p ? (double)a.top_p[m] : a.p;
+  r.mp = a.min_p ? (double)a.min_p[m] : a.mp;
+  const int64_t k = a.top_k ? (int64_t)a.top_k[m] : a.k;
+  r.K = k > 0 && k < (int64_t)valid ? (uint32_t)k : valid;
+  r.greedy = !(r.T > 0.0) || r.p <= 0.0 || r.mp > 1.0 || r.K == 1;
+  const double u = a.draws_f64 ? static_cast<const double*>(a.draws)[m]
+                               : (double)static_cast<const float*>(a.draws)[m];
+  r.u = u > 0.0 ? (u < 1.0 ? (uint64_t)(u * 18446744073709551616.0) : ~0ull) : 0;
+  return r;
+}
+// ceil(p * mass), at least 1.
+__device__ __forceinline__ uint64_t share_of(double p, uint64_t mass) {
+  const uint64_t f = (uint64_t)(p * 18446744073709551616.0);
+  return max((uint64_t)1, (uint64_t)__umul64hi(f, mass) + (f * mass ? 1 : 0));
+}
+
+// Where a search ends: the value, the tokens before it in sorted order, how many of those that
+// hold it are needed (1 or more), the mass up to the last of them.
+struct Leaf {
+  uint32_t key, before, in;
+  uint64_t total;
+};
+
+// The cuts and the draw, from a search(P, K) for the first place where the mass reaches P (0: no
+// such bound) or the count K; `near` tokens pass min_p, `all` is the row's mass.
+template <typename Search>
+__device__ __forceinline__ Leaf draw_of(const Row& r, uint32_t valid, uint32_t near, uint64_t all,
+                                        uint32_t& kept, Search&& search) {
+  uint64_t P = 0;
+  if (r.p < 1.0) P = share_of(r.p, r.K < valid ? search(0, r.K).total : all);
+  const uint32_t K = r.mp > 0.0 ? min(r.K, max(near, 1u)) : r.K;
+  kept = valid;
+  uint64_t mass = all;
+  if (P || K < valid) {
+    const Leaf cut = search(P, K);
+    kept = cut.before + cut.in;
+    mass = cut.total;
+  }
+  return search(__umul64hi(r.u, mass) + 1, kept);
+}
+__device__ __forceinline__ bool reached(uint64_t mass, uint32_t count, uint64_t P, uint32_t K) {
+  return (P && mass >= P) || count >= K;
+}
+
+struct Found {
+  uint64_t mass, own;  // before the bin, of the bin
+  uint32_t bin, before, group;
+};
+struct Slots {
   uint64_t s64[TT / 64];
   uint32_t s32[TT / 64];
-  uint64_t f_mass;  // of find()
-  uint32_t f_bin, f_cnt;
+  Found found;
+  Leaf leaf;
   uint32_t n_list, best;
 };
 
-// Where a search ends: the value (key), what stands before it in sorted order, how many tokens
-// hold it and how many of those are needed.
-struct Leaf {
-  uint32_t key;
-  uint64_t mass;
-  uint32_t before, group, in;
-  uint64_t w;
-  int bin;
-  __device__ uint32_t count() const { return before + in; }
-  __device__ uint64_t total() const { return mass + in * w; }
-};
-
-// The first of N bins at whose end the mass reaches P (0: no such bound) or the count K.
-template <int N>
-__device__ __forceinline__ void find(Lds& s, const unsigned long long* mass, const uint32_t* cnt,
-                                     uint64_t mb, uint32_t cb, uint64_t P, uint32_t K) {
-  constexpr int PER = N / TT;
-  const int b0 = threadIdx.x * PER;
-  uint64_t m = 0;
-  uint32_t c = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    m += mass ? mass[b0 + j] : 0;
-    c += cnt[b0 + j];
-  }
-  uint64_t pm = m;
-  uint32_t pc = c;
-  if (threadIdx.x == 0) {  // (a bound always lies within the bins)
-    s.f_bin = N - 1;
-    s.f_mass = mb;
-    s.f_cnt = cb;
-  }
-  block_excl_scan(pm, pc, s.s64, s.s32);
-  pm += mb;
-  pc += cb;
-  auto reached = [&](uint64_t a, uint32_t b) { return (P && a >= P) || b >= K; };
-  if (!reached(pm, pc) && reached(pm + m, pc + c)) {
-    for (int j = 0; j < PER; ++j) {
-      const uint64_t mj = mass ? mass[b0 + j] : 0;
-      const uint32_t cj = cnt[b0 + j];
-      if (reached(pm + mj, pc + cj)) {
-        s.f_bin = b0 + j;
-        s.f_mass = pm;
-        s.f_cnt = pc;
-        break;
-      }
-      pm += mj;
-      pc += cj;
-    }
-  }
+// First index of the value with key `key` (all threads get it).
+template <int DT>
+__device__ __forceinline__ uint32_t first_index(const typename Elem<DT>::type* row, int V,
+                                                uint32_t key, Slots& s) {
+  if (threadIdx.x == 0) s.best = 0xFFFFFFFFu;
   __syncthreads();
+  uint32_t best = 0xFFFFFFFFu;
+  for_row<DT>(row, V, [&](int i, float x) {
+    if (key_of<DT>(x) == key) best = min(best, (uint32_t)i);
+  });
+  if (best != 0xFFFFFFFFu) atomicMin(&s.best, best);
+  __syncthreads();
+  return s.best;
 }
 
-// Smallest key in [1, kmax] whose bin is at most j: 64 candidates at a time.
+// The token of rank `rank` (from 0) by index among those of value `key`, whose numbers per
+// segment of seg tokens stand in count: the segment, then the place in it.
 template <int DT>
-__device__ __forceinline__ uint32_t first_key(const Scale& sc, uint32_t kmax, int j) {
-  uint32_t lo = 1, hi = kmax;  // hi holds
-  while (lo < hi) {
-    const uint32_t step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
-    const uint32_t c = (uint32_t)min((uint64_t)lo + (uint64_t)lane * step, (uint64_t)hi);
-    const uint64_t is = __ballot(bin_of(sc.below(key_value<DT>(c))) <= j);
-    const uint32_t f = is ? __builtin_ctzll(is) : 64;
-    const uint32_t at = lo;
-    if (f < 64) hi = (uint32_t)min((uint64_t)at + (uint64_t)f * step, (uint64_t)hi);
-    lo = f ? at + (f - 1) * step + 1 : at;
-    if (f == 0) hi = at;
-  }
-  return hi;
-}
-
-template <int DT>
-__global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
-  typedef typename Elem<DT>::type E;
-  extern __shared__ __align__(16) char lds_raw[];
-  Lds& s = *reinterpret_cast<Lds*>(lds_raw);
-  const int tid = threadIdx.x, m = blockIdx.x, V = a.V;
-  const E* const row = static_cast<const E*>(a.logits) + (int64_t)m * a.ld;
-
-  uint32_t kmax = 0, valid = 0;
-  for_row<DT>(row, V, [&](int, float x) {
-    const uint32_t k = key_of<DT>(x);
-    kmax = max(kmax, k);
-    valid += k ? 1u : 0u;
-  });
-  kmax = block_max<TT / 64>(kmax, s.s32);
-  valid = block_sum<TT / 64>(valid, s.s32);
-  if (kmax == 0) {  // nothing to draw
-    if (tid == 0) {
-      a.tokens[m] = -1;
-      if (a.kept) a.kept[m] = 0;
-    }
-    return;
-  }
-  const double T = a.temperature ? (double)a.temperature[m] : a.t;
-  const int64_t topk = a.top_k ? (int64_t)a.top_k[m] : a.k;
-  const double p = a.top_p ? (double)a.top_p[m] : a.p;
-  const double mp = a.min_p ? (double)a.min_p[m] : a.mp;
-  uint32_t K = topk > 0 && topk < (int64_t)valid ? (uint32_t)topk : valid;
-  if (!(T > 0.0) || p <= 0.0 || mp > 1.0) K = 1;
-  if (K == 1) {  // the lowest index of the maximum
-    if (tid == 0) s.best = 0xFFFFFFFFu;
-    __syncthreads();
-    uint32_t best = 0xFFFFFFFFu;
-    for_row<DT>(row, V, [&](int i, float x) {
-      if (key_of<DT>(x) == kmax) best = min(best, (uint32_t)i);
-    });
-    if (best != 0xFFFFFFFFu) atomicMin(&s.best, best);
-    __syncthreads();
-    if (tid == 0) {
-      a.tokens[m] = s.best;
-      if (a.kept) a.kept[m] = 1;
-    }
-    return;
-  }
-
-  const Scale sc{key_value<DT>(kmax), 1.4426950408889634 / T};
-  const double ymin = mp > 0.0 ? -log2(mp) : INFINITY;
-  for (int j = tid; j < NB; j += TT) {
-    s.mass[j] = 0;
-    s.cnt[j] = 0;
-  }
-  if (tid == 0) s.n_list = 0;
-  __syncthreads();
-  uint32_t near = 0;  // tokens that min_p leaves
-  uint64_t all = 0;
-  for_row<DT>(row, V, [&](int, float x) {
-    if (!key_of<DT>(x)) return;
-    const double y = sc.below(x);
-    const int b = bin_of(y);
-    const uint64_t w = mass_of(y, a.shift);
-    atomicAdd(&s.mass[b], (unsigned long long)w);
-    atomicAdd(&s.cnt[b], 1u);
-    all += w;
-    near += y <= ymin ? 1u : 0u;
-  });
-  near = block_sum<TT / 64>(near, s.s32);
-  all = block_sum<TT / 64>(all, s.s64);
-
-  int listed = -1;  // the bin whose tokens stand in the list
-  auto descend = [&](uint64_t P, uint32_t bound) {
-    find<NB>(s, s.mass, s.cnt, 0, 0, P, bound);
-    Leaf r;
-    const int bin = r.bin = s.f_bin;
-    r.mass = s.f_mass;
-    r.before = s.f_cnt;
-    r.group = s.cnt[bin];
-    uint32_t lo = first_key<DT>(sc, kmax, bin);
-    uint32_t hi = bin ? first_key<DT>(sc, kmax, bin - 1) - 1 : kmax;
-    const bool list = r.group <= LIST;
-    __syncthreads();
-    if (list && listed != bin) {
-      if (tid == 0) s.n_list = 0;
-      __syncthreads();
-      for_row<DT>(row, V, [&](int i, float x) {
-        const uint32_t k = key_of<DT>(x);
-        if (k < lo || k > hi) return;
-        const uint32_t at = atomicAdd(&s.n_list, 1u);
-        if (at >= LIST) return;  // (never: the bin holds as many)
-        s.lkey[at] = k;
-        s.lidx[at] = i;
-      });
-      listed = bin;
-      __syncthreads();
-    }
-    while (lo < hi) {
-      const int sh = max(0, 32 - __clz(hi - lo) - KEY_BITS);
-      for (int j = tid; j < NK; j += TT) {
-        s.kmass[j] = 0;
-        s.kcnt[j] = 0;
-      }
-      __syncthreads();
-      auto add = [&](uint32_t k) {
-        if (k < lo || k > hi) return;
-        const uint32_t q = (hi - k) >> sh;
-        atomicAdd(&s.kmass[q], (unsigned long long)mass_of(sc.below(key_value<DT>(k)), a.shift));
-        atomicAdd(&s.kcnt[q], 1u);
-      };
-      if (list) {
-        for (uint32_t i = tid; i < min(s.n_list, (uint32_t)LIST); i += TT) add(s.lkey[i]);
-      } else {
-        for_row<DT>(row, V, [&](int, float x) { add(key_of<DT>(x)); });
-      }
-      __syncthreads();
-      find<NK>(s, s.kmass, s.kcnt, r.mass, r.before, P, bound);
-      const uint32_t q = min(s.f_bin, (hi - lo) >> sh);
-      r.mass = s.f_mass;
-      r.before = s.f_cnt;
-      r.group = s.kcnt[q];
-      hi -= q << sh;
-      const uint32_t width = (1u << sh) - 1;
-      if (hi - lo > width) lo = hi - width;
-      __syncthreads();
-    }
-    r.key = hi;
-    r.w = mass_of(sc.below(key_value<DT>(hi)), a.shift);
-    r.in = min(r.group, bound - r.before);
-    if (P && r.w) {
-      const uint64_t need = (P - r.mass + r.w - 1) / r.w;
-      if (need < r.in) r.in = (uint32_t)need;
-    }
-    return r;
-  };
-
-  uint64_t P = 0;
-  if (p < 1.0) {
-    const uint64_t most = K < valid ? descend(0, K).total() : all;
-    const uint64_t pf = (uint64_t)(p * 18446744073709551616.0);
-    P = __umul64hi(pf, most) + (pf * most ? 1 : 0);
-    if (P == 0) P = 1;
-  }
-  K = min(K, max(near, 1u));
-  uint32_t kept = valid;
-  uint64_t mass = all;
-  if (P || K < valid) {
-    const Leaf cut = descend(P, K);
-    kept = cut.count();
-    mass = cut.total();
-  }
-  const double u = a.draws_f64 ? static_cast<const double*>(a.draws)[m]
-                               : (double)static_cast<const float*>(a.draws)[m];
-  const uint64_t uf = u > 0.0 ? (u < 1.0 ? (uint64_t)(u * 18446744073709551616.0) : ~0ull) : 0;
-  const Leaf d = descend(__umul64hi(uf, mass) + 1, 0xFFFFFFFFu);
-
-  // The token of rank d.in - 1 among those of value d.key, by index: the segment of the row
-  // that holds it, then its place there.
-  const int seg = (V + SEGS - 1) / SEGS;
-  for (int j = tid; j < SEGS; j += TT) s.kcnt[j] = 0;
-  __syncthreads();
-  if (listed == d.bin) {
-    for (uint32_t i = tid; i < min(s.n_list, (uint32_t)LIST); i += TT)
-      if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] / seg], 1u);
-  } else {
-    for_row<DT>(row, V, [&](int i, float x) {
-      if (key_of<DT>(x) == d.key) atomicAdd(&s.kcnt[i / seg], 1u);
-    });
+__device__ __forceinline__ void pick(const TokArgs& a, const typename Elem<DT>::type* row, int m,
+                                     uint32_t key, uint32_t rank, const uint32_t* count, int seg,
+                                     uint32_t kept, Slots& s) {
+  const int tid = threadIdx.x, V = a.V;
+  uint64_t unused = 0;
+  const uint32_t mine = count[tid];
+  uint32_t upto = mine;
+  block_excl_scan(unused, upto, s.s64, s.s32);
+  if (upto <= rank && rank < upto + mine) {
+    s.found.bin = tid;
+    s.found.before = upto;
   }
   __syncthreads();
-  find<NK>(s, nullptr, s.kcnt, 0, 0, 0, d.in);
   if (tid >= 64) return;
-  const int i0 = (int)s.f_bin * seg, i1 = min(V, i0 + seg);
-  uint32_t left = d.in - 1 - s.f_cnt;
+  const int i0 = (int)s.found.bin * seg, i1 = min(V, i0 + seg);
+  uint32_t left = rank - s.found.before;
   for (int i = i0; i < i1; i += 64) {
     const int at = i + tid;
-    bool hit = false;
-    if (at < i1) {
-      if constexpr (DT == 2)
-        hit = key_of<DT>(row[at]) == d.key;
-      else
-        hit = key_of<DT>(value_of<DT>(row[at])) == d.key;
-    }
+    const bool hit = at < i1 && key_of<DT>(value_of<DT>(row[min(at, V - 1)])) == key;
     const uint64_t hits = __ballot(hit);
     const uint32_t n = __popcll(hits);
     if (left < n) {
@@ -429,11 +270,443 @@ __global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
   }
 }
 
+// ------------------------------------------------- bins of the distance --
+// 64 bins per doubling below the maximum. A token adds one 64-bit number to its bin: 1 to the
+// count in the upper bits, and (1 - 2^-(f / 64)) 2^UNIT to a sum in the lower ones, f its place in
+// the bin. A bin's mass is 2^-(bin / 64) (count - sum): one LDS atomic and 5 FMAs per token
+// instead of two and an exponential. Within a bin the tokens' weights are relative to the bin's
+// first, and P is a share of the bin's mass.
+constexpr int NB = 4096;
+constexpr int PER = NB / TT;   // bins of a thread
+constexpr int NK = TT;         // bins of keys
+constexpr int KEY_BITS = 10;
+constexpr int LIST = 4096;     // tokens of one bin that LDS holds
+constexpr double A64 = 0.010830424696249145;  // ln(2) / 64
+
+struct General {
+  unsigned long long bins[NB];
+  unsigned long long kmass[NK];
+  uint32_t kcnt[NK];
+  uint32_t lkey[LIST];
+  uint32_t lidx[LIST];
+  Slots s;
+};
+
+__device__ __forceinline__ double bin_place(double y) { return fmin(y * 64.0, (double)(NB - 1)); }
+
+// Smallest key in [1, kmax] whose bin is at most j: 64 candidates at a time.
 template <int DT>
+__device__ __forceinline__ uint32_t first_key(const Scale& sc, uint32_t kmax, int j) {
+  uint32_t lo = 1, hi = kmax;  // hi holds
+  while (lo < hi) {
+    const uint32_t step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
+    const uint32_t c = (uint32_t)min((uint64_t)lo + (uint64_t)lane * step, (uint64_t)hi);
+    const uint64_t is = __ballot((int)bin_place(sc.below(key_value<DT>(c))) <= j);
+    const uint32_t f = is ? __builtin_ctzll(is) : 64;
+    const uint32_t at = lo;
+    if (f < 64) hi = (uint32_t)min((uint64_t)at + (uint64_t)f * step, (uint64_t)hi);
+    lo = f ? at + (f - 1) * step + 1 : hi;
+  }
+  return hi;
+}
+
+template <int DT>
+__device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s, uint32_t kmax,
+                                            uint32_t valid, const Row& r) {
+  typedef typename Elem<DT>::type E;
+  const int tid = threadIdx.x, V = a.V;
+  const E* const row = static_cast<const E*>(a.logits) + (int64_t)m * a.ld;
+  const Scale sc{key_value<DT>(kmax), 1.4426950408889634 / r.T};
+  const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
+  // units of a place's sum: the sum of V of them, below V A64, stays in the lower bits
+  const int cbits = a.V < 1 << 18 ? 18 : 21, unit = 70 - 2 * cbits;
+  const int sbits = 64 - cbits;
+  for (int j = tid; j < NB; j += TT) s.bins[j] = 0;
+  if (tid == 0) s.s.n_list = 0;
+  __syncthreads();
+  uint32_t near = 0;  // tokens that min_p leaves
+  {
+    const double sl = ldexp(1.0, unit), k1 = A64 * sl, k2 = -A64 * A64 / 2 * sl,
+                 k3 = A64 * A64 * A64 / 6 * sl, k4 = -A64 * A64 * A64 * A64 / 24 * sl,
+                 k5 = A64 * A64 * A64 * A64 * A64 / 120 * sl;
+    for_row<DT>(row, V, [&](int, float x) {
+      if (!(x > -INFINITY)) return;
+      const double y = sc.below(x);
+      near += y <= ymin ? 1u : 0u;
+      const double z = bin_place(y);
+      const int b = (int)z;
+      const double f = z - b;
+      // (the double's last place is 1 after 2^52 is added)
+      const double q = fma(fma(fma(fma(fma(k5, f, k4), f, k3), f, k2), f, k1), f, 4503599627370496.0);
+      const uint64_t lo = (uint64_t)__double_as_longlong(q) & ((1ull << 52) - 1);
+      atomicAdd(&s.bins[b], (unsigned long long)(lo + (1ull << sbits)));
+    });
+  }
+  near = block_sum<TT / 64>(near, s.s.s32);
+  // this thread's bins: masses, counts, and what stands before them
+  uint64_t bm[PER], pm = 0;
+  uint32_t bc[PER], pc = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const uint64_t v = s.bins[tid * PER + j];
+    bc[j] = (uint32_t)(v >> sbits);
+    const double part = (double)bc[j] - ldexp((double)(v & ((1ull << sbits) - 1)), -unit);
+    bm[j] = bc[j] ? (uint64_t)rint(part * exp2_neg((tid * PER + j) * (1.0 / 64), a.shift)) : 0;
+    pm += bm[j];
+    pc += bc[j];
+  }
+  const uint64_t tm = pm;
+  const uint32_t tc = pc;
+  block_excl_scan(pm, pc, s.s.s64, s.s.s32);
+  const uint64_t all = block_sum<TT / 64>(tm, s.s.s64);
+
+  int listed = -1, last = -1;  // bins: whose tokens stand in the list, that held the last place
+  auto search = [&](uint64_t P, uint32_t K) {
+    if (P > all) P = all;
+    if (!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K)) {
+      uint64_t mj = pm;
+      uint32_t cj = pc;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (!reached(mj, cj, P, K) && reached(mj + bm[j], cj + bc[j], P, K))
+          s.s.found = Found{mj, bm[j], (uint32_t)(tid * PER + j), cj, bc[j]};
+        mj += bm[j];
+        cj += bc[j];
+      }
+    }
+    __syncthreads();
+    const Found top = s.s.found;
+    const int bin = last = top.bin;
+    uint32_t lo = first_key<DT>(sc, kmax, bin);
+    uint32_t hi = bin ? first_key<DT>(sc, kmax, bin - 1) - 1 : kmax;
+    const bool list = top.group <= LIST;
+    if (list && listed != bin) {
+      if (tid == 0) s.s.n_list = 0;
+      __syncthreads();
+      for_row<DT>(row, V, [&](int i, float x) {
+        const uint32_t k = key_of<DT>(x);
+        if (k < lo || k > hi) return;
+        const uint32_t at = atomicAdd(&s.s.n_list, 1u);
+        if (at >= LIST) return;  // (never: the bin holds as many)
+        s.lkey[at] = k;
+        s.lidx[at] = i;
+      });
+      listed = bin;
+    }
+    __syncthreads();
+    const uint32_t n = min(s.s.n_list, (uint32_t)LIST);
+    // weights relative to the bin's start: 2^44 of it at most
+    auto rel = [&](uint32_t k) {
+      return (uint64_t)rint(exp2_neg(fmax(sc.below(key_value<DT>(k)) - bin * (1.0 / 64), 0.0), a.shift));
+    };
+    uint64_t Q = 0, mb = 0, sum = 0;  // P in those, before the range, of the whole bin
+    uint32_t cb = top.before, group = top.group;
+    bool first = true;
+    while (lo < hi) {
+      const int sh = max(0, 32 - __clz(hi - lo) - KEY_BITS);
+      for (int j = tid; j < NK; j += TT) {
+        s.kmass[j] = 0;
+        s.kcnt[j] = 0;
+      }
+      __syncthreads();
+      auto add = [&](uint32_t k) {
+        if (k < lo || k > hi) return;
+        atomicAdd(&s.kmass[(hi - k) >> sh], (unsigned long long)rel(k));
+        atomicAdd(&s.kcnt[(hi - k) >> sh], 1u);
+      };
+      if (list) {
+        for (uint32_t i = tid; i < n; i += TT) add(s.lkey[i]);
+      } else {
+        for_row<DT>(row, V, [&](int, float x) { add(key_of<DT>(x)); });
+      }
+      __syncthreads();
+      const uint64_t mt = s.kmass[tid];
+      const uint32_t ct = s.kcnt[tid];
+      uint64_t before = mt;
+      uint32_t upto = ct;
+      block_excl_scan(before, upto, s.s.s64, s.s.s32);
+      if (first) {
+        sum = block_sum<TT / 64>(mt, s.s.s64);
+        // (a bin whose tokens have no mass of their own: the last one)
+        Q = P ? (top.own ? (uint64_t)ceil((double)(P - top.mass) / (double)top.own * (double)sum)
+                         : sum) : 0;
+        Q = P > top.mass + top.own ? 0 : min(max(Q, (uint64_t)(P ? 1 : 0)), sum);
+        first = false;
+      }
+      before += mb;
+      upto += cb;
+      if (!reached(before, upto, Q, K) && reached(before + mt, upto + ct, Q, K))
+        s.s.found = Found{before, mt, (uint32_t)tid, upto, ct};
+      __syncthreads();
+      const Found f = s.s.found;
+      const uint32_t q = min(f.bin, (hi - lo) >> sh), width = (1u << sh) - 1;
+      mb = f.mass;
+      cb = f.before;
+      group = f.group;
+      hi -= q << sh;
+      if (hi - lo > width) lo = hi - width;
+      __syncthreads();
+    }
+    const uint64_t w = rel(hi);
+    if (first) {  // the bin is one value
+      sum = w * group;
+      Q = P && P <= top.mass + top.own && top.own
+              ? max((uint64_t)1, (uint64_t)ceil((double)(P - top.mass) / (double)top.own * (double)sum))
+              : 0;
+    }
+    Leaf l;
+    l.key = hi;
+    l.before = cb;
+    l.in = min(group, K - cb);
+    if (Q) {
+      const uint64_t need = (Q - mb + w - 1) / w;  // (w >= 2^43 / 2^(1/64))
+      if (need < l.in) l.in = (uint32_t)need;
+    }
+    l.in = max(l.in, 1u);
+    const uint64_t end = mb + l.in * w;
+    l.total = top.mass + (end >= sum ? top.own
+                                     : (uint64_t)rint((double)end / (double)sum * (double)top.own));
+    if (l.total == 0) l.total = 1;
+    return l;
+  };
+
+  uint32_t kept;
+  const Leaf d = draw_of(r, valid, near, all, kept, search);
+  const int seg = (V + SEGS - 1) / SEGS;
+  s.kcnt[tid] = 0;
+  __syncthreads();
+  if (listed == last) {
+    for (uint32_t i = tid; i < min(s.s.n_list, (uint32_t)LIST); i += TT)
+      if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] / seg], 1u);
+  } else {
+    for_row<DT>(row, V, [&](int i, float x) {
+      if (key_of<DT>(x) == d.key) atomicAdd(&s.kcnt[i / seg], 1u);
+    });
+  }
+  __syncthreads();
+  pick<DT>(a, row, m, d.key, d.in - 1, s.kcnt, seg, kept, s.s);
+}
+
+template <int DT>
+__device__ __forceinline__ void maximum(const typename Elem<DT>::type* row, int V, uint32_t& kmax,
+                                        uint32_t& valid, Slots& s) {
+  kmax = valid = 0;
+  for_row<DT>(row, V, [&](int, float x) {
+    const uint32_t k = key_of<DT>(x);
+    kmax = max(kmax, k);
+    valid += k ? 1u : 0u;
+  });
+  kmax = block_max<TT / 64>(kmax, s.s32);
+  valid = block_sum<TT / 64>(valid, s.s32);
+}
+
+// Rows with nothing to draw, or whose maximum is taken; true if done.
+template <int DT>
+__device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kmax, const Row& r,
+                                           Slots& s) {
+  typedef typename Elem<DT>::type E;
+  if (kmax && !r.greedy) return false;
+  int64_t token = -1;
+  if (kmax)
+    token = first_index<DT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, s);
+  if (threadIdx.x == 0) {
+    a.tokens[m] = token;
+    if (a.kept) a.kept[m] = kmax ? 1 : 0;
+  }
+  return true;
+}
+
+// ------------------------------------------------------- bf16: its values --
+// A bf16 row has few distinct values: their counts, one 32-bit LDS atomic per token, and a
+// weight per value. Bins by t(maximum) - t(x), t the value's bits as a 16-bit integer in the
+// order of the values; 34816 of them reach from the maximum m down past 0 to about -m. A row with
+// mass further down (an extreme temperature) takes the bins of the distance.
+constexpr int CB = 34 * TT;
+constexpr int CPER = CB / TT;
+typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+struct Counts {
+  uint32_t n[CB + 32];  // n[CB]: further down
+  Slots s;
+};
+
+// +0 -> 0, -0 -> -1; +inf, and what is a NaN above it; -inf, and what is a NaN below it.
+constexpr int T_INF = 0x7F80, T_NINF = 0x7F - 0x8000;
+__device__ __forceinline__ s16x2 order_of(uint32_t pair) {
+  const s16x2 x = __builtin_bit_cast(s16x2, pair);
+  return x ^ ((x >> 15) & (int16_t)0x7FFF);
+}
+__device__ __forceinline__ float ordered_value(int t) {
+  return bf2f((uint16_t)(t < 0 ? t ^ 0x7FFF : t));
+}
+
+template <typename One, typename Pair>
+__device__ __forceinline__ void for_pairs(const uint16_t* row, int V, One&& one, Pair&& pair) {
+  for_groups<0, 8>(row, V, one, [&](int i, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pair(i + 2 * e, w[e]);
+  });
+}
+
+// False if the row needs the bins of the distance.
+__device__ __forceinline__ bool count_row(const TokArgs& a, int m, Counts& s, int tmax, bool odd,
+                                          uint32_t valid, const Row& r) {
+  const int tid = threadIdx.x, lane = tid & 63, V = a.V;
+  const uint16_t* const row = static_cast<const uint16_t*>(a.logits) + (int64_t)m * a.ld;
+  const Scale sc{ordered_value(tmax), 1.4426950408889634 / r.T};
+  const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
+  for (int j = tid; j < (CB + 32) / 4; j += TT)
+    reinterpret_cast<uint4*>(s.n)[j] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  auto one = [&](int, uint16_t x) {
+    const int t = (int)order_of(x)[0];
+    if (t <= T_NINF || t > T_INF) return;
+    atomicAdd(&s.n[min(tmax - t, CB)], 1u);
+  };
+  if (odd) {
+    for_pairs(row, V, one, [&](int i, uint32_t w) {
+      one(i, (uint16_t)w);
+      one(i + 1, (uint16_t)(w >> 16));
+    });
+  } else {
+    const u16x2 top = (uint16_t)tmax, most = (uint16_t)CB;
+    for_pairs(row, V, one, [&](int, uint32_t w) {
+      const u16x2 d = __builtin_elementwise_min(top - __builtin_bit_cast(u16x2, order_of(w)), most);
+      atomicAdd(&s.n[d[0]], 1u);
+      atomicAdd(&s.n[d[1]], 1u);
+    });
+  }
+  __syncthreads();
+  if (s.n[CB]) {  // (what lies there begins at a distance of bin CB)
+    const double y = sc.below(ordered_value(max(tmax - CB, T_NINF + 1)));
+    if (y < a.shift + 2 || (r.mp > 0.0 && y <= ymin)) return false;
+  }
+  if (tid == 0 && tmax >= 0) {  // -0 with +0
+    s.n[tmax] += s.n[tmax + 1];
+    s.n[tmax + 1] = 0;
+  }
+  __syncthreads();
+  auto distance = [&](int bin) { return sc.below(ordered_value(tmax - bin)); };
+  uint64_t pm = 0;
+  uint32_t pc = 0, near = 0;
+#pragma unroll 2
+  for (int j = 0; j < CPER; ++j) {
+    const uint32_t c = s.n[tid * CPER + j];
+    if (!c) continue;
+    const double y = distance(tid * CPER + j);
+    pm += c * mass_of(y, a.shift);
+    pc += c;
+    near += y <= ymin ? c : 0u;
+  }
+  const uint64_t tm = pm;
+  const uint32_t tc = pc;
+  block_excl_scan(pm, pc, s.s.s64, s.s.s32);
+  near = block_sum<TT / 64>(near, s.s.s32);
+  const uint64_t all = block_sum<TT / 64>(tm, s.s.s64);
+  const uint32_t counted = valid - s.n[CB];
+
+  int found = 0;  // bin of the last search
+  auto search = [&](uint64_t P, uint32_t K) {
+    if (!P && K > counted) return Leaf{0u, K - 1, 1u, all};  // among those without mass
+    if (!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K))
+      s.s.found = Found{pm, 0, (uint32_t)tid, pc, 0};
+    __syncthreads();
+    const Found f = s.s.found;
+    // its 34 bins, one per lane
+    const int bin = (int)f.bin * CPER + min(lane, CPER - 1);
+    const uint32_t c = lane < CPER ? s.n[bin] : 0u;
+    const uint64_t w = c ? mass_of(distance(bin), a.shift) : 0, own = c * w;
+    const uint64_t end = wave_prefix(own, Add()) + f.mass;
+    const uint32_t upto = wave_prefix(c, Add()) + f.before;
+    const uint64_t hits = __ballot(reached(end, upto, P, K));
+    const int at = hits ? __builtin_ctzll(hits) : CPER - 1;
+    found = (int)f.bin * CPER + at;
+    const uint64_t own_at = lane_value(own, at), w_at = lane_value(w, at);
+    const uint64_t before = lane_value(end, at) - own_at;
+    const uint32_t c_at = lane_value(c, at);
+    Leaf l;
+    l.before = lane_value(upto, at) - c_at;
+    l.in = min(c_at, K - l.before);
+    if (P && w_at) l.in = (uint32_t)min((uint64_t)l.in, (P - before + w_at - 1) / w_at);
+    l.key = 0;
+    l.total = before + l.in * w_at;
+    __syncthreads();  // found has been read
+    return l;
+  };
+  uint32_t kept;
+  const Leaf d = draw_of(r, valid, near, all, kept, search);
+
+  const int seg = (V + SEGS - 1) / SEGS;
+  const int t = tmax - found;
+  const uint32_t bits = (uint32_t)(t < 0 ? t ^ 0x7FFF : t) & 0xFFFFu;
+  const uint32_t mask = bits << 1 & 0xFFFFu ? 0xFFFFFFFFu : 0x7FFF7FFFu;
+  const uint32_t want = (bits | bits << 16) & mask;
+  s.n[tid] = 0;
+  __syncthreads();
+  for_pairs(
+      row, V,
+      [&](int i, uint16_t x) {
+        if (((x ^ want) & mask & 0xFFFFu) == 0) atomicAdd(&s.n[i / seg], 1u);
+      },
+      [&](int i, uint32_t w) {
+        const uint32_t x = (w ^ want) & mask;
+        if (x >> 16 == 0) atomicAdd(&s.n[(i + 1) / seg], 1u);
+        if ((x & 0xFFFFu) == 0) atomicAdd(&s.n[i / seg], 1u);
+      });
+  __syncthreads();
+  pick<0>(a, row, m, key_of<0>(ordered_value(t)), d.in - 1, s.n, seg, kept, s.s);
+  return true;
+}
+
+__global__ void __launch_bounds__(TT) sample_tokens_bf16_kernel(TokArgs a) {
+  extern __shared__ __align__(16) char lds_raw[];
+  Counts& s = *reinterpret_cast<Counts*>(lds_raw);
+  const int m = blockIdx.x, V = a.V;
+  const uint16_t* const row = static_cast<const uint16_t*>(a.logits) + (int64_t)m * a.ld;
+  s16x2 hi = (int16_t)-0x8000, lo = (int16_t)0x7FFF;
+  auto pair = [&](int, uint32_t w) {
+    const s16x2 t = order_of(w);
+    hi = __builtin_elementwise_max(hi, t);
+    lo = __builtin_elementwise_min(lo, t);
+  };
+  for_pairs(row, V, [&](int i, uint16_t x) { pair(i, x | (uint32_t)x << 16); }, pair);
+  const int top = max((int)hi[0], (int)hi[1]), least = min((int)lo[0], (int)lo[1]);
+  int tmax = (int)block_max<TT / 64>((uint32_t)(top + 0x8000), s.s.s32) - 0x8000;
+  const int tmin = 0x8000 - (int)block_max<TT / 64>((uint32_t)(0x8000 - least), s.s.s32);
+  const bool odd = tmax > T_INF || tmin <= T_NINF;  // NaN or -inf among them
+  uint32_t kmax = 1, valid = (uint32_t)V;
+  if (odd) {
+    maximum<0>(row, V, kmax, valid, s.s);
+    tmax = (int)kmax - 0x8000;
+  } else {
+    kmax = key_of<0>(ordered_value(tmax));
+  }
+  const Row r = row_of(a, m, valid);
+  if (simple_row<0>(a, m, kmax, r, s.s)) return;
+  if (count_row(a, m, s, tmax, odd, valid, r)) return;
+  __syncthreads();
+  general_row<0>(a, m, *reinterpret_cast<General*>(lds_raw), kmax, valid, r);
+}
+
+template <int DT>
+__global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
+  typedef typename Elem<DT>::type E;
+  extern __shared__ __align__(16) char lds_raw[];
+  General& s = *reinterpret_cast<General*>(lds_raw);
+  const int m = blockIdx.x;
+  uint32_t kmax, valid;
+  maximum<DT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, valid, s.s);
+  const Row r = row_of(a, m, valid);
+  if (simple_row<DT>(a, m, kmax, r, s.s)) return;
+  general_row<DT>(a, m, s, kmax, valid, r);
+}
+
+template <auto KERN, int LDS>
 int go(const TokArgs& a, hipStream_t st) {
-  constexpr auto kern = sample_tokens_kernel<DT>;
-  if (int rc = allow_dynamic_lds<kern, (int)sizeof(Lds)>()) return rc;
-  kern<<<a.M, TT, sizeof(Lds), st>>>(a);
+  if (int rc = allow_dynamic_lds<KERN, LDS>()) return rc;
+  KERN<<<a.M, TT, LDS, st>>>(a);
   return launch_check("sample_tokens");
 }
 
@@ -456,5 +729,8 @@ extern "C" int grpo_sample_tokens(const void* logits, int dtype, int64_t ld, int
                   sampler->temperature, sampler->top_p, sampler->min_p, sampler->top_k,
                   min(44, 62 - bits), tokens, kept};
   hipStream_t st = as_stream(stream);
-  return dtype == 0 ? go<0>(a, st) : dtype == 1 ? go<1>(a, st) : go<2>(a, st);
+  constexpr int LDS = (int)sizeof(General);
+  if (dtype == 0) return go<sample_tokens_bf16_kernel, (int)std::max(sizeof(Counts), sizeof(General))>(a, st);
+  return dtype == 1 ? go<sample_tokens_kernel<1>, LDS>(a, st)
+                    : go<sample_tokens_kernel<2>, LDS>(a, st);
 }

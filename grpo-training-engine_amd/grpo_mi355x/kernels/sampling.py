@@ -15,7 +15,7 @@ from .. import _lib
 from .policy_loss import _run
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_MAX_VOCAB = 1 << 24
+_MAX_VOCAB = 1 << 20
 _MAX_ROWS = 1 << 31
 Setting = Union[float, torch.Tensor]
 

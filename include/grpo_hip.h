@@ -1075,7 +1075,7 @@ int grpo_draft_tree_accept(const int64_t* drafted, int64_t drafted_stride, const
  * 1, min_p <= 0: no such bound. NaN and -inf are never drawn; where +inf is the maximum only
  * +inf is. A row with nothing to draw gives token -1, kept 0.
  *   tokens : int64 [M];  kept : int32 [M], the tokens that the filters leave, or NULL */
-#define GRPO_SAMPLE_MAX_VOCAB (1 << 24)
+#define GRPO_SAMPLE_MAX_VOCAB (1 << 20)
 typedef struct {
   double temperature, top_p, min_p;
   int64_t top_k;

@@ -199,7 +199,7 @@ def test_drafted_tree_argument_errors(lib):
         return lib.grpo_sample_tokens(logits, dtype, ld, m, v, draws, 0,
                                       ctypes.byref(s) if sampler else None, tokens, None, None)
 
-    for kw in (dict(m=-1), dict(v=0), dict(v=(1 << 24) + 1), dict(dtype=3), dict(dtype=-1),
+    for kw in (dict(m=-1), dict(v=0), dict(v=(1 << 20) + 1), dict(dtype=3), dict(dtype=-1),
                dict(ld=99), dict(logits=None), dict(draws=None), dict(tokens=None),
                dict(sampler=False), dict(logits=p + 1), dict(logits=p + 2, dtype=2)):
         assert sample(**kw) < 0, kw
