@@ -17,6 +17,7 @@
 //
 // A workgroup of 1024 threads per row.
 #include <math.h>
+#include <stddef.h>
 
 #include <algorithm>
 
@@ -192,17 +193,21 @@ struct Leaf {
 template <typename Search>
 __device__ __forceinline__ Leaf draw_of(const Row& r, uint32_t valid, uint32_t near, uint64_t all,
                                         uint32_t& kept, Search&& search) {
-  uint64_t P = 0;
-  if (r.p < 1.0) P = share_of(r.p, r.K < valid ? search(0, r.K).total : all);
   const uint32_t K = r.mp > 0.0 ? min(r.K, max(near, 1u)) : r.K;
+  uint64_t mass = r.K < valid && r.p < 1.0 ? 0 : all;  // of what top_k leaves; then of what is kept
   kept = valid;
-  uint64_t mass = all;
-  if (P || K < valid) {
-    const Leaf cut = search(P, K);
-    kept = cut.before + cut.in;
-    mass = cut.total;
+  Leaf l;
+  // (one place that calls it: the code is large, and once it is there it is there for all three)
+#pragma unroll 1
+  for (int stage = mass ? 1 : 0; stage < 3; ++stage) {
+    const uint64_t P = stage == 0 ? 0 : stage == 2 ? __umul64hi(r.u, mass) + 1
+                                  : r.p < 1.0 ? share_of(r.p, mass) : 0;
+    if (stage == 1 && !P && K >= valid) continue;
+    l = search(P, stage == 0 ? r.K : stage == 1 ? K : kept);
+    mass = l.total;
+    if (stage == 1) kept = l.before + l.in;
   }
-  return search(__umul64hi(r.u, mass) + 1, kept);
+  return l;
 }
 __device__ __forceinline__ bool reached(uint64_t mass, uint32_t count, uint64_t P, uint32_t K) {
   return (P && mass >= P) || count >= K;
@@ -235,8 +240,12 @@ __device__ __forceinline__ uint32_t first_index(const typename Elem<DT>::type* r
   return s.best;
 }
 
+// Segments of 2^seg_bits tokens, at most SEGS of them.
+__device__ __forceinline__ int seg_bits(int V) { return max(0, 32 - __clz(V - 1) - 10); }
+static_assert(SEGS == 1 << 10, "");
+
 // The token of rank `rank` (from 0) by index among those of value `key`, whose numbers per
-// segment of seg tokens stand in count: the segment, then the place in it.
+// segment of 2^seg tokens stand in count: the segment, then the place in it.
 template <int DT>
 __device__ __forceinline__ void pick(const TokArgs& a, const typename Elem<DT>::type* row, int m,
                                      uint32_t key, uint32_t rank, const uint32_t* count, int seg,
@@ -252,7 +261,7 @@ __device__ __forceinline__ void pick(const TokArgs& a, const typename Elem<DT>::
   }
   __syncthreads();
   if (tid >= 64) return;
-  const int i0 = (int)s.found.bin * seg, i1 = min(V, i0 + seg);
+  const int i0 = (int)s.found.bin << seg, i1 = min(V, i0 + (1 << seg));
   uint32_t left = rank - s.found.before;
   for (int i = i0; i < i1; i += 64) {
     const int at = i + tid;
@@ -472,15 +481,15 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
 
   uint32_t kept;
   const Leaf d = draw_of(r, valid, near, all, kept, search);
-  const int seg = (V + SEGS - 1) / SEGS;
+  const int seg = seg_bits(V);
   s.kcnt[tid] = 0;
   __syncthreads();
   if (listed == last) {
     for (uint32_t i = tid; i < min(s.s.n_list, (uint32_t)LIST); i += TT)
-      if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] / seg], 1u);
+      if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] >> seg], 1u);
   } else {
     for_row<DT>(row, V, [&](int i, float x) {
-      if (key_of<DT>(x) == d.key) atomicAdd(&s.kcnt[i / seg], 1u);
+      if (key_of<DT>(x) == d.key) atomicAdd(&s.kcnt[i >> seg], 1u);
     });
   }
   __syncthreads();
@@ -518,20 +527,31 @@ __device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kma
 
 // ------------------------------------------------------- bf16: its values --
 // A bf16 row has few distinct values: their counts, one 32-bit LDS atomic per token, and a
-// weight per value. Bins by t(maximum) - t(x), t the value's bits as a 16-bit integer in the
-// order of the values; 34816 of them reach from the maximum m down past 0 to about -m. A row with
-// mass further down (an extreme temperature) takes the bins of the distance.
-constexpr int CB = 34 * TT;
-constexpr int CPER = CB / TT;
+// weight per value. The bins are fixed, the values of magnitude below 512 in descending order,
+// so that one pass over the row makes the counts and finds the maximum. A row with a larger
+// maximum, or with mass at -512 and below (an extreme temperature), takes the bins of the distance.
+// (The row in registers instead of its second reading: 8 / 512 rows of 151936 39 / 155 us against
+// 35 / 100, in code without loops that runs at the rate of its instruction fetches.)
+constexpr int CW = 64;              // bins of a group: one per lane
+constexpr int CG = 544;             // groups: one per thread
+constexpr int CB = CW * CG;
+constexpr int CI = CG / (TT / 64);  // groups of a wave
+constexpr int TOP = CB / 2;         // the bin of t is TOP - 1 - t
+static_assert(CG % (TT / 64) == 0 && CG <= TT, "groups split evenly");
+static_assert(TOP == 0x4400, "the bits of 512");
+constexpr int SEG_PER = 3;          // segments of a thread in the search for a token
 typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct Counts {
-  uint32_t n[CB + 32];  // n[CB]: further down
+  uint32_t n[CB + 32];  // n[CB]: of what has no bin
+  uint64_t mass[CG];    // of the groups
+  uint32_t count[CG];   // (all of these are zero at first)
   Slots s;
 };
 
-// +0 -> 0, -0 -> -1; +inf, and what is a NaN above it; -inf, and what is a NaN below it.
+// The value's bits as a 16-bit integer in the order of the values: +0 -> 0, -0 -> -1; +inf,
+// and what is a NaN above it; -inf, and what is a NaN below it.
 constexpr int T_INF = 0x7F80, T_NINF = 0x7F - 0x8000;
 __device__ __forceinline__ s16x2 order_of(uint32_t pair) {
   const s16x2 x = __builtin_bit_cast(s16x2, pair);
@@ -541,71 +561,144 @@ __device__ __forceinline__ float ordered_value(int t) {
   return bf2f((uint16_t)(t < 0 ? t ^ 0x7FFF : t));
 }
 
-template <typename One, typename Pair>
-__device__ __forceinline__ void for_pairs(const uint16_t* row, int V, One&& one, Pair&& pair) {
-  for_groups<0, 8>(row, V, one, [&](int i, const uint4& v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// Where the row's 16-byte groups begin, and how many they are.
+struct Groups {
+  const uint16_t* row;
+  int V, head, G;
+  __device__ __forceinline__ Groups(const TokArgs& a, int m)
+      : row(static_cast<const uint16_t*>(a.logits) + (int64_t)m * a.ld), V(a.V) {
+    const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / 2);
+    head = min(V, mis ? 8 - mis : 0);
+    G = (V - head) / 8;
+  }
+  __device__ __forceinline__ uint4 at(int g) const {
+    return *reinterpret_cast<const uint4*>(row + head + 8 * (int64_t)g);
+  }
+  // one(0 or 1, index, value) of the values before and after the groups, many(g, group)
+  template <typename One, typename Many>
+  __device__ __forceinline__ void each(One&& one, Many&& many) const {
+    constexpr int U = 8;
+    const int tid = threadIdx.x, tail = head + 8 * G + tid;
+    if (tid < head) one(0, tid, row[tid]);
+#pragma unroll 1
+    for (int g = tid; g < G; g += U * TT) {
+      uint4 w[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pair(i + 2 * e, w[e]);
-  });
+      for (int u = 0; u < U; ++u) w[u] = at(min(g + u * TT, G - 1));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (g + u * TT < G) many(g + u * TT, w[u]);
+    }
+    if (tail < V) one(1, tail, row[tail]);
+  }
+};
+
+// The token of rank `rank` among those whose bits are want (two of them, compared in mask),
+// counted per wave's groups; all threads get it.
+__device__ __forceinline__ void pick_bits(const TokArgs& a, const Groups& x, int m, uint32_t want,
+                                          uint32_t mask, uint32_t rank, uint32_t kept, Counts& s) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int segs = 2 + (x.G + 63) / 64;  // before the groups, 64 groups each, after them
+  for (int j = tid; j < SEG_PER * TT; j += TT) s.n[j] = 0;
+  __syncthreads();
+  auto matches = [&](const uint4& w) {
+    const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+    const u16x2 one = (uint16_t)1;
+    u16x2 not_it = (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      not_it += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (p[i] ^ want) & mask), one);
+    return 8u - not_it[0] - not_it[1];
+  };
+  auto is = [&](uint16_t v) { return ((v ^ want) & mask & 0xFFFFu) == 0; };
+  x.each(
+      [&](int end, int, uint16_t v) {
+        if (is(v)) atomicAdd(&s.n[end ? segs - 1 : 0], 1u);
+      },
+      [&](int g, const uint4& w) {
+        const uint32_t c = matches(w);
+        if (c) atomicAdd(&s.n[1 + g / 64], c);
+      });
+  __syncthreads();
+  uint32_t c[SEG_PER], mine = 0, upto;
+#pragma unroll
+  for (int j = 0; j < SEG_PER; ++j) mine += c[j] = s.n[SEG_PER * tid + j];
+  upto = mine;
+  uint64_t unused = 0;
+  block_excl_scan(unused, upto, s.s.s64, s.s.s32);
+  if (upto <= rank && rank < upto + mine) {
+#pragma unroll
+    for (int j = 0; j < SEG_PER; ++j) {
+      if (upto <= rank && rank < upto + c[j]) s.s.found = Found{0, 0, (uint32_t)(SEG_PER * tid + j), upto, 0};
+      upto += c[j];
+    }
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  const int seg = (int)s.s.found.bin;
+  const uint32_t left = rank - s.s.found.before;
+  // a lane's values: a group's eight, or one of an end
+  const int g = 64 * (seg - 1) + lane;
+  const bool ends = seg == 0 || seg == segs - 1;
+  const int first = ends ? (seg ? x.head + 8 * x.G : 0) + lane : x.head + 8 * g;
+  const int count = ends ? (first < (seg ? x.V : x.head) ? 1 : 0) : (g < x.G ? 8 : 0);
+  uint32_t bits = 0;
+  for (int i = 0; i < count; ++i) bits |= (uint32_t)is(x.row[first + i]) << i;
+  const uint32_t before = wave_prefix((uint32_t)__popc(bits), Add()) - __popc(bits);
+  if (before <= left && left < before + __popc(bits)) {
+    for (uint32_t k = left - before; k; --k) bits &= bits - 1;
+    a.tokens[m] = first + __builtin_ctz(bits);
+    if (a.kept) a.kept[m] = (int32_t)kept;
+  }
 }
 
 // False if the row needs the bins of the distance.
-__device__ __forceinline__ bool count_row(const TokArgs& a, int m, Counts& s, int tmax, bool odd,
-                                          uint32_t valid, const Row& r) {
-  const int tid = threadIdx.x, lane = tid & 63, V = a.V;
-  const uint16_t* const row = static_cast<const uint16_t*>(a.logits) + (int64_t)m * a.ld;
-  const Scale sc{ordered_value(tmax), 1.4426950408889634 / r.T};
+__device__ __forceinline__ bool count_row(const TokArgs& a, int m, const Groups& x, Counts& s,
+                                          uint32_t kmax, uint32_t valid, const Row& r) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Scale sc{key_value<0>(kmax), 1.4426950408889634 / r.T};
   const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
-  for (int j = tid; j < (CB + 32) / 4; j += TT)
-    reinterpret_cast<uint4*>(s.n)[j] = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  auto one = [&](int, uint16_t x) {
-    const int t = (int)order_of(x)[0];
-    if (t <= T_NINF || t > T_INF) return;
-    atomicAdd(&s.n[min(tmax - t, CB)], 1u);
-  };
-  if (odd) {
-    for_pairs(row, V, one, [&](int i, uint32_t w) {
-      one(i, (uint16_t)w);
-      one(i + 1, (uint16_t)(w >> 16));
-    });
-  } else {
-    const u16x2 top = (uint16_t)tmax, most = (uint16_t)CB;
-    for_pairs(row, V, one, [&](int, uint32_t w) {
-      const u16x2 d = __builtin_elementwise_min(top - __builtin_bit_cast(u16x2, order_of(w)), most);
-      atomicAdd(&s.n[d[0]], 1u);
-      atomicAdd(&s.n[d[1]], 1u);
-    });
-  }
-  __syncthreads();
-  if (s.n[CB]) {  // (what lies there begins at a distance of bin CB)
-    const double y = sc.below(ordered_value(max(tmax - CB, T_NINF + 1)));
+  if (!(fabs(sc.top) < 512.0)) return false;
+  if (s.n[CB]) {
+    const double y = sc.below(-512.f);
     if (y < a.shift + 2 || (r.mp > 0.0 && y <= ymin)) return false;
   }
-  if (tid == 0 && tmax >= 0) {  // -0 with +0
-    s.n[tmax] += s.n[tmax + 1];
-    s.n[tmax + 1] = 0;
+  auto distance = [&](int bin) { return sc.below(ordered_value(TOP - 1 - bin)); };
+  // The groups' masses and counts, a wave per group and a bin per lane: most groups are empty,
+  // and the others stand side by side.
+  uint32_t near = 0;
+  {
+    uint64_t some = 0;  // of this wave's groups
+#pragma unroll
+    for (int i = 0; i < CI; ++i)
+      some |= (uint64_t)(__ballot(s.n[CW * (wave + i * (TT / 64)) + lane] != 0) != 0) << i;
+#pragma unroll 1
+    for (; some; some &= some - 1) {
+      const int g = wave + __builtin_ctzll(some) * (TT / 64);
+      const uint32_t c = s.n[CW * g + lane];
+      const double y = distance(CW * g + lane);
+      const uint64_t mass = wave_prefix(c * mass_of(y, a.shift), Add());
+      const uint32_t count = wave_prefix(c, Add());
+      near += y <= ymin ? c : 0u;
+      if (lane == 63) {
+        s.mass[g] = mass;
+        s.count[g] = count;
+      }
+    }
   }
   __syncthreads();
-  auto distance = [&](int bin) { return sc.below(ordered_value(tmax - bin)); };
-  uint64_t pm = 0;
-  uint32_t pc = 0, near = 0;
-#pragma unroll 2
-  for (int j = 0; j < CPER; ++j) {
-    const uint32_t c = s.n[tid * CPER + j];
-    if (!c) continue;
-    const double y = distance(tid * CPER + j);
-    pm += c * mass_of(y, a.shift);
-    pc += c;
-    near += y <= ymin ? c : 0u;
-  }
-  const uint64_t tm = pm;
-  const uint32_t tc = pc;
+  const uint64_t tm = tid < CG ? s.mass[tid] : 0;
+  const uint32_t tc = tid < CG ? s.count[tid] : 0;
+  uint64_t pm = tm;
+  uint32_t pc = tc;
   block_excl_scan(pm, pc, s.s.s64, s.s.s32);
-  near = block_sum<TT / 64>(near, s.s.s32);
-  const uint64_t all = block_sum<TT / 64>(tm, s.s.s64);
-  const uint32_t counted = valid - s.n[CB];
+  if (tid == TT - 1) s.s.found = Found{0, pm + tm, 0, pc + tc, 0};
+  if (r.mp > 0.0) near = block_sum<TT / 64>(near, s.s.s32);
+  __syncthreads();
+  const uint64_t all = s.s.found.own;
+  const uint32_t counted = s.s.found.before;
+  __syncthreads();
 
   int found = 0;  // bin of the last search
   auto search = [&](uint64_t P, uint32_t K) {
@@ -614,15 +707,14 @@ __device__ __forceinline__ bool count_row(const TokArgs& a, int m, Counts& s, in
       s.s.found = Found{pm, 0, (uint32_t)tid, pc, 0};
     __syncthreads();
     const Found f = s.s.found;
-    // its 34 bins, one per lane
-    const int bin = (int)f.bin * CPER + min(lane, CPER - 1);
-    const uint32_t c = lane < CPER ? s.n[bin] : 0u;
-    const uint64_t w = c ? mass_of(distance(bin), a.shift) : 0, own = c * w;
+    const int bin = (int)f.bin * CW + lane;
+    const uint32_t c = s.n[bin];
+    const uint64_t w = mass_of(distance(bin), a.shift), own = c * w;
     const uint64_t end = wave_prefix(own, Add()) + f.mass;
     const uint32_t upto = wave_prefix(c, Add()) + f.before;
     const uint64_t hits = __ballot(reached(end, upto, P, K));
-    const int at = hits ? __builtin_ctzll(hits) : CPER - 1;
-    found = (int)f.bin * CPER + at;
+    const int at = hits ? __builtin_ctzll(hits) : 63;
+    found = (int)f.bin * CW + at;
     const uint64_t own_at = lane_value(own, at), w_at = lane_value(w, at);
     const uint64_t before = lane_value(end, at) - own_at;
     const uint32_t c_at = lane_value(c, at);
@@ -637,55 +729,53 @@ __device__ __forceinline__ bool count_row(const TokArgs& a, int m, Counts& s, in
   };
   uint32_t kept;
   const Leaf d = draw_of(r, valid, near, all, kept, search);
-
-  const int seg = (V + SEGS - 1) / SEGS;
-  const int t = tmax - found;
+  const int t = TOP - 1 - found;  // (-0 stands with +0)
   const uint32_t bits = (uint32_t)(t < 0 ? t ^ 0x7FFF : t) & 0xFFFFu;
-  const uint32_t mask = bits << 1 & 0xFFFFu ? 0xFFFFFFFFu : 0x7FFF7FFFu;
-  const uint32_t want = (bits | bits << 16) & mask;
-  s.n[tid] = 0;
-  __syncthreads();
-  for_pairs(
-      row, V,
-      [&](int i, uint16_t x) {
-        if (((x ^ want) & mask & 0xFFFFu) == 0) atomicAdd(&s.n[i / seg], 1u);
-      },
-      [&](int i, uint32_t w) {
-        const uint32_t x = (w ^ want) & mask;
-        if (x >> 16 == 0) atomicAdd(&s.n[(i + 1) / seg], 1u);
-        if ((x & 0xFFFFu) == 0) atomicAdd(&s.n[i / seg], 1u);
-      });
-  __syncthreads();
-  pick<0>(a, row, m, key_of<0>(ordered_value(t)), d.in - 1, s.n, seg, kept, s.s);
+  pick_bits(a, x, m, bits | bits << 16, bits ? 0xFFFFFFFFu : 0x7FFF7FFFu, d.in - 1, kept, s);
   return true;
 }
 
 __global__ void __launch_bounds__(TT) sample_tokens_bf16_kernel(TokArgs a) {
   extern __shared__ __align__(16) char lds_raw[];
   Counts& s = *reinterpret_cast<Counts*>(lds_raw);
-  const int m = blockIdx.x, V = a.V;
-  const uint16_t* const row = static_cast<const uint16_t*>(a.logits) + (int64_t)m * a.ld;
+  const int m = blockIdx.x;
+  const Groups x(a, m);
+  static_assert(offsetof(Counts, s) % 16 == 0, "cleared 16 bytes at a time");
+  for (int j = threadIdx.x; j < (int)offsetof(Counts, s) / 16; j += TT)
+    reinterpret_cast<uint4*>(s.n)[j] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
   s16x2 hi = (int16_t)-0x8000, lo = (int16_t)0x7FFF;
-  auto pair = [&](int, uint32_t w) {
+  const u16x2 top = (uint16_t)(TOP - 1), none = (uint16_t)CB;
+  auto pair = [&](uint32_t w) {
     const s16x2 t = order_of(w);
     hi = __builtin_elementwise_max(hi, t);
     lo = __builtin_elementwise_min(lo, t);
+    return __builtin_elementwise_min(top - __builtin_bit_cast(u16x2, t), none);
   };
-  for_pairs(row, V, [&](int i, uint16_t x) { pair(i, x | (uint32_t)x << 16); }, pair);
-  const int top = max((int)hi[0], (int)hi[1]), least = min((int)lo[0], (int)lo[1]);
-  int tmax = (int)block_max<TT / 64>((uint32_t)(top + 0x8000), s.s.s32) - 0x8000;
+  x.each([&](int, int, uint16_t v) { atomicAdd(&s.n[pair(v * 0x10001u)[0]], 1u); },
+         [&](int, const uint4& v) {
+           const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+           for (int i = 0; i < 4; ++i) {
+             const u16x2 d = pair(w[i]);
+             atomicAdd(&s.n[d[0]], 1u);
+             atomicAdd(&s.n[d[1]], 1u);
+           }
+         });
+  const int most = max((int)hi[0], (int)hi[1]), least = min((int)lo[0], (int)lo[1]);
+  const int tmax = (int)block_max<TT / 64>((uint32_t)(most + 0x8000), s.s.s32) - 0x8000;
   const int tmin = 0x8000 - (int)block_max<TT / 64>((uint32_t)(0x8000 - least), s.s.s32);
-  const bool odd = tmax > T_INF || tmin <= T_NINF;  // NaN or -inf among them
-  uint32_t kmax = 1, valid = (uint32_t)V;
-  if (odd) {
-    maximum<0>(row, V, kmax, valid, s.s);
-    tmax = (int)kmax - 0x8000;
-  } else {
-    kmax = key_of<0>(ordered_value(tmax));
+  uint32_t kmax = key_of<0>(ordered_value(tmax)), valid = (uint32_t)a.V;
+  if (tmax > T_INF || tmin <= T_NINF)  // NaN or -inf among them
+    maximum<0>(x.row, a.V, kmax, valid, s.s);
+  if (threadIdx.x == 0) {  // -0 with +0
+    s.n[TOP - 1] += s.n[TOP];
+    s.n[TOP] = 0;
   }
+  __syncthreads();
   const Row r = row_of(a, m, valid);
   if (simple_row<0>(a, m, kmax, r, s.s)) return;
-  if (count_row(a, m, s, tmax, odd, valid, r)) return;
+  if (count_row(a, m, x, s, kmax, valid, r)) return;
   __syncthreads();
   general_row<0>(a, m, *reinterpret_cast<General*>(lds_raw), kmax, valid, r);
 }
@@ -730,7 +820,8 @@ extern "C" int grpo_sample_tokens(const void* logits, int dtype, int64_t ld, int
                   min(44, 62 - bits), tokens, kept};
   hipStream_t st = as_stream(stream);
   constexpr int LDS = (int)sizeof(General);
-  if (dtype == 0) return go<sample_tokens_bf16_kernel, (int)std::max(sizeof(Counts), sizeof(General))>(a, st);
+  constexpr int LDS16 = (int)std::max(sizeof(Counts), sizeof(General));
+  if (dtype == 0) return go<sample_tokens_bf16_kernel, LDS16>(a, st);
   return dtype == 1 ? go<sample_tokens_kernel<1>, LDS>(a, st)
                     : go<sample_tokens_kernel<2>, LDS>(a, st);
 }
