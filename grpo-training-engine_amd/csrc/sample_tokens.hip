@@ -15,7 +15,9 @@
 //    its values in bf16, else of 4096 distances from the maximum and then, within the one of
 //    them that holds the place, of the order-preserving keys until a bin is one value.
 //
-// A workgroup of 1024 threads per row.
+// A workgroup per row: of 1024 threads, or of 512 where there are more rows than CUs (two bf16 rows
+// on a CU take turns at its atomics and its arithmetic: 512 x 151936 57 us against 70; 8 rows 29
+// with 1024, 32 with 512).
 #include <math.h>
 #include <stddef.h>
 
@@ -26,9 +28,6 @@
 using namespace grpo;
 
 namespace {
-
-constexpr int TT = 1024;  // threads
-constexpr int SEGS = TT;  // segments of the row in which a tied token is looked for
 
 struct TokArgs {
   const void* logits;
@@ -81,46 +80,39 @@ __device__ __forceinline__ float value_of(typename Elem<DT>::type x) {
   if constexpr (DT == 2) return x;
 }
 
-// one(index, value) of the row's values before the first and after the last 16-byte boundary,
-// many(index of the first, 16 bytes) of what is between, U loads in flight per thread.
-template <int DT, int U, typename One, typename Many>
-__device__ __forceinline__ void for_groups(const typename Elem<DT>::type* row, int V, One&& one,
-                                           Many&& many) {
+// f(index, value as float) of every value of the row; 16-byte loads from the first boundary on.
+template <int DT, int TT, typename F>
+__device__ __forceinline__ void for_row(const typename Elem<DT>::type* row, int V, F&& f) {
   typedef typename Elem<DT>::type E;
-  constexpr int N = Elem<DT>::N;
+  constexpr int N = Elem<DT>::N, U = 4;
   const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(E));
   const int head = min(V, mis ? N - mis : 0), G = (V - head) / N, tid = threadIdx.x;
-  if (tid < head) one(tid, row[tid]);
+  if (tid < head) f(tid, value_of<DT>(row[tid]));
   const E* const body = row + head;
+#pragma unroll 1
   for (int g = tid; g < G; g += U * TT) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       v[u] = *reinterpret_cast<const uint4*>(body + (int64_t)N * min(g + u * TT, G - 1));
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (g + u * TT < G) many(head + N * (g + u * TT), v[u]);
+    for (int u = 0; u < U; ++u) {
+      if (g + u * TT >= G) continue;
+      const int at = head + N * (g + u * TT);
+      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (DT == 2) {
+          f(at + e, __uint_as_float(w[e]));
+        } else {
+          f(at + 2 * e, value_of<DT>((uint16_t)w[e]));
+          f(at + 2 * e + 1, value_of<DT>((uint16_t)(w[e] >> 16)));
+        }
+      }
+    }
   }
   const int tail = head + N * G + tid;
-  if (tail < V) one(tail, row[tail]);
-}
-// f(index, value as float) of every value.
-template <int DT, typename F>
-__device__ __forceinline__ void for_row(const typename Elem<DT>::type* row, int V, F&& f) {
-  for_groups<DT, 4>(
-      row, V, [&](int i, typename Elem<DT>::type x) { f(i, value_of<DT>(x)); },
-      [&](int i, const uint4& v) {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (DT == 2) {
-            f(i + e, __uint_as_float(w[e]));
-          } else {
-            f(i + 2 * e, value_of<DT>((uint16_t)w[e]));
-            f(i + 2 * e + 1, value_of<DT>((uint16_t)(w[e] >> 16)));
-          }
-        }
-      });
+  if (tail < V) f(tail, value_of<DT>(row[tail]));
 }
 
 // 2^-y as a double, y >= 0, times 2^up: Taylor polynomial of 2^f on [-1/2, 1/2], below 1e-14.
@@ -140,9 +132,14 @@ __device__ __forceinline__ double exp2_neg(double y, int up) {
   p = fma(p, f, 1.0);
   return ldexp(p, up - (int)n);
 }
-// A weight in units of 2^-shift; nothing more than shift + 1 doublings below the maximum.
+// A double in [0, 2^52) as the nearest integer: its last place is 1 after 2^52 is added.
+__device__ __forceinline__ uint64_t nearest(double x) {
+  return (uint64_t)__double_as_longlong(x + 4503599627370496.0) & ((1ull << 52) - 1);
+}
+// A weight in units of 2^-shift (at most 2^-44); nothing more than shift + 1 doublings below the
+// maximum.
 __device__ __forceinline__ uint64_t mass_of(double y, int shift) {
-  return y < (double)(shift + 1) ? (uint64_t)rint(exp2_neg(y, shift)) : 0;
+  return y < (double)(shift + 1) ? nearest(exp2_neg(y, shift)) : 0;
 }
 
 // Distance from the maximum in doublings: 0 at the maximum itself (an infinite one included),
@@ -180,6 +177,15 @@ __device__ __forceinline__ uint64_t share_of(double p, uint64_t mass) {
   const uint64_t f = (uint64_t)(p * 18446744073709551616.0);
   return max((uint64_t)1, (uint64_t)__umul64hi(f, mass) + (f * mass ? 1 : 0));
 }
+// How many weights w > 0 reach P > 0, at most `most` of them.
+__device__ __forceinline__ uint32_t weights_for(uint64_t P, uint64_t w, uint32_t most) {
+  double q = (double)P / (double)w;
+  if (!(q < (double)most)) return most;
+  uint32_t n = (uint32_t)q;  // the quotient or a neighbour of it
+  while (n && n * w >= P) --n;
+  while (n * w < P) ++n;
+  return min(n, most);
+}
 
 // Where a search ends: the value, the tokens before it in sorted order, how many of those that
 // hold it are needed (1 or more), the mass up to the last of them.
@@ -197,11 +203,14 @@ __device__ __forceinline__ Leaf draw_of(const Row& r, uint32_t valid, uint32_t n
   uint64_t mass = r.K < valid && r.p < 1.0 ? 0 : all;  // of what top_k leaves; then of what is kept
   kept = valid;
   Leaf l;
-  // (one place that calls it: the code is large, and once it is there it is there for all three)
+  // (one place that calls it: the code is large, and runs at the rate of its instruction
+  // fetches the first time)
 #pragma unroll 1
   for (int stage = mass ? 1 : 0; stage < 3; ++stage) {
-    const uint64_t P = stage == 0 ? 0 : stage == 2 ? __umul64hi(r.u, mass) + 1
-                                  : r.p < 1.0 ? share_of(r.p, mass) : 0;
+    const uint64_t P = stage == 0   ? 0
+                       : stage == 2 ? __umul64hi(r.u, mass) + 1
+                       : r.p < 1.0  ? share_of(r.p, mass)
+                                    : 0;
     if (stage == 1 && !P && K >= valid) continue;
     l = search(P, stage == 0 ? r.K : stage == 1 ? K : kept);
     mass = l.total;
@@ -218,84 +227,71 @@ struct Found {
   uint32_t bin, before, group;
 };
 struct Slots {
-  uint64_t s64[TT / 64];
-  uint32_t s32[TT / 64];
+  uint64_t s64[16];  // (the scans read a row of lanes of them)
+  uint32_t s32[16];
   Found found;
   Leaf leaf;
-  uint32_t n_list, best;
+  uint32_t n_list, best, range[2];
 };
 
 // First index of the value with key `key` (all threads get it).
-template <int DT>
+template <int DT, int TT>
 __device__ __forceinline__ uint32_t first_index(const typename Elem<DT>::type* row, int V,
                                                 uint32_t key, Slots& s) {
   if (threadIdx.x == 0) s.best = 0xFFFFFFFFu;
   __syncthreads();
+  const float x = key_value<DT>(key);  // (-0 is equal to it too)
   uint32_t best = 0xFFFFFFFFu;
-  for_row<DT>(row, V, [&](int i, float x) {
-    if (key_of<DT>(x) == key) best = min(best, (uint32_t)i);
-  });
+  for_row<DT, TT>(row, V, [&](int i, float v) { best = v == x ? min(best, (uint32_t)i) : best; });
   if (best != 0xFFFFFFFFu) atomicMin(&s.best, best);
   __syncthreads();
   return s.best;
 }
 
-// Segments of 2^seg_bits tokens, at most SEGS of them.
-__device__ __forceinline__ int seg_bits(int V) { return max(0, 32 - __clz(V - 1) - 10); }
-static_assert(SEGS == 1 << 10, "");
+template <int DT, int TT>
+__device__ __forceinline__ void maximum(const typename Elem<DT>::type* row, int V, uint32_t& kmax,
+                                        uint32_t& valid, Slots& s) {
+  float top = -INFINITY;
+  uint32_t n = 0;
+  for_row<DT, TT>(row, V, [&](int, float x) {
+    top = fmaxf(top, x);
+    n += x > -INFINITY ? 1u : 0u;
+  });
+  kmax = block_max<TT / 64>(key_of<DT>(top), s.s32);
+  valid = block_sum<TT / 64>(n, s.s32);
+}
 
-// The token of rank `rank` (from 0) by index among those of value `key`, whose numbers per
-// segment of 2^seg tokens stand in count: the segment, then the place in it.
-template <int DT>
-__device__ __forceinline__ void pick(const TokArgs& a, const typename Elem<DT>::type* row, int m,
-                                     uint32_t key, uint32_t rank, const uint32_t* count, int seg,
-                                     uint32_t kept, Slots& s) {
-  const int tid = threadIdx.x, V = a.V;
-  uint64_t unused = 0;
-  const uint32_t mine = count[tid];
-  uint32_t upto = mine;
-  block_excl_scan(unused, upto, s.s64, s.s32);
-  if (upto <= rank && rank < upto + mine) {
-    s.found.bin = tid;
-    s.found.before = upto;
+// Rows with nothing to draw, or whose maximum is taken; true if done.
+template <int DT, int TT>
+__device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kmax, const Row& r,
+                                           Slots& s) {
+  typedef typename Elem<DT>::type E;
+  if (kmax && !r.greedy) return false;
+  int64_t token = -1;
+  if (kmax)
+    token = first_index<DT, TT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, s);
+  if (threadIdx.x == 0) {
+    a.tokens[m] = token;
+    if (a.kept) a.kept[m] = kmax ? 1 : 0;
   }
-  __syncthreads();
-  if (tid >= 64) return;
-  const int i0 = (int)s.found.bin << seg, i1 = min(V, i0 + (1 << seg));
-  uint32_t left = rank - s.found.before;
-  for (int i = i0; i < i1; i += 64) {
-    const int at = i + tid;
-    const bool hit = at < i1 && key_of<DT>(value_of<DT>(row[min(at, V - 1)])) == key;
-    const uint64_t hits = __ballot(hit);
-    const uint32_t n = __popcll(hits);
-    if (left < n) {
-      if (hit && (uint32_t)__popcll(hits & ((1ull << tid) - 1)) == left) {
-        a.tokens[m] = at;
-        if (a.kept) a.kept[m] = (int32_t)kept;
-      }
-      return;
-    }
-    left -= n;
-  }
+  return true;
 }
 
 // ------------------------------------------------- bins of the distance --
 // 64 bins per doubling below the maximum. A token adds one 64-bit number to its bin: 1 to the
 // count in the upper bits, and (1 - 2^-(f / 64)) 2^UNIT to a sum in the lower ones, f its place in
-// the bin. A bin's mass is 2^-(bin / 64) (count - sum): one LDS atomic and 5 FMAs per token
-// instead of two and an exponential. Within a bin the tokens' weights are relative to the bin's
-// first, and P is a share of the bin's mass.
+// the bin. A bin's mass is 2^-(bin / 64) (count - sum): one LDS atomic and 4 FMAs per token
+// (2e-14 of its weight) instead of two and an exponential. Within a bin the tokens' weights are
+// relative to the bin's first, and P is a share of the bin's mass.
 constexpr int NB = 4096;
-constexpr int PER = NB / TT;   // bins of a thread
-constexpr int NK = TT;         // bins of keys
-constexpr int KEY_BITS = 10;
 constexpr int LIST = 4096;     // tokens of one bin that LDS holds
 constexpr double A64 = 0.010830424696249145;  // ln(2) / 64
 
+template <int TT>
 struct General {
   unsigned long long bins[NB];
-  unsigned long long kmass[NK];
-  uint32_t kcnt[NK];
+  unsigned long long kmass[TT];  // bins of keys, one per thread
+  uint32_t kcnt[TT];
   uint32_t lkey[LIST];
   uint32_t lidx[LIST];
   Slots s;
@@ -303,10 +299,11 @@ struct General {
 
 __device__ __forceinline__ double bin_place(double y) { return fmin(y * 64.0, (double)(NB - 1)); }
 
-// Smallest key in [1, kmax] whose bin is at most j: 64 candidates at a time.
+// Smallest key in [1, kmax] whose bin is at most j: 64 candidates at a time, by one wave.
 template <int DT>
 __device__ __forceinline__ uint32_t first_key(const Scale& sc, uint32_t kmax, int j) {
   uint32_t lo = 1, hi = kmax;  // hi holds
+#pragma unroll 1
   while (lo < hi) {
     const uint32_t step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
     const uint32_t c = (uint32_t)min((uint64_t)lo + (uint64_t)lane * step, (uint64_t)hi);
@@ -319,39 +316,43 @@ __device__ __forceinline__ uint32_t first_key(const Scale& sc, uint32_t kmax, in
   return hi;
 }
 
-template <int DT>
-__device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s, uint32_t kmax,
+template <int DT, int TT>
+__device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>& s, uint32_t kmax,
                                             uint32_t valid, const Row& r) {
   typedef typename Elem<DT>::type E;
-  const int tid = threadIdx.x, V = a.V;
+  constexpr int PER = NB / TT, KEY_BITS = TT == 1024 ? 10 : 9;
+  static_assert(TT == 1 << KEY_BITS, "a bin of keys per thread");
+  const int tid = threadIdx.x, V = a.V, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const E* const row = static_cast<const E*>(a.logits) + (int64_t)m * a.ld;
   const Scale sc{key_value<DT>(kmax), 1.4426950408889634 / r.T};
   const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
-  // units of a place's sum: the sum of V of them, below V A64, stays in the lower bits
-  const int cbits = a.V < 1 << 18 ? 18 : 21, unit = 70 - 2 * cbits;
-  const int sbits = 64 - cbits;
+  // The sum of V places, below V A64 2^unit, stays in the lower bits, their count in the upper.
+  const int cbits = a.V < 1 << 18 ? 18 : 21, unit = 70 - 2 * cbits, sbits = 64 - cbits;
   for (int j = tid; j < NB; j += TT) s.bins[j] = 0;
-  if (tid == 0) s.s.n_list = 0;
   __syncthreads();
   uint32_t near = 0;  // tokens that min_p leaves
   {
     const double sl = ldexp(1.0, unit), k1 = A64 * sl, k2 = -A64 * A64 / 2 * sl,
-                 k3 = A64 * A64 * A64 / 6 * sl, k4 = -A64 * A64 * A64 * A64 / 24 * sl,
-                 k5 = A64 * A64 * A64 * A64 * A64 / 120 * sl;
-    for_row<DT>(row, V, [&](int, float x) {
-      if (!(x > -INFINITY)) return;
-      const double y = sc.below(x);
-      near += y <= ymin ? 1u : 0u;
-      const double z = bin_place(y);
+                 k3 = A64 * A64 * A64 / 6 * sl, k4 = -A64 * A64 * A64 * A64 / 24 * sl;
+    auto add = [&](double z) {
+      near += z <= ymin * 64.0 ? 1u : 0u;
+      z = fmin(z, (double)(NB - 1));
       const int b = (int)z;
       const double f = z - b;
-      // (the double's last place is 1 after 2^52 is added)
-      const double q = fma(fma(fma(fma(fma(k5, f, k4), f, k3), f, k2), f, k1), f, 4503599627370496.0);
-      const uint64_t lo = (uint64_t)__double_as_longlong(q) & ((1ull << 52) - 1);
-      atomicAdd(&s.bins[b], (unsigned long long)(lo + (1ull << sbits)));
-    });
+      const uint64_t place = nearest(f * fma(fma(fma(k4, f, k3), f, k2), f, k1));
+      atomicAdd(&s.bins[b], (unsigned long long)(place + (1ull << sbits)));
+    };
+    if (valid == (uint32_t)V && sc.top < INFINITY) {
+      const double c = sc.c * 64.0;
+      for_row<DT, TT>(row, V, [&](int, float x) { add((sc.top - (double)x) * c); });
+    } else {
+      for_row<DT, TT>(row, V, [&](int, float x) {
+        if (x > -INFINITY) add(sc.below(x) * 64.0);
+      });
+    }
   }
-  near = block_sum<TT / 64>(near, s.s.s32);
+  if (r.mp > 0.0) near = block_sum<TT / 64>(near, s.s.s32);
+  __syncthreads();
   // this thread's bins: masses, counts, and what stands before them
   uint64_t bm[PER], pm = 0;
   uint32_t bc[PER], pc = 0;
@@ -386,18 +387,21 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
     __syncthreads();
     const Found top = s.s.found;
     const int bin = last = top.bin;
-    uint32_t lo = first_key<DT>(sc, kmax, bin);
-    uint32_t hi = bin ? first_key<DT>(sc, kmax, bin - 1) - 1 : kmax;
+    if (wave < 2) {  // the bin's keys: below the first one of the bin before
+      const uint32_t k = bin >= wave ? first_key<DT>(sc, kmax, bin - wave) : kmax + 1;
+      if ((tid & 63) == 0) s.s.range[wave] = k - wave;
+    }
+    if (tid == 0 && listed != bin) s.s.n_list = 0;
+    __syncthreads();
+    uint32_t lo = s.s.range[0], hi = s.s.range[1];
     const bool list = top.group <= LIST;
     if (list && listed != bin) {
-      if (tid == 0) s.s.n_list = 0;
-      __syncthreads();
-      for_row<DT>(row, V, [&](int i, float x) {
-        const uint32_t k = key_of<DT>(x);
-        if (k < lo || k > hi) return;
+      const float xlo = key_value<DT>(lo), xhi = key_value<DT>(hi);
+      for_row<DT, TT>(row, V, [&](int i, float x) {
+        if (!(x >= xlo && x <= xhi)) return;
         const uint32_t at = atomicAdd(&s.s.n_list, 1u);
         if (at >= LIST) return;  // (never: the bin holds as many)
-        s.lkey[at] = k;
+        s.lkey[at] = key_of<DT>(x);
         s.lidx[at] = i;
       });
       listed = bin;
@@ -406,17 +410,23 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
     const uint32_t n = min(s.s.n_list, (uint32_t)LIST);
     // weights relative to the bin's start: 2^44 of it at most
     auto rel = [&](uint32_t k) {
-      return (uint64_t)rint(exp2_neg(fmax(sc.below(key_value<DT>(k)) - bin * (1.0 / 64), 0.0), a.shift));
+      return nearest(
+          exp2_neg(fmin(fmax(sc.below(key_value<DT>(k)) - bin * (1.0 / 64), 0.0), 1000.0), a.shift));
+    };
+    // P among those, if it lies in this bin; a bin whose tokens have no mass of their own: all
+    auto share = [&](uint64_t sum) -> uint64_t {
+      if (!P || P > top.mass + top.own) return 0;
+      const double x = top.own ? (double)(P - top.mass) / (double)top.own * (double)sum : (double)sum;
+      return min(max((uint64_t)ceil(x), (uint64_t)1), max(sum, (uint64_t)1));
     };
     uint64_t Q = 0, mb = 0, sum = 0;  // P in those, before the range, of the whole bin
     uint32_t cb = top.before, group = top.group;
     bool first = true;
+#pragma unroll 1
     while (lo < hi) {
       const int sh = max(0, 32 - __clz(hi - lo) - KEY_BITS);
-      for (int j = tid; j < NK; j += TT) {
-        s.kmass[j] = 0;
-        s.kcnt[j] = 0;
-      }
+      s.kmass[tid] = 0;
+      s.kcnt[tid] = 0;
       __syncthreads();
       auto add = [&](uint32_t k) {
         if (k < lo || k > hi) return;
@@ -424,9 +434,10 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
         atomicAdd(&s.kcnt[(hi - k) >> sh], 1u);
       };
       if (list) {
+#pragma unroll 1
         for (uint32_t i = tid; i < n; i += TT) add(s.lkey[i]);
       } else {
-        for_row<DT>(row, V, [&](int, float x) { add(key_of<DT>(x)); });
+        for_row<DT, TT>(row, V, [&](int, float x) { add(key_of<DT>(x)); });
       }
       __syncthreads();
       const uint64_t mt = s.kmass[tid];
@@ -436,10 +447,7 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
       block_excl_scan(before, upto, s.s.s64, s.s.s32);
       if (first) {
         sum = block_sum<TT / 64>(mt, s.s.s64);
-        // (a bin whose tokens have no mass of their own: the last one)
-        Q = P ? (top.own ? (uint64_t)ceil((double)(P - top.mass) / (double)top.own * (double)sum)
-                         : sum) : 0;
-        Q = P > top.mass + top.own ? 0 : min(max(Q, (uint64_t)(P ? 1 : 0)), sum);
+        Q = share(sum);
         first = false;
       }
       before += mb;
@@ -459,109 +467,125 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General& s,
     const uint64_t w = rel(hi);
     if (first) {  // the bin is one value
       sum = w * group;
-      Q = P && P <= top.mass + top.own && top.own
-              ? max((uint64_t)1, (uint64_t)ceil((double)(P - top.mass) / (double)top.own * (double)sum))
-              : 0;
+      Q = share(sum);
     }
     Leaf l;
     l.key = hi;
     l.before = cb;
     l.in = min(group, K - cb);
-    if (Q) {
-      const uint64_t need = (Q - mb + w - 1) / w;  // (w >= 2^43 / 2^(1/64))
-      if (need < l.in) l.in = (uint32_t)need;
-    }
+    if (Q > mb && w) l.in = weights_for(Q - mb, w, l.in);
     l.in = max(l.in, 1u);
     const uint64_t end = mb + l.in * w;
     l.total = top.mass + (end >= sum ? top.own
                                      : (uint64_t)rint((double)end / (double)sum * (double)top.own));
-    if (l.total == 0) l.total = 1;
+    l.total = max(l.total, (uint64_t)1);
     return l;
   };
 
   uint32_t kept;
   const Leaf d = draw_of(r, valid, near, all, kept, search);
-  const int seg = seg_bits(V);
+  // The token of rank d.in - 1 by index among those of this value: the segment of 2^seg tokens
+  // that holds it, then the place in it.
+  const int seg = max(0, 32 - __clz(V - 1) - KEY_BITS);
   s.kcnt[tid] = 0;
   __syncthreads();
   if (listed == last) {
+#pragma unroll 1
     for (uint32_t i = tid; i < min(s.s.n_list, (uint32_t)LIST); i += TT)
       if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] >> seg], 1u);
   } else {
-    for_row<DT>(row, V, [&](int i, float x) {
-      if (key_of<DT>(x) == d.key) atomicAdd(&s.kcnt[i >> seg], 1u);
+    const float x = key_value<DT>(d.key);
+    for_row<DT, TT>(row, V, [&](int i, float v) {
+      if (v == x) atomicAdd(&s.kcnt[i >> seg], 1u);
     });
   }
   __syncthreads();
-  pick<DT>(a, row, m, d.key, d.in - 1, s.kcnt, seg, kept, s.s);
-}
-
-template <int DT>
-__device__ __forceinline__ void maximum(const typename Elem<DT>::type* row, int V, uint32_t& kmax,
-                                        uint32_t& valid, Slots& s) {
-  kmax = valid = 0;
-  for_row<DT>(row, V, [&](int, float x) {
-    const uint32_t k = key_of<DT>(x);
-    kmax = max(kmax, k);
-    valid += k ? 1u : 0u;
-  });
-  kmax = block_max<TT / 64>(kmax, s.s32);
-  valid = block_sum<TT / 64>(valid, s.s32);
-}
-
-// Rows with nothing to draw, or whose maximum is taken; true if done.
-template <int DT>
-__device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kmax, const Row& r,
-                                           Slots& s) {
-  typedef typename Elem<DT>::type E;
-  if (kmax && !r.greedy) return false;
-  int64_t token = -1;
-  if (kmax)
-    token = first_index<DT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, s);
-  if (threadIdx.x == 0) {
-    a.tokens[m] = token;
-    if (a.kept) a.kept[m] = kmax ? 1 : 0;
+  const uint32_t rank = d.in - 1, mine = s.kcnt[tid];
+  uint64_t unused = 0;
+  uint32_t upto = mine;
+  block_excl_scan(unused, upto, s.s.s64, s.s.s32);
+  if (upto <= rank && rank < upto + mine) {
+    s.s.found.bin = tid;
+    s.s.found.before = upto;
   }
-  return true;
+  __syncthreads();
+  if (tid >= 64) return;
+  const int i0 = (int)s.s.found.bin << seg, i1 = min(V, i0 + (1 << seg));
+  uint32_t left = rank - s.s.found.before;
+#pragma unroll 1
+  for (int i = i0; i < i1; i += 64) {
+    const int at = i + tid;
+    const bool hit = at < i1 && key_of<DT>(value_of<DT>(row[min(at, V - 1)])) == d.key;
+    const uint64_t hits = __ballot(hit);
+    const uint32_t c = __popcll(hits);
+    if (left < c) {
+      if (hit && (uint32_t)__popcll(hits & ((1ull << tid) - 1)) == left) {
+        a.tokens[m] = at;
+        if (a.kept) a.kept[m] = (int32_t)kept;
+      }
+      return;
+    }
+    left -= c;
+  }
+}
+
+template <int DT, int TT>
+__global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
+  typedef typename Elem<DT>::type E;
+  extern __shared__ __align__(16) char lds_raw[];
+  General<TT>& s = *reinterpret_cast<General<TT>*>(lds_raw);
+  const int m = blockIdx.x;
+  uint32_t kmax, valid;
+  maximum<DT, TT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, valid, s.s);
+  const Row r = row_of(a, m, valid);
+  if (simple_row<DT, TT>(a, m, kmax, r, s.s)) return;
+  general_row<DT, TT>(a, m, s, kmax, valid, r);
 }
 
 // ------------------------------------------------------- bf16: its values --
 // A bf16 row has few distinct values: their counts, one 32-bit LDS atomic per token, and a
-// weight per value. The bins are fixed, the values of magnitude below 512 in descending order,
-// so that one pass over the row makes the counts and finds the maximum. A row with a larger
-// maximum, or with mass at -512 and below (an extreme temperature), takes the bins of the distance.
-// (The row in registers instead of its second reading: 8 / 512 rows of 151936 39 / 155 us against
-// 35 / 100, in code without loops that runs at the rate of its instruction fetches.)
-constexpr int CW = 64;              // bins of a group: one per lane
-constexpr int CG = 544;             // groups: one per thread
-constexpr int CB = CW * CG;
-constexpr int CI = CG / (TT / 64);  // groups of a wave
-constexpr int TOP = CB / 2;         // the bin of t is TOP - 1 - t
-static_assert(CG % (TT / 64) == 0 && CG <= TT, "groups split evenly");
-static_assert(TOP == 0x4400, "the bits of 512");
-constexpr int SEG_PER = 3;          // segments of a thread in the search for a token
-typedef int16_t s16x2 __attribute__((ext_vector_type(2)));
+// weight per value. The bins are fixed, the values of magnitude 2^-30 to 512 (without) in
+// descending order with one bin for 0 and what is smaller among them, so that one pass over the
+// row makes the counts, which tell the maximum too. A row with smaller values than 2^-30 other
+// than 0, with a larger maximum, or with mass at -512 and below (an extreme temperature) takes
+// the bins of the distance. The second pass over the row looks for the token and ends where it is
+// found.
+// Bound on its CU by the atomics (8 of 29 us at 151936 tokens) and by the issue of what is done
+// per token (1 us per instruction). (The row in registers instead of its second reading: 8 / 512
+// rows 39 / 155 us, in code without loops that runs at the rate of its instruction fetches.)
+constexpr int LEAST = 0x3080, LARGE = 0x4400;  // the bits of 2^-30 and 512
+constexpr int ZERO = LARGE - LEAST + 1;        // bin of 0; 0 and 2 ZERO: from +-512 on
+constexpr int CW = 64;                         // bins of a group: one per lane
+constexpr int CG = (2 * ZERO + 1 + CW - 1) / CW;
+constexpr int U16 = 5;                         // 16-byte groups in flight per thread
+constexpr int SEGS = GRPO_SAMPLE_MAX_VOCAB / (8 * 64 * U16) + 17 + 2;
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct Counts {
-  uint32_t n[CB + 32];  // n[CB]: of what has no bin
-  uint64_t mass[CG];    // of the groups
-  uint32_t count[CG];   // (all of these are zero at first)
+  uint32_t n[CG * CW];
+  uint64_t mass[CG + 1];  // of the groups
+  uint32_t count[CG + 3]; // (all of these are zero at first)
   Slots s;
 };
+static_assert(offsetof(Counts, s) % 16 == 0, "cleared 16 bytes at a time");
+static_assert(CG <= 512 && SEGS <= 512, "a group, a segment per thread");
 
-// The value's bits as a 16-bit integer in the order of the values: +0 -> 0, -0 -> -1; +inf,
-// and what is a NaN above it; -inf, and what is a NaN below it.
-constexpr int T_INF = 0x7F80, T_NINF = 0x7F - 0x8000;
-__device__ __forceinline__ s16x2 order_of(uint32_t pair) {
-  const s16x2 x = __builtin_bit_cast(s16x2, pair);
-  return x ^ ((x >> 15) & (int16_t)0x7FFF);
+__device__ __forceinline__ u16x2 bin_of(uint32_t pair) {
+  const u16x2 x = __builtin_bit_cast(u16x2, pair);
+  const u16x2 size = __builtin_elementwise_min(
+      __builtin_elementwise_sub_sat((u16x2)(x & (uint16_t)0x7FFF), (u16x2)(uint16_t)(LEAST - 1)),
+      (u16x2)(uint16_t)ZERO);
+  const u16x2 sign = (x >> 15) * (uint16_t)2 - (uint16_t)1;  // -1 for what is positive
+  return size * sign + (uint16_t)ZERO;
 }
-__device__ __forceinline__ float ordered_value(int t) {
-  return bf2f((uint16_t)(t < 0 ? t ^ 0x7FFF : t));
+__device__ __forceinline__ uint32_t bin_bits(int bin) {
+  const int size = bin < ZERO ? ZERO - bin : bin - ZERO;
+  return size ? (uint32_t)(size + LEAST - 1) | (bin > ZERO ? 0x8000u : 0u) : 0u;
 }
 
-// Where the row's 16-byte groups begin, and how many they are.
+// Where the row's 16-byte groups begin, and how many they are. A wave takes 64 U16 neighbouring
+// groups at a time (a segment), 64 of them by each load.
+template <int TT>
 struct Groups {
   const uint16_t* row;
   int V, head, G;
@@ -572,118 +596,177 @@ struct Groups {
     G = (V - head) / 8;
   }
   __device__ __forceinline__ uint4 at(int g) const {
-    return *reinterpret_cast<const uint4*>(row + head + 8 * (int64_t)g);
+    return *reinterpret_cast<const uint4*>(row + head + 8 * (int64_t)min(g, G - 1));
   }
-  // one(0 or 1, index, value) of the values before and after the groups, many(g, group)
-  template <typename One, typename Many>
-  __device__ __forceinline__ void each(One&& one, Many&& many) const {
-    constexpr int U = 8;
+  // one(0 or 1, value) of the values before and after the groups, many(group), done(segment) of
+  // all threads after each of its wave's segments; true ends it.
+  template <typename One, typename Many, typename Done>
+  __device__ __forceinline__ void each(One&& one, Many&& many, Done&& done) const {
     const int tid = threadIdx.x, tail = head + 8 * G + tid;
-    if (tid < head) one(0, tid, row[tid]);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < head) one(0, row[tid]);
+    if (tail < V) one(1, row[tail]);
 #pragma unroll 1
-    for (int g = tid; g < G; g += U * TT) {
-      uint4 w[U];
+    for (int s = wave; s - wave < (G + 64 * U16 - 1) / (64 * U16); s += TT / 64) {
+      const int g = 64 * U16 * s + (tid & 63);
+      uint4 w[U16];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = at(min(g + u * TT, G - 1));
+      for (int u = 0; u < U16; ++u) w[u] = at(g + 64 * u);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (g + u * TT < G) many(g + u * TT, w[u]);
+      for (int u = 0; u < U16; ++u)
+        if (g + 64 * u < G) many(w[u]);
+      if (done(s)) break;
     }
-    if (tail < V) one(1, tail, row[tail]);
   }
 };
+struct Never {
+  __device__ __forceinline__ bool operator()(int) const { return false; }
+};
 
-// The token of rank `rank` among those whose bits are want (two of them, compared in mask),
-// counted per wave's groups; all threads get it.
-__device__ __forceinline__ void pick_bits(const TokArgs& a, const Groups& x, int m, uint32_t want,
-                                          uint32_t mask, uint32_t rank, uint32_t kept, Counts& s) {
+// The token of rank `rank` among those whose bits are want (two of them, compared in mask).
+template <int TT>
+__device__ __forceinline__ void pick_bits(const TokArgs& a, const Groups<TT>& x, int m,
+                                          uint32_t want, uint32_t mask, uint32_t rank,
+                                          uint32_t kept, Counts& s) {
   const int tid = threadIdx.x, lane = tid & 63;
-  const int segs = 2 + (x.G + 63) / 64;  // before the groups, 64 groups each, after them
-  for (int j = tid; j < SEG_PER * TT; j += TT) s.n[j] = 0;
+  // segments: before the groups, the waves' (an unfinished round's too), after them
+  const int segs = 2 + (x.G + 64 * U16 - 1) / (64 * U16) + TT / 64;
+  if (tid < SEGS) s.n[tid] = 0;
+  if (tid == 0) s.s.n_list = 0;
   __syncthreads();
-  auto matches = [&](const uint4& w) {
+  auto differ = [&](const uint4& w) {  // in the halves of the sum: how many of the values do
     const uint32_t p[4] = {w.x, w.y, w.z, w.w};
-    const u16x2 one = (uint16_t)1;
-    u16x2 not_it = (uint16_t)0;
+    u16x2 n = (uint16_t)0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      not_it += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (p[i] ^ want) & mask), one);
-    return 8u - not_it[0] - not_it[1];
+      n += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (p[i] ^ want) & mask),
+                                     (u16x2)(uint16_t)1);
+    return n;
   };
   auto is = [&](uint16_t v) { return ((v ^ want) & mask & 0xFFFFu) == 0; };
+  u16x2 not_it = (uint16_t)0;
+  uint32_t looked = 0;
   x.each(
-      [&](int end, int, uint16_t v) {
-        if (is(v)) atomicAdd(&s.n[end ? segs - 1 : 0], 1u);
+      [&](int end, uint16_t v) {
+        if (!is(v)) return;
+        atomicAdd(&s.n[end ? segs - 1 : 0], 1u);
+        if (!end) atomicAdd(&s.s.n_list, 1u);
       },
-      [&](int g, const uint4& w) {
-        const uint32_t c = matches(w);
-        if (c) atomicAdd(&s.n[1 + g / 64], c);
+      [&](const uint4& w) {
+        not_it += differ(w);
+        looked += 8;
+      },
+      [&](int seg) {  // is the token among those looked at so far?
+        const uint32_t c = wave_prefix(looked - not_it[0] - not_it[1], Add());
+        if (lane == 63 && c) {
+          s.n[1 + seg] = c;
+          atomicAdd(&s.s.n_list, c);
+        }
+        not_it = (uint16_t)0;
+        looked = 0;
+        __syncthreads();
+        const bool is_there = s.s.n_list > rank;
+        __syncthreads();  // (read by all before more is added)
+        return is_there;
       });
   __syncthreads();
-  uint32_t c[SEG_PER], mine = 0, upto;
-#pragma unroll
-  for (int j = 0; j < SEG_PER; ++j) mine += c[j] = s.n[SEG_PER * tid + j];
-  upto = mine;
+  const uint32_t mine = tid < segs ? s.n[tid] : 0;
+  uint32_t upto = mine;
   uint64_t unused = 0;
   block_excl_scan(unused, upto, s.s.s64, s.s.s32);
   if (upto <= rank && rank < upto + mine) {
-#pragma unroll
-    for (int j = 0; j < SEG_PER; ++j) {
-      if (upto <= rank && rank < upto + c[j]) s.s.found = Found{0, 0, (uint32_t)(SEG_PER * tid + j), upto, 0};
-      upto += c[j];
-    }
+    s.s.found.bin = tid;
+    s.s.found.before = upto;
   }
   __syncthreads();
   if (tid >= 64) return;
   const int seg = (int)s.s.found.bin;
-  const uint32_t left = rank - s.s.found.before;
-  // a lane's values: a group's eight, or one of an end
-  const int g = 64 * (seg - 1) + lane;
-  const bool ends = seg == 0 || seg == segs - 1;
-  const int first = ends ? (seg ? x.head + 8 * x.G : 0) + lane : x.head + 8 * g;
-  const int count = ends ? (first < (seg ? x.V : x.head) ? 1 : 0) : (g < x.G ? 8 : 0);
-  uint32_t bits = 0;
-  for (int i = 0; i < count; ++i) bits |= (uint32_t)is(x.row[first + i]) << i;
-  const uint32_t before = wave_prefix((uint32_t)__popc(bits), Add()) - __popc(bits);
-  if (before <= left && left < before + __popc(bits)) {
-    for (uint32_t k = left - before; k; --k) bits &= bits - 1;
-    a.tokens[m] = first + __builtin_ctz(bits);
-    if (a.kept) a.kept[m] = (int32_t)kept;
+  uint32_t left = rank - s.s.found.before;
+  auto finish = [&](int first, uint32_t bits) {  // a lane's values, from index first on
+    const uint32_t c = __popc(bits), end = wave_prefix(c, Add());
+    if (end - c <= left && left < end) {
+      for (uint32_t k = left - (end - c); k; --k) bits &= bits - 1;
+      a.tokens[m] = first + __builtin_ctz(bits);
+      if (a.kept) a.kept[m] = (int32_t)kept;
+    }
+    return lane_value(end, 63);
+  };
+  if (seg == 0 || seg == segs - 1) {
+    const int first = (seg ? x.head + 8 * x.G : 0) + lane;
+    finish(first, first < (seg ? x.V : x.head) && is(x.row[min(first, x.V - 1)]));
+    return;
+  }
+  const int g = 64 * U16 * (seg - 1) + lane;
+  uint4 w[U16];
+#pragma unroll
+  for (int u = 0; u < U16; ++u) w[u] = x.at(g + 64 * u);
+#pragma unroll 1
+  for (int u = 0; u < U16; ++u) {
+    uint32_t bits = 0;
+    const uint32_t p[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      bits |= (uint32_t)is((uint16_t)p[i]) << (2 * i) | (uint32_t)is((uint16_t)(p[i] >> 16)) << (2 * i + 1);
+    const uint32_t n = finish(x.head + 8 * (g + 64 * u), g + 64 * u < x.G ? bits : 0u);
+    if (left < n) return;
+    left -= n;
+#pragma unroll
+    for (int i = 0; i + 1 < U16; ++i) w[i] = w[i + 1];
   }
 }
 
-// False if the row needs the bins of the distance.
-__device__ __forceinline__ bool count_row(const TokArgs& a, int m, const Groups& x, Counts& s,
-                                          uint32_t kmax, uint32_t valid, const Row& r) {
+// False if the row needs the bins of the distance. some: this wave's groups wave + i TT / 64 that
+// are not empty.
+template <int TT>
+__device__ __forceinline__ bool count_row(const TokArgs& a, int m, const Groups<TT>& x, Counts& s,
+                                          uint32_t kmax, uint32_t valid, const Row& r,
+                                          uint32_t some) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Scale sc{key_value<0>(kmax), 1.4426950408889634 / r.T};
   const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
   if (!(fabs(sc.top) < 512.0)) return false;
-  if (s.n[CB]) {
+  if (s.n[2 * ZERO]) {
     const double y = sc.below(-512.f);
     if (y < a.shift + 2 || (r.mp > 0.0 && y <= ymin)) return false;
   }
-  auto distance = [&](int bin) { return sc.below(ordered_value(TOP - 1 - bin)); };
-  // The groups' masses and counts, a wave per group and a bin per lane: most groups are empty,
-  // and the others stand side by side.
+  // (what is in the bins of +-512 and beyond is not looked for: NaN and no mass)
+  auto weight = [&](int bin, double& y) {
+    y = sc.below(bf2f((uint16_t)bin_bits(bin)));
+    return bin > 0 && bin < 2 * ZERO ? mass_of(y, a.shift) : 0;
+  };
+  auto number = [&](int bin) { return bin > 0 && bin < 2 * ZERO ? s.n[bin] : 0; };
+  // The groups' masses and counts, a wave per group and a bin per lane, two groups at a time:
+  // many are empty.
   uint32_t near = 0;
-  {
-    uint64_t some = 0;  // of this wave's groups
-#pragma unroll
-    for (int i = 0; i < CI; ++i)
-      some |= (uint64_t)(__ballot(s.n[CW * (wave + i * (TT / 64)) + lane] != 0) != 0) << i;
 #pragma unroll 1
-    for (; some; some &= some - 1) {
-      const int g = wave + __builtin_ctzll(some) * (TT / 64);
-      const uint32_t c = s.n[CW * g + lane];
-      const double y = distance(CW * g + lane);
-      const uint64_t mass = wave_prefix(c * mass_of(y, a.shift), Add());
-      const uint32_t count = wave_prefix(c, Add());
-      near += y <= ymin ? c : 0u;
-      if (lane == 63) {
-        s.mass[g] = mass;
-        s.count[g] = count;
+  while (some) {
+    int g[2];
+    uint32_t c[2];
+    uint64_t mass[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      g[i] = wave + (some ? __builtin_ctz(some) : 31) * (TT / 64);
+      c[i] = some ? number(CW * g[i] + lane) : 0;
+      some &= some - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      double y;
+      mass[i] = c[i] * weight(CW * g[i] + lane, y);
+      near += y <= ymin ? c[i] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mass[i] = wave_prefix(mass[i], Add());
+      c[i] = wave_prefix(c[i], Add());
+    }
+    if (lane == 63) {
+      s.mass[g[0]] = mass[0];
+      s.count[g[0]] = c[0];
+      if (c[1]) {
+        s.mass[g[1]] = mass[1];
+        s.count[g[1]] = c[1];
       }
     }
   }
@@ -698,106 +781,107 @@ __device__ __forceinline__ bool count_row(const TokArgs& a, int m, const Groups&
   __syncthreads();
   const uint64_t all = s.s.found.own;
   const uint32_t counted = s.s.found.before;
-  __syncthreads();
 
-  int found = 0;  // bin of the last search
   auto search = [&](uint64_t P, uint32_t K) {
     if (!P && K > counted) return Leaf{0u, K - 1, 1u, all};  // among those without mass
-    if (!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K))
-      s.s.found = Found{pm, 0, (uint32_t)tid, pc, 0};
+    const uint64_t here = __ballot(!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K));
+    if (here) {  // this wave has the group: its bins, one per lane
+      const int from = __builtin_ctzll(here);
+      const int bin = (64 * wave + from) * CW + lane;
+      double y;
+      const uint32_t c = number(bin);
+      const uint64_t w = weight(bin, y), own = c * w;
+      const uint64_t end = wave_prefix(own, Add()) + lane_value(pm, from);
+      const uint32_t upto = wave_prefix(c, Add()) + lane_value(pc, from);
+      const uint64_t hits = __ballot(reached(end, upto, P, K));
+      if (lane == (hits ? __builtin_ctzll(hits) : 63)) {
+        Leaf l;
+        l.key = (uint32_t)bin;
+        l.before = upto - c;
+        l.in = min(c, K - l.before);
+        if (P && w) l.in = weights_for(P - (end - own), w, l.in);
+        l.total = end - own + l.in * w;
+        s.s.leaf = l;
+      }
+    }
     __syncthreads();
-    const Found f = s.s.found;
-    const int bin = (int)f.bin * CW + lane;
-    const uint32_t c = s.n[bin];
-    const uint64_t w = mass_of(distance(bin), a.shift), own = c * w;
-    const uint64_t end = wave_prefix(own, Add()) + f.mass;
-    const uint32_t upto = wave_prefix(c, Add()) + f.before;
-    const uint64_t hits = __ballot(reached(end, upto, P, K));
-    const int at = hits ? __builtin_ctzll(hits) : 63;
-    found = (int)f.bin * CW + at;
-    const uint64_t own_at = lane_value(own, at), w_at = lane_value(w, at);
-    const uint64_t before = lane_value(end, at) - own_at;
-    const uint32_t c_at = lane_value(c, at);
-    Leaf l;
-    l.before = lane_value(upto, at) - c_at;
-    l.in = min(c_at, K - l.before);
-    if (P && w_at) l.in = (uint32_t)min((uint64_t)l.in, (P - before + w_at - 1) / w_at);
-    l.key = 0;
-    l.total = before + l.in * w_at;
-    __syncthreads();  // found has been read
+    const Leaf l = s.s.leaf;
+    __syncthreads();
     return l;
   };
   uint32_t kept;
   const Leaf d = draw_of(r, valid, near, all, kept, search);
-  const int t = TOP - 1 - found;  // (-0 stands with +0)
-  const uint32_t bits = (uint32_t)(t < 0 ? t ^ 0x7FFF : t) & 0xFFFFu;
-  pick_bits(a, x, m, bits | bits << 16, bits ? 0xFFFFFFFFu : 0x7FFF7FFFu, d.in - 1, kept, s);
+  const uint32_t bits = bin_bits((int)d.key);
+  pick_bits<TT>(a, x, m, bits | bits << 16, bits ? 0xFFFFFFFFu : 0x7FFF7FFFu, d.in - 1, kept, s);
   return true;
 }
 
-__global__ void __launch_bounds__(TT) sample_tokens_bf16_kernel(TokArgs a) {
+template <int TT>
+__global__ void __launch_bounds__(TT, 4) sample_tokens_bf16_kernel(TokArgs a) {
+  constexpr int CI = (CG + TT / 64 - 1) / (TT / 64);  // groups of a wave
+  static_assert(CI < 31, "a bit each");
   extern __shared__ __align__(16) char lds_raw[];
   Counts& s = *reinterpret_cast<Counts*>(lds_raw);
-  const int m = blockIdx.x;
-  const Groups x(a, m);
-  static_assert(offsetof(Counts, s) % 16 == 0, "cleared 16 bytes at a time");
-  for (int j = threadIdx.x; j < (int)offsetof(Counts, s) / 16; j += TT)
+  const int m = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Groups<TT> x(a, m);
+  for (int j = tid; j < (int)offsetof(Counts, s) / 16; j += TT)
     reinterpret_cast<uint4*>(s.n)[j] = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  s16x2 hi = (int16_t)-0x8000, lo = (int16_t)0x7FFF;
-  const u16x2 top = (uint16_t)(TOP - 1), none = (uint16_t)CB;
-  auto pair = [&](uint32_t w) {
-    const s16x2 t = order_of(w);
-    hi = __builtin_elementwise_max(hi, t);
-    lo = __builtin_elementwise_min(lo, t);
-    return __builtin_elementwise_min(top - __builtin_bit_cast(u16x2, t), none);
-  };
-  x.each([&](int, int, uint16_t v) { atomicAdd(&s.n[pair(v * 0x10001u)[0]], 1u); },
-         [&](int, const uint4& v) {
+  x.each([&](int, uint16_t v) { atomicAdd(&s.n[bin_of(v)[0]], 1u); },
+         [&](const uint4& v) {
            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
            for (int i = 0; i < 4; ++i) {
-             const u16x2 d = pair(w[i]);
+             const u16x2 d = bin_of(w[i]);
              atomicAdd(&s.n[d[0]], 1u);
              atomicAdd(&s.n[d[1]], 1u);
            }
-         });
-  const int most = max((int)hi[0], (int)hi[1]), least = min((int)lo[0], (int)lo[1]);
-  const int tmax = (int)block_max<TT / 64>((uint32_t)(most + 0x8000), s.s.s32) - 0x8000;
-  const int tmin = 0x8000 - (int)block_max<TT / 64>((uint32_t)(0x8000 - least), s.s.s32);
-  uint32_t kmax = key_of<0>(ordered_value(tmax)), valid = (uint32_t)a.V;
-  if (tmax > T_INF || tmin <= T_NINF)  // NaN or -inf among them
-    maximum<0>(x.row, a.V, kmax, valid, s.s);
-  if (threadIdx.x == 0) {  // -0 with +0
-    s.n[TOP - 1] += s.n[TOP];
-    s.n[TOP] = 0;
+         },
+         Never());
+  __syncthreads();
+  // This wave's groups that are not empty, and the row's first bin that is not.
+  uint32_t some = 0, first = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = CI - 1; i >= 0; --i) {
+    const int g = wave + i * (TT / 64);
+    const uint64_t is = __ballot(g < CG && s.n[min(CW * g, CW * (CG - 1)) + lane] != 0);
+    some |= (uint32_t)(is != 0) << i;
+    if (is) first = CW * g + __builtin_ctzll(is);
   }
-  __syncthreads();
+  first = ~block_max<TT / 64>(~first, s.s.s32);
+  uint32_t kmax = key_of<0>(bf2f((uint16_t)bin_bits((int)first))), valid = (uint32_t)a.V;
+  bool tiny = false;
+  if (s.n[ZERO]) {  // is it 0?
+    uint32_t bad = 0;
+    auto look = [&](uint32_t w) {
+      bad |= ((w & 0x7FFFu) - 1u < LEAST - 1u) | ((w >> 16 & 0x7FFFu) - 1u < LEAST - 1u);
+    };
+    x.each([&](int, uint16_t v) { look(v * 0x10001u); },
+           [&](const uint4& v) { look(v.x), look(v.y), look(v.z), look(v.w); }, Never());
+    tiny = block_max<TT / 64>(bad, s.s.s32) != 0;
+  }
+  if (tiny || s.n[0] || s.n[2 * ZERO]) maximum<0, TT>(x.row, a.V, kmax, valid, s.s);
   const Row r = row_of(a, m, valid);
-  if (simple_row<0>(a, m, kmax, r, s.s)) return;
-  if (count_row(a, m, x, s, kmax, valid, r)) return;
+  if (simple_row<0, TT>(a, m, kmax, r, s.s)) return;
+  if (!tiny && count_row<TT>(a, m, x, s, kmax, valid, r, some)) return;
   __syncthreads();
-  general_row<0>(a, m, *reinterpret_cast<General*>(lds_raw), kmax, valid, r);
+  general_row<0, TT>(a, m, *reinterpret_cast<General<TT>*>(lds_raw), kmax, valid, r);
 }
 
-template <int DT>
-__global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
-  typedef typename Elem<DT>::type E;
-  extern __shared__ __align__(16) char lds_raw[];
-  General& s = *reinterpret_cast<General*>(lds_raw);
-  const int m = blockIdx.x;
-  uint32_t kmax, valid;
-  maximum<DT>(static_cast<const E*>(a.logits) + (int64_t)m * a.ld, a.V, kmax, valid, s.s);
-  const Row r = row_of(a, m, valid);
-  if (simple_row<DT>(a, m, kmax, r, s.s)) return;
-  general_row<DT>(a, m, s, kmax, valid, r);
-}
-
-template <auto KERN, int LDS>
+template <auto KERN, int TT, int LDS>
 int go(const TokArgs& a, hipStream_t st) {
   if (int rc = allow_dynamic_lds<KERN, LDS>()) return rc;
   KERN<<<a.M, TT, LDS, st>>>(a);
   return launch_check("sample_tokens");
+}
+template <int TT>
+int go_type(const TokArgs& a, int dtype, hipStream_t st) {
+  constexpr int LDS = (int)sizeof(General<TT>);
+  if (dtype == 0)
+    return go<sample_tokens_bf16_kernel<TT>, TT, std::max((int)sizeof(Counts), LDS)>(a, st);
+  return dtype == 1 ? go<sample_tokens_kernel<1, TT>, TT, LDS>(a, st)
+                    : go<sample_tokens_kernel<2, TT>, TT, LDS>(a, st);
 }
 
 }  // namespace
@@ -819,9 +903,5 @@ extern "C" int grpo_sample_tokens(const void* logits, int dtype, int64_t ld, int
                   sampler->temperature, sampler->top_p, sampler->min_p, sampler->top_k,
                   min(44, 62 - bits), tokens, kept};
   hipStream_t st = as_stream(stream);
-  constexpr int LDS = (int)sizeof(General);
-  constexpr int LDS16 = (int)std::max(sizeof(Counts), sizeof(General));
-  if (dtype == 0) return go<sample_tokens_bf16_kernel, LDS16>(a, st);
-  return dtype == 1 ? go<sample_tokens_kernel<1>, LDS>(a, st)
-                    : go<sample_tokens_kernel<2>, LDS>(a, st);
+  return M > 256 ? go_type<512>(a, dtype, st) : go_type<1024>(a, dtype, st);
 }

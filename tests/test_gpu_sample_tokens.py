@@ -175,3 +175,28 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             sample_tokens(x, u, **kw)
     assert sample_tokens(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_values_of_every_size(dev, dtype):
+    """Logits from the smallest to the largest of the type, zeros, and few of a size: the ways
+    in which a row is counted, and their borders."""
+    g = torch.Generator().manual_seed(21)
+    n, dt = 3001, DTYPES[dtype]
+    sign = torch.randint(0, 2, (n,), generator=g) * 2.0 - 1
+    spread = sign * torch.exp2(torch.rand(n, generator=g) * 250 - 126)
+    x = torch.stack([
+        spread.clamp(-torch.finfo(dt).max, torch.finfo(dt).max),  # most far from each other
+        (sign * 600 * torch.rand(n, generator=g)),  # around 512
+        torch.where(torch.rand(n, generator=g) < 0.5, 0.0, sign * torch.rand(n, generator=g)),
+        sign * torch.exp2(-29 - 2 * torch.rand(n, generator=g)),  # around 2^-30
+        sign * 2.0 ** -35,
+        -510 - 4 * torch.rand(n, generator=g),
+        510 + 4 * torch.rand(n, generator=g),
+        torch.full((n,), -512.0),
+        torch.full((n,), 2.0 ** -30),
+        -spread.abs().clamp(max=torch.finfo(dt).max)]).to(dt)
+    u = torch.rand(len(x), generator=g, dtype=torch.float64)
+    for kw in (dict(), dict(temperature=300.0, top_p=0.95), dict(top_k=1000), dict(min_p=0.3),
+               dict(temperature=1e5, top_k=2500, top_p=0.99), dict(temperature=0.01)):
+        check(dev, x, u, **kw)
