@@ -179,15 +179,17 @@ __device__ __forceinline__ uint4 turn(const uint32_t (&v)[8][VW], int t) {
                     perm(v[5][w], v[4][w], sel), perm(v[7][w], v[6][w], sel));
 }
 
-template <int D, int TW>
-constexpr int RING_OF = D * TW <= 128 ? 4 : (D * TW <= 256 ? 3 : 2);
+// Steps in LDS at a time, of 32 PT TW tokens.
+template <int D, int TW, int PT>
+constexpr int RING_OF = D * TW * PT <= 128 ? 4 : (D * TW * PT <= 256 ? 3 : 2);
 
-template <bool F16, int D, int RW, int TW>
+template <bool F16, int D, int RW, int TW, int PT>
 __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
-  constexpr int W = RW * TW, STEP = 32 * TW, RING = RING_OF<D, TW>;
-  constexpr int ROWB = 2 * D, NCH = D / 8;          // bytes and 16-byte chunks of a row
-  constexpr int HALF_B = 32 * ROWB, PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
-  constexpr int TPP = 1024 / ROWB, PPK = 32 / TPP;  // tokens of a 1-KiB piece, pieces of K
+  constexpr int W = RW * TW, PTOK = 32 * PT, STEP = PTOK * TW, RING = RING_OF<D, TW, PT>;
+  constexpr int ROWB = 2 * D, NCH = D / 8;            // bytes and 16-byte chunks of a row
+  constexpr int TILE_B = 32 * ROWB, HALF_B = PT * TILE_B;
+  constexpr int PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
+  constexpr int TPP = 1024 / ROWB, PPK = PTOK / TPP;  // tokens of a 1-KiB piece, pieces of K
   constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
   static_assert(PIECES % W == 0, "every wave loads as many pieces");
   constexpr int KS = D / 16, DT = D / 32, VW = DT / 2;  // steps of K, tiles of V, its words
@@ -226,14 +228,16 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
 
   const uint32_t lbase = lds_address(lds);
   auto fetch = [&](int s) __attribute__((always_inline)) {
+    int l = lane;
+    asm volatile("" : "+v"(l));
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const int pc = wave + W * i, pt = pc / (2 * PPK);
-      const int tok = (pc & (PPK - 1)) * TPP + lane / NCH;
-      const int r = max(rows[s * STEP + 32 * pt + tok], 0);  // a missing one reads row 0
+      const int tok = (pc & (PPK - 1)) * TPP + l / NCH;
+      const int r = max(rows[s * STEP + PTOK * pt + tok], 0);  // a missing one reads row 0
       const uint16_t* const base = (pc / PPK) & 1 ? a.vc : a.kc;
       dma16_at(lbase + (s % RING) * STEP_B + pc * 1024,
-               base + (int64_t)r * D + 8 * ((lane ^ tok) & (NCH - 1)));
+               base + (int64_t)r * D + 8 * ((l ^ tok) & (NCH - 1)));
     }
   };
 
@@ -243,9 +247,83 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
-  const int kx = 16 * ((lh ^ ln) & (NCH - 1)), ky = ln * ROWB;
-  const int vx = 16 * (((ln * 4 * VW / 16) ^ (4 * lh)) & (NCH - 1));
+  // Where a lane's operands stand in a tile of K, and in a tile of V less its token.
+  int kx = 16 * ((lh ^ ln) & (NCH - 1)), vx = 16 * ((ln * 4 * VW / 16 ^ 4 * lh) & (NCH - 1));
+  const int ky = ln * ROWB;
   const int vy = 4 * lh * ROWB + ln * 4 * VW % 16;
+  // S^T of 32 tokens (tile q of the part at kb).
+  auto scores = [&](const char* kb, int q) __attribute__((always_inline)) {
+    f32x16_t sc;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+      sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kb + ky + (kx ^ 32 * i) + q * TILE_B),
+                       qf[i], sc);
+    return sc;
+  };
+  // V of half of them (product j), a lane's dims of token 16 j + 8 (e / 4) + 4 lh + e % 4 in v[e].
+  auto values = [&](const char* vt, int j, uint32_t (&v)[8][VW]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = 8 * (e >> 2) + (e & 3);
+      const char* const p = vt + vy + (vx ^ 16 * (k & (NCH - 1))) + (16 * j + k) * ROWB;
+      if constexpr (VW == 2) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        v[e][0] = w.x, v[e][VW - 1] = w.y;
+      } else {
+        v[e][0] = *reinterpret_cast<const uint32_t*>(p);
+      }
+    }
+  };
+  // V of half a tile that some row does not attend as a whole. there, some: bit k, its token k is
+  // there, it is and not every row attends it. A value that is not finite in a token of `some`
+  // would be NaN times 0: it leaves V (and is looked at again in the end).
+  bool odd = false;
+  auto mask_values = [&](uint32_t (&v)[8][VW], int j, uint32_t there, uint32_t some)
+                         __attribute__((always_inline)) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = 16 * j + 8 * (e >> 2) + (e & 3);
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t d = there >> (4 * lh) >> k & 1 ? v[e][w] : 0u;
+        const uint32_t x = some >> (4 * lh) >> k & 1 ? inf_halves<F16>(d) : 0u;
+        v[e][w] = d & ~x;
+        any |= x;
+      }
+    }
+    odd = odd || __ballot(any != 0) != 0;
+  };
+  // The running maximum, ahead of scores up to top. It stands still while they are less than 2^8
+  // above it: the weights stay below 2^8, and the sums need no factor.
+  auto rescale = [&](float top) __attribute__((always_inline)) {
+    const bool up = top > m_run + 8.f;  // (the first score that is not -inf too)
+    if (__ballot(up)) {
+      const float m_new = up ? top : m_run;
+      const float corr = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= corr;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) oacc[t] *= corr;
+      m_run = m_new;
+    }
+  };
+  // P of half a tile and its products with V.
+  auto add_half = [&](const f32x16_t& sc, int j, const uint32_t (&v)[8][VW])
+                      __attribute__((always_inline)) {
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no token yet: every P is 0
+    float pv[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pv[i] = __builtin_amdgcn_exp2f(fmaf(sc[8 * j + i], sl2, -m_use));
+      l_run += pv[i];
+    }
+    const uint4 p = make_uint4(pack_e2<F16>(pv[0], pv[1]), pack_e2<F16>(pv[2], pv[3]),
+                               pack_e2<F16>(pv[4], pv[5]), pack_e2<F16>(pv[6], pv[7]));
+#pragma unroll
+    for (int t = 0; t < DT; ++t) oacc[t] = mfma32<F16>(turn<VW>(v, t), p, oacc[t]);
+  };
   // Wait for q here: at its first use the compiler, which does not count the fetches, would
   // wait for all of them, in every step.
 #pragma unroll
@@ -272,111 +350,82 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       asm volatile("" ::: "memory");
       // The slot filled now was read a step ago: every wave is past that.
       if (s + RING - 1 < nstep) fetch(s + RING - 1);
-      const int t0 = w0 + s * STEP + 32 * part;
+      const int t0 = w0 + s * STEP + PTOK * part;
       if (t0 >= wend || row0 >= R) continue;
+      // (the addresses made of these are made again in each step, not kept in registers)
+      asm volatile("" : "+v"(kx), "+v"(vx));
       const char* const kb = lds + (s % RING) * STEP_B + part * PART_B;
-      const char* const vb = kb + HALF_B + vy;
-      f32x16_t sc;
+      const char* const vb = kb + HALF_B;
+      // What of the part's tokens is there; a part that every row attends needs no masks.
+      const uint64_t there =
+          __ballot(rows[s * STEP + PTOK * part + (lane & (PTOK - 1))] >= 0);
+      if (t0 + PTOK <= c.context && there == ~0ull) {
+        f32x16_t sc[PT];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+        for (int q = 0; q < PT; ++q) sc[q] = scores(kb, q);
+        float top = sc[0][0];
 #pragma unroll
-      for (int i = 0; i < KS; ++i)
-        sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kb + ky + (kx ^ (32 * i))), qf[i], sc);
-      uint32_t v[2][8][VW];
+        for (int i = 1; i < 16 * PT; ++i) top = fmaxf(top, sc[i / 16][i % 16]);
+        rescale(pair32_max(top) * sl2);
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = 8 * (e >> 2) + (e & 3);
-          const char* const p = vb + (16 * j + k) * ROWB + (vx ^ (16 * (k & (NCH - 1))));
-          if constexpr (VW == 2) {
-            const uint2 w = *reinterpret_cast<const uint2*>(p);
-            v[j][e][0] = w.x, v[j][e][VW - 1] = w.y;
-          } else {
-            v[j][e][0] = *reinterpret_cast<const uint32_t*>(p);
-          }
+        for (int q = 0; q < 2 * PT; ++q) {
+          uint32_t v[8][VW];
+          values(vb + (q >> 1) * TILE_B, q & 1, v);
+          add_half(sc[q >> 1], q & 1, v);
         }
-      const uint32_t there = (uint32_t)__ballot(rows[s * STEP + 32 * part + ln] >= 0);
-      if (t0 + 32 > c.context || there != ~0u) {
-        // Bit k: this row attends token t0 + k; of the tokens from `past` on not every row does.
-        const int past = max(c.context - t0, 0);
-        uint32_t on = past >= 32 ? ~0u
-                                 : (past ? (uint32_t)(mask << past) | ((1u << past) - 1)
-                                         : (uint32_t)(mask >> (t0 - c.context)));
-        on = (on & there) >> (4 * lh);
-        const uint32_t gone = ~there >> (4 * lh);
-        const uint32_t some = (past >= 32 ? 0u : ~0u << past) >> (4 * lh);
-        uint32_t odd = 0;
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < PT; ++q) {
+          const int t1 = t0 + 32 * q;
+          if (t1 >= wend) break;
+          const uint32_t here = (uint32_t)(there >> (32 * q));
+          // of its tokens from `past` on not every row attends each
+          const int past = max(c.context - t1, 0);
+          const uint32_t on = here & (past >= 32 ? ~0u
+                                      : past     ? (uint32_t)(mask << past) | ((1u << past) - 1)
+                                                 : (uint32_t)(mask >> (t1 - c.context)));
+          const uint32_t some = past >= 32 ? 0u : here & ~0u << past;
+          f32x16_t sc = scores(kb, q);
+          float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = 8 * (i >> 2) + (i & 3);  // register i, and token e = i % 8 of product i / 8
-          sc[i] = (on >> k) & 1 ? sc[i] : -INFINITY;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            uint32_t& d = v[i >> 3][i & 7][w];
-            d = (gone >> k) & 1 ? 0u : d;
-            odd |= (some >> k) & 1 ? inf_halves<F16>(d) : 0u;
+          for (int i = 0; i < 16; ++i) {
+            sc[i] = on >> (4 * lh) >> (8 * (i >> 2) + (i & 3)) & 1 ? sc[i] : -INFINITY;
+            top = fmaxf(top, sc[i]);
           }
-        }
-        // A value that is not finite, in a token that some row does not attend: 0 times it would
-        // be NaN. It leaves V; the rows that attend its token become NaN there.
-        if (__builtin_expect(__ballot(odd != 0) != 0, 0)) {
-          constexpr uint32_t ONE = F16 ? 0x3C003C00u : 0x3F803F80u;
+          rescale(pair32_max(top) * sl2);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            uint32_t one[4], u[8][VW];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int k = 16 * j + 8 * (e >> 2) + (e & 3);
-              const uint32_t bit = (on >> k) & 1 ? ONE & (e & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
-              one[e >> 1] = e & 1 ? one[e >> 1] | bit : bit;
-#pragma unroll
-              for (int w = 0; w < VW; ++w) {
-                const uint32_t x = (some >> k) & 1 ? inf_halves<F16>(v[j][e][w]) : 0u;
-                u[e][w] = x & ONE;
-                v[j][e][w] &= ~x;
-              }
-            }
-            const uint4 ob = make_uint4(one[0], one[1], one[2], one[3]);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) {
-              f32x16_t n;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) n[i] = 0.f;
-              n = mfma32<F16>(turn<VW>(u, t), ob, n);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) oacc[t][i] = n[i] > 0.f ? NAN : oacc[t][i];
-            }
+            uint32_t v[8][VW];
+            values(vb + q * TILE_B, j, v);
+            mask_values(v, j, here, some);
+            add_half(sc, j, v);
           }
         }
       }
-      float top = sc[0];
+    }
+  }
+  l_run = pair32_sum(l_run);
+  if (__builtin_expect(odd, 0)) {  // the rows that attend a value that is not finite are NaN there
+#pragma unroll 1
+    for (int k = max(begin, c.context); k < end; ++k) {
+      const int64_t r = a.pages.row(b, k);
+      if (r < 0) continue;
+      const bool mine = (mask >> (k - c.context)) & 1;
+      const uint4* const d = reinterpret_cast<const uint4*>(
+          a.vc + (r + (int64_t)kvh * a.pages.block_size) * D);
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-      const float m_new = fmaxf(m_run, pair32_max(top) * sl2);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no token yet: every P is 0
-      const float corr = __builtin_amdgcn_exp2f(m_run - m_use);
-      float pv[16], ps = 0.f;
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        pv[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], sl2, -m_use));
-        ps += pv[i];
-      }
-      l_run = l_run * corr + pair32_sum(ps);
-      m_run = m_new;
-      if (__ballot(corr != 1.f)) {
+        for (int h = 0; h < VW; ++h) {  // eight dims of the 4 DT of this i
+          const uint4 x = d[VW * (2 * i + lh) + h];
+          const uint32_t w[4] = {inf_halves<F16>(x.x), inf_halves<F16>(x.y), inf_halves<F16>(x.z),
+                                 inf_halves<F16>(x.w)};
 #pragma unroll
-        for (int t = 0; t < DT; ++t) oacc[t] *= corr;
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint4 p = make_uint4(pack_e2<F16>(pv[8 * j], pv[8 * j + 1]),
-                                   pack_e2<F16>(pv[8 * j + 2], pv[8 * j + 3]),
-                                   pack_e2<F16>(pv[8 * j + 4], pv[8 * j + 5]),
-                                   pack_e2<F16>(pv[8 * j + 6], pv[8 * j + 7]));
-#pragma unroll
-        for (int t = 0; t < DT; ++t) oacc[t] = mfma32<F16>(turn<VW>(v[j], t), p, oacc[t]);
-      }
+          for (int e = 0; e < 8; ++e) {
+            const int t = (8 * h + e) % DT, n = 4 * i + (8 * h + e) / DT;
+            oacc[t][n] = mine && (e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu) ? NAN : oacc[t][n];
+          }
+        }
     }
   }
 
@@ -505,10 +554,10 @@ Plan plan_of(int B, int T, int Hq, int Hkv) {
 }
 bool fast_dim(int D) { return D == 64 || D == 128; }
 
-template <bool F16, int D, int RW, int TW>
+template <bool F16, int D, int RW, int TW, int PT>
 int go(const FastArgs& a, const Plan& p, hipStream_t st) {
-  constexpr int LDS = RING_OF<D, TW> * TW * 128 * D + WIN * 4;
-  constexpr auto kern = tree_attn_kernel<F16, D, RW, TW>;
+  constexpr int LDS = RING_OF<D, TW, PT> * TW * PT * 128 * D + WIN * 4;
+  constexpr auto kern = tree_attn_kernel<F16, D, RW, TW, PT>;
   if (int rc = allow_dynamic_lds<kern, LDS>()) return rc;
   // Blocks of rows that read the same tokens run on one XCD: their ids are equal modulo 8.
   int64_t x = (int64_t)a.t.B * a.t.pages.Hkv * p.splits;
@@ -518,16 +567,16 @@ int go(const FastArgs& a, const Plan& p, hipStream_t st) {
     const int R = a.t.T * (a.t.Hq / a.t.pages.Hkv);
     tree_attn_join_kernel<F16, D><<<dim3((unsigned)cdiv(R, JT / (D / 4)),
                                          (unsigned)(a.t.B * a.t.pages.Hkv)), JT, 0, st>>>(
-        a, 32 * TW);
+        a, 32 * PT * TW);
   }
   return launch_check("paged_tree_attn");
 }
 template <bool F16, int D>
 int go_form(const FastArgs& a, const Plan& p, hipStream_t st) {
-  return p.rw == 1   ? go<F16, D, 1, 4>(a, p, st)
-         : p.rw == 2 ? go<F16, D, 2, 4>(a, p, st)
-         : p.rw == 4 ? go<F16, D, 4, 2>(a, p, st)
-                     : go<F16, D, 8, 1>(a, p, st);
+  return p.rw == 1   ? go<F16, D, 1, 4, 1>(a, p, st)
+         : p.rw == 2 ? go<F16, D, 2, 4, 1>(a, p, st)
+         : p.rw == 4 ? go<F16, D, 4, 2, 2>(a, p, st)
+                     : go<F16, D, 8, 1, 2>(a, p, st);
 }
 
 }  // namespace
