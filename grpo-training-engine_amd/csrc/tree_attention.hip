@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 
 constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
 constexpr int MAX_SPLITS = 64;
+constexpr int LEAST_CHUNK = 128; // tokens of a split at least
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -152,14 +153,15 @@ __device__ __forceinline__ void dma16_at(uint32_t lds, const void* p) {
 struct Cut {
   int context, nodes, total, chunk, splits;
 };
-__device__ __forceinline__ Cut cut_of(const TreeArgs& a, int b, int splits, int step) {
+__device__ __forceinline__ Cut cut_of(const TreeArgs& a, int len, int count, int splits, int step) {
   Cut c;
-  const int len = a.cl[b], cap = a.pages.max_blocks * a.pages.block_size;
-  c.nodes = nodes_of(a.counts, b, a.T, len);
+  const int cap = a.pages.max_blocks * a.pages.block_size;
+  c.nodes = len < 0 ? 0 : min(max(count, 0), a.T);
   c.context = min(max(len, 0), cap);
-  c.total = c.nodes ? (int)min((int64_t)len + c.nodes, (int64_t)cap) : 0;
-  c.chunk = (int)cdiv(cdiv(c.total, splits), step) * step;
-  c.splits = c.total ? (c.total + c.chunk - 1) / c.chunk : 0;
+  c.total = c.nodes ? c.context + min(c.nodes, cap - c.context) : 0;
+  const uint32_t part = ((uint32_t)c.total + splits - 1) / (uint32_t)splits;
+  c.chunk = max((int)((part + step - 1) / step) * step, LEAST_CHUNK);
+  c.splits = ((uint32_t)c.total + c.chunk - 1) / (uint32_t)c.chunk;
   return c;
 }
 
@@ -205,25 +207,24 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   const int pair = blockIdx.x / f.splits, split = blockIdx.x - pair * f.splits;
   const int b = pair / Hkv, kvh = pair - b * Hkv;
   if (b >= a.B) return;
-  const Cut c = cut_of(a, b, f.splits, STEP);
-  if (split >= max(c.splits, 1)) return;
+  // What does not depend on the sequence's length is asked for together with it.
+  const int len = a.cl[b], count = a.counts ? a.counts[b] : a.T;
   const int row0 = (blockIdx.y * RW + wave % RW) * 32, row = row0 + ln, rowc = min(row, R - 1);
   const int node = rowc / G, head = kvh * G + rowc - node * G;
-  const uint64_t all = sees(a, b);
-  const uint64_t mask = (uint64_t)__shfl((long long)all, node);
-
+  int up = lane - 1;
+  if (a.parents) up = lane < a.T ? a.parents[(int64_t)b * a.ps + lane] : -1;
   uint4 qf[KS];
   {
     const uint16_t* const q =
         a.q + (int64_t)b * a.qsb + (int64_t)node * a.qst + (int64_t)head * a.qsh + 8 * lh;
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      qf[i] = *reinterpret_cast<const uint4*>(q + 16 * i);
-      qf[i].x ^= flip, qf[i].y ^= flip, qf[i].z ^= flip, qf[i].w ^= flip;
-    }
+    for (int i = 0; i < KS; ++i) qf[i] = *reinterpret_cast<const uint4*>(q + 16 * i);
   }
+  const Cut c = cut_of(a, len, count, f.splits, STEP);
+  if (split >= max(c.splits, 1)) return;
   const float sl2 = fmaxf(fabsf(a.scale) * LOG2E, 1e-30f);  // (-inf stays -inf)
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+  uint64_t mask = 0;  // the nodes that row ln's node attends
   const int begin = split * c.chunk, end = min(c.total, begin + c.chunk);
 
   const uint32_t lbase = lds_address(lds);
@@ -324,18 +325,23 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
 #pragma unroll
     for (int t = 0; t < DT; ++t) oacc[t] = mfma32<F16>(turn<VW>(v, t), p, oacc[t]);
   };
-  // Wait for q here: at its first use the compiler, which does not count the fetches, would
-  // wait for all of them, in every step.
-#pragma unroll
-  for (int i = 0; i < KS; ++i)
-    asm volatile("" : "+v"(qf[i].x), "+v"(qf[i].y), "+v"(qf[i].z), "+v"(qf[i].w));
-
   for (int w0 = begin; w0 < end; w0 += WIN) {
     const int wend = min(end, w0 + WIN), nstep = (wend - w0 + STEP - 1) / STEP;
     if (w0 != begin) __syncthreads();  // the last window has been read
     for (int i = tid; i < nstep * STEP; i += 64 * W) {
       const int64_t at = w0 + i < wend ? a.pages.row(b, w0 + i) : -1;
       rows[i] = at < 0 ? -1 : (int)at + kvh * a.pages.block_size;
+    }
+    if (w0 == begin) {  // (while the block tables are on their way)
+      const uint64_t all = a.parents ? ancestors(node_parent(up, lane)) : ~0ull >> (63 - lane);
+      mask = (uint64_t)__shfl((long long)all, node);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        qf[i].x ^= flip, qf[i].y ^= flip, qf[i].z ^= flip, qf[i].w ^= flip;
+        // wait for q here: at its first use the compiler, which does not count the fetches, would
+        // wait for all of them, in every step
+        asm volatile("" : "+v"(qf[i].x), "+v"(qf[i].y), "+v"(qf[i].z), "+v"(qf[i].w));
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(JT) tree_attn_join_kernel(FastArgs f, int step
   const TreeArgs& a = f.t;
   const int Hkv = a.pages.Hkv, G = a.Hq / Hkv, R = a.T * G;
   const int pair = blockIdx.y, b = pair / Hkv, kvh = pair - b * Hkv;
-  const Cut c = cut_of(a, b, f.splits, step);
+  const Cut c = cut_of(a, a.cl[b], a.counts ? a.counts[b] : a.T, f.splits, step);
   if (c.splits <= 1) return;
   const int row = blockIdx.x * RPB + threadIdx.x / L, l = threadIdx.x % L;
   if (row >= R) return;
@@ -548,7 +554,7 @@ Plan plan_of(int B, int T, int Hq, int Hkv) {
   p.tw = std::min(8 / p.rw, 4);
   p.rb = (int)cdiv(R, 32 * p.rw);
   const int64_t groups = (int64_t)B * Hkv * p.rb;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS, 512 / groups));
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS, 256 / groups));
   p.values = p.splits > 1 ? (size_t)B * Hkv * p.splits * p.rb * 32 * p.rw : 0;
   return p;
 }
