@@ -183,7 +183,7 @@ __device__ __forceinline__ uint4 turn(const uint32_t (&v)[8][VW], int t) {
 
 // Steps in LDS at a time, of 32 PT TW tokens.
 template <int D, int TW, int PT>
-constexpr int RING_OF = D * TW * PT <= 128 ? 4 : (D * TW * PT <= 256 ? 3 : 2);
+constexpr int RING_OF = D * TW * PT <= 256 ? 4 : 2;
 
 template <bool F16, int D, int RW, int TW, int PT>
 __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   constexpr int ROWB = 2 * D, NCH = D / 8;            // bytes and 16-byte chunks of a row
   constexpr int TILE_B = 32 * ROWB, HALF_B = PT * TILE_B;
   constexpr int PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
+  constexpr int AHEAD = RING > 2;  // the next tile's scores are made while this one is added
   constexpr int TPP = 1024 / ROWB, PPK = PTOK / TPP;  // tokens of a 1-KiB piece, pieces of K
   constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
   static_assert(PIECES % W == 0, "every wave loads as many pieces");
@@ -252,15 +253,15 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   int kx = 16 * ((lh ^ ln) & (NCH - 1)), vx = 16 * ((ln * 4 * VW / 16 ^ 4 * lh) & (NCH - 1));
   const int ky = ln * ROWB;
   const int vy = 4 * lh * ROWB + ln * 4 * VW % 16;
-  // S^T of 32 tokens (tile q of the part at kb).
-  auto scores = [&](const char* kb, int q) __attribute__((always_inline)) {
+  // S^T of 32 tokens, tile q of step s.
+  auto scores = [&](int s, int q) __attribute__((always_inline)) {
+    const char* const kt = lds + (s % RING) * STEP_B + part * PART_B + q * TILE_B + ky;
     f32x16_t sc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
-      sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kb + ky + (kx ^ 32 * i) + q * TILE_B),
-                       qf[i], sc);
+      sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kt + (kx ^ 32 * i)), qf[i], sc);
     return sc;
   };
   // V of half of them (product j), a lane's dims of token 16 j + 8 (e / 4) + 4 lh + e % 4 in v[e].
@@ -347,66 +348,62 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
 #pragma unroll
     for (int s = 0; s < RING - 1; ++s)
       if (s < nstep) fetch(s);
+    f32x16_t sc;  // of the tile at hand
+    if constexpr (AHEAD) {
+      if (nstep >= RING - 1)
+        wait_vm<(RING - 2) * LD>();  // step 0 has landed
+      else
+        wait_vm<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      sc = scores(0, 0);
+    }
+#pragma unroll 1
     for (int s = 0; s < nstep; ++s) {
       if (nstep - 1 - s >= RING - 2)
-        wait_vm<(RING - 2) * LD>();  // step s has landed
+        wait_vm<(RING - 2 - AHEAD) * LD>();  // step s (s + 1) has landed
       else
         wait_vm<0>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       // The slot filled now was read a step ago: every wave is past that.
       if (s + RING - 1 < nstep) fetch(s + RING - 1);
-      const int t0 = w0 + s * STEP + PTOK * part;
-      if (t0 >= wend || row0 >= R) continue;
+      if (row0 >= R) continue;
       // (the addresses made of these are made again in each step, not kept in registers)
       asm volatile("" : "+v"(kx), "+v"(vx));
-      const char* const kb = lds + (s % RING) * STEP_B + part * PART_B;
-      const char* const vb = kb + HALF_B;
-      // What of the part's tokens is there; a part that every row attends needs no masks.
-      const uint64_t there =
-          __ballot(rows[s * STEP + PTOK * part + (lane & (PTOK - 1))] >= 0);
-      if (t0 + PTOK <= c.context && there == ~0ull) {
-        f32x16_t sc[PT];
 #pragma unroll
-        for (int q = 0; q < PT; ++q) sc[q] = scores(kb, q);
-        float top = sc[0][0];
-#pragma unroll
-        for (int i = 1; i < 16 * PT; ++i) top = fmaxf(top, sc[i / 16][i % 16]);
-        rescale(pair32_max(top) * sl2);
-#pragma unroll
-        for (int q = 0; q < 2 * PT; ++q) {
-          uint32_t v[8][VW];
-          values(vb + (q >> 1) * TILE_B, q & 1, v);
-          add_half(sc[q >> 1], q & 1, v);
-        }
-      } else {
-#pragma unroll 1
-        for (int q = 0; q < PT; ++q) {
-          const int t1 = t0 + 32 * q;
-          if (t1 >= wend) break;
-          const uint32_t here = (uint32_t)(there >> (32 * q));
-          // of its tokens from `past` on not every row attends each
-          const int past = max(c.context - t1, 0);
+      for (int q = 0; q < PT; ++q) {
+        const int t1 = w0 + s * STEP + PTOK * part + 32 * q;
+        f32x16_t next;
+        if constexpr (AHEAD)
+          next = q + 1 < PT ? scores(s, q + 1) : scores(s + 1, 0);  // (of nothing after the last)
+        else
+          sc = scores(s, q);
+        const uint32_t here = (uint32_t)__ballot(rows[s * STEP + PTOK * part + 32 * q + ln] >= 0);
+        const bool masked = t1 + 32 > c.context || here != ~0u;
+        // of the tile's tokens from `past` on not every row attends each
+        const int past = max(c.context - t1, 0);
+        if (masked) {
           const uint32_t on = here & (past >= 32 ? ~0u
                                       : past     ? (uint32_t)(mask << past) | ((1u << past) - 1)
-                                                 : (uint32_t)(mask >> (t1 - c.context)));
-          const uint32_t some = past >= 32 ? 0u : here & ~0u << past;
-          f32x16_t sc = scores(kb, q);
-          float top = -INFINITY;
+                                                 : (uint32_t)(mask >> min(t1 - c.context, 63)));
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 16; ++i)
             sc[i] = on >> (4 * lh) >> (8 * (i >> 2) + (i & 3)) & 1 ? sc[i] : -INFINITY;
-            top = fmaxf(top, sc[i]);
-          }
-          rescale(pair32_max(top) * sl2);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t v[8][VW];
-            values(vb + q * TILE_B, j, v);
-            mask_values(v, j, here, some);
-            add_half(sc, j, v);
-          }
         }
+        float top = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
+        rescale(pair32_max(top) * sl2);
+        const char* const vt = lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t v[8][VW];
+          values(vt, j, v);
+          if (masked) mask_values(v, j, here, past >= 32 ? 0u : here & ~0u << past);
+          add_half(sc, j, v);
+        }
+        if constexpr (AHEAD) sc = next;
       }
     }
   }
@@ -581,7 +578,7 @@ template <bool F16, int D>
 int go_form(const FastArgs& a, const Plan& p, hipStream_t st) {
   return p.rw == 1   ? go<F16, D, 1, 4, 1>(a, p, st)
          : p.rw == 2 ? go<F16, D, 2, 4, 1>(a, p, st)
-         : p.rw == 4 ? go<F16, D, 4, 2, 2>(a, p, st)
+         : p.rw == 4 ? go<F16, D, 4, 2, 1>(a, p, st)
                      : go<F16, D, 8, 1, 2>(a, p, st);
 }
 
