@@ -108,9 +108,8 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //  * A wave owns 32 rows; a workgroup RW waves side by side on rows times TW on tokens, which
 //    take the 32-token parts of each step and meet in LDS at the end. A sequence's tokens are
 //    cut over workgroups where there are few of them (a second kernel joins the parts).
-//  * K and V of a step come to LDS by loads of their own, RING - 1 steps ahead. A token's
-//    16-byte chunks are stored at chunk ^ token, so that the readers (32 tokens, one chunk)
-//    spread over the banks. The cache rows of WIN tokens stand in LDS too.
+//  * K and V of a step come to LDS by loads of their own, RING - 1 steps ahead. The cache rows of
+//    WIN tokens stand in LDS too.
 //  * S^T = K Q^T leaves lane (row ln, half lh) with 16 of 32 tokens' scores of its row, which
 //    are the operand P^T of O^T = V^T P^T if its contraction index (lh, e) of product j means
 //    token 16 j + 8 (e / 4) + 4 lh + e % 4: P never leaves the lane. V is read as rows, D / 32
@@ -118,7 +117,9 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //  * P is rounded to 16 bits (2^-8 of each weight in bf16, 2^-11 in float16), the sum is of the
 //    float32 weights: the roundings are independent, so over many tokens they stay below the
 //    rounding of the result.
-//  * Only steps that reach past the cached tokens, or hold a missing block, look at masks.
+//  * Steps that reach past the cached tokens, or a window that holds a missing block, have V
+//    cleaned in LDS first and the scores masked: the same loop adds them, so that O stays in one
+//    set of registers.
 
 constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
 constexpr int MAX_SPLITS = 64;
@@ -181,6 +182,18 @@ __device__ __forceinline__ uint4 turn(const uint32_t (&v)[8][VW], int t) {
                     perm(v[5][w], v[4][w], sel), perm(v[7][w], v[6][w], sel));
 }
 
+// LDS: pieces of 1 KiB, each an instruction's, 16 bytes apart so that four (eight) of them start
+// in different banks. Within one a token's 16-byte chunk c stands at c ^ swizzle(token).
+template <int D>
+constexpr int TPP = 512 / D;  // tokens of a piece
+constexpr int PIECE = 1024 + 16;
+template <int D>
+constexpr int TILE = 32 / TPP<D> * PIECE;  // 32 tokens
+template <int D>
+__device__ __forceinline__ int swizzle(int token) {
+  return D == 128 ? (token & 3) * 4 : token & 6;
+}
+
 // Steps in LDS at a time, of 32 PT TW tokens.
 template <int D, int TW, int PT>
 constexpr int RING_OF = D * TW * PT <= 256 ? 4 : 2;
@@ -189,10 +202,10 @@ template <bool F16, int D, int RW, int TW, int PT>
 __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   constexpr int W = RW * TW, PTOK = 32 * PT, STEP = PTOK * TW, RING = RING_OF<D, TW, PT>;
   constexpr int ROWB = 2 * D, NCH = D / 8;            // bytes and 16-byte chunks of a row
-  constexpr int TILE_B = 32 * ROWB, HALF_B = PT * TILE_B;
+  constexpr int TILE_B = TILE<D>, HALF_B = PT * TILE_B;
   constexpr int PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
   constexpr int AHEAD = RING > 2;  // the next tile's scores are made while this one is added
-  constexpr int TPP = 1024 / ROWB, PPK = PTOK / TPP;  // tokens of a 1-KiB piece, pieces of K
+  constexpr int PPK = PTOK / TPP<D>;                  // pieces of K
   constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
   static_assert(PIECES % W == 0, "every wave loads as many pieces");
   constexpr int KS = D / 16, DT = D / 32, VW = DT / 2;  // steps of K, tiles of V, its words
@@ -232,14 +245,19 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   auto fetch = [&](int s) __attribute__((always_inline)) {
     int l = lane;
     asm volatile("" : "+v"(l));
+    int r[LD];
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
-      const int pc = wave + W * i, pt = pc / (2 * PPK);
-      const int tok = (pc & (PPK - 1)) * TPP + l / NCH;
-      const int r = max(rows[s * STEP + PTOK * pt + tok], 0);  // a missing one reads row 0
+      const int pc = wave + W * i, tok = (pc & (PPK - 1)) * TPP<D> + l / NCH;
+      r[i] = rows[s * STEP + PTOK * (pc / (2 * PPK)) + tok];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const int pc = wave + W * i, tok = (pc & (PPK - 1)) * TPP<D> + l / NCH;
       const uint16_t* const base = (pc / PPK) & 1 ? a.vc : a.kc;
-      dma16_at(lbase + (s % RING) * STEP_B + pc * 1024,
-               base + (int64_t)r * D + 8 * ((l ^ tok) & (NCH - 1)));
+      dma16_at(lbase + (s % RING) * STEP_B + pc * PIECE,  // (a missing one reads row 0)
+               base + (int64_t)max(r[i], 0) * D + 8 * ((l & (NCH - 1)) ^ swizzle<D>(tok)));
     }
   };
 
@@ -249,27 +267,38 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
-  // Where a lane's operands stand in a tile of K, and in a tile of V less its token.
-  int kx = 16 * ((lh ^ ln) & (NCH - 1)), vx = 16 * ((ln * 4 * VW / 16 ^ 4 * lh) & (NCH - 1));
-  const int ky = ln * ROWB;
-  const int vy = 4 * lh * ROWB + ln * 4 * VW % 16;
+  // Where a lane's operands stand in a tile, less what is the same for all lanes: of K product
+  // KS / 4 i's, of V the tokens' whose swizzles are alike.
+  constexpr int VA = D == 128 ? 4 : 2;
+  int ka[4], va[VA];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    ka[i] = ln / TPP<D> * PIECE + ln % TPP<D> * ROWB + 16 * (NCH / 4 * i ^ swizzle<D>(ln)) + 16 * lh;
+#pragma unroll
+  for (int i = 0; i < VA; ++i) {
+    const int tok = 4 * lh + 4 / VA * i, at = 4 * VW * ln;
+    va[i] = tok / TPP<D> * PIECE + tok % TPP<D> * ROWB + 16 * (at / 16 ^ swizzle<D>(tok)) + at % 16;
+  }
+  auto k_of = [&](const char* kt, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const uint4*>(kt + ka[i / (KS / 4)] + 32 * (i % (KS / 4)));
+  };
   // S^T of 32 tokens, tile q of step s.
   auto scores = [&](int s, int q) __attribute__((always_inline)) {
-    const char* const kt = lds + (s % RING) * STEP_B + part * PART_B + q * TILE_B + ky;
+    const char* const kt = lds + (s % RING) * STEP_B + part * PART_B + q * TILE_B;
     f32x16_t sc;
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
-      sc = mfma32<F16>(*reinterpret_cast<const uint4*>(kt + (kx ^ 32 * i)), qf[i], sc);
+      sc = mfma32<F16>(k_of(kt, i), qf[i], sc);
     return sc;
   };
   // V of half of them (product j), a lane's dims of token 16 j + 8 (e / 4) + 4 lh + e % 4 in v[e].
   auto values = [&](const char* vt, int j, uint32_t (&v)[8][VW]) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int k = 8 * (e >> 2) + (e & 3);
-      const char* const p = vt + vy + (vx ^ 16 * (k & (NCH - 1))) + (16 * j + k) * ROWB;
+      const char* const p = vt + va[(e & 3) / (4 / VA)] + (e & (4 / VA - 1)) * ROWB +
+                            (16 * j + 8 * (e >> 2)) / TPP<D> * PIECE;
       if constexpr (VW == 2) {
         const uint2 w = *reinterpret_cast<const uint2*>(p);
         v[e][0] = w.x, v[e][VW - 1] = w.y;
@@ -278,25 +307,36 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       }
     }
   };
-  // V of half a tile that some row does not attend as a whole. there, some: bit k, its token k is
-  // there, it is and not every row attends it. A value that is not finite in a token of `some`
-  // would be NaN times 0: it leaves V (and is looked at again in the end).
+  // V of a step that some row does not attend as a whole: a missing token's row is 0, and so is a
+  // value that is not finite in a token that not every row attends, which would be NaN times 0
+  // (it is looked at again in the end).
   bool odd = false;
-  auto mask_values = [&](uint32_t (&v)[8][VW], int j, uint32_t there, uint32_t some)
-                         __attribute__((always_inline)) {
-    uint32_t any = 0;
+  auto clean = [&](int s, int t0) __attribute__((always_inline)) {
+    constexpr int N = STEP * NCH / (64 * W);
+    bool any = false;
+    int r[N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int k = 16 * j + 8 * (e >> 2) + (e & 3);
+    for (int i = 0; i < N; ++i) r[i] = rows[s * STEP + (tid + 64 * W * i) / NCH];
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t d = there >> (4 * lh) >> k & 1 ? v[e][w] : 0u;
-        const uint32_t x = some >> (4 * lh) >> k & 1 ? inf_halves<F16>(d) : 0u;
-        v[e][w] = d & ~x;
-        any |= x;
+    for (int i = 0; i < N; ++i) {
+      const int tok = (tid + 64 * W * i) / NCH, at = tok % PTOK;
+      uint4* const d = reinterpret_cast<uint4*>(lds + (s % RING) * STEP_B + tok / PTOK * PART_B +
+                                                HALF_B + at / TPP<D> * PIECE + at % TPP<D> * ROWB) +
+                       tid % NCH;
+      if (r[i] < 0) {
+        *d = make_uint4(0u, 0u, 0u, 0u);
+      } else if (t0 + tok >= c.context) {
+        uint4 v = *d;
+        const uint4 x = make_uint4(inf_halves<F16>(v.x), inf_halves<F16>(v.y),
+                                   inf_halves<F16>(v.z), inf_halves<F16>(v.w));
+        if (x.x | x.y | x.z | x.w) {
+          v.x &= ~x.x, v.y &= ~x.y, v.z &= ~x.z, v.w &= ~x.w;
+          *d = v;
+          any = true;
+        }
       }
     }
-    odd = odd || __ballot(any != 0) != 0;
+    odd |= __syncthreads_or(any) != 0;
   };
   // The running maximum, ahead of scores up to top. It stands still while they are less than 2^8
   // above it: the weights stay below 2^8, and the sums need no factor.
@@ -311,27 +351,79 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       m_run = m_new;
     }
   };
-  // P of half a tile and its products with V.
-  auto add_half = [&](const f32x16_t& sc, int j, const uint32_t (&v)[8][VW])
-                      __attribute__((always_inline)) {
+  auto weight = [&](float x) __attribute__((always_inline)) {
     const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no token yet: every P is 0
-    float pv[8];
+    const float p = __builtin_amdgcn_exp2f(fmaf(x, sl2, -m_use));
+    l_run += p;
+    return p;
+  };
+  auto top_of = [&](const f32x16_t& x) __attribute__((always_inline)) {
+    float top = x[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      pv[i] = __builtin_amdgcn_exp2f(fmaf(sc[8 * j + i], sl2, -m_use));
-      l_run += pv[i];
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+    return top;
+  };
+  // P V of a tile, and the next tile's scores (K at kn) with their maximum. In this order the
+  // vector instructions stand between products that they do not depend on: the compiler would
+  // put a tile's products one after another, and its arithmetic behind them.
+  auto add = [&](f32x16_t& sc, const char* vt, const char* kn, float& top)
+                 __attribute__((always_inline)) {
+    constexpr int A = KS < 4 ? KS : 4, E = 16 / KS;  // fragments of K ahead, weights per product
+    uint4 k[KS];
+    uint32_t v[2][8][VW];
+    uint32_t p[8];
+    f32x16_t next;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) next[i] = 0.f;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    const uint4 p = make_uint4(pack_e2<F16>(pv[0], pv[1]), pack_e2<F16>(pv[2], pv[3]),
-                               pack_e2<F16>(pv[4], pv[5]), pack_e2<F16>(pv[6], pv[7]));
 #pragma unroll
-    for (int t = 0; t < DT; ++t) oacc[t] = mfma32<F16>(turn<VW>(v, t), p, oacc[t]);
+    for (int i = 0; i < KS; ++i) {
+      if constexpr (AHEAD) {
+        next = mfma32<F16>(k[i], qf[i], next);
+        if (i + A < KS) k[i + A] = k_of(kn, i + A);
+      }
+#pragma unroll
+      for (int e = E * i; e < E * (i + 1); e += 2) {
+        const float x = weight(sc[e]), y = weight(sc[e + 1]);
+        p[e / 2] = pack_e2<F16>(x, y);
+      }
+      if (i == KS - 2) values(vt, 0, v[0]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint4 vv = turn<VW>(v[0], 0);
+    const uint4 p0 = make_uint4(p[0], p[1], p[2], p[3]), p1 = make_uint4(p[4], p[5], p[6], p[7]);
+    values(vt, 1, v[1]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2 * DT; ++t) {
+      oacc[t % DT] = mfma32<F16>(vv, t < DT ? p0 : p1, oacc[t % DT]);
+      if (t + 1 < 2 * DT) vv = turn<VW>(v[(t + 1) / DT], (t + 1) % DT);
+      if constexpr (AHEAD) {
+        if (t >= DT) {
+          constexpr int M = 16 / DT;
+#pragma unroll
+          for (int i = 0; i < M; ++i) {
+            const float x = next[M * (t - DT) + i];
+            top = t == DT && i == 0 ? x : fmaxf(top, x);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (AHEAD) sc = next;
   };
   for (int w0 = begin; w0 < end; w0 += WIN) {
     const int wend = min(end, w0 + WIN), nstep = (wend - w0 + STEP - 1) / STEP;
     if (w0 != begin) __syncthreads();  // the last window has been read
+    int hole = 0;  // a missing block
     for (int i = tid; i < nstep * STEP; i += 64 * W) {
       const int64_t at = w0 + i < wend ? a.pages.row(b, w0 + i) : -1;
       rows[i] = at < 0 ? -1 : (int)at + kvh * a.pages.block_size;
+      hole |= at < 0 && w0 + i < wend;
     }
     if (w0 == begin) {  // (while the block tables are on their way)
       const uint64_t all = a.parents ? ancestors(node_parent(up, lane)) : ~0ull >> (63 - lane);
@@ -344,11 +436,12 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
         asm volatile("" : "+v"(qf[i].x), "+v"(qf[i].y), "+v"(qf[i].z), "+v"(qf[i].w));
       }
     }
-    __syncthreads();
+    const bool holes = __syncthreads_or(hole);
 #pragma unroll
     for (int s = 0; s < RING - 1; ++s)
       if (s < nstep) fetch(s);
-    f32x16_t sc;  // of the tile at hand
+    f32x16_t sc;  // of the tile at hand, and each lane's maximum of them
+    float top;
     if constexpr (AHEAD) {
       if (nstep >= RING - 1)
         wait_vm<(RING - 2) * LD>();  // step 0 has landed
@@ -357,6 +450,7 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       sc = scores(0, 0);
+      top = top_of(sc);
     }
 #pragma unroll 1
     for (int s = 0; s < nstep; ++s) {
@@ -368,42 +462,30 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       asm volatile("" ::: "memory");
       // The slot filled now was read a step ago: every wave is past that.
       if (s + RING - 1 < nstep) fetch(s + RING - 1);
+      const int t0 = w0 + s * STEP;
+      const bool masked = t0 + STEP > c.context || holes;
+      if (masked) clean(s, t0);
       if (row0 >= R) continue;
-      // (the addresses made of these are made again in each step, not kept in registers)
-      asm volatile("" : "+v"(kx), "+v"(vx));
 #pragma unroll
       for (int q = 0; q < PT; ++q) {
-        const int t1 = w0 + s * STEP + PTOK * part + 32 * q;
-        f32x16_t next;
-        if constexpr (AHEAD)
-          next = q + 1 < PT ? scores(s, q + 1) : scores(s + 1, 0);  // (of nothing after the last)
-        else
-          sc = scores(s, q);
-        const uint32_t here = (uint32_t)__ballot(rows[s * STEP + PTOK * part + 32 * q + ln] >= 0);
-        const bool masked = t1 + 32 > c.context || here != ~0u;
-        // of the tile's tokens from `past` on not every row attends each
-        const int past = max(c.context - t1, 0);
+        if constexpr (!AHEAD) sc = scores(s, q), top = top_of(sc);
         if (masked) {
+          const int at = PTOK * part + 32 * q;
+          const uint32_t here = (uint32_t)__ballot(rows[s * STEP + at + ln] >= 0);
+          // of the tile's tokens from `past` on not every row attends each
+          const int past = max(c.context - t0 - at, 0);
           const uint32_t on = here & (past >= 32 ? ~0u
                                       : past     ? (uint32_t)(mask << past) | ((1u << past) - 1)
-                                                 : (uint32_t)(mask >> min(t1 - c.context, 63)));
+                                                 : (uint32_t)(mask >> min(t0 + at - c.context, 63)));
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             sc[i] = on >> (4 * lh) >> (8 * (i >> 2) + (i & 3)) & 1 ? sc[i] : -INFINITY;
+          top = top_of(sc);
         }
-        float top = sc[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
         rescale(pair32_max(top) * sl2);
-        const char* const vt = lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t v[8][VW];
-          values(vt, j, v);
-          if (masked) mask_values(v, j, here, past >= 32 ? 0u : here & ~0u << past);
-          add_half(sc, j, v);
-        }
-        if constexpr (AHEAD) sc = next;
+        const int sn = s + (q + 1) / PT, qn = (q + 1) % PT;  // (behind the last tile: of nothing)
+        add(sc, lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B,
+            lds + (sn % RING) * STEP_B + part * PART_B + qn * TILE_B, top);
       }
     }
   }
@@ -559,7 +641,7 @@ bool fast_dim(int D) { return D == 64 || D == 128; }
 
 template <bool F16, int D, int RW, int TW, int PT>
 int go(const FastArgs& a, const Plan& p, hipStream_t st) {
-  constexpr int LDS = RING_OF<D, TW, PT> * TW * PT * 128 * D + WIN * 4;
+  constexpr int LDS = RING_OF<D, TW, PT> * TW * PT * 2 * TILE<D> + WIN * 4;
   constexpr auto kern = tree_attn_kernel<F16, D, RW, TW, PT>;
   if (int rc = allow_dynamic_lds<kern, LDS>()) return rc;
   // Blocks of rows that read the same tokens run on one XCD: their ids are equal modulo 8.
