@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //    WIN tokens stand in LDS too.
 //  * S^T = K Q^T leaves lane (row ln, half lh) with 16 of 32 tokens' scores of its row, which
 //    are the operand P^T of O^T = V^T P^T if its contraction index (lh, e) of product j means
-//    token 16 j + 8 (e / 4) + 4 lh + e % 4: P never leaves the lane. V is read as rows, D / 32
-//    neighbouring dims per lane, and its pairs of tokens are turned with v_perm.
+//    token 16 j + 8 (e / 4) + 4 lh + e % 4: P never leaves the lane. V is turned as it is read
+//    from LDS.
 //  * P is rounded to 16 bits (2^-8 of each weight in bf16, 2^-11 in float16), the sum is of the
 //    float32 weights: the roundings are independent, so over many tokens they stay below the
 //    rounding of the result.
@@ -173,13 +173,12 @@ __device__ __forceinline__ uint32_t inf_halves(uint32_t d) {
   return ((d & X) == X ? 0xFFFFu : 0u) | ((d & (X << 16)) == X << 16 ? 0xFFFF0000u : 0u);
 }
 
-// V^T operand of dims DT row + t from eight tokens' words.
-template <int VW>
-__device__ __forceinline__ uint4 turn(const uint32_t (&v)[8][VW], int t) {
-  const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
-  const int w = t >> 1;
-  return make_uint4(perm(v[1][w], v[0][w], sel), perm(v[3][w], v[2][w], sel),
-                    perm(v[5][w], v[4][w], sel), perm(v[7][w], v[6][w], sel));
+// Four 16-bit values per lane, turned: of 16 lanes' rows 0 to 3, which lanes 4 r to 4 r + 3 name with
+// an address for four values each, lane n gets value n of each.
+__device__ __forceinline__ uint2 turned(const char* p) {
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4_t*)p));
 }
 
 // LDS: pieces of 1 KiB, each an instruction's, 16 bytes apart so that four (eight) of them start
@@ -208,7 +207,7 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   constexpr int PPK = PTOK / TPP<D>;                  // pieces of K
   constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
   static_assert(PIECES % W == 0, "every wave loads as many pieces");
-  constexpr int KS = D / 16, DT = D / 32, VW = DT / 2;  // steps of K, tiles of V, its words
+  constexpr int KS = D / 16, DT = D / 32;             // steps of K, tiles of V
   constexpr int XCH = 2 + 16 * DT;                      // values per lane in the waves' merge
   static_assert((TW - 1) * RW * XCH * 256 <= RING * STEP_B, "the merge fits the ring");
   extern __shared__ __align__(16) char lds[];           // [RING][STEP_B], then WIN rows
@@ -242,7 +241,22 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   const int begin = split * c.chunk, end = min(c.total, begin + c.chunk);
 
   const uint32_t lbase = lds_address(lds);
+  // Where a block of the cache holds whole pieces, a piece is 1 KiB of it.
+  const bool by_piece = a.pages.block_size % TPP<D> == 0;
+  const uint32_t piece_at =
+      lane / NCH * ROWB + 16 * ((lane & (NCH - 1)) ^ swizzle<D>(lane / NCH));
   auto fetch = [&](int s) __attribute__((always_inline)) {
+    if (by_piece) {  // piece i's first row in lane i
+      const int pc = wave + W * (lane % LD);
+      const int first = rows[s * STEP + PTOK * (pc / (2 * PPK)) + (pc & (PPK - 1)) * TPP<D>];
+#pragma unroll
+      for (int i = 0; i < LD; ++i) {
+        const int pi = wave + W * i, r = max(__builtin_amdgcn_readlane(first, i), 0);
+        const uint16_t* const base = (pi / PPK) & 1 ? a.vc : a.kc;
+        dma16(lbase + (s % RING) * STEP_B + pi * PIECE, piece_at, base + (int64_t)r * D);
+      }
+      return;
+    }
     int l = lane;
     asm volatile("" : "+v"(l));
     int r[LD];
@@ -262,22 +276,21 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   };
 
   float m_run = -INFINITY, l_run = 0.f;  // of row ln
-  f32x16_t oacc[DT];  // O[ln][DT (8 (i / 4) + 4 lh + i % 4) + t] in oacc[t][i]
+  f32x16_t oacc[DT];  // O[ln][32 t + 8 (i / 4) + 4 lh + i % 4] in oacc[t][i]
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
   // Where a lane's operands stand in a tile, less what is the same for all lanes: of K product
-  // KS / 4 i's, of V the tokens' whose swizzles are alike.
-  constexpr int VA = D == 128 ? 4 : 2;
-  int ka[4], va[VA];
+  // KS / 4 i's, of V those of dims from 32 t on.
+  int ka[4], va[DT];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     ka[i] = ln / TPP<D> * PIECE + ln % TPP<D> * ROWB + 16 * (NCH / 4 * i ^ swizzle<D>(ln)) + 16 * lh;
 #pragma unroll
-  for (int i = 0; i < VA; ++i) {
-    const int tok = 4 * lh + 4 / VA * i, at = 4 * VW * ln;
-    va[i] = tok / TPP<D> * PIECE + tok % TPP<D> * ROWB + 16 * (at / 16 ^ swizzle<D>(tok)) + at % 16;
+  for (int t = 0; t < DT; ++t) {
+    const int tok = 4 * lh + lane % 16 / 4, chunk = 4 * t + ln / 16 * 2 + lane % 4 / 2;
+    va[t] = tok / TPP<D> * PIECE + tok % TPP<D> * ROWB + 16 * (chunk ^ swizzle<D>(tok)) + lane % 2 * 8;
   }
   auto k_of = [&](const char* kt, int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const uint4*>(kt + ka[i / (KS / 4)] + 32 * (i % (KS / 4)));
@@ -293,18 +306,14 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       sc = mfma32<F16>(k_of(kt, i), qf[i], sc);
     return sc;
   };
-  // V of half of them (product j), a lane's dims of token 16 j + 8 (e / 4) + 4 lh + e % 4 in v[e].
-  auto values = [&](const char* vt, int j, uint32_t (&v)[8][VW]) __attribute__((always_inline)) {
+  // V^T of half of them (product j): of dim 32 t + ln token 16 j + 8 (e / 4) + 4 lh + e % 4 as
+  // value e of v[t].
+  auto values = [&](const char* vt, int j, uint4 (&v)[DT]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const char* const p = vt + va[(e & 3) / (4 / VA)] + (e & (4 / VA - 1)) * ROWB +
-                            (16 * j + 8 * (e >> 2)) / TPP<D> * PIECE;
-      if constexpr (VW == 2) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        v[e][0] = w.x, v[e][VW - 1] = w.y;
-      } else {
-        v[e][0] = *reinterpret_cast<const uint32_t*>(p);
-      }
+    for (int t = 0; t < DT; ++t) {
+      const uint2 x = turned(vt + va[t] + 16 * j / TPP<D> * PIECE);
+      const uint2 y = turned(vt + va[t] + (16 * j + 8) / TPP<D> * PIECE);
+      v[t] = make_uint4(x.x, x.y, y.x, y.y);
     }
   };
   // V of a step that some row does not attend as a whole: a missing token's row is 0, and so is a
@@ -366,20 +375,17 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   // P V of a tile, and the next tile's scores (K at kn) with their maximum. In this order the
   // vector instructions stand between products that they do not depend on: the compiler would
   // put a tile's products one after another, and its arithmetic behind them.
-  auto add = [&](f32x16_t& sc, const char* vt, const char* kn, float& top)
+  constexpr int A = KS < 4 ? KS : 4;  // fragments of K ahead
+  auto add = [&](f32x16_t& sc, const char* vt, const char* kn, uint4 (&k)[KS], float& top)
                  __attribute__((always_inline)) {
-    constexpr int A = KS < 4 ? KS : 4, E = 16 / KS;  // fragments of K ahead, weights per product
-    uint4 k[KS];
-    uint32_t v[2][8][VW];
+    constexpr int E = 16 / KS;  // weights per product
+    uint4 v[2][DT];
     uint32_t p[8];
     f32x16_t next;
 #pragma unroll
     for (int i = 0; i < 16; ++i) next[i] = 0.f;
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    values(vt, 0, v[0]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       if constexpr (AHEAD) {
@@ -391,17 +397,14 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
         const float x = weight(sc[e]), y = weight(sc[e + 1]);
         p[e / 2] = pack_e2<F16>(x, y);
       }
-      if (i == KS - 2) values(vt, 0, v[0]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    uint4 vv = turn<VW>(v[0], 0);
     const uint4 p0 = make_uint4(p[0], p[1], p[2], p[3]), p1 = make_uint4(p[4], p[5], p[6], p[7]);
     values(vt, 1, v[1]);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < 2 * DT; ++t) {
-      oacc[t % DT] = mfma32<F16>(vv, t < DT ? p0 : p1, oacc[t % DT]);
-      if (t + 1 < 2 * DT) vv = turn<VW>(v[(t + 1) / DT], (t + 1) % DT);
+      oacc[t % DT] = mfma32<F16>(v[t / DT][t % DT], t < DT ? p0 : p1, oacc[t % DT]);
       if constexpr (AHEAD) {
         if (t >= DT) {
           constexpr int M = 16 / DT;
@@ -468,7 +471,16 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       if (row0 >= R) continue;
 #pragma unroll
       for (int q = 0; q < PT; ++q) {
-        if constexpr (!AHEAD) sc = scores(s, q), top = top_of(sc);
+        const int sn = s + (q + 1) / PT, qn = (q + 1) % PT;  // (behind the last tile: of nothing)
+        const char* const kn = lds + (sn % RING) * STEP_B + part * PART_B + qn * TILE_B;
+        uint4 k[KS];
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+          sc = scores(s, q), top = top_of(sc);
+        }
         if (masked) {
           const int at = PTOK * part + 32 * q;
           const uint32_t here = (uint32_t)__ballot(rows[s * STEP + at + ln] >= 0);
@@ -483,9 +495,7 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
           top = top_of(sc);
         }
         rescale(pair32_max(top) * sl2);
-        const int sn = s + (q + 1) / PT, qn = (q + 1) % PT;  // (behind the last tile: of nothing)
-        add(sc, lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B,
-            lds + (sn % RING) * STEP_B + part * PART_B + qn * TILE_B, top);
+        add(sc, lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B, kn, k, top);
       }
     }
   }
@@ -496,20 +506,17 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       const int64_t r = a.pages.row(b, k);
       if (r < 0) continue;
       const bool mine = (mask >> (k - c.context)) & 1;
-      const uint4* const d = reinterpret_cast<const uint4*>(
-          a.vc + (r + (int64_t)kvh * a.pages.block_size) * D);
+      const uint16_t* const d = a.vc + (r + (int64_t)kvh * a.pages.block_size) * D + 4 * lh;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int h = 0; h < VW; ++h) {  // eight dims of the 4 DT of this i
-          const uint4 x = d[VW * (2 * i + lh) + h];
-          const uint32_t w[4] = {inf_halves<F16>(x.x), inf_halves<F16>(x.y), inf_halves<F16>(x.z),
-                                 inf_halves<F16>(x.w)};
+        for (int i = 0; i < 4; ++i) {
+          const uint2 x = *reinterpret_cast<const uint2*>(d + 32 * t + 8 * i);
+          const uint32_t w[2] = {inf_halves<F16>(x.x), inf_halves<F16>(x.y)};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int t = (8 * h + e) % DT, n = 4 * i + (8 * h + e) / DT;
-            oacc[t][n] = mine && (e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu) ? NAN : oacc[t][n];
-          }
+          for (int e = 0; e < 4; ++e)
+            oacc[t][4 * i + e] = mine && (e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu)
+                                     ? NAN : oacc[t][4 * i + e];
         }
     }
   }
@@ -553,36 +560,31 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   if (row >= R) return;
   if (c.splits <= 1) {
     const float inv = node < c.nodes && l_run != 0.f ? 1.f / l_run : 0.f;
-    uint16_t* const o = a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * DT * lh;
+    uint16_t* const o = a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 8 * lh;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int h = 0; h < DT / 2; ++h) {  // eight neighbouring dims
+      for (int i = 0; i < 16; i += 8) {
+        // 4 dims of 8 each: the halves of the wave exchange them for 8 that are neighbours
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 8 * h + 2 * e;  // of the 4 DT dims of this i
-          const float x0 = oacc[d % DT][4 * i + d / DT];
-          const float x1 = oacc[(d + 1) % DT][4 * i + (d + 1) / DT];
-          w[e] = inv == 0.f ? 0u : pack_e2<F16>(x0 * inv, x1 * inv);
-        }
-        *reinterpret_cast<uint4*>(o + 8 * DT * i + 8 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < 4; ++e)
+          w[e] = inv == 0.f ? 0u
+                            : pack_e2<F16>(oacc[t][i + 2 * e] * inv, oacc[t][i + 2 * e + 1] * inv);
+        const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        *reinterpret_cast<uint4*>(o + 32 * t + 2 * i) = make_uint4(x[0], y[0], x[1], y[1]);
       }
     return;
   }
   const int64_t at = ((int64_t)pair * f.splits + split) * f.RP + row;
-  float* const o = f.ws_o + at * D + 4 * DT * lh;
+  float* const o = f.ws_o + at * D + 4 * lh;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int t = 0; t < DT; ++t)
 #pragma unroll
-    for (int h = 0; h < DT; ++h) {
-      float4 w;
-      w.x = oacc[(4 * h) % DT][4 * i + 4 * h / DT];
-      w.y = oacc[(4 * h + 1) % DT][4 * i + (4 * h + 1) / DT];
-      w.z = oacc[(4 * h + 2) % DT][4 * i + (4 * h + 2) / DT];
-      w.w = oacc[(4 * h + 3) % DT][4 * i + (4 * h + 3) / DT];
-      *reinterpret_cast<float4*>(o + 8 * DT * i + 4 * h) = w;
-    }
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<float4*>(o + 32 * t + 2 * i) =
+          make_float4(oacc[t][i], oacc[t][i + 1], oacc[t][i + 2], oacc[t][i + 3]);
   if (lh == 0) *reinterpret_cast<float2*>(f.ws_ml + 2 * at) = make_float2(m_run, l_run);
 }
 
