@@ -378,9 +378,17 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   constexpr int A = KS < 4 ? KS : 4;  // fragments of K ahead
   auto add = [&](f32x16_t& sc, const char* vt, const char* kn, uint4 (&k)[KS], float& top)
                  __attribute__((always_inline)) {
-    constexpr int E = 16 / KS;  // weights per product
+    constexpr int E = 10;  // weights between the scores' products; the others between V's first
     uint4 v[2][DT];
+    float x[16];
     uint32_t p[8];
+    auto weights = [&](int from, int to) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = from; i < to; ++i) {
+        x[i] = weight(sc[i]);
+        if (i & 1) p[i / 2] = pack_e2<F16>(x[i - 1], x[i]);
+      }
+    };
     f32x16_t next;
 #pragma unroll
     for (int i = 0; i < 16; ++i) next[i] = 0.f;
@@ -392,26 +400,25 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
         next = mfma32<F16>(k[i], qf[i], next);
         if (i + A < KS) k[i + A] = k_of(kn, i + A);
       }
-#pragma unroll
-      for (int e = E * i; e < E * (i + 1); e += 2) {
-        const float x = weight(sc[e]), y = weight(sc[e + 1]);
-        p[e / 2] = pack_e2<F16>(x, y);
-      }
+      weights(E * i / KS, E * (i + 1) / KS);
       __builtin_amdgcn_sched_barrier(0);
     }
-    const uint4 p0 = make_uint4(p[0], p[1], p[2], p[3]), p1 = make_uint4(p[4], p[5], p[6], p[7]);
     values(vt, 1, v[1]);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < 2 * DT; ++t) {
-      oacc[t % DT] = mfma32<F16>(v[t / DT][t % DT], t < DT ? p0 : p1, oacc[t % DT]);
+      oacc[t % DT] =
+          mfma32<F16>(v[t / DT][t % DT],
+                      t < DT ? make_uint4(p[0], p[1], p[2], p[3]) : make_uint4(p[4], p[5], p[6], p[7]),
+                      oacc[t % DT]);
+      if (t < DT) weights(E + (16 - E) * t / DT, E + (16 - E) * (t + 1) / DT);
       if constexpr (AHEAD) {
         if (t >= DT) {
           constexpr int M = 16 / DT;
 #pragma unroll
           for (int i = 0; i < M; ++i) {
-            const float x = next[M * (t - DT) + i];
-            top = t == DT && i == 0 ? x : fmaxf(top, x);
+            const float y = next[M * (t - DT) + i];
+            top = t == DT && i == 0 ? y : fmaxf(top, y);
           }
         }
       }
