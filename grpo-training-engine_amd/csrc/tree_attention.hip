@@ -611,23 +611,46 @@ __global__ void __launch_bounds__(JT) tree_attn_join_kernel(FastArgs f, int step
   const int64_t at = (int64_t)pair * f.splits * f.RP + row;
   const float2* const ml = reinterpret_cast<const float2*>(f.ws_ml) + at;
   const float4* const o = reinterpret_cast<const float4*>(f.ws_o) + at * L + l;
+  // A lane has every L-th split's weight, and four dims of all.
+  constexpr int N = MAX_SPLITS / L, AT_ONCE = 8;
+  float2 w[N];
   float m = -INFINITY;
-  for (int z = 0; z < c.splits; ++z) m = fmaxf(m, ml[(int64_t)z * f.RP].x);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int z = i * L + l;
+    w[i] = z < c.splits ? ml[(int64_t)z * f.RP] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, w[i].x);
+  }
+#pragma unroll
+  for (int x = L / 2; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
   const float m_use = m == -INFINITY ? 0.f : m;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-#pragma unroll 4
-  for (int z = 0; z < c.splits; ++z) {
-    const float2 w = ml[(int64_t)z * f.RP];
-    const float4 v = o[(int64_t)z * f.RP * L];
-    const float x = __builtin_amdgcn_exp2f(w.x - m_use);
-    sum += x * w.y;
-    acc.x += x * v.x, acc.y += x * v.y, acc.z += x * v.z, acc.w += x * v.w;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float mine = __builtin_amdgcn_exp2f(w[i].x - m_use);
+    sum += mine * w[i].y;
+#pragma unroll
+    for (int z0 = i * L; z0 < (i + 1) * L; z0 += AT_ONCE) {
+      if (z0 >= c.splits) break;
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int z = 0; z < AT_ONCE; ++z)
+        if (z0 + z < c.splits) v[z] = o[(int64_t)(z0 + z) * f.RP * L];
+#pragma unroll
+      for (int z = 0; z < AT_ONCE; ++z) {
+        if (z0 + z >= c.splits) break;
+        const float x = __shfl(mine, (threadIdx.x & 63 & ~(L - 1)) + z0 % L + z);
+        acc.x += x * v[z].x, acc.y += x * v[z].y, acc.z += x * v[z].z, acc.w += x * v[z].w;
+      }
+    }
   }
+#pragma unroll
+  for (int x = L / 2; x; x >>= 1) sum += __shfl_xor(sum, x);
   const float inv = node < c.nodes && sum != 0.f ? 1.f / sum : 0.f;
-  uint2 w = make_uint2(pack_e2<F16>(acc.x * inv, acc.y * inv), pack_e2<F16>(acc.z * inv, acc.w * inv));
-  if (inv == 0.f) w = make_uint2(0u, 0u);
-  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * l) = w;
+  uint2 y = make_uint2(pack_e2<F16>(acc.x * inv, acc.y * inv), pack_e2<F16>(acc.z * inv, acc.w * inv));
+  if (inv == 0.f) y = make_uint2(0u, 0u);
+  *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * l) = y;
 }
 
 struct Plan {
