@@ -38,65 +38,74 @@ _I32 = torch.int32
 
 
 def _check_cache(k_cache, v_cache, layered: bool):
-    """(layers, num_blocks, Hkv, block_size, D) of checked caches."""
-    shape = k_cache.shape
+    """(layers, num_blocks, Hkv, block_size, D), type and device of checked caches."""
+    shape, dtype, device = k_cache.shape, k_cache.dtype, k_cache.device
     if len(shape) != 4 and not (layered and len(shape) == 5):
         raise ValueError("k_cache/v_cache must be [num_blocks, heads, block, head_dim]"
                          + (" or [layers, ...]." if layered else "."))
     if v_cache.shape != shape:
         raise ValueError("k_cache and v_cache must have identical shapes.")
-    if k_cache.dtype not in _HALF or v_cache.dtype != k_cache.dtype:
+    if dtype not in _HALF or v_cache.dtype is not dtype:
         raise ValueError("k_cache/v_cache must be bfloat16 or float16, both the same.")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache/v_cache must be contiguous.")
-    if not k_cache.is_cuda or v_cache.device != k_cache.device:
+    if not k_cache.is_cuda or v_cache.get_device() != device.index:
         raise ValueError("k_cache/v_cache must be on the ROCm/HIP device, both on one.")
-    if 0 in shape:
+    if not k_cache.numel():
         raise ValueError("k_cache/v_cache must not be empty.")
-    return shape if len(shape) == 5 else (1, *shape)
+    return shape if len(shape) == 5 else (1, *shape), dtype, device
 
 
 def _check_ints(t: torch.Tensor, name: str, shape, device, dtype=_I32) -> None:
-    if t.dtype != dtype or t.device != device or t.shape != shape:
+    if t.dtype is not dtype or t.get_device() != device.index or t.shape != shape:
         raise ValueError(f"{name} must be {str(dtype)[6:]} {list(shape)} on {device}, got "
                          f"{str(t.dtype)[6:]} {list(t.shape)} on {t.device}.")
 
 
 def _check_tables(block_tables, context_lens, counts, b: int, device):
-    """(context_lens, counts, (address, row stride) of the tables, their width)."""
+    """(context_lens, address of counts or None, the tables, their row stride and width), and
+    counts, which has to live as long."""
     if block_tables.ndim != 2 or not block_tables.shape[1]:
         raise ValueError("block_tables must be [batch, max_blocks].")
-    _check_ints(block_tables, "block_tables", (b, block_tables.shape[1]), device)
+    width = block_tables.shape[1]
+    _check_ints(block_tables, "block_tables", (b, width), device)
     _check_ints(context_lens, "context_lens", (b,), device)
+    at = None
     if counts is not None:
         _check_ints(counts, "counts", (b,), device)
         counts = counts.contiguous()
-    if block_tables.stride(1) != 1 and block_tables.shape[1] > 1:
+        at = counts.data_ptr()
+    stride, step = block_tables.stride()
+    if step != 1 and width > 1:
         block_tables = block_tables.contiguous()
-    return context_lens.contiguous(), counts, block_tables
+        stride = width
+    return context_lens.contiguous(), at, block_tables, stride, width, counts
 
 
 def _rows(t: Optional[torch.Tensor], name: str, shape, device, dtype=_I32):
-    """``t`` [B, T] with contiguous rows (an expanded row stays one)."""
+    """``t`` [B, T] with contiguous rows (an expanded row stays one), its address and row
+    stride."""
     if t is None:
-        return None, 0
+        return None, None, 0
     _check_ints(t, name, shape, device, dtype)
     if t.stride(1) != 1 and shape[1] > 1:
         t = t.contiguous()
-    return t, t.stride(0)
+    return t, t.data_ptr(), t.stride(0)
 
 
-def _heads(t: torch.Tensor, name: str, shape, cache) -> torch.Tensor:
-    """``t`` [B, T, H, D] of the cache's type, its last dim contiguous."""
-    if t.ndim != 4 or t.shape[:2] != shape[:2] or t.shape[3] != shape[3] or \
-            (shape[2] and t.shape[2] != shape[2]):
-        want = [*shape[:2], shape[2] or "heads", shape[3]]
-        raise ValueError(f"{name} must be {want}, got {list(t.shape)}.")
-    if t.dtype != cache.dtype:
-        raise ValueError(f"{name} must be {cache.dtype} like the caches, got {t.dtype}.")
-    if t.device != cache.device:
-        raise ValueError(f"{name} must be on {cache.device}, got {t.device}.")
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+def _heads(t: torch.Tensor, name: str, shape, dtype, device):
+    """``t`` [B, T, H, D] of the cache's type, its last dim contiguous, and three strides."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}.")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype} like the caches, got {t.dtype}.")
+    if t.get_device() != device.index:
+        raise ValueError(f"{name} must be on {device}, got {t.device}.")
+    sb, st, sh, sd = t.stride()
+    if sd != 1 and shape[3] > 1:
+        t = t.contiguous()
+        sb, st, sh, _ = t.stride()
+    return t, sb, st, sh
 
 
 def _grouped(hq: int, hkv: int) -> None:
@@ -117,33 +126,32 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: to
     token ``i``: ``positions[b, i]`` (int32; clamped to the table), else ``context_lens[b] + i``.
     The rotation is float32, rounded once. Rows past ``counts[b]`` are not stored and their
     ``q`` is 0; slots past the block table, or in blocks outside the cache, are skipped."""
-    _, nb, hkv, bs, d = _check_cache(k_cache, v_cache, False)
+    (_, nb, hkv, bs, d), dtype, dev = _check_cache(k_cache, v_cache, False)
     if q.ndim != 4:
         raise ValueError(f"q must be [B, T, heads, {d}], got {list(q.shape)}.")
     b, t, hq, _ = q.shape
-    q = _heads(q, "q", (b, t, 0, d), k_cache)
-    k = _heads(k, "k", (b, t, hkv, d), k_cache)
-    v = _heads(v, "v", (b, t, hkv, d), k_cache)
+    q, qb, qt, qh = _heads(q, "q", (b, t, hq, d), dtype, dev)
+    k, kb, kt, kh = _heads(k, "k", (b, t, hkv, d), dtype, dev)
+    v, vb, vt, vh = _heads(v, "v", (b, t, hkv, d), dtype, dev)
     _grouped(hq, hkv)
-    dev = k_cache.device
     if d % 2:
         raise ValueError(f"head_dim must be even, got {d}.")
     if cos.ndim != 2 or cos.shape[1] != d or not cos.shape[0] or sin.shape != cos.shape:
         raise ValueError(f"cos/sin must be [max_pos, {d}], both the same.")
-    if cos.dtype not in (torch.float32, k_cache.dtype) or sin.dtype != cos.dtype:
+    wide = cos.dtype is torch.float32
+    if not (wide or cos.dtype is dtype) or sin.dtype is not cos.dtype:
         raise ValueError("cos/sin must be float32 or of q's type, both the same.")
-    if cos.device != dev or sin.device != dev:
+    if cos.get_device() != dev.index or sin.get_device() != dev.index:
         raise ValueError(f"cos/sin must be on {dev}.")
     cos, sin = cos.contiguous(), sin.contiguous()
-    lens, counts, tables = _check_tables(block_tables, context_lens, counts, b, dev)
-    positions, pos_stride = _rows(positions, "positions", (b, t), dev)
-    out = torch.empty((b, t, hq, d), dtype=q.dtype, device=dev)
-    _run(dev, "grpo_paged_rope_append", q.data_ptr(), *q.stride()[:3], k.data_ptr(),
-         *k.stride()[:3], v.data_ptr(), *v.stride()[:3], q.dtype == torch.float16, cos.data_ptr(),
-         sin.data_ptr(), cos.dtype == torch.float32, cos.shape[0], _lib.ptr(positions), pos_stride,
-         lens.data_ptr(), _lib.ptr(counts), out.data_ptr(), k_cache.data_ptr(),
-         v_cache.data_ptr(), nb, tables.data_ptr(), tables.stride(0), bs, tables.shape[1], b, t,
-         hq, hkv, d)
+    lens, n_at, tables, bt_stride, width, counts = _check_tables(block_tables, context_lens,
+                                                                 counts, b, dev)
+    positions, p_at, p_stride = _rows(positions, "positions", (b, t), dev)
+    out = q.new_empty((b, t, hq, d))
+    _run(dev, "grpo_paged_rope_append", q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh,
+         v.data_ptr(), vb, vt, vh, dtype is torch.float16, cos.data_ptr(), sin.data_ptr(), wide,
+         cos.shape[0], p_at, p_stride, lens.data_ptr(), n_at, out.data_ptr(), k_cache.data_ptr(),
+         v_cache.data_ptr(), nb, tables.data_ptr(), bt_stride, bs, width, b, t, hq, hkv, d)
     return out
 
 
@@ -170,26 +178,26 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     node ``i - 1`` being the parent of ``i``. ``scale``: 1 / sqrt(D) unless given. Nodes past
     ``counts[b]``, and nodes that attend nothing, get 0. Tokens that a node does not attend do
     not reach it, whatever stands in their slots."""
-    _, nb, hkv, bs, d = _check_cache(k_cache, v_cache, False)
+    (_, nb, hkv, bs, d), dtype, dev = _check_cache(k_cache, v_cache, False)
     if q.ndim != 4:
         raise ValueError(f"q must be [B, T, heads, {d}], got {list(q.shape)}.")
     b, t, hq, _ = q.shape
-    q = _heads(q, "q", (b, t, 0, d), k_cache)
+    q, qb, qt, qh = _heads(q, "q", (b, t, hq, d), dtype, dev)
     _grouped(hq, hkv)
     _check_nodes(t)
     if d > 512:
         raise ValueError(f"head_dim at most 512, got {d}.")
-    dev = k_cache.device
-    lens, counts, tables = _check_tables(block_tables, context_lens, counts, b, dev)
-    parents, p_stride = _rows(parents, "parents", (b, t), dev)
+    lens, n_at, tables, bt_stride, width, counts = _check_tables(block_tables, context_lens,
+                                                                 counts, b, dev)
+    parents, p_at, p_stride = _rows(parents, "parents", (b, t), dev)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    out = torch.empty((b, t, hq, d), dtype=q.dtype, device=dev)
+    out = q.new_empty((b, t, hq, d))
     nbytes = _attn_bytes(b, t, hq, hkv, d)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _run(dev, "grpo_paged_tree_attn", q.data_ptr(), *q.stride()[:3], q.dtype == torch.float16,
-         k_cache.data_ptr(), v_cache.data_ptr(), nb, tables.data_ptr(), tables.stride(0), bs,
-         tables.shape[1], lens.data_ptr(), _lib.ptr(parents), p_stride, _lib.ptr(counts), scale,
-         out.data_ptr(), b, t, hq, hkv, d, _lib.ptr(ws), nbytes)
+    _run(dev, "grpo_paged_tree_attn", q.data_ptr(), qb, qt, qh, dtype is torch.float16,
+         k_cache.data_ptr(), v_cache.data_ptr(), nb, tables.data_ptr(), bt_stride, bs, width,
+         lens.data_ptr(), p_at, p_stride, n_at, scale, out.data_ptr(), b, t, hq, hkv, d,
+         _lib.ptr(ws), nbytes)
     return out
 
 
@@ -211,26 +219,27 @@ def accept_draft_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, sampled
     path, the last of them pending; ``pad_token_id`` behind them), how many they are ``[B]``
     int32, and the accepted nodes ``[B, T]`` int32 (-1 behind them). What is drawn with
     ``sample_tokens`` has the model's own distribution, whatever was drafted."""
-    layers, nb, hkv, bs, d = _check_cache(k_cache, v_cache, True)
-    if draft_tokens.ndim != 2:
-        raise ValueError(f"draft_tokens must be [B, T], got {list(draft_tokens.shape)}.")
-    b, t = shape = draft_tokens.shape
+    (layers, nb, hkv, bs, d), _, dev = _check_cache(k_cache, v_cache, True)
+    shape = draft_tokens.shape
+    if len(shape) != 2:
+        raise ValueError(f"draft_tokens must be [B, T], got {list(shape)}.")
+    b, t = shape
     _check_nodes(t)
-    dev = k_cache.device
-    drafted, d_stride = _rows(draft_tokens, "draft_tokens", shape, dev, torch.int64)
-    sampled, s_stride = _rows(sampled, "sampled", shape, dev, torch.int64)
-    parents, p_stride = _rows(parents, "parents", shape, dev)
+    drafted, d_at, d_stride = _rows(draft_tokens, "draft_tokens", shape, dev, torch.int64)
+    sampled, s_at, s_stride = _rows(sampled, "sampled", shape, dev, torch.int64)
+    parents, p_at, p_stride = _rows(parents, "parents", shape, dev)
     if b > 65535:
         raise ValueError(f"at most 65535 sequences, got {b}.")
-    lens, counts, tables = _check_tables(block_tables, context_lens, counts, b, dev)
-    tokens = torch.empty(shape, dtype=torch.int64, device=dev)
-    path = torch.empty(shape, dtype=_I32, device=dev)
-    accepted = torch.empty(b, dtype=_I32, device=dev)
-    _run(dev, "grpo_draft_tree_accept", drafted.data_ptr(), d_stride, parents.data_ptr(), p_stride,
-         sampled.data_ptr(), s_stride, lens.data_ptr(), _lib.ptr(counts), k_cache.data_ptr(),
-         v_cache.data_ptr(), layers, nb, tables.data_ptr(), tables.stride(0), bs, tables.shape[1],
-         b, t, hkv, d, -1 if eos_token_id is None else int(eos_token_id), int(pad_token_id),
-         tokens.data_ptr(), accepted.data_ptr(), path.data_ptr())
+    lens, n_at, tables, bt_stride, width, counts = _check_tables(block_tables, context_lens,
+                                                                 counts, b, dev)
+    tokens = drafted.new_empty(shape)
+    path = lens.new_empty(shape)
+    accepted = lens.new_empty(b)
+    _run(dev, "grpo_draft_tree_accept", d_at, d_stride, p_at, p_stride, s_at, s_stride,
+         lens.data_ptr(), n_at, k_cache.data_ptr(), v_cache.data_ptr(), layers, nb,
+         tables.data_ptr(), bt_stride, bs, width, b, t, hkv, d,
+         -1 if eos_token_id is None else int(eos_token_id), int(pad_token_id), tokens.data_ptr(),
+         accepted.data_ptr(), path.data_ptr())
     return tokens, accepted, path
 
 
