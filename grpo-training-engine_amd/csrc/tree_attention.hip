@@ -6,6 +6,7 @@
 // A token that a node does not attend is not read for it: whatever stands there (NaN of a slot
 // never written, another branch) stays out. A node that attends nothing gets 0.
 #include <algorithm>
+#include <cmath>
 
 #include "lds_dma.hpp"
 #include "tree.hpp"
@@ -507,26 +508,6 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
     }
   }
   l_run = pair32_sum(l_run);
-  if (__builtin_expect(odd, 0)) {  // the rows that attend a value that is not finite are NaN there
-#pragma unroll 1
-    for (int k = max(begin, c.context); k < end; ++k) {
-      const int64_t r = a.pages.row(b, k);
-      if (r < 0) continue;
-      const bool mine = (mask >> (k - c.context)) & 1;
-      const uint16_t* const d = a.vc + (r + (int64_t)kvh * a.pages.block_size) * D + 4 * lh;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint2 x = *reinterpret_cast<const uint2*>(d + 32 * t + 8 * i);
-          const uint32_t w[2] = {inf_halves<F16>(x.x), inf_halves<F16>(x.y)};
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            oacc[t][4 * i + e] = mine && (e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xFFFFu)
-                                     ? NAN : oacc[t][4 * i + e];
-        }
-    }
-  }
 
   // The other parts' waves hand (max, sum, O) to the first part's: XCH values per lane.
   if constexpr (TW > 1) {
@@ -563,6 +544,25 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
         for (int i = 0; i < 16; ++i) oacc[t][i] += fp * w[64 * (2 + 16 * t + i)];
     }
     m_run = m;
+  }
+  if (__builtin_expect(odd, 0)) {  // the values that were taken out, for the rows that attend them
+#pragma unroll 1
+    for (int k = max(begin, c.context); k < end; ++k) {
+      const int64_t r = a.pages.row(b, k);
+      if (r < 0) continue;
+      const bool mine = (mask >> (k - c.context)) & 1;
+      const uint16_t* const d = a.vc + (r + (int64_t)kvh * a.pages.block_size) * D + 4 * lh;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint2 x = *reinterpret_cast<const uint2*>(d + 32 * t + 8 * i);
+          const uint32_t w[2] = {x.x & inf_halves<F16>(x.x), x.y & inf_halves<F16>(x.y)};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            oacc[t][4 * i + e] += mine ? e2f<F16>((uint16_t)(w[e / 2] >> (e & 1) * 16)) : 0.f;
+        }
+    }
   }
   if (row >= R) return;
   if (c.splits <= 1) {
@@ -717,6 +717,7 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
     return einval("bad attention dimensions");
   if (T > TREE_MAX) return einval("a drafted tree has at most 64 nodes");
   if (D > GD) return einval("head_dim at most 512");
+  if (!std::isfinite(scale)) return einval("the scale must be finite");
   if (Hq > 65535 || (int64_t)B * T >= (1ll << 31)) return einval("too many rows or heads");
   if (B == 0) return GRPO_OK;
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out)
@@ -741,7 +742,8 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
   hipStream_t st = as_stream(stream);
   if (fast_dim(D) && ((q_sb | q_st | q_sh) & 7) == 0 && aligned16(q) && aligned16(k_cache) &&
       aligned16(v_cache) && aligned16(out) && (int64_t)B * Hkv < 65536 &&
-      num_blocks * Hkv * block_size < (1ll << 31)) {
+      num_blocks * Hkv * block_size < (1ll << 31) &&
+      (int64_t)max_blocks * block_size <= (1ll << 31) - 2 * WIN) {
     const Plan p = plan_of(B, T, Hq, Hkv);
     const size_t need = p.values * (D + 2) * sizeof(float);
     if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {

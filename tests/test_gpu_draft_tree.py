@@ -252,6 +252,60 @@ def test_tree_attention_without_blocks(dev):
     assert (out[1] == 0).all() and (out[2] == 0).all()
 
 
+@pytest.mark.parametrize("t,hq,hkv,d", [(2, 12, 2, 128), (8, 12, 2, 128), (20, 12, 2, 128),
+                                        (64, 7, 1, 128), (3, 4, 2, 64), (33, 14, 2, 64)])
+@pytest.mark.parametrize("block", [16, 5])
+def test_tree_attention_over_long_tables_with_holes(dev, t, hq, hkv, d, block):
+    """Missing blocks in every part of a long table, and slots that hold NaN beside them."""
+    args = attend_inputs(2, t, hq, hkv, d, block, "bf16", [9001, 4500], "random", None, seed=5)
+    kc, vc, tables, lens = args[1:5]
+    gone = torch.rand(tables.shape, generator=torch.Generator().manual_seed(t)) < 0.01
+    gone[:, 3] = True
+    gone[1, 4500 // block:] = False
+    for x in (kc, vc):
+        x[tables[gone].long()] = float("nan")
+        blk = tables[1, (4500 + t) // block]  # what stands behind the last node
+        x[blk, :, (4500 + t) % block:] = float("nan")
+    tables[gone] = -1
+    check_attention(attend(dev, *args), *args)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("t,hq,hkv,d", [(20, 12, 2, 128), (64, 8, 1, 128), (7, 4, 2, 64),
+                                        (5, 2, 1, 80)])
+def test_infinite_values_arrive_as_such(dev, dtype, t, hq, hkv, d):
+    """An infinite value of an attended node makes that dim infinite, of its sign, and no other
+    dim; two of opposite signs make it NaN."""
+    q, kc, vc, tables, lens, parents, _ = attend_inputs(2, t, hq, hkv, d, 16, dtype, [50, 111],
+                                                        "random", None, seed=6)
+    parents[0, 3] = 1
+    parents[0, 4] = 3
+
+    def put(slot, dim, x):
+        blk, off = ref.slot_of(tables[0].tolist(), slot, 16, kc.shape[0])
+        vc[blk, :, off, dim] = x
+
+    first = attend(dev, q, kc, vc, tables, lens, parents).cpu()
+    put(50 + 1, 3, float("inf"))
+    put(50 + 1, 4, -float("inf"))
+    put(50 + 1, 5, float("nan"))
+    put(50 + 1, 6, float("inf"))
+    put(50 + 3, 6, -float("inf"))
+    put(20, 9, float("inf"))
+    out = attend(dev, q, kc, vc, tables, lens, parents).cpu()
+    sees = torch.from_numpy(ref.sees(parents[0].numpy(), t))
+    one, both = sees[:, 1], sees[:, 1] & sees[:, 3]
+    assert one.any() and not one.all() and both.any()
+    inf = float("inf")
+    assert (out[0, one, :, 3] == inf).all() and (out[0, one, :, 4] == -inf).all()
+    assert out[0, one, :, 5].isnan().all() and out[0, both, :, 6].isnan().all()
+    assert (out[0, one & ~both, :, 6] == inf).all() and (out[0, :, :, 9] == inf).all()
+    for dim in (3, 4, 5):
+        assert torch.equal(out[0, ~one, :, dim], first[0, ~one, :, dim])
+    same = [i for i in range(d) if i not in (3, 4, 5, 6, 9)]
+    assert torch.equal(out[..., same], first[..., same])
+
+
 def test_tree_attention_takes_odd_parents(dev):
     """A parent that is no earlier node is none; one tree may serve all sequences."""
     q, kc, vc, tables, lens, _, _ = attend_inputs(2, 6, 4, 2, 128, 16, "bf16", [40, 7], "chain",
@@ -595,6 +649,10 @@ def test_refusals(dev):
         call(kernels.accept_draft_tree, draft_tokens=ids, sampled=ids)
     with pytest.raises(ValueError, match="multiple"):
         call(kernels.paged_tree_attention, q=base["q"][:, :, :3])
+    for scale in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="finite"):
+            kernels.paged_tree_attention(*(base[n] for n in uses[kernels.paged_tree_attention][0]
+                                           .split()), scale=scale)
     with pytest.raises(ValueError, match="512"):
         c = torch.zeros(2, 1, 16, 514, dtype=torch.bfloat16, device=dev)
         kernels.paged_tree_attention(torch.zeros(2, 4, 1, 514, dtype=c.dtype, device=dev), c, c,
