@@ -106,23 +106,34 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 // ------------------------------------------------------------ MFMA kernel --
 // The T (Hq / Hkv) rows (node, head of the group) of one KV head are the columns of 32x32x16
 // MFMAs, so that K and V are read once for all of them:
-//  * A wave owns 32 rows; a workgroup RW waves side by side on rows times TW on tokens, which
-//    take the 32-token parts of each step and meet in LDS at the end. A sequence's tokens are
-//    cut over workgroups where there are few of them (a second kernel joins the parts).
-//  * K and V of a step come to LDS by loads of their own, RING - 1 steps ahead. The cache rows of
-//    WIN tokens stand in LDS too.
+//  * A wave owns 32 rows. A workgroup has RW waves side by side on rows times 8 / RW on tokens,
+//    which take the 32-token parts of each step and meet in LDS at the end. A sequence's tokens
+//    are cut over workgroups, one per CU, where there are few of them (a second kernel joins the
+//    parts).
+//  * K and V of a step come to LDS by loads of their own, RING - 1 steps ahead (96 KiB on their
+//    way per CU). The cache rows of WIN tokens stand in LDS too.
 //  * S^T = K Q^T leaves lane (row ln, half lh) with 16 of 32 tokens' scores of its row, which
 //    are the operand P^T of O^T = V^T P^T if its contraction index (lh, e) of product j means
 //    token 16 j + 8 (e / 4) + 4 lh + e % 4: P never leaves the lane. V is turned as it is read
 //    from LDS.
+//  * The scores of the next tile are made between the weights of this one: on a SIMD a product
+//    takes 32 cycles, an exponential 16, another instruction 4, side by side.
 //  * P is rounded to 16 bits (2^-8 of each weight in bf16, 2^-11 in float16), the sum is of the
 //    float32 weights: the roundings are independent, so over many tokens they stay below the
 //    rounding of the result.
 //  * Steps that reach past the cached tokens, or a window that holds a missing block, have V
 //    cleaned in LDS first and the scores masked: the same loop adds them, so that O stays in one
 //    set of registers.
+// Measured at 28 and 4 heads of 128 dims, blocks of 16, contexts of half to one and a half times
+// the mean: 64 trees of 4 nodes over 2500 tokens 79 us (4.2 TB/s: the reading of the cache), 64
+// of 32 120 us (361 MB, 74 GFLOP), one of 61 over 30 thousand 51 us. With many rows the two waves
+// of a SIMD take 1.9 thousand cycles for a tile each, of which 1024 are products, and the longest
+// sequence ends last: 64 of 32 take 105 us without any reading of the cache. (Equal shares of all
+// tokens for every workgroup instead, of up to three sequences each: 164 against 146 us, the
+// parts' sums are 60 MB.)
 
 constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
+constexpr int RING = 4;          // steps of K and V that stand there
 constexpr int MAX_SPLITS = 64;
 constexpr int LEAST_CHUNK = 128; // tokens of a split at least
 
@@ -174,8 +185,8 @@ __device__ __forceinline__ uint32_t inf_halves(uint32_t d) {
   return ((d & X) == X ? 0xFFFFu : 0u) | ((d & (X << 16)) == X << 16 ? 0xFFFF0000u : 0u);
 }
 
-// Four 16-bit values per lane, turned: of 16 lanes' rows 0 to 3, which lanes 4 r to 4 r + 3 name with
-// an address for four values each, lane n gets value n of each.
+// Four 16-bit values per lane, turned: of 16 lanes' rows 0 to 3, which lanes 4 r to 4 r + 3 name
+// with an address for four values each, lane n gets value n of each.
 __device__ __forceinline__ uint2 turned(const char* p) {
   typedef short s16x4_t __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -194,17 +205,18 @@ __device__ __forceinline__ int swizzle(int token) {
   return D == 128 ? (token & 3) * 4 : token & 6;
 }
 
-// Steps in LDS at a time, of 32 PT TW tokens.
-template <int D, int TW, int PT>
-constexpr int RING_OF = D * TW * PT <= 256 ? 4 : 2;
+// Of a step's tokens a wave has one tile of 32 or two.
+template <int RW>
+constexpr int TILES = RW == 8 ? 2 : 1;
+template <int RW>
+constexpr int step_of() { return 32 * TILES<RW> * (8 / RW); }
 
-template <bool F16, int D, int RW, int TW, int PT>
-__global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
-  constexpr int W = RW * TW, PTOK = 32 * PT, STEP = PTOK * TW, RING = RING_OF<D, TW, PT>;
+template <bool F16, int D, int RW>
+__global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
+  constexpr int W = 8, TW = W / RW, PT = TILES<RW>, PTOK = 32 * PT, STEP = step_of<RW>();
   constexpr int ROWB = 2 * D, NCH = D / 8;            // bytes and 16-byte chunks of a row
   constexpr int TILE_B = TILE<D>, HALF_B = PT * TILE_B;
   constexpr int PART_B = 2 * HALF_B, STEP_B = TW * PART_B;
-  constexpr int AHEAD = RING > 2;  // the next tile's scores are made while this one is added
   constexpr int PPK = PTOK / TPP<D>;                  // pieces of K
   constexpr int PIECES = 2 * PPK * TW, LD = PIECES / W;
   static_assert(PIECES % W == 0, "every wave loads as many pieces");
@@ -287,11 +299,13 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
   int ka[4], va[DT];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    ka[i] = ln / TPP<D> * PIECE + ln % TPP<D> * ROWB + 16 * (NCH / 4 * i ^ swizzle<D>(ln)) + 16 * lh;
+    ka[i] = ln / TPP<D> * PIECE + ln % TPP<D> * ROWB +
+            16 * ((NCH / 4 * i ^ swizzle<D>(ln)) + lh);
 #pragma unroll
   for (int t = 0; t < DT; ++t) {
     const int tok = 4 * lh + lane % 16 / 4, chunk = 4 * t + ln / 16 * 2 + lane % 4 / 2;
-    va[t] = tok / TPP<D> * PIECE + tok % TPP<D> * ROWB + 16 * (chunk ^ swizzle<D>(tok)) + lane % 2 * 8;
+    va[t] = tok / TPP<D> * PIECE + tok % TPP<D> * ROWB + 16 * (chunk ^ swizzle<D>(tok)) +
+            lane % 2 * 8;
   }
   auto k_of = [&](const char* kt, int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const uint4*>(kt + ka[i / (KS / 4)] + 32 * (i % (KS / 4)));
@@ -303,8 +317,7 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) sc[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
-      sc = mfma32<F16>(k_of(kt, i), qf[i], sc);
+    for (int i = 0; i < KS; ++i) sc = mfma32<F16>(k_of(kt, i), qf[i], sc);
     return sc;
   };
   // V^T of half of them (product j): of dim 32 t + ln token 16 j + 8 (e / 4) + 4 lh + e % 4 as
@@ -397,10 +410,8 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      if constexpr (AHEAD) {
-        next = mfma32<F16>(k[i], qf[i], next);
-        if (i + A < KS) k[i + A] = k_of(kn, i + A);
-      }
+      next = mfma32<F16>(k[i], qf[i], next);
+      if (i + A < KS) k[i + A] = k_of(kn, i + A);
       weights(E * i / KS, E * (i + 1) / KS);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -408,24 +419,21 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < 2 * DT; ++t) {
-      oacc[t % DT] =
-          mfma32<F16>(v[t / DT][t % DT],
-                      t < DT ? make_uint4(p[0], p[1], p[2], p[3]) : make_uint4(p[4], p[5], p[6], p[7]),
-                      oacc[t % DT]);
+      const int j = t / DT * 4;
+      oacc[t % DT] = mfma32<F16>(v[t / DT][t % DT], make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]),
+                                 oacc[t % DT]);
       if (t < DT) weights(E + (16 - E) * t / DT, E + (16 - E) * (t + 1) / DT);
-      if constexpr (AHEAD) {
-        if (t >= DT) {
-          constexpr int M = 16 / DT;
+      if (t >= DT) {
+        constexpr int M = 16 / DT;
 #pragma unroll
-          for (int i = 0; i < M; ++i) {
-            const float y = next[M * (t - DT) + i];
-            top = t == DT && i == 0 ? y : fmaxf(top, y);
-          }
+        for (int i = 0; i < M; ++i) {
+          const float y = next[M * (t - DT) + i];
+          top = t == DT && i == 0 ? y : fmaxf(top, y);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (AHEAD) sc = next;
+    sc = next;
   };
   for (int w0 = begin; w0 < end; w0 += WIN) {
     const int wend = min(end, w0 + WIN), nstep = (wend - w0 + STEP - 1) / STEP;
@@ -453,20 +461,18 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
       if (s < nstep) fetch(s);
     f32x16_t sc;  // of the tile at hand, and each lane's maximum of them
     float top;
-    if constexpr (AHEAD) {
-      if (nstep >= RING - 1)
-        wait_vm<(RING - 2) * LD>();  // step 0 has landed
-      else
-        wait_vm<0>();
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      sc = scores(0, 0);
-      top = top_of(sc);
-    }
+    if (nstep >= RING - 1)
+      wait_vm<(RING - 2) * LD>();  // step 0 has landed
+    else
+      wait_vm<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    sc = scores(0, 0);
+    top = top_of(sc);
 #pragma unroll 1
     for (int s = 0; s < nstep; ++s) {
       if (nstep - 1 - s >= RING - 2)
-        wait_vm<(RING - 2 - AHEAD) * LD>();  // step s (s + 1) has landed
+        wait_vm<(RING - 3) * LD>();  // step s + 1 has landed
       else
         wait_vm<0>();
       __builtin_amdgcn_s_barrier();
@@ -482,21 +488,16 @@ __global__ void __launch_bounds__(64 * RW * TW) tree_attn_kernel(FastArgs f) {
         const int sn = s + (q + 1) / PT, qn = (q + 1) % PT;  // (behind the last tile: of nothing)
         const char* const kn = lds + (sn % RING) * STEP_B + part * PART_B + qn * TILE_B;
         uint4 k[KS];
-        if constexpr (AHEAD) {
 #pragma unroll
-          for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
-          __builtin_amdgcn_sched_barrier(0);
-        } else {
-          sc = scores(s, q), top = top_of(sc);
-        }
+        for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
+        __builtin_amdgcn_sched_barrier(0);
         if (masked) {
           const int at = PTOK * part + 32 * q;
           const uint32_t here = (uint32_t)__ballot(rows[s * STEP + at + ln] >= 0);
           // of the tile's tokens from `past` on not every row attends each
           const int past = max(c.context - t0 - at, 0);
-          const uint32_t on = here & (past >= 32 ? ~0u
-                                      : past     ? (uint32_t)(mask << past) | ((1u << past) - 1)
-                                                 : (uint32_t)(mask >> min(t0 + at - c.context, 63)));
+          const uint64_t tree = past ? mask << min(past, 63) : mask >> min(t0 + at - c.context, 63);
+          const uint32_t on = here & (past >= 32 ? ~0u : (uint32_t)tree | ((1u << past) - 1));
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             sc[i] = on >> (4 * lh) >> (8 * (i >> 2) + (i & 3)) & 1 ? sc[i] : -INFINITY;
@@ -648,21 +649,24 @@ __global__ void __launch_bounds__(JT) tree_attn_join_kernel(FastArgs f, int step
 #pragma unroll
   for (int x = L / 2; x; x >>= 1) sum += __shfl_xor(sum, x);
   const float inv = node < c.nodes && sum != 0.f ? 1.f / sum : 0.f;
-  uint2 y = make_uint2(pack_e2<F16>(acc.x * inv, acc.y * inv), pack_e2<F16>(acc.z * inv, acc.w * inv));
+  uint2 y =
+      make_uint2(pack_e2<F16>(acc.x * inv, acc.y * inv), pack_e2<F16>(acc.z * inv, acc.w * inv));
   if (inv == 0.f) y = make_uint2(0u, 0u);
   *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.T + node) * a.Hq + head) * D + 4 * l) = y;
 }
 
 struct Plan {
-  int rw, tw;      // waves side by side on rows, on tokens
+  int rw;          // waves side by side on rows; 8 / rw on tokens
   int rb, splits;  // blocks of 32 rw rows, parts of a sequence's tokens
   size_t values;   // rows of the workspace
 };
-Plan plan_of(int B, int T, int Hq, int Hkv) {
+Plan plan_of(int B, int T, int Hq, int Hkv, int D) {
   const int R = T * (Hq / Hkv);
   Plan p;
-  p.rw = R <= 32 ? 1 : (R <= 64 ? 2 : (R <= 128 ? 4 : 8));
-  p.tw = std::min(8 / p.rw, 4);
+  // The fewest waves on rows that hold them, of 4 and 8: 64 trees over 2500 tokens, 28 rows, 79
+  // us with 4 and 81 with 8, 112 rows 85 and 88; of 2 where a token is 128 bytes: 28 rows of 64
+  // dims 26 us with 2, 32 with 4 and 34 with 8, 56 rows 28, 33 and 37 (of 128 dims 81, 81, 83).
+  p.rw = R <= 64 && D == 64 ? 2 : (R <= 128 ? 4 : 8);
   p.rb = (int)cdiv(R, 32 * p.rw);
   const int64_t groups = (int64_t)B * Hkv * p.rb;
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS, 256 / groups));
@@ -671,36 +675,35 @@ Plan plan_of(int B, int T, int Hq, int Hkv) {
 }
 bool fast_dim(int D) { return D == 64 || D == 128; }
 
-template <bool F16, int D, int RW, int TW, int PT>
+template <bool F16, int D, int RW>
 int go(const FastArgs& a, const Plan& p, hipStream_t st) {
-  constexpr int LDS = RING_OF<D, TW, PT> * TW * PT * 2 * TILE<D> + WIN * 4;
-  constexpr auto kern = tree_attn_kernel<F16, D, RW, TW, PT>;
+  constexpr int LDS = RING * step_of<RW>() / 32 * 2 * TILE<D> + WIN * 4;
+  constexpr auto kern = tree_attn_kernel<F16, D, RW>;
   if (int rc = allow_dynamic_lds<kern, LDS>()) return rc;
   // Blocks of rows that read the same tokens run on one XCD: their ids are equal modulo 8.
   int64_t x = (int64_t)a.t.B * a.t.pages.Hkv * p.splits;
   if (p.rb > 1) x = cdiv(x, 8) * 8;
-  kern<<<dim3((unsigned)x, (unsigned)p.rb), 64 * RW * TW, LDS, st>>>(a);
+  kern<<<dim3((unsigned)x, (unsigned)p.rb), 512, LDS, st>>>(a);
   if (p.splits > 1) {
     const int R = a.t.T * (a.t.Hq / a.t.pages.Hkv);
     tree_attn_join_kernel<F16, D><<<dim3((unsigned)cdiv(R, JT / (D / 4)),
                                          (unsigned)(a.t.B * a.t.pages.Hkv)), JT, 0, st>>>(
-        a, 32 * PT * TW);
+        a, step_of<RW>());
   }
   return launch_check("paged_tree_attn");
 }
 template <bool F16, int D>
 int go_form(const FastArgs& a, const Plan& p, hipStream_t st) {
-  return p.rw == 1   ? go<F16, D, 1, 4, 1>(a, p, st)
-         : p.rw == 2 ? go<F16, D, 2, 4, 1>(a, p, st)
-         : p.rw == 4 ? go<F16, D, 4, 2, 1>(a, p, st)
-                     : go<F16, D, 8, 1, 2>(a, p, st);
+  if constexpr (D == 64)
+    if (p.rw == 2) return go<F16, D, 2>(a, p, st);
+  return p.rw == 4 ? go<F16, D, 4>(a, p, st) : go<F16, D, 8>(a, p, st);
 }
 
 }  // namespace
 
 extern "C" size_t grpo_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D) {
   if (B < 1 || T < 1 || T > TREE_MAX || Hkv < 1 || Hq < 1 || Hq % Hkv || !fast_dim(D)) return 0;
-  return plan_of(B, T, Hq, Hkv).values * (D + 2) * sizeof(float);
+  return plan_of(B, T, Hq, Hkv, D).values * (D + 2) * sizeof(float);
 }
 
 extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
@@ -744,7 +747,7 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
       aligned16(v_cache) && aligned16(out) && (int64_t)B * Hkv < 65536 &&
       num_blocks * Hkv * block_size < (1ll << 31) &&
       (int64_t)max_blocks * block_size <= (1ll << 31) - 2 * WIN) {
-    const Plan p = plan_of(B, T, Hq, Hkv);
+    const Plan p = plan_of(B, T, Hq, Hkv, D);
     const size_t need = p.values * (D + 2) * sizeof(float);
     if (need && (!workspace || !aligned16(workspace) || workspace_bytes < need)) {
       set_error("tree attention workspace: %zu bytes, 16-byte aligned", need);
