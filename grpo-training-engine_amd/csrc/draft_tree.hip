@@ -156,8 +156,7 @@ struct AcceptArgs {
 // takes at most T steps and the node at depth j moves from a slot >= j: its new slot has been
 // read before it is written, in one thread's program order. A thread moves N values of one
 // (layer, K or V, head). 8 trees of 7 nodes, 28 layers of 2 heads of 128: 4.2 us; 64 of 61 with 4
-// heads 8.8 us (20 MB moved), of which the lengths, the tree and the tables, one after another, are
-// 3.
+// heads 8.8 us (20 MB moved).
 template <int N>
 __global__ void __launch_bounds__(RT) tree_accept_kernel(AcceptArgs a) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
