@@ -370,7 +370,9 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
   block_excl_scan(pm, pc, s.s.s64, s.s.s32);
   const uint64_t all = block_sum<TT / 64>(tm, s.s.s64);
 
-  int listed = -1, last = -1;  // bins: whose tokens stand in the list, that held the last place
+  // The list holds the tokens of bins list0 to list1: of all down to a search's bin, if they are
+  // that few (the searches that follow end in or before it), else of that bin alone.
+  int list0 = 0, list1 = -1, last = -1;  // last: the bin that held the last place
   auto search = [&](uint64_t P, uint32_t K) {
     if (P > all) P = all;
     if (!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K)) {
@@ -387,26 +389,42 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
     __syncthreads();
     const Found top = s.s.found;
     const int bin = last = top.bin;
-    if (wave < 2) {  // the bin's keys: below the first one of the bin before
-      const uint32_t k = bin >= wave ? first_key<DT>(sc, kmax, bin - wave) : kmax + 1;
-      if ((tid & 63) == 0) s.s.range[wave] = k - wave;
+    const bool all_before = top.before + top.group <= LIST;
+    bool list = bin >= list0 && bin <= list1;
+    if (list) {  // the bin's keys
+      if (tid < 2) s.s.range[tid] = tid ? 0u : 0xFFFFFFFFu;
+      __syncthreads();
+      for (uint32_t i = tid; i < min(s.s.n_list, (uint32_t)LIST); i += TT) {
+        const uint32_t k = s.lkey[i];
+        if ((int)bin_place(sc.below(key_value<DT>(k))) != bin) continue;
+        atomicMin(&s.s.range[0], k);
+        atomicMax(&s.s.range[1], k);
+      }
+    } else {
+      if (wave < 2) {  // they are below the first one of the bin before
+        const uint32_t k = bin >= wave ? first_key<DT>(sc, kmax, bin - wave) : kmax + 1;
+        if ((tid & 63) == 0) s.s.range[wave] = k - wave;
+      }
+      if (tid == 0) s.s.n_list = 0;
+      list0 = all_before ? 0 : bin;
+      list1 = top.group <= LIST ? bin : -1;
     }
-    if (tid == 0 && listed != bin) s.s.n_list = 0;
     __syncthreads();
     uint32_t lo = s.s.range[0], hi = s.s.range[1];
-    const bool list = top.group <= LIST;
-    if (list && listed != bin) {
-      const float xlo = key_value<DT>(lo), xhi = key_value<DT>(hi);
+    if (!list && top.group <= LIST) {
+      // (the last bin begins at a key of NaN)
+      const float xlo = fmaxf(key_value<DT>(lo), -__FLT_MAX__);
+      const float xhi = all_before ? INFINITY : key_value<DT>(hi);
       for_row<DT, TT>(row, V, [&](int i, float x) {
         if (!(x >= xlo && x <= xhi)) return;
         const uint32_t at = atomicAdd(&s.s.n_list, 1u);
-        if (at >= LIST) return;  // (never: the bin holds as many)
+        if (at >= LIST) return;  // (never: the bins hold as many)
         s.lkey[at] = key_of<DT>(x);
         s.lidx[at] = i;
       });
-      listed = bin;
+      list = true;
+      __syncthreads();
     }
-    __syncthreads();
     const uint32_t n = min(s.s.n_list, (uint32_t)LIST);
     // weights relative to the bin's start: 2^44 of it at most
     auto rel = [&](uint32_t k) {
@@ -463,6 +481,13 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
       hi -= q << sh;
       if (hi - lo > width) lo = hi - width;
       __syncthreads();
+      if (list && group == 1 && lo < hi) {  // the token itself
+#pragma unroll 1
+        for (uint32_t i = tid; i < n; i += TT)
+          if (s.lkey[i] >= lo && s.lkey[i] <= hi) s.s.range[0] = s.lkey[i];
+        __syncthreads();
+        lo = hi = s.s.range[0];
+      }
     }
     const uint64_t w = rel(hi);
     if (first) {  // the bin is one value
@@ -489,7 +514,7 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
   const int seg = max(0, 32 - __clz(V - 1) - KEY_BITS);
   s.kcnt[tid] = 0;
   __syncthreads();
-  if (listed == last) {
+  if (last >= list0 && last <= list1) {
 #pragma unroll 1
     for (uint32_t i = tid; i < min(s.s.n_list, (uint32_t)LIST); i += TT)
       if (s.lkey[i] == d.key) atomicAdd(&s.kcnt[s.lidx[i] >> seg], 1u);
