@@ -212,7 +212,7 @@ __device__ __forceinline__ Leaf draw_of(const Row& r, uint32_t valid, uint32_t n
                        : r.p < 1.0  ? share_of(r.p, mass)
                                     : 0;
     if (stage == 1 && !P && K >= valid) continue;
-    l = search(P, stage == 0 ? r.K : stage == 1 ? K : kept);
+    l = search(P, stage == 0 ? r.K : stage == 1 ? K : kept, stage < 2);
     mass = l.total;
     if (stage == 1) kept = l.before + l.in;
   }
@@ -285,6 +285,7 @@ __device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kma
 // relative to the bin's first, and P is a share of the bin's mass.
 constexpr int NB = 4096;
 constexpr int LIST = 4096;     // tokens of one bin that LDS holds
+constexpr int ALL = 1024;      // of all bins down to one (512 to 4096: no difference)
 constexpr double A64 = 0.010830424696249145;  // ln(2) / 64
 
 template <int TT>
@@ -371,9 +372,9 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
   const uint64_t all = block_sum<TT / 64>(tm, s.s.s64);
 
   // The list holds the tokens of bins list0 to list1: of all down to a search's bin, if they are
-  // that few (the searches that follow end in or before it), else of that bin alone.
+  // few and searches follow (which end in or before it), else of that bin alone.
   int list0 = 0, list1 = -1, last = -1;  // last: the bin that held the last place
-  auto search = [&](uint64_t P, uint32_t K) {
+  auto search = [&](uint64_t P, uint32_t K, bool more) {
     if (P > all) P = all;
     if (!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K)) {
       uint64_t mj = pm;
@@ -389,7 +390,7 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
     __syncthreads();
     const Found top = s.s.found;
     const int bin = last = top.bin;
-    const bool all_before = top.before + top.group <= LIST;
+    const bool all_before = more && top.before + top.group <= ALL;
     bool list = bin >= list0 && bin <= list1;
     if (list) {  // the bin's keys
       if (tid < 2) s.s.range[tid] = tid ? 0u : 0xFFFFFFFFu;
@@ -807,7 +808,7 @@ __device__ __forceinline__ bool count_row(const TokArgs& a, int m, const Groups<
   const uint64_t all = s.s.found.own;
   const uint32_t counted = s.s.found.before;
 
-  auto search = [&](uint64_t P, uint32_t K) {
+  auto search = [&](uint64_t P, uint32_t K, bool) {
     if (!P && K > counted) return Leaf{0u, K - 1, 1u, all};  // among those without mass
     const uint64_t here = __ballot(!reached(pm, pc, P, K) && reached(pm + tm, pc + tc, P, K));
     if (here) {  // this wave has the group: its bins, one per lane
