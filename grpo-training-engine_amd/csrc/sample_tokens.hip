@@ -194,8 +194,9 @@ struct Leaf {
   uint64_t total;
 };
 
-// The cuts and the draw, from a search(P, K) for the first place where the mass reaches P (0: no
-// such bound) or the count K; `near` tokens pass min_p, `all` is the row's mass.
+// The cuts and the draw, from a search(P, K, more) for the first place where the mass reaches P
+// (0: no such bound) or the count K (more: others follow); `near` tokens pass min_p, `all` is the
+// row's mass.
 template <typename Search>
 __device__ __forceinline__ Leaf draw_of(const Row& r, uint32_t valid, uint32_t near, uint64_t all,
                                         uint32_t& kept, Search&& search) {
@@ -429,13 +430,14 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
     const uint32_t n = min(s.s.n_list, (uint32_t)LIST);
     // weights relative to the bin's start: 2^44 of it at most
     auto rel = [&](uint32_t k) {
-      return nearest(
-          exp2_neg(fmin(fmax(sc.below(key_value<DT>(k)) - bin * (1.0 / 64), 0.0), 1000.0), a.shift));
+      const double y = sc.below(key_value<DT>(k)) - bin * (1.0 / 64);
+      return nearest(exp2_neg(fmin(fmax(y, 0.0), 1000.0), a.shift));
     };
     // P among those, if it lies in this bin; a bin whose tokens have no mass of their own: all
     auto share = [&](uint64_t sum) -> uint64_t {
       if (!P || P > top.mass + top.own) return 0;
-      const double x = top.own ? (double)(P - top.mass) / (double)top.own * (double)sum : (double)sum;
+      const double x =
+          top.own ? (double)(P - top.mass) / (double)top.own * (double)sum : (double)sum;
       return min(max((uint64_t)ceil(x), (uint64_t)1), max(sum, (uint64_t)1));
     };
     uint64_t Q = 0, mb = 0, sum = 0;  // P in those, before the range, of the whole bin
@@ -732,7 +734,7 @@ __device__ __forceinline__ void pick_bits(const TokArgs& a, const Groups<TT>& x,
     const uint32_t p[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      bits |= (uint32_t)is((uint16_t)p[i]) << (2 * i) | (uint32_t)is((uint16_t)(p[i] >> 16)) << (2 * i + 1);
+      bits |= ((uint32_t)is((uint16_t)p[i]) | (uint32_t)is((uint16_t)(p[i] >> 16)) << 1) << 2 * i;
     const uint32_t n = finish(x.head + 8 * (g + 64 * u), g + 64 * u < x.G ? bits : 0u);
     if (left < n) return;
     left -= n;

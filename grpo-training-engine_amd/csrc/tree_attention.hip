@@ -407,6 +407,9 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) next[i] = 0.f;
     values(vt, 0, v[0]);
+    // ahead of the SIMD's other wave, if that is between its tiles (64 trees of 36 nodes over 5000
+    // tokens 238 against 245 us)
+    __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
@@ -433,6 +436,7 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     sc = next;
   };
   for (int w0 = begin; w0 < end; w0 += WIN) {
