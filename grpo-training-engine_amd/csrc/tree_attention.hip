@@ -126,11 +126,11 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //    set of registers.
 // Measured at 28 and 4 heads of 128 dims, blocks of 16, contexts of half to one and a half times
 // the mean: 64 trees of 4 nodes over 2500 tokens 79 us (4.2 TB/s: the reading of the cache), 64
-// of 32 120 us (361 MB, 74 GFLOP), one of 61 over 30 thousand 51 us. With many rows the two waves
+// of 32 114 us (361 MB, 74 GFLOP), one of 61 over 30 thousand 49 us. With many rows the two waves
 // of a SIMD take 1.9 thousand cycles for a tile each, of which 1024 are products, and the longest
 // sequence ends last: 64 of 32 take 105 us without any reading of the cache. (Equal shares of all
 // tokens for every workgroup instead, of up to three sequences each: 164 against 146 us, the
-// parts' sums are 60 MB.)
+// parts' sums are 60 MB; second parts of the longest sequences only: 143 against 119.)
 
 constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
 constexpr int RING = 4;          // steps of K and V that stand there
