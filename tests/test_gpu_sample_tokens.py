@@ -105,6 +105,24 @@ def test_settings_of_each_row(dev, dtype):
           min_p=[0.0, 0.1, 0.0, 0.01, 0.5, 0.0, 0.2, 0.0, 1.0])
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("std", [0.3, 1.5])
+def test_cuts_one_after_another(dev, dtype, std):
+    """Few and many tokens before each cut and before the draw, few and many of one size."""
+    x, u = rows(13, 12, 20011, dtype, std)
+    x[:, ::7] = x[:, :1]  # 2859 of a value
+    k = [3, 50, 900, 1023, 1024, 1025, 1100, 4096, 5000, 0, 700, 12000]
+    for p in (0.05, 0.9, 0.999999):
+        check(dev, x, u, top_k=k, top_p=p)
+        check(dev, x, u, top_k=k, top_p=[p] * 6 + [1.0] * 6, min_p=0.2, temperature=1.1)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_more_rows_than_compute_units(dev, dtype):
+    x, u = rows(14, 300, 1501, dtype)
+    check(dev, x, u, temperature=0.9, top_k=300, top_p=0.95)
+
+
 def test_ends_of_the_unit_interval(dev):
     x, _ = rows(7, 6, 1000, "f32")
     u = torch.tensor([0.0, 1 - 2.0 ** -53, 0.5, 2.0 ** -60, 1 - 2.0 ** -24, 0.25],
