@@ -67,10 +67,14 @@ def _check_tables(block_tables, context_lens, counts, b: int, device):
     counts, which has to live as long."""
     if block_tables.ndim != 2 or not block_tables.shape[1]:
         raise ValueError("block_tables must be [batch, max_blocks].")
-    width = block_tables.shape[1]
-    _check_ints(block_tables, "block_tables", (b, width), device)
-    _check_ints(context_lens, "context_lens", (b,), device)
-    at = None
+    rows, width = block_tables.shape
+    at, index = None, device.index
+    # (one look at what is right; what is not is found below)
+    if not (rows == b and block_tables.dtype is _I32 and block_tables.get_device() == index
+            and context_lens.dtype is _I32 and context_lens.get_device() == index
+            and context_lens.ndim == 1 and context_lens.shape[0] == b):
+        _check_ints(block_tables, "block_tables", (b, width), device)
+        _check_ints(context_lens, "context_lens", (b,), device)
     if counts is not None:
         _check_ints(counts, "counts", (b,), device)
         counts = counts.contiguous()
@@ -193,7 +197,7 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     out = q.new_empty((b, t, hq, d))
     nbytes = _attn_bytes(b, t, hq, hkv, d)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = q.new_empty(nbytes // 2) if nbytes else None
     _run(dev, "grpo_paged_tree_attn", q.data_ptr(), qb, qt, qh, dtype is torch.float16,
          k_cache.data_ptr(), v_cache.data_ptr(), nb, tables.data_ptr(), bt_stride, bs, width,
          lens.data_ptr(), p_at, p_stride, n_at, scale, out.data_ptr(), b, t, hq, hkv, d,
