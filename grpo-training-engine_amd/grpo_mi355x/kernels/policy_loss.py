@@ -40,9 +40,8 @@ _MAX_VOCAB = 1 << 30
 def _run(device: torch.device, name: str, *args) -> None:
     """The C entry point on the device's current stream."""
     fn = getattr(_lib.device_library(), name)
-    index = device.index
-    if index == torch._C._cuda_getDevice():  # (a tensor of the device is there: it is set up)
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_handle(device))
     else:
         with torch.cuda.device(device):
             rc = fn(*args, _lib.stream_handle(device))
