@@ -596,6 +596,40 @@ def test_calls_on_two_streams_at_once(dev):
             assert torch.equal(x[0], w[0]) and torch.equal(x[1], w[1])
 
 
+def test_where_another_device_is_current(dev, monkeypatch):
+    """Every operator makes its tensors' device the current one for its launch."""
+    from grpo_mi355x import kernels
+
+    q, kc, vc, tables, lens, parents, _ = (
+        None if x is None else x.to(dev) for x in
+        attend_inputs(2, 5, 4, 2, 64, 16, "bf16", [40, 9], "random", None))
+    cos, sin = (x.to(dev) for x in tables_of_angles(64, 64, torch.float32))
+    ids = torch.ones(2, 5, dtype=torch.int64, device=dev)
+    logits, draws = torch.randn(5, 300, device=dev), torch.rand(5, device=dev)
+
+    def go():
+        k, v = kc.clone(), vc.clone()
+        return [kernels.paged_rope_append(q, q[:, :, :2], q[:, :, 2:], cos, sin, k, v, tables, lens),
+                kernels.paged_tree_attention(q, k, v, tables, lens, parents),
+                kernels.sample_tokens(logits, draws, top_p=0.9),
+                *kernels.accept_draft_tree(ids, parents, ids, lens, k, v, tables), k, v]
+
+    want, entered = go(), []
+
+    class Entered(torch.cuda.device):
+        def __init__(self, d):
+            entered.append(d)
+            super().__init__(d)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", Entered)
+    got = go()
+    monkeypatch.undo()
+    assert len(entered) == 4 and all(d.index == 0 for d in entered)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
 # --------------------------------------------------------------- refusals --
 
 def test_refusals(dev):
