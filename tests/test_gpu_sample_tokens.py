@@ -118,6 +118,14 @@ def test_cuts_one_after_another(dev, dtype, std):
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("v", [(1 << 18) - 1, 1 << 18, 1 << 20])
+def test_the_largest_vocabularies(dev, dtype, v):
+    x, u = rows(15, 2, v, dtype)
+    for kw in (dict(), dict(temperature=0.8, top_k=5000, top_p=0.9), dict(top_p=0.99, min_p=1e-4)):
+        check(dev, x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
 def test_more_rows_than_compute_units(dev, dtype):
     x, u = rows(14, 300, 1501, dtype)
     check(dev, x, u, temperature=0.9, top_k=300, top_p=0.95)
