@@ -343,6 +343,37 @@ def test_large_scores_keep_their_order(dev):
     check_attention(out, q, kc, vc, tables, lens, parents, None)
 
 
+@pytest.mark.parametrize("d,block,t", [(128, 16, 20), (64, 4, 33), (80, 16, 3)])
+def test_blocks_past_32_bits(dev, d, block, t):
+    """Blocks whose values stand 2^31 values and more into the cache: as in a small cache."""
+    from grpo_mi355x import kernels
+
+    q, kc, vc, tables, lens, parents, _ = attend_inputs(2, t, 6, 2, d, block, "bf16", [150, 33],
+                                                        "random", None, seed=9)
+    n, far = kc.shape[0], (1 << 31) // (2 * block * d) + 5
+    small = [x[None].to(dev) for x in (kc, vc)]  # [1, blocks, ...]: one layer
+    big = []
+    for x in small:
+        y = torch.empty(1, far + n, 2, block, d, dtype=x.dtype, device=dev)
+        y[:, far:] = x
+        big.append(y)
+    g = torch.Generator().manual_seed(1)
+    k = randn(g, 2, t, 2, d, dtype=torch.bfloat16).to(dev)
+    cos, sin = (x.to(dev) for x in tables_of_angles(d, 256, torch.float32))
+    drafted = torch.randint(0, 2, (2, t), generator=g).to(dev)
+    drawn = torch.randint(0, 2, (2, t), generator=g).to(dev)
+    q, tables, lens, parents = (x.to(dev) for x in (q, tables, lens, parents))
+    out = []
+    for (kk, vv), at in ((small, tables), (big, tables + far)):
+        r = kernels.paged_rope_append(q, k, k, cos, sin, kk[0], vv[0], at, lens)
+        out.append([r, kernels.paged_tree_attention(r, kk[0], vv[0], at, lens, parents),
+                    *kernels.accept_draft_tree(drafted, parents, drawn, lens, kk, vv, at)])
+        out[-1] += [x[:, -n:] for x in (kk, vv)]
+    for x, y in zip(*out):
+        assert torch.equal(x, y)
+    assert (out[0][3] > 1).any()  # something moved
+
+
 # ----------------------------------------------------------------- accept --
 
 def accept_inputs(g, b, t, hkv, d, block, layers, vocab=3):
