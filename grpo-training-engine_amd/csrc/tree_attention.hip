@@ -386,12 +386,14 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
     return top;
   };
-  // P V of a tile, and the next tile's scores (K at kn) with their maximum. In this order the
-  // vector instructions stand between products that they do not depend on: the compiler would
-  // put a tile's products one after another, and its arithmetic behind them.
+  // P V of a tile, and the next tile's scores (K at kn, its first fragments in k) with their
+  // maximum. In this order the vector instructions stand between products that they do not depend
+  // on: the compiler would put a tile's products one after another, and its arithmetic behind them.
+  // With two tiles a step the tile after the next has landed too, and its first fragments come
+  // into k (one tree of 61 nodes over 30 thousand tokens 52 -> 50.5 us; V's too: no faster).
   constexpr int A = KS < 4 ? KS : 4;  // fragments of K ahead
-  auto add = [&](f32x16_t& sc, const char* vt, const char* kn, uint4 (&k)[KS], float& top)
-                 __attribute__((always_inline)) {
+  auto add = [&](f32x16_t& sc, const char* vt, const char* kn, const char* after, uint4 (&k)[KS],
+                 float& top) __attribute__((always_inline)) {
     constexpr int E = 10;  // weights between the scores' products; the others between V's first
     uint4 v[2][DT];
     float x[16];
@@ -426,6 +428,11 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
       oacc[t % DT] = mfma32<F16>(v[t / DT][t % DT], make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]),
                                  oacc[t % DT]);
       if (t < DT) weights(E + (16 - E) * t / DT, E + (16 - E) * (t + 1) / DT);
+      if constexpr (PT == 2) {
+        if (t == DT)
+#pragma unroll
+          for (int i = 0; i < A; ++i) k[i] = k_of(after, i);
+      }
       if (t >= DT) {
         constexpr int M = 16 / DT;
 #pragma unroll
@@ -473,6 +480,10 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     asm volatile("" ::: "memory");
     sc = scores(0, 0);
     top = top_of(sc);
+    uint4 k[KS];
+    if constexpr (PT == 2)
+#pragma unroll
+      for (int i = 0; i < A; ++i) k[i] = k_of(lds + part * PART_B + TILE_B, i);
 #pragma unroll 1
     for (int s = 0; s < nstep; ++s) {
       if (nstep - 1 - s >= RING - 2)
@@ -489,12 +500,16 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
       if (row0 >= R) continue;
 #pragma unroll
       for (int q = 0; q < PT; ++q) {
-        const int sn = s + (q + 1) / PT, qn = (q + 1) % PT;  // (behind the last tile: of nothing)
-        const char* const kn = lds + (sn % RING) * STEP_B + part * PART_B + qn * TILE_B;
-        uint4 k[KS];
+        auto tile = [&](int ahead) {  // (behind the last: of nothing)
+          const int st = s + (q + ahead) / PT;
+          return lds + (st % RING) * STEP_B + part * PART_B + (q + ahead) % PT * TILE_B;
+        };
+        const char* const kn = tile(1);
+        if constexpr (PT == 1) {
 #pragma unroll
-        for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < A; ++i) k[i] = k_of(kn, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if (masked) {
           const int at = PTOK * part + 32 * q;
           const uint32_t here = (uint32_t)__ballot(rows[s * STEP + at + ln] >= 0);
@@ -508,7 +523,7 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
           top = top_of(sc);
         }
         rescale(pair32_max(top) * sl2);
-        add(sc, lds + (s % RING) * STEP_B + part * PART_B + HALF_B + q * TILE_B, kn, k, top);
+        add(sc, tile(0) + HALF_B, kn, tile(2), k, top);
       }
     }
   }
