@@ -167,6 +167,9 @@ __device__ __forceinline__ Row row_of(const TokArgs& a, int m, uint32_t valid) {
   const int64_t k = a.top_k ? (int64_t)a.top_k[m] : a.k;
   r.K = k > 0 && k < (int64_t)valid ? (uint32_t)k : valid;
   r.greedy = !(r.T > 0.0) || r.p <= 0.0 || r.mp > 1.0 || r.K == 1;
+  // Two logits of any type differ by 2^-149 or not at all, so from 1e-300 down every weight but
+  // the maximum's is 0, and log2(e) / T times 64 would become infinite: NaN at the maximum.
+  r.T = fmax(r.T, 1e-300);
   const double u = a.draws_f64 ? static_cast<const double*>(a.draws)[m]
                                : (double)static_cast<const float*>(a.draws)[m];
   r.u = u > 0.0 ? (u < 1.0 ? (uint64_t)(u * 18446744073709551616.0) : ~0ull) : 0;

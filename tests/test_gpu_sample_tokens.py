@@ -226,3 +226,22 @@ def test_values_of_every_size(dev, dtype):
     for kw in (dict(), dict(temperature=300.0, top_p=0.95), dict(top_k=1000), dict(min_p=0.3),
                dict(temperature=1e5, top_k=2500, top_p=0.99), dict(temperature=0.01)):
         check(dev, x, u, **kw)
+
+
+@pytest.mark.filterwarnings("ignore:overflow")  # of the oracle's quotients: -inf, as meant
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("temperature", [5e-324, 2.2250738585072014e-308, 5e-307, 1e-300, 1e-250,
+                                         1e-45])
+def test_temperatures_next_to_zero(dev, dtype, temperature):
+    """A draw among the maxima alone, down to the smallest number above 0; the filters count as
+    ever."""
+    x, u = rows(31, 7, 2003, dtype)
+    x[1, 4::500] = x[1].max()  # five maxima
+    x[2] = x[2, 0]  # nothing but maxima
+    x[3] *= 300  # past 512, below it too
+    x[4] = x[4] * 300 - 5000
+    x[5, ::3] = -float("inf")
+    x[6, 9] = float("inf")
+    for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.5),
+               dict(top_k=900, top_p=0.99, min_p=1e-9)):
+        check(dev, x, u, temperature=temperature, **kw)
