@@ -118,9 +118,13 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //    from LDS.
 //  * The scores of the next tile are made between the weights of this one: on a SIMD a product
 //    takes 32 cycles, an exponential 16, another instruction 4, side by side.
-//  * P is rounded to 16 bits (2^-8 of each weight in bf16, 2^-11 in float16), the sum is of the
-//    float32 weights: the roundings are independent, so over many tokens they stay below the
-//    rounding of the result.
+//  * P is two 16-bit values, a weight's rounding and the rest's (2^-17 of the weight off in bf16,
+//    2^-23 in float16), as in the decode attention: V times each is summed in float32. One value
+//    alone would add as much error as the rounding of the result, 0.0022 against 0.0017 of it in
+//    bf16, for 117 instead of 149 us (64 trees of 32, 2500 tokens), 50 instead of 62 (one of 61, 30
+//    thousand), 26 instead of 28.6 (32 of 16, 1500). In float16 a row's largest weight is 2^12 or
+//    more, so that what a small one loses below 2^-24 is 2^-37 of the largest: a long tail of faint
+//    tokens beside one that stands out keeps its mass.
 //  * Steps that reach past the cached tokens, or a window that holds a missing block, have V
 //    cleaned in LDS first and the scores masked: the same loop adds them, so that O stays in one
 //    set of registers.
@@ -361,12 +365,14 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     }
     odd |= __syncthreads_or(any) != 0;
   };
-  // The running maximum, ahead of scores up to top. It stands still while they are less than 2^8
-  // above it: the weights stay below 2^8, and the sums need no factor.
+  // The running maximum less FIRST (room below for float16's small weights), ahead of scores up to
+  // top. It stands still while they are less than MOST above it: the weights stay below 2^MOST, and
+  // the sums need no factor.
+  constexpr float FIRST = F16 ? 12.f : 0.f, MOST = F16 ? 15.f : 8.f;
   auto rescale = [&](float top) __attribute__((always_inline)) {
-    const bool up = top > m_run + 8.f;  // (the first score that is not -inf too)
+    const bool up = top > m_run + MOST;  // (the first score that is not -inf too)
     if (__ballot(up)) {
-      const float m_new = up ? top : m_run;
+      const float m_new = up ? top - FIRST : m_run;
       const float corr = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= corr;
 #pragma unroll
@@ -394,15 +400,22 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
   constexpr int A = KS < 4 ? KS : 4;  // fragments of K ahead
   auto add = [&](f32x16_t& sc, const char* vt, const char* kn, const char* after, uint4 (&k)[KS],
                  float& top) __attribute__((always_inline)) {
-    constexpr int E = 10;  // weights between the scores' products; the others between V's first
+    // weights between the scores' products (the first half's at least); the others between V's
+    // first
+    constexpr int E = 12;
     uint4 v[2][DT];
     float x[16];
-    uint32_t p[8];
+    uint32_t p[2][8];  // the weights' first parts, and the rest of them
     auto weights = [&](int from, int to) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = from; i < to; ++i) {
         x[i] = weight(sc[i]);
-        if (i & 1) p[i / 2] = pack_e2<F16>(x[i - 1], x[i]);
+        if (i & 1) {
+          const uint32_t h = pack_e2<F16>(x[i - 1], x[i]);
+          p[0][i / 2] = h;
+          p[1][i / 2] = pack_e2<F16>(x[i - 1] - e2f<F16>((uint16_t)h),
+                                     x[i] - e2f<F16>((uint16_t)(h >> 16)));
+        }
       }
     };
     f32x16_t next;
@@ -423,22 +436,22 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     values(vt, 1, v[1]);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < 2 * DT; ++t) {
-      const int j = t / DT * 4;
-      oacc[t % DT] = mfma32<F16>(v[t / DT][t % DT], make_uint4(p[j], p[j + 1], p[j + 2], p[j + 3]),
-                                 oacc[t % DT]);
-      if (t < DT) weights(E + (16 - E) * t / DT, E + (16 - E) * (t + 1) / DT);
+    for (int n = 0; n < 4 * DT; ++n) {  // product j of both parts, of all dims
+      const int j = n / (2 * DT), t = n % DT, m = n - 2 * DT;
+      const uint32_t* const w = p[n / DT % 2] + 4 * j;
+      oacc[t] = mfma32<F16>(v[j][t], make_uint4(w[0], w[1], w[2], w[3]), oacc[t]);
+      if (m < 0) weights(E + (16 - E) * n / (2 * DT), E + (16 - E) * (n + 1) / (2 * DT));
       if constexpr (PT == 2) {
-        if (t == DT)
+        if (m == 0)
 #pragma unroll
           for (int i = 0; i < A; ++i) k[i] = k_of(after, i);
       }
-      if (t >= DT) {
-        constexpr int M = 16 / DT;
+      if (m >= 0) {
+        constexpr int M = 8 / DT;
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-          const float y = next[M * (t - DT) + i];
-          top = t == DT && i == 0 ? y : fmaxf(top, y);
+          const float y = next[M * m + i];
+          top = m == 0 && i == 0 ? y : fmaxf(top, y);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -565,12 +578,24 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     }
     m_run = m;
   }
-  if (__builtin_expect(odd, 0)) {  // the values that were taken out, for the rows that attend them
+  // A value of V that is not finite: it was taken out, or the two parts of its weights made NaN of
+  // it. Such values' sum, of its row's attended tokens, takes the place of the dim's.
+  float finite = 0.f;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) finite = fmaf(oacc[t][i], 0.f, finite);
+  if (__builtin_expect(odd || __ballot(finite != 0.f && l_run == l_run), 0)) {
+    f32x16_t e[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[t][i] = 0.f;
 #pragma unroll 1
-    for (int k = max(begin, c.context); k < end; ++k) {
+    for (int k = begin; k < end; ++k) {
       const int64_t r = a.pages.row(b, k);
       if (r < 0) continue;
-      const bool mine = (mask >> (k - c.context)) & 1;
+      const bool mine = k < c.context || ((mask >> (k - c.context)) & 1);
       const uint16_t* const d = a.vc + (r + (int64_t)kvh * a.pages.block_size) * D + 4 * lh;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
@@ -579,10 +604,14 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
           const uint2 x = *reinterpret_cast<const uint2*>(d + 32 * t + 8 * i);
           const uint32_t w[2] = {x.x & inf_halves<F16>(x.x), x.y & inf_halves<F16>(x.y)};
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            oacc[t][4 * i + e] += mine ? e2f<F16>((uint16_t)(w[e / 2] >> (e & 1) * 16)) : 0.f;
+          for (int n = 0; n < 4; ++n)
+            e[t][4 * i + n] += mine ? e2f<F16>((uint16_t)(w[n / 2] >> (n & 1) * 16)) : 0.f;
         }
     }
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) oacc[t][i] = e[t][i] == 0.f ? oacc[t][i] : e[t][i];
   }
   if (row >= R) return;
   if (c.splits <= 1) {

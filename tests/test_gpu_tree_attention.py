@@ -1,0 +1,85 @@
+"""``paged_tree_attention`` where its weights are all there is to lose, against float64
+(oracle/draft_tree.py)."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import draft_tree as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def attend(dev, *args, **kw):
+    from grpo_mi355x.kernels import paged_tree_attention
+
+    return f64(paged_tree_attention(*(x if x is None else x.to(dev) for x in args), **kw))
+
+
+def check(out, want, size, dtype, scores, adds, faint):
+    """A weight is two 16-bit values (2^-17 of it off in bf16, 2^-23 in float16, and there 2^-37 of
+    the largest weight: `faint` sums that over the tokens) of an exponential (2^-20) of a score of
+    one product, which a few roundings of at most `scores` doublings move by 2^-22 of them. So is
+    the mean of the |v|, twice. A sum of `adds` float32 values one after another is off by 2^-24 of
+    itself for each. One rounding of the result."""
+    weight = {"bf16": 2.0 ** -17, "f16": 2.0 ** -23}[dtype] + 2.0 ** -20 + scores * 2.0 ** -22
+    f = torch.finfo(HALF[dtype])
+    bound = 2 * (weight + adds * 2.0 ** -24) * size + faint + f.eps / 2 * (np.abs(want) + f.tiny)
+    worst = float((np.abs(out - want) / bound).max())
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("t,hq,hkv,d", [(8, 4, 2, 128), (40, 8, 2, 128), (1, 16, 4, 128),
+                                        (6, 4, 2, 64), (20, 4, 1, 64), (40, 8, 2, 64),
+                                        (3, 2, 1, 80)])
+def test_weights_are_not_rounded_to_16_bits(dev, dtype, t, hq, hkv, d):
+    """Means of values of both signs that almost cancel: their weights, of two sizes, would show
+    in the result with 2^-9 (2^-12) of them lost."""
+    g = torch.Generator().manual_seed(d + t)
+    n, block, dt = 200, 16, HALF[dtype]
+    nb = -(-(n + t) // block)
+    kc, vc = (torch.zeros(nb, hkv, block, d, dtype=dt) for _ in range(2))
+    faint = torch.rand(nb, hkv, block, generator=g) < 0.6
+    kc[..., 0] = torch.where(faint, -1.0, 0.0).to(dt)
+    vc[:] = (torch.randint(0, 2, vc.shape, generator=g) * 2 - 1).to(dt)
+    q = torch.zeros(1, t, hq, d, dtype=dt)
+    q[..., 0] = (torch.rand(1, t, hq, generator=g) * 3).to(dt)  # weights of 1 and exp(-0 .. -3)
+    tables = torch.randperm(nb, generator=g).view(1, nb).int()
+    lens = torch.tensor([n], dtype=torch.int32)
+    out = attend(dev, q, kc, vc, tables, lens, scale=1.0)
+    want, size = ref.tree_attention(f64(q), f64(kc), f64(vc), tables.numpy(), lens.numpy(),
+                                    scale=1.0)
+    # (a lane adds every fourth weight, with other dims than 64 and 128 a thread every one)
+    check(out, want, size, dtype, 5, n + t if d == 80 else (n + t) / 4, (n + t) * 2.0 ** -37)
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nats", [9.0, 17.0, 20.0])
+def test_a_long_tail_beside_one_token_that_stands_out(dev, dtype, d, nats):
+    """The first token has nearly all the mass and a value of 0; what the tail gives is its mass.
+    One workgroup takes it all: there are more (sequence, head) pairs than parts."""
+    b, n, block, dt = 130, 131071, 16, HALF[dtype]
+    nb = -(-(n + 1) // block)
+    kc, vc = (torch.zeros(nb, 1, block, d, dtype=dt) for _ in range(2))
+    kc[..., 0] = -nats
+    vc[:] = torch.linspace(-1, 1, d).to(dt)
+    tables = torch.arange(nb).int()[None].repeat(b, 1)
+    kc[0, :, 0] = 0
+    vc[0, :, 0] = 0
+    lens = torch.zeros(b, dtype=torch.int32)
+    lens[77] = n
+    q = torch.zeros(b, 1, 2, d, dtype=dt)
+    q[..., 0] = 1
+    q[..., 1, :] *= 0.5  # half the distance
+    out = attend(dev, q, kc, vc, tables, lens, scale=1.0)[77:78]
+    want, size = ref.tree_attention(f64(q[77:78]), f64(kc), f64(vc), tables[77:78].numpy(),
+                                    lens[77:78].numpy(), scale=1.0)
+    check(out, want, size, dtype, 1.5 * nats, (n + 1) / 4, (n + 1) * 2.0 ** -37)
