@@ -58,7 +58,9 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
   const int64_t head = (int64_t)kvh * a.pages.block_size;
   const uint16_t* const q = a.q + (int64_t)b * a.qsb + (int64_t)t * a.qst + (int64_t)h * a.qsh;
   for (int d = tid; d < D; d += GT) qs[d] = e2f<F16>(q[d]);
-  const int64_t last = used ? (int64_t)context + t + 1 : 0;
+  // (no further than the table: a length past it would be walked for seconds)
+  const int64_t cap = (int64_t)a.pages.max_blocks * a.pages.block_size;
+  const int64_t last = used ? min((int64_t)context + t + 1, cap) : 0;
   float m_run = -INFINITY, l_run = 0.f, acc[GD / GT] = {};
   for (int64_t t0 = 0; t0 < last; t0 += GT) {
     __syncthreads();

@@ -83,3 +83,21 @@ def test_a_long_tail_beside_one_token_that_stands_out(dev, dtype, d, nats):
     want, size = ref.tree_attention(f64(q[77:78]), f64(kc), f64(vc), tables[77:78].numpy(),
                                     lens[77:78].numpy(), scale=1.0)
     check(out, want, size, dtype, 1.5 * nats, (n + 1) / 4, (n + 1) * 2.0 ** -37)
+
+
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("parents", [None, [[-1, 0, 0]]])
+def test_lengths_past_the_table(dev, d, parents):
+    """A length past the block table is all of the table, and no node has a slot."""
+    g = torch.Generator().manual_seed(d)
+    kc, vc = (torch.randn(12, 2, 16, d, generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(3, 3, 4, d, generator=g).bfloat16()
+    tables = torch.arange(12).view(3, 4).int()
+    if parents is not None:
+        parents = torch.tensor(parents, dtype=torch.int32).expand(3, 3)
+    full = attend(dev, q, kc, vc, tables, torch.full((3,), 64, dtype=torch.int32), parents)
+    want, _ = ref.tree_attention(f64(q), f64(kc), f64(vc), tables.numpy(), [64] * 3)
+    assert np.abs(full - want).max() < 0.02
+    for most in (65, 1 << 20, (1 << 31) - 3, (1 << 31) - 1):
+        lens = torch.tensor([most, 64, most], dtype=torch.int32)
+        assert (attend(dev, q, kc, vc, tables, lens, parents) == full).all(), most
