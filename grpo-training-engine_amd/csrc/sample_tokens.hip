@@ -900,6 +900,8 @@ __global__ void __launch_bounds__(TT, 4) sample_tokens_bf16_kernel(TokArgs a) {
   general_row<0, TT>(a, m, *reinterpret_cast<General<TT>*>(lds_raw), kmax, valid, r);
 }
 
+constexpr int MOST_ROWS = 1 << 22;  // of a launch
+
 template <auto KERN, int TT, int LDS>
 int go(const TokArgs& a, hipStream_t st) {
   if (int rc = allow_dynamic_lds<KERN, LDS>()) return rc;
@@ -929,14 +931,27 @@ extern "C" int grpo_sample_tokens(const void* logits, int dtype, int64_t ld, int
     return einval("logits must be aligned to their type");
   int bits = 0;
   while ((1 << bits) < V) ++bits;
-  const TokArgs a{logits, ld, M, V, draws, draws_f64, sampler->temperature_rows,
-                  sampler->top_k_rows, sampler->top_p_rows, sampler->min_p_rows,
-                  sampler->temperature, sampler->top_p, sampler->min_p, sampler->top_k,
-                  min(44, 62 - bits), tokens, kept};
+  TokArgs a{logits, ld, M, V, draws, draws_f64, sampler->temperature_rows,
+            sampler->top_k_rows, sampler->top_p_rows, sampler->min_p_rows,
+            sampler->temperature, sampler->top_p, sampler->min_p, sampler->top_k,
+            min(44, 62 - bits), tokens, kept};
   hipStream_t st = as_stream(stream);
   // Fewer waves wait less at the searches' barriers, more read a long row faster: 16 rows of 8000
   // float32 logits 18 us with 512 threads and 24 with 1024, of 40000 29-34 and 33-35, 37 of 50257
   // 38 and 36 (bf16 rows: 1024 from 8000 on).
-  return M > 256 || (dtype != 0 && V <= 49152) ? go_type<512>(a, dtype, st)
-                                               : go_type<1024>(a, dtype, st);
+  const bool small = M > 256 || (dtype != 0 && V <= 49152);
+  // (a launch has fewer than 2^32 threads)
+  for (int64_t left = M; left > 0; left -= MOST_ROWS) {
+    a.M = (int)std::min<int64_t>(left, MOST_ROWS);
+    if (int rc = small ? go_type<512>(a, dtype, st) : go_type<1024>(a, dtype, st)) return rc;
+    a.logits = static_cast<const char*>(a.logits) + MOST_ROWS * ld * (dtype == 2 ? 4 : 2);
+    a.draws = static_cast<const char*>(a.draws) + MOST_ROWS * (draws_f64 ? 8 : 4);
+    if (a.temperature) a.temperature += MOST_ROWS;
+    if (a.top_k) a.top_k += MOST_ROWS;
+    if (a.top_p) a.top_p += MOST_ROWS;
+    if (a.min_p) a.min_p += MOST_ROWS;
+    a.tokens += MOST_ROWS;
+    if (a.kept) a.kept += MOST_ROWS;
+  }
+  return GRPO_OK;
 }

@@ -245,3 +245,23 @@ def test_temperatures_next_to_zero(dev, dtype, temperature):
     for kw in (dict(), dict(top_k=50), dict(top_p=0.9), dict(min_p=0.5),
                dict(top_k=900, top_p=0.99, min_p=1e-9)):
         check(dev, x, u, temperature=temperature, **kw)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_more_rows_than_a_launch_takes(dev, dtype):
+    """8 million draws from one expanded row, settings of each row's own: every thousandth as in a
+    call of its own."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    m, g = (1 << 23) + 1234, torch.Generator().manual_seed(41)
+    x = (torch.randn(1, 5, generator=g) * 2).to(DTYPES[dtype]).to(dev).expand(m, 5)
+    u = torch.rand(m, generator=g).to(dev)
+    kw = dict(temperature=torch.rand(m, generator=g).to(dev) + 0.2,
+              top_k=torch.randint(0, 6, (m,), generator=g).int().to(dev),
+              top_p=1 - torch.rand(m, generator=g).to(dev) / 2,
+              min_p=torch.rand(m, generator=g).to(dev) / 4)
+    tokens, kept = sample_tokens(x, u, return_kept=True, **kw)
+    some = slice(7, None, 1000)
+    want = sample_tokens(x[some], u[some], return_kept=True, **{k: v[some] for k, v in kw.items()})
+    assert torch.equal(tokens[some], want[0]) and torch.equal(kept[some], want[1])
+    assert len(set(want[0].tolist())) > 2
