@@ -230,7 +230,8 @@ extern "C" int grpo_paged_rope_append(
   if (B < 0 || T < 0 || D % 2 || max_pos <= 0 ||
       !pages_ok(num_blocks, block_size, max_blocks, Hq, Hkv, D))
     return einval("bad rope/append dimensions");
-  if ((int64_t)B * T >= (1ll << 31)) return einval("too many rows");
+  // (256 threads for each row, fewer than 2^32 in a launch)
+  if ((int64_t)B * T >= (1ll << 24)) return einval("at most 2^24 - 1 tokens");
   if (B == 0 || T == 0) return GRPO_OK;
   if (!q || !k || !v || !cos_table || !sin_table || !context_lens || !q_out || !k_cache ||
       !v_cache || !block_tables)

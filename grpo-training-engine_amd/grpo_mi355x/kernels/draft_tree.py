@@ -125,7 +125,8 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: to
     """Rotate ``q [B, T, Hq, D]`` and ``k [B, T, Hkv, D]`` to their positions and store the
     rotated ``k`` and ``v`` at slots ``context_lens[b] + i``; returns the rotated ``q``.
 
-    Any number of tokens ``T`` (a tree's nodes, or a chunk of a prompt), any strides.
+    Any number of tokens ``T`` (a tree's nodes, or a chunk of a prompt; fewer than 2^24 in all),
+    any strides.
     ``cos``/``sin`` ``[max_pos, D]`` in float32 or q's type (``rotary_emb.tables``); position of
     token ``i``: ``positions[b, i]`` (int32; clamped to the table), else ``context_lens[b] + i``.
     The rotation is float32, rounded once. Rows past ``counts[b]`` are not stored and their

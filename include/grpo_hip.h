@@ -1012,7 +1012,7 @@ int grpo_paged_attn_prefill(const void* q, int64_t q_stride_b, int64_t q_stride_
 
 /* Rotation of queries and keys to their positions, and the keys and values into the cache:
  * fused_qkv_rope + the KV update (src/triton_kernels/fused_ops.py:198-219, paged_kv.py:253-319)
- * for T >= 0 tokens per sequence (any number here).
+ * for T >= 0 tokens per sequence (any number here, B T < 2^24).
  *   q [B, T, Hq, D], k, v [B, T, Hkv, D]: strides of sequence, token and head in values
  *   cos_table, sin_table : [max_pos, D], float32 (table_f32) or the 16-bit type
  *   positions : int32 [B, T] (row stride pos_stride; clamped to the table), or NULL:

@@ -204,3 +204,16 @@ def test_drafted_tree_argument_errors(lib):
                dict(sampler=False), dict(logits=p + 1), dict(logits=p + 2, dtype=2)):
         assert sample(**kw) < 0, kw
     assert sample(m=0) == 0
+
+
+def test_more_tokens_than_a_launch_takes(lib):
+    """Refused where 256 threads for each would be 2^32 (addresses are never dereferenced)."""
+    p = 1 << 20
+
+    def append(b, t):
+        return lib.grpo_paged_rope_append(p, 0, 0, 0, p, 0, 0, 0, p, 0, 0, 0, 0, p, p, 1, 64, None,
+                                          0, p, None, p, p, p, 8, p, 4, 16, 4, b, t, 4, 2, 32, None)
+
+    for b, t in ((1, 1 << 24), (1 << 24, 1), (1 << 12, 1 << 12), (1 << 16, 1 << 10),
+                 (1 << 16, 1 << 14)):
+        assert append(b, t) == -1, (b, t)
