@@ -771,7 +771,9 @@ extern "C" int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, i
   if (T > TREE_MAX) return einval("a drafted tree has at most 64 nodes");
   if (D > GD) return einval("head_dim at most 512");
   if (!std::isfinite(scale)) return einval("the scale must be finite");
-  if (Hq > 65535 || (int64_t)B * T >= (1ll << 31)) return einval("too many rows or heads");
+  // (the plain kernel: 256 threads for each node, fewer than 2^32 in a row of its grid)
+  if (Hq > 65535 || (int64_t)B * T >= (1ll << 24))
+    return einval("at most 65535 heads and 2^24 - 1 nodes");
   if (B == 0) return GRPO_OK;
   if (!q || !k_cache || !v_cache || !block_tables || !context_lens || !out)
     return einval("null pointer");

@@ -175,9 +175,9 @@ def paged_tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          parents: Optional[torch.Tensor] = None, *,
                          counts: Optional[torch.Tensor] = None,
                          scale: Optional[float] = None) -> torch.Tensor:
-    """Attention of the nodes' (rotated) ``q [B, T, Hq, D]``, ``T <= 64``, each over its
-    sequence's ``context_lens[b]`` cached tokens, its ancestors and itself; ``[B, T, Hq, D]`` in
-    q's type.
+    """Attention of the nodes' (rotated) ``q [B, T, Hq, D]``, ``T <= 64`` (fewer than 2^24 nodes in
+    all), each over its sequence's ``context_lens[b]`` cached tokens, its ancestors and itself;
+    ``[B, T, Hq, D]`` in q's type.
 
     ``parents`` int32 ``[B, T]`` (one tree for all: ``parents.expand(B, -1)``), None: a chain,
     node ``i - 1`` being the parent of ``i``. ``scale``: 1 / sqrt(D) unless given. Nodes past

@@ -1035,7 +1035,7 @@ int grpo_paged_rope_append(const void* q, int64_t q_sb, int64_t q_st, int64_t q_
  * itself (the decode attention of paged_kv.py:63-251 for a tree): out[b, i, h] = sum_t
  * softmax_t(scale * q[b, i, h].k_t) v_t, KV head h / (Hq / Hkv). Rows past counts[b], and rows
  * that attend nothing, are 0. parents: int32 [B, T] (row stride parents_stride), or NULL: a
- * chain. out: [B, T, Hq, D] in q's type. D <= 512. */
+ * chain. out: [B, T, Hq, D] in q's type. D <= 512, Hq < 65536, B T < 2^24. */
 size_t grpo_paged_tree_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D);
 int grpo_paged_tree_attn(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int f16,
                          const void* k_cache, const void* v_cache, int64_t num_blocks,

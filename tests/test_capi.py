@@ -217,3 +217,10 @@ def test_more_tokens_than_a_launch_takes(lib):
     for b, t in ((1, 1 << 24), (1 << 24, 1), (1 << 12, 1 << 12), (1 << 16, 1 << 10),
                  (1 << 16, 1 << 14)):
         assert append(b, t) == -1, (b, t)
+
+    def attend(b, t, d):
+        return lib.grpo_paged_tree_attn(p, 0, 0, 0, 0, p, p, 8, p, 4, 16, 4, p, None, 0, None, 1.0,
+                                        p, b, t, 4, 2, d, None, 0, None)
+
+    for b, t in ((1 << 24, 1), (1 << 18, 64), (1 << 20, 32)):
+        assert attend(b, t, 80) == attend(b, t, 128) == -1, (b, t)
