@@ -9,7 +9,8 @@
 //
 //  * Masses are integers, in units of 2^-S of the largest weight, S = 62 - ceil(log2 V), at most
 //    44: their sums do not depend on the order in which threads add them, so the token is a
-//    function of the inputs alone. Weights are doubles.
+//    function of the inputs alone. Weights are doubles, rounded once to a unit where a bf16 row is
+//    counted by its values; where bins of the distance stand for them, see there.
 //  * "The first place in sorted order where the mass reaches P or the count reaches K" gives the
 //    top-k, top-p and min-p cuts and the draw itself. It is found in a histogram of the row: of
 //    its values in bf16, else of 4096 distances from the maximum and then, within the one of
@@ -285,8 +286,10 @@ __device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kma
 // 64 bins per doubling below the maximum. A token adds one 64-bit number to its bin: 1 to the
 // count in the upper bits, and (1 - 2^-(f / 64)) 2^UNIT to a sum in the lower ones, f its place in
 // the bin. A bin's mass is 2^-(bin / 64) (count - sum): one LDS atomic and 4 FMAs per token
-// (2e-14 of its weight) instead of two and an exponential. Within a bin the tokens' weights are
-// relative to the bin's first, and P is a share of the bin's mass.
+// instead of two and an exponential. A token's weight in it is off by 1.3e-12 of itself at most for
+// the series and half a unit for its place: 2^-(71 - 2 bits of V), 2e-12 up to 65535 tokens, 3e-11 up
+// to 262143, 2e-9 for 2^20. Within a bin the tokens' weights are relative to the bin's first (2^-44),
+// and P is a share of the bin's mass.
 constexpr int NB = 4096;
 constexpr int LIST = 4096;     // tokens of one bin that LDS holds
 constexpr int ALL = 1024;      // of all bins down to one (512 to 4096: no difference)
@@ -331,8 +334,9 @@ __device__ __forceinline__ void general_row(const TokArgs& a, int m, General<TT>
   const E* const row = static_cast<const E*>(a.logits) + (int64_t)m * a.ld;
   const Scale sc{key_value<DT>(kmax), 1.4426950408889634 / r.T};
   const double ymin = r.mp > 0.0 ? -log2(r.mp) : INFINITY;
-  // The sum of V places, below V A64 2^unit, stays in the lower bits, their count in the upper.
-  const int cbits = a.V < 1 << 18 ? 18 : 21, unit = 70 - 2 * cbits, sbits = 64 - cbits;
+  // The sum of V places, below V A64 2^unit, stays in the lower bits, their count in the upper
+  // (13 at least: a place of 2^-44 is as fine as a mass).
+  const int cbits = max(13, 32 - __clz(V)), unit = 70 - 2 * cbits, sbits = 64 - cbits;
   for (int j = tid; j < NB; j += TT) s.bins[j] = 0;
   __syncthreads();
   uint32_t near = 0;  // tokens that min_p leaves

@@ -42,7 +42,9 @@ def sample_tokens(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Set
     it is below ``top_p`` times the mass of those ``top_k``, and ``w >= min_p``; the first
     always is. The token is the first kept one at which the running mass passes ``draws`` times
     the kept mass. Masses are integers (units of 2^-44 of the largest weight; 2^-(62 - log2 V)
-    for more than 2^18 tokens), so the same inputs give the same token, whatever runs beside.
+    for more than 2^18 tokens), so the same inputs give the same token, whatever runs beside. A
+    weight in them is rounded to a unit for most bf16 rows, else off by 3e-11 of itself at most
+    (2e-9 for 2^20 tokens): a draw or a border closer than that to a sum may go to its other side.
 
     Each setting is a number or a tensor of the leading shape. ``temperature`` 0 (or below):
     the lowest index of the maximum; ``top_k`` 0 (or below), ``top_p`` 1, ``min_p`` 0: no such

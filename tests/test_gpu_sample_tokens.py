@@ -265,3 +265,24 @@ def test_more_rows_than_a_launch_takes(dev, dtype):
     want = sample_tokens(x[some], u[some], return_kept=True, **{k: v[some] for k, v in kw.items()})
     assert torch.equal(tokens[some], want[0]) and torch.equal(kept[some], want[1])
     assert len(set(want[0].tolist())) > 2
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("v,apart", [(1 << 13, 1e-6), (50257, 1e-6), (151936, 3e-5), (1 << 18, 1e-4)])
+def test_draws_next_to_a_border(dev, dtype, v, apart):
+    """One token and v - 1 equal ones far below it, draws next to the border between two of these, by
+    `apart` of one's weight. All of their weights are off by the same 2^-(71 - 2 bits of v) at most,
+    and 1.3e-12, which moves a border by v - 1 times as much of one weight."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    off = 2.0 ** -(71 - 2 * max(13, v.bit_length())) + 1.3e-12
+    assert (v - 1) * off < 0.5 * apart
+    x = torch.full((1, v), -13.828125, dtype=DTYPES[dtype])
+    x[0, 0] = 0
+    w = float(np.exp(np.longdouble(-13.828125)))
+    total = 1 + (v - 1) * np.longdouble(w)
+    rank = np.arange(1, 200)
+    u = np.concatenate([(1 + np.longdouble(w) * (rank + s * np.longdouble(apart))) / total
+                        for s in (-1, 1)]).astype(np.float64)
+    tokens = sample_tokens(x.to(dev).expand(len(u), v), torch.from_numpy(u).to(dev)).cpu().numpy()
+    assert (tokens[:199] == rank).all() and (tokens[199:] == rank + 1).all()
