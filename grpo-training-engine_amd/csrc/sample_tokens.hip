@@ -1,6 +1,8 @@
 // A token from each row of logits with temperature, top-k, top-p and min-p, from given
-// uniform numbers (grpo_sample_tokens): the filters of the reference's _sample_tokens
-// (src/triton_kernels/paged_kv.py:418-450) in exact arithmetic, without a sort.
+// uniform numbers (grpo_sample_tokens), without a sort. The place of the reference's _sample_tokens
+// (src/triton_kernels/paged_kv.py:418-450) but not its top-p: the token at which the mass passes
+// top_p is kept here, as the last of the shortest head that holds top_p of the mass, and cut there
+// and in grpo_sample_top_p. Of .5, .3, .15, .05 at .9 three are kept here, two there.
 //
 // Row m: w_v = exp((x_v - max) / T), the row in descending order of x (ties by index). Kept
 // is the head of that order with rank < k, then a mass before it below top_p times the mass
@@ -287,9 +289,9 @@ __device__ __forceinline__ bool simple_row(const TokArgs& a, int m, uint32_t kma
 // count in the upper bits, and (1 - 2^-(f / 64)) 2^UNIT to a sum in the lower ones, f its place in
 // the bin. A bin's mass is 2^-(bin / 64) (count - sum): one LDS atomic and 4 FMAs per token
 // instead of two and an exponential. A token's weight in it is off by 1.3e-12 of itself at most for
-// the series and half a unit for its place: 2^-(71 - 2 bits of V), 2e-12 up to 65535 tokens, 3e-11 up
-// to 262143, 2e-9 for 2^20. Within a bin the tokens' weights are relative to the bin's first (2^-44),
-// and P is a share of the bin's mass.
+// the series and half a unit for its place: 2^-(71 - 2 bits of V), 2e-12 up to 65535 tokens, 3e-11
+// up to 262143, 2e-9 for 2^20. Within a bin the tokens' weights are relative to the bin's first
+// (2^-44), and P is a share of the bin's mass.
 constexpr int NB = 4096;
 constexpr int LIST = 4096;     // tokens of one bin that LDS holds
 constexpr int ALL = 1024;      // of all bins down to one (512 to 4096: no difference)

@@ -222,8 +222,9 @@ def accept_draft_tree(draft_tokens: torch.Tensor, parents: torch.Tensor, sampled
 
     Returns ``(tokens, accepted, path)``: the new tokens ``[B, T]`` int64 (``sampled`` along the
     path, the last of them pending; ``pad_token_id`` behind them), how many they are ``[B]``
-    int32, and the accepted nodes ``[B, T]`` int32 (-1 behind them). What is drawn with
-    ``sample_tokens`` has the model's own distribution, whatever was drafted."""
+    int32, and the accepted nodes ``[B, T]`` int32 (-1 behind them). The tokens
+    have the distribution of drawing one at a time in the way ``sampled`` was drawn, whatever was
+    drafted."""
     (layers, nb, hkv, bs, d), _, dev = _check_cache(k_cache, v_cache, True)
     shape = draft_tokens.shape
     if len(shape) != 2:

@@ -1,6 +1,11 @@
 """``sample_tokens`` -- a token from each row of logits, from given uniform numbers
-(``csrc/sample_tokens.hip``): the filters of ``src/triton_kernels/paged_kv.py:418-450`` in exact
-arithmetic, with top-k and min-p, for any vocabulary, type and row.
+(``csrc/sample_tokens.hip``), with temperature, top-k, top-p and min-p, for any vocabulary, type
+and row.
+
+Its top-p is not that of ``src/triton_kernels/paged_kv.py:418-450``, which the framework's sampled
+decode keeps (``paged_kv_decode_model``, ``grpo_sample_top_p``): the token at which the mass passes
+``top_p`` is kept here (the shortest head that holds ``top_p`` of the mass) and cut there. Of .5,
+.3, .15 and .05 at .9 three are kept here, two there.
 """
 
 from __future__ import annotations
@@ -41,10 +46,12 @@ def sample_tokens(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Set
     (ties by index), a token is kept while fewer than ``top_k`` stand before it, the mass before
     it is below ``top_p`` times the mass of those ``top_k``, and ``w >= min_p``; the first
     always is. The token is the first kept one at which the running mass passes ``draws`` times
-    the kept mass. Masses are integers (units of 2^-44 of the largest weight; 2^-(62 - log2 V)
-    for more than 2^18 tokens), so the same inputs give the same token, whatever runs beside. A
-    weight in them is rounded to a unit for most bf16 rows, else off by 3e-11 of itself at most
-    (2e-9 for 2^20 tokens): a draw or a border closer than that to a sum may go to its other side.
+    the kept mass. (The sampled decode's ``top_p`` also cuts the token that passes it.)
+
+    Masses are integers (units of 2^-44 of the largest weight; 2^-(62 - log2 V) for more than 2^18
+    tokens), so the same inputs give the same token, whatever runs beside. A weight in them is
+    rounded to a unit for most bf16 rows, else off by 3e-11 of itself at most (2e-9 for 2^20
+    tokens): a draw or a border closer than that to a sum may go to its other side.
 
     Each setting is a number or a tensor of the leading shape. ``temperature`` 0 (or below):
     the lowest index of the maximum; ``top_k`` 0 (or below), ``top_p`` 1, ``min_p`` 0: no such

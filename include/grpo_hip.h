@@ -1064,14 +1064,15 @@ int grpo_draft_tree_accept(const int64_t* drafted, int64_t drafted_stride, const
                            grpo_stream_t stream);
 
 /* One token per row of logits [M, V] (row stride ld in values; dtype as in the policy update),
- * with temperature, top-k, top-p and min-p (src/triton_kernels/paged_kv.py:418-450), from given
- * uniform numbers in [0, 1) (draws: float32, or float64 when draws_f64). w_v = exp((x_v - max)
- * / T); in descending order of x (ties by index) a token is kept while fewer than top_k stand
- * before it, the mass before it is below top_p times the mass of those top_k, and w >= min_p;
- * the first always. The token is the first kept one at which the running mass passes u times
- * the kept mass. Masses are integers in units of 2^-44 of the largest weight (2^-(62 - log2 V) for
- * V > 2^18); a weight in them is rounded to a unit where a bf16 row is counted by its values, else
- * off by 3e-11 of itself at most up to 2^18 tokens, 2e-9 for 2^20.
+ * with temperature, top-k, top-p and min-p, from given uniform numbers in [0, 1) (draws: float32,
+ * or float64 when draws_f64). w_v = exp((x_v - max) / T); in descending order of x (ties by index)
+ * a token is kept while fewer than top_k stand before it, the mass before it is below top_p times
+ * the mass of those top_k, and w >= min_p; the first always (grpo_sample_top_p and
+ * src/triton_kernels/paged_kv.py:418-434 also cut the token at which the mass passes top_p). The
+ * token is the first kept one at which the running mass passes u times the kept mass. Masses are
+ * integers in units of 2^-44 of the largest weight (2^-(62 - log2 V) for V > 2^18); a weight in
+ * them is rounded to a unit where a bf16 row is counted by its values, else off by 3e-11 of itself
+ * at most up to 2^18 tokens, 2e-9 for 2^20.
  * Each setting is one number, or one per row where its _rows pointer is not NULL. temperature
  * <= 0 (or NaN), top_p <= 0 or min_p > 1: the lowest index of the maximum. top_k <= 0, top_p >=
  * 1, min_p <= 0: no such bound. NaN and -inf are never drawn; where +inf is the maximum only

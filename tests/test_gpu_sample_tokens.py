@@ -268,11 +268,12 @@ def test_more_rows_than_a_launch_takes(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("v,apart", [(1 << 13, 1e-6), (50257, 1e-6), (151936, 3e-5), (1 << 18, 1e-4)])
+@pytest.mark.parametrize("v,apart", [(1 << 13, 1e-6), (50257, 1e-6), (151936, 3e-5),
+                                     (1 << 18, 1e-4)])
 def test_draws_next_to_a_border(dev, dtype, v, apart):
-    """One token and v - 1 equal ones far below it, draws next to the border between two of these, by
-    `apart` of one's weight. All of their weights are off by the same 2^-(71 - 2 bits of v) at most,
-    and 1.3e-12, which moves a border by v - 1 times as much of one weight."""
+    """One token and v - 1 equal ones far below it, draws next to the border between two of these,
+    by `apart` of one's weight. All of their weights are off by the same 2^-(71 - 2 bits of v) at
+    most, and 1.3e-12, which moves a border by v - 1 times as much of one weight."""
     from grpo_mi355x.kernels import sample_tokens
 
     off = 2.0 ** -(71 - 2 * max(13, v.bit_length())) + 1.3e-12
@@ -286,3 +287,18 @@ def test_draws_next_to_a_border(dev, dtype, v, apart):
                         for s in (-1, 1)]).astype(np.float64)
     tokens = sample_tokens(x.to(dev).expand(len(u), v), torch.from_numpy(u).to(dev)).cpu().numpy()
     assert (tokens[:199] == rank).all() and (tokens[199:] == rank + 1).all()
+
+
+def test_top_p_keeps_the_token_that_passes_it(dev):
+    """The shortest head that holds top_p of the mass; the sampled decode's rule cuts its last
+    token."""
+    from grpo_mi355x.kernels import sample_tokens
+    from grpo_mi355x.kernels.paged_kv import _apply_top_p
+
+    p = torch.tensor([0.15, 0.5, 0.05, 0.3], dtype=torch.float64)
+    x = p.log().float()[None].to(dev).expand(4, 4)
+    # the draws' places among .5, .3, .15
+    u = torch.tensor([0.5, 0.55, 0.8, 0.86], dtype=torch.float64, device=dev)
+    tokens, kept = sample_tokens(x, u, top_p=0.9, return_kept=True)
+    assert kept.tolist() == [3] * 4 and tokens.tolist() == [1, 3, 3, 0]
+    assert torch.isfinite(_apply_top_p(x, 0.9)).sum(1).tolist() == [2] * 4
