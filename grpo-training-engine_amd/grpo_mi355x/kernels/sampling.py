@@ -33,6 +33,8 @@ def _row_setting(t: torch.Tensor, name: str, lead, device, dtype) -> torch.Tenso
         raise ValueError(f"{name} must be on {device}, got {t.device}.")
     if t.dtype.is_complex or (dtype == torch.int32 and t.dtype.is_floating_point):
         raise ValueError(f"{name} cannot be {t.dtype}.")
+    if dtype == torch.int32 and t.dtype in (torch.int64, torch.uint32, torch.uint64):
+        t = t.long().clamp(0, _MAX_VOCAB)
     return t.to(dtype).contiguous()
 
 
@@ -53,7 +55,8 @@ def sample_tokens(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Set
     rounded to a unit for most bf16 rows, else off by 3e-11 of itself at most (2e-9 for 2^20
     tokens): a draw or a border closer than that to a sum may go to its other side.
 
-    Each setting is a number or a tensor of the leading shape. ``temperature`` 0 (or below):
+    Each setting is a number or a tensor of the leading shape (float32; ``top_k`` integers).
+    ``temperature`` 0 (or below):
     the lowest index of the maximum; ``top_k`` 0 (or below), ``top_p`` 1, ``min_p`` 0: no such
     filter. NaN and -inf logits are never drawn; beside +inf only +inf is. A row with nothing to
     draw gives -1. With ``return_kept`` also the number of kept tokens (int32)."""
@@ -88,9 +91,11 @@ def sample_tokens(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Set
             held.append(_row_setting(value, name, lead, dev, dtype))
             setattr(s, name + "_rows", held[-1].data_ptr())
             continue
-        number = int(value) if name == "top_k" else float(value)
+        number = value if name == "top_k" and isinstance(value, int) else float(value)
         if number != number or number in (math.inf, -math.inf):
             raise ValueError(f"{name} must be a finite number, got {value}.")
+        if name == "top_k":
+            number = min(max(int(number), 0), _MAX_VOCAB)
         setattr(s, name, number)
     tokens = torch.empty(lead, dtype=torch.int64, device=dev)
     kept = torch.empty(lead, dtype=torch.int32, device=dev) if return_kept else None

@@ -302,3 +302,26 @@ def test_top_p_keeps_the_token_that_passes_it(dev):
     tokens, kept = sample_tokens(x, u, top_p=0.9, return_kept=True)
     assert kept.tolist() == [3] * 4 and tokens.tolist() == [1, 3, 3, 0]
     assert torch.isfinite(_apply_top_p(x, 0.9)).sum(1).tolist() == [2] * 4
+
+
+def test_top_k_past_32_bits(dev):
+    """More than the vocabulary is no bound, however large; below 0 is none either."""
+    from grpo_mi355x.kernels import sample_tokens
+
+    x, u = rows(51, 6, 900, "f32")
+    x, u = x.to(dev), u.to(dev)
+    want, kept = sample_tokens(x, u, return_kept=True)
+    assert kept.tolist() == [900] * 6
+    for k in (1 << 31, (1 << 32) + 3, (1 << 63) + 2, (1 << 64) + 3, -(1 << 64) + 3, 1e30):
+        got = sample_tokens(x, u, top_k=k, return_kept=True)
+        assert torch.equal(got[0], want) and torch.equal(got[1], kept), k
+    at = torch.tensor([(1 << 31) + 1, (1 << 32) + 1, (1 << 62) + 1, -(1 << 62) + 1, 0, 901],
+                      device=dev)
+    got = sample_tokens(x, u, top_k=at, return_kept=True)
+    assert torch.equal(got[0], want) and torch.equal(got[1], kept)
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64):
+        at = torch.arange(1, 7, device=dev).to(dtype)
+        assert sample_tokens(x, u, top_k=at, return_kept=True)[1].tolist() == [1, 2, 3, 4, 5, 6]
+    for k in (float("inf"), -float("inf"), float("nan")):
+        with pytest.raises(ValueError):
+            sample_tokens(x, u, top_k=k)
