@@ -77,9 +77,9 @@ def sample_tokens(logits: torch.Tensor, draws: torch.Tensor, *, temperature: Set
     x = logits.detach()
     if x.ndim != 2:
         x = x.reshape(-1, v)
-    if v > 1 and x.stride(1) != 1:
-        x = x.contiguous()
     m = x.shape[0]
+    if (v > 1 and x.stride(1) != 1) or (m > 1 and 0 < x.stride(0) < v):  # (rows that overlap)
+        x = x.contiguous()
     if m >= _MAX_ROWS:
         raise ValueError(f"at most {_MAX_ROWS - 1} rows of logits in a call.")
     draws = draws.contiguous()

@@ -325,3 +325,15 @@ def test_top_k_past_32_bits(dev):
     for k in (float("inf"), -float("inf"), float("nan")):
         with pytest.raises(ValueError):
             sample_tokens(x, u, top_k=k)
+
+
+def test_rows_that_overlap(dev):
+    from grpo_mi355x.kernels import sample_tokens
+
+    x, u = rows(61, 1, 1500, "bf16")
+    some = x[0].to(dev).unfold(0, 1000, 100)  # row m begins at 100 m
+    u = torch.rand(len(some), generator=torch.Generator().manual_seed(2)).to(dev)
+    for kw in (dict(), dict(top_k=30, temperature=0.8), dict(top_p=0.9)):
+        assert torch.equal(sample_tokens(some, u, **kw), sample_tokens(some.contiguous(), u, **kw))
+    one = torch.randn(9, 4).to(dev).t()  # tokens 4 apart, a row of one token
+    assert sample_tokens(one[:, :1], u[:4]).tolist() == [0] * 4
