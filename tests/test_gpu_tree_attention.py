@@ -101,3 +101,92 @@ def test_lengths_past_the_table(dev, d, parents):
     for most in (65, 1 << 20, (1 << 31) - 3, (1 << 31) - 1):
         lens = torch.tensor([most, 64, most], dtype=torch.int32)
         assert (attend(dev, q, kc, vc, tables, lens, parents) == full).all(), most
+
+
+def long_inputs(t, hq, hkv, d, block, dtype, contexts, rest, seed):
+    """Sequences of the given contexts among others of up to `rest` tokens, so many that each
+    (sequence, KV head) is one workgroup's; blocks in no order; the nodes' parents at random."""
+    g = torch.Generator().manual_seed(seed)
+    b, dt = -(-130 // hkv) + 1, HALF[dtype]
+    lens = torch.randint(0, rest, (b,), generator=g).int()
+    at = torch.randperm(b, generator=g)[:len(contexts)].tolist()
+    lens[at] = torch.tensor(contexts, dtype=torch.int32)
+    need = -(-(lens + t) // block)
+    nb = int(need.sum()) + 3
+    ids, used = torch.randperm(nb, generator=g).int(), 0
+    tables = torch.full((b, int(need.max())), -1, dtype=torch.int32)
+    for i, n in enumerate(need.tolist()):
+        tables[i, :n] = ids[used:used + n]
+        used += n
+    kc, vc = (torch.randn(nb, hkv, block, d, generator=g).to(dt) for _ in range(2))
+    q = (torch.randn(b, t, hq, d, generator=g) * 1.5).to(dt)
+    parents = torch.full((b, t), -1, dtype=torch.int32)
+    for i in range(1, t):
+        parents[:, i] = torch.randint(0, i, (b,), generator=g)
+    counts = torch.randint(t // 2 + 1, t + 1, (b,), generator=g).int()
+    return [q, kc, vc, tables, lens, parents, counts], at
+
+
+def check_some(out, args, some):
+    """The sequences `some`, as test_gpu_draft_tree bounds them; nodes past the counts are 0."""
+    from test_gpu_draft_tree import check_attention
+
+    q, kc, vc, tables, lens, parents, counts = args
+    assert np.isfinite(out).all()
+    check_attention(torch.from_numpy(out[some]), q[some], kc, vc, tables[some], lens[some],
+                    parents[some], counts[some])
+    for i, n in enumerate(counts.tolist()):
+        assert (out[i, n:] == 0).all()
+
+
+WHOLE = [
+    # t, hq, hkv, d, block: by rows of a KV head, 2 (64 dims), 4 and 8 waves side by side on them,
+    # blocks that hold whole pieces of 1 KiB and others
+    (8, 4, 2, 64, 16),
+    (9, 7, 1, 64, 5),
+    (20, 5, 1, 64, 16),
+    (31, 4, 1, 64, 12),
+    (33, 4, 1, 64, 64),
+    (64, 7, 1, 64, 6),
+    (9, 3, 1, 128, 16),
+    (16, 14, 2, 128, 7),
+    (40, 3, 1, 128, 12),
+    (43, 3, 1, 128, 16),
+    (64, 7, 1, 128, 10),
+]
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("case", WHOLE, ids=lambda c: "-".join(map(str, c)))
+def test_long_sequences_of_one_workgroup_each(dev, dtype, case):
+    """More steps than the ring of K and V holds, many times over, and more tokens than one window
+    of cache rows (4096): contexts that end, and trees that lie, on both sides of its borders."""
+    t = case[0]
+    contexts = [1000, 4096 - t // 2, 4096, 4095, 8192 - t, 8192 + 77]
+    args, at = long_inputs(*case, dtype, contexts, 200, seed=t)
+    out = attend(dev, *args[:6], counts=args[6].to(dev))
+    check_some(out, args, at + list(range(8)))
+
+
+@pytest.mark.parametrize("case", WHOLE, ids=lambda c: "-".join(map(str, c)))
+def test_long_sequences_of_one_workgroup_each_with_holes(dev, case):
+    """The same with missing blocks in some windows and none in others, NaN where nothing is
+    attended."""
+    t, block = case[0], case[4]
+    contexts = [1500, 4096 - t // 2, 8192 + 77]
+    args, at = long_inputs(*case, "bf16", contexts, 100, seed=t + 1)
+    q, kc, vc, tables, lens, parents, counts = args
+    gone = torch.zeros(tables.shape, dtype=torch.bool)
+    gone[at] = torch.rand(3, tables.shape[1], generator=torch.Generator().manual_seed(t)) < 0.02
+    gone[at[2], 5000 // block:] = False  # the last of its windows is whole
+    gone[at[1], 4000 // block:] = False
+    gone &= tables >= 0
+    for x in (kc, vc):
+        x[tables[gone].long()] = float("nan")
+        for i in range(len(lens)):  # behind the last node
+            end = int(lens[i] + counts[i])
+            if end % block:
+                x[tables[i, end // block], :, end % block:] = float("nan")
+    tables[gone] = -1
+    out = attend(dev, *args[:6], counts=counts.to(dev))
+    check_some(out, args, at + list(range(8)))
