@@ -51,7 +51,7 @@ int allow_dynamic_lds() {
   return rc;
 }
 
-__host__ __device__ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 __host__ __device__ inline bool aligned16(const void* ptr) {
   return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0;
