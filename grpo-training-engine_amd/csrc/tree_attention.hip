@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //  * The scores of the next tile are made between the weights of this one: on a SIMD a product
 //    takes 32 cycles, an exponential 16, another instruction 4, side by side.
 //  * P is two 16-bit values, a weight's rounding and the rest's (2^-17 of the weight off in bf16,
-//    2^-23 in float16), as in the decode attention: V times each is summed in float32. One value
+//    2^-22 in float16), as in the decode attention: V times each is summed in float32. One value
 //    alone would add as much error as the rounding of the result, 0.0022 against 0.0017 of it in
-//    bf16, for 117 instead of 149 us (64 trees of 32, 2500 tokens), 50 instead of 62 (one of 61, 30
+//    bf16, for 117 instead of 150 us (64 trees of 32, 2500 tokens), 50 instead of 62 (one of 61, 30
 //    thousand), 26 instead of 28.6 (32 of 16, 1500). In float16 a row's largest weight is 2^12 or
 //    more, so that what a small one loses below 2^-24 is 2^-37 of the largest: a long tail of faint
 //    tokens beside one that stands out keeps its mass.
@@ -131,12 +131,13 @@ __global__ void __launch_bounds__(GT) tree_attn_plain_kernel(TreeArgs a) {
 //    cleaned in LDS first and the scores masked: the same loop adds them, so that O stays in one
 //    set of registers.
 // Measured at 28 and 4 heads of 128 dims, blocks of 16, contexts of half to one and a half times
-// the mean: 64 trees of 4 nodes over 2500 tokens 79 us (4.2 TB/s: the reading of the cache), 64
-// of 32 114 us (361 MB, 74 GFLOP), one of 61 over 30 thousand 49 us. With many rows the two waves
-// of a SIMD take 1.9 thousand cycles for a tile each, of which 1024 are products, and the longest
-// sequence ends last: 64 of 32 take 105 us without any reading of the cache. (Equal shares of all
-// tokens for every workgroup instead, of up to three sequences each: 164 against 146 us, the
-// parts' sums are 60 MB; second parts of the longest sequences only: 143 against 119.)
+// the mean: 64 trees of 4 nodes over 2500 tokens 88 us (3.8 TB/s: the reading of the cache), 64
+// of 32 150 us (361 MB, 74 GFLOP), one of 61 over 30 thousand 62 us, 64 of 32 and 64 dims 102 us.
+// With many rows the two waves of a SIMD take 2.5 thousand cycles for a tile each, of which 1536 are
+// products, and the longest sequence ends last. (With P in one value: equal shares of all tokens for
+// every workgroup instead, of up to three sequences each, 164 against 146 us, the parts' sums are 60
+// MB; second parts of the longest sequences only, 143 against 119; 105 of 119 us without any
+// reading of the cache.)
 
 constexpr int WIN = 4096;        // tokens whose cache rows stand in LDS at a time
 constexpr int RING = 4;          // steps of K and V that stand there
@@ -398,7 +399,8 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
   // maximum. In this order the vector instructions stand between products that they do not depend
   // on: the compiler would put a tile's products one after another, and its arithmetic behind them.
   // With two tiles a step the tile after the next has landed too, and its first fragments come
-  // into k (one tree of 61 nodes over 30 thousand tokens 52 -> 50.5 us; V's too: no faster).
+  // into k (one tree of 61 nodes over 30 thousand tokens, P in one value: 52 -> 50.5 us; V's too:
+  // no faster).
   constexpr int A = KS < 4 ? KS : 4;  // fragments of K ahead
   auto add = [&](f32x16_t& sc, const char* vt, const char* kn, const char* after, uint4 (&k)[KS],
                  float& top) __attribute__((always_inline)) {
@@ -413,7 +415,10 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
       for (int i = from; i < to; ++i) {
         x[i] = weight(sc[i]);
         if (i & 1) {
-          const uint32_t h = pack_e2<F16>(x[i - 1], x[i]);
+          // (float16's first part is cut, one instruction instead of five: the rest is exact)
+          const uint32_t h =
+              F16 ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[i - 1], x[i]))
+                  : pack_bf2(x[i - 1], x[i]);
           p[0][i / 2] = h;
           p[1][i / 2] = pack_e2<F16>(x[i - 1] - e2f<F16>((uint16_t)h),
                                      x[i] - e2f<F16>((uint16_t)(h >> 16)));
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
     for (int i = 0; i < 16; ++i) next[i] = 0.f;
     values(vt, 0, v[0]);
     // ahead of the SIMD's other wave, if that is between its tiles (64 trees of 36 nodes over 5000
-    // tokens 238 against 245 us)
+    // tokens, P in one value: 238 against 245 us)
     __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -582,7 +587,7 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
   }
   // A value of V that is not finite: it was taken out, or the two parts of its weights made NaN of
   // it. Such values' sum, of its row's attended tokens, takes the place of the dim's.
-  float finite = 0.f;
+  float finite = 0.f;  // (0 of finite sums, else NaN)
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -713,9 +718,10 @@ struct Plan {
 Plan plan_of(int B, int T, int Hq, int Hkv, int D) {
   const int R = T * (Hq / Hkv);
   Plan p;
-  // The fewest waves on rows that hold them, of 4 and 8: 64 trees over 2500 tokens, 28 rows, 79
-  // us with 4 and 81 with 8, 112 rows 85 and 88; of 2 where a token is 128 bytes: 28 rows of 64
-  // dims 26 us with 2, 32 with 4 and 34 with 8, 56 rows 28, 33 and 37 (of 128 dims 81, 81, 83).
+  // The fewest waves on rows that hold them, of 4 and 8: 64 trees over 2500 tokens, 4 KV heads of
+  // 128 dims, 28 rows, 88 us with 4 and 92 with 8, 112 rows 102 and 105, 224 rows 192 and 152; of 2
+  // where a token is 128 bytes: 28 rows of 64 dims 45 us with 2, 62 with 4 and 68 with 8, 56 rows
+  // 48, 65 and 71, 112 rows 84, 71 and 74.
   p.rw = R <= 64 && D == 64 ? 2 : (R <= 128 ? 4 : 8);
   p.rb = (int)cdiv(R, 32 * p.rw);
   const int64_t groups = (int64_t)B * Hkv * p.rb;
