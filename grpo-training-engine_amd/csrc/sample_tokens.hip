@@ -587,8 +587,8 @@ __global__ void __launch_bounds__(TT) sample_tokens_kernel(TokArgs a) {
 // than 0, with a larger maximum, or with mass at -512 and below (an extreme temperature) takes
 // the bins of the distance. The second pass over the row looks for the token and ends where it is
 // found.
-// Bound on its CU by the atomics (8 of 29 us at 151936 tokens) and by the issue of what is done
-// per token (1 us per instruction). (The row in registers instead of its second reading: 8 / 512
+// Bound on its CU by loading and counting (16 of 28 us at 151936 tokens; stores in place of the
+// atomics take as long) and by the issue of what is done per token (1 us per instruction). (The row in registers instead of its second reading: 8 / 512
 // rows 39 / 155 us, in code without loops that runs at the rate of its instruction fetches.)
 constexpr int LEAST = 0x3080, LARGE = 0x4400;  // the bits of 2^-30 and 512
 constexpr int ZERO = LARGE - LEAST + 1;        // bin of 0; 0 and 2 ZERO: from +-512 on

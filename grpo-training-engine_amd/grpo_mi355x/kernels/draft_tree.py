@@ -129,7 +129,8 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: to
     any strides.
     ``cos``/``sin`` ``[max_pos, D]`` in float32 or q's type (``rotary_emb.tables``); position of
     token ``i``: ``positions[b, i]`` (int32; clamped to the table), else ``context_lens[b] + i``.
-    The rotation is float32, rounded once. Rows past ``counts[b]`` are not stored and their
+    The rotation is float32, rounded once (the decode step's rounds three times in bf16, so its
+    cached keys differ in last bits). Rows past ``counts[b]`` are not stored and their
     ``q`` is 0; slots past the block table, or in blocks outside the cache, are skipped."""
     (_, nb, hkv, bs, d), dtype, dev = _check_cache(k_cache, v_cache, False)
     if q.ndim != 4:
