@@ -592,14 +592,15 @@ __global__ void __launch_bounds__(512) tree_attn_kernel(FastArgs f) {
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) finite = fmaf(oacc[t][i], 0.f, finite);
-  if (__builtin_expect(odd || __ballot(finite != 0.f && l_run == l_run), 0)) {
+  const bool whole = __ballot(finite != 0.f && l_run == l_run) != 0;  // else among the nodes only
+  if (__builtin_expect(odd || whole, 0)) {
     f32x16_t e[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) e[t][i] = 0.f;
 #pragma unroll 1
-    for (int k = begin; k < end; ++k) {
+    for (int k = whole ? begin : max(begin, c.context); k < end; ++k) {
       const int64_t r = a.pages.row(b, k);
       if (r < 0) continue;
       const bool mine = k < c.context || ((mask >> (k - c.context)) & 1);

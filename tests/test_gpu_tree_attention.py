@@ -191,3 +191,41 @@ def test_long_sequences_of_one_workgroup_each_with_holes(dev, case):
     tables[gone] = -1
     out = attend(dev, *args[:6], counts=counts.to(dev))
     check_some(out, args, at + list(range(8)))
+
+
+@pytest.mark.parametrize("dtype", list(HALF))
+@pytest.mark.parametrize("many", [False, True])  # one workgroup for a whole sequence
+@pytest.mark.parametrize("t,hq,hkv,d", [(4, 12, 2, 128), (20, 12, 2, 128), (64, 8, 1, 128),
+                                        (7, 4, 2, 64), (20, 5, 1, 64), (40, 8, 2, 64),
+                                        (5, 2, 1, 80)])
+def test_infinite_values_of_cached_tokens(dev, dtype, many, t, hq, hkv, d):
+    """An infinite value of a cached token makes that dim infinite, of its sign, for every node,
+    however small its weight; two of opposite signs make it NaN; other dims stay as they are."""
+    g, dt = torch.Generator().manual_seed(d + t), HALF[dtype]
+    b, n, block = (140 if many else 2), 1000, 16
+    nb = -(-(n + t) // block) + 1
+    kc, vc = (torch.randn(nb, hkv, block, d, generator=g).to(dt) for _ in range(2))
+    q = torch.randn(b, t, hq, d, generator=g).to(dt)
+    lens = torch.full((b,), 100, dtype=torch.int32)
+    lens[1] = n
+    tables = torch.randperm(nb - 1, generator=g).int().expand(b, -1)
+    first = attend(dev, q, kc, vc, tables, lens)
+
+    def put(slot, dim, x):
+        vc[tables[0, slot // block], :, slot % block, dim] = x
+
+    put(200, 3, float("inf"))  # past the others' contexts and nodes
+    put(500, 4, -float("inf"))
+    put(333, 5, float("nan"))
+    put(333, 6, float("inf"))
+    put(900, 6, -float("inf"))
+    put(701, 8, float("inf"))
+    put(800, 8, float("inf"))
+    out = attend(dev, q, kc, vc, tables, lens)
+    inf = float("inf")
+    assert (out[1][..., [3, 8]] == inf).all() and (out[1][..., 4] == -inf).all()
+    assert np.isnan(out[1][..., [5, 6]]).all()
+    same = [i for i in range(d) if i not in (3, 4, 5, 6, 8)]
+    assert (out[..., same] == first[..., same]).all()
+    others = [i for i in range(b) if i != 1]
+    assert (out[others] == first[others]).all()
