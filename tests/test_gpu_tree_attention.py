@@ -23,12 +23,13 @@ def attend(dev, *args, **kw):
 
 
 def check(out, want, size, dtype, scores, adds, faint):
-    """A weight in [1, 2) is two 16-bit values: in bf16 its rounding and the rest, at most 2^-8, whose
-    own is 2^-17 off; in float16 what it is cut to and the rest, below 2^-10 and 2^-22 off (where it
-    is subnormal 2^-25, the largest weight being 2^12 or more: 2^-37 of that, which `faint` sums over
-    the tokens). It is of an exponential (2^-20) of a score of one product, which a few roundings of
-    at most `scores` doublings move by 2^-22 of them. Twice that of the mean of |v|. A sum of `adds` float32 values one after another is off by 2^-24 of
-    itself for each. One rounding of the result."""
+    """A weight in [1, 2) is two 16-bit values: in bf16 its rounding and the rest, at most 2^-8,
+    whose own is 2^-17 off; in float16 what it is cut to and the rest, below 2^-10 and 2^-22 off
+    (where it is subnormal 2^-25, the largest weight being 2^12 or more: 2^-37 of that, which
+    `faint` sums over the tokens). It is of an exponential (2^-20) of a score of one product, which
+    a few roundings of at most `scores` doublings move by 2^-22 of them. Twice that of the mean of
+    |v|. A sum of `adds` float32 values one after another is off by 2^-24 of itself for each. One
+    rounding of the result."""
     weight = {"bf16": 2.0 ** -17, "f16": 2.0 ** -22}[dtype] + 2.0 ** -20 + scores * 2.0 ** -22
     f = torch.finfo(HALF[dtype])
     bound = 2 * (weight + adds * 2.0 ** -24) * size + faint + f.eps / 2 * (np.abs(want) + f.tiny)
